@@ -30,6 +30,17 @@ from .eager import (
     quantize_signed_int4_rowwise,
 )
 from .int8_eager import quantize_signed_int8_rowwise as _quantize_int8_rowwise
+from .mx4 import (
+    convrot_mx4_attention,
+    convrot_mx4_cache_append,
+    convrot_mx4_cache_read,
+    convrot_mx4_linear,
+    dequantize_convrot_mx4,
+    mx4_cache_empty,
+    mx4_scales_from_rows,
+    mx4_scales_to_rows,
+    quantize_convrot_mx4,
+)
 
 __all__ = [
     "quantize_convrot_w4a4_weight",
@@ -38,6 +49,15 @@ __all__ = [
     "convrot_w8a8_linear",
     "convrot_w4a4_linear_lora",
     "set_unpacked_weights",
+    "quantize_convrot_mx4",
+    "dequantize_convrot_mx4",
+    "mx4_scales_to_rows",
+    "mx4_scales_from_rows",
+    "convrot_mx4_linear",
+    "mx4_cache_empty",
+    "convrot_mx4_cache_append",
+    "convrot_mx4_cache_read",
+    "convrot_mx4_attention",
     "is_available",
     "pick_groupsize",
 ]

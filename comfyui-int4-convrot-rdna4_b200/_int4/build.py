@@ -13,8 +13,9 @@ import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(os.path.dirname(_HERE), "csrc")
-SOURCES = ["convrot_b200.cu", "noalloc.cu"]
-HEADERS = ["sm100_ptx.cuh", "gemm_pair.cuh", "gemm_a8t.cuh", "lora_down.cuh", "linear_api.cuh"]
+SOURCES = ["convrot_b200.cu", "noalloc.cu", "mx4.cu"]
+HEADERS = ["sm100_ptx.cuh", "gemm_pair.cuh", "gemm_a8t.cuh", "lora_down.cuh", "linear_api.cuh", "hadamard.cuh",
+           "host_launch.cuh", "mx4_common.cuh", "mx4_quant.cuh", "mx4_gemm.cuh", "mx4_cache.cuh", "mx4_attn.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -54,7 +55,7 @@ def build(verbose: bool = False) -> str:
         raise RuntimeError("nvcc not found; cannot build libconvrot_b200.so")
     out = lib_path()
     tmp = out + ".tmp"
-    cmd = [nvcc, *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared",
+    cmd = [nvcc, *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared", "--threads", "0",
            "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
            "-o", tmp, *src_paths()]
     if verbose:

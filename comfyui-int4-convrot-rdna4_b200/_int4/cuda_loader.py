@@ -23,6 +23,7 @@ _IN_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_longlong
 _SIGNATURES = {
     "ck_convrot_quant_int4": [_P, _I, _P, _P, _I, _I, _I, _P],
     "ck_int4_quant_rowwise": [_P, _I, _P, _P, _I, _I, _P],
@@ -53,6 +54,16 @@ _SIGNATURES = {
     "ck_convrot_quant_int4_unpacked": [_P, _I, _P, _P, _I, _I, _I, _P],
     "ck_convrot_w4a4_linear_unpacked_workspace_size": [_I, _I],
     "ck_convrot_w4a4_linear_unpacked": [_P, _I, _P, _P, _P, _I, _P] + [_I] * 5 + [_P, ctypes.c_size_t, _P],
+    "ck_mx4_scales_size": [_I, _I],
+    "ck_mx4_quant": [_P, _I, _L, _P, _P, _I, _I, _I, _P],
+    "ck_mx4_dequant": [_P, _P, _P, _I, _I, _I, _I, _P],
+    "ck_mx4_linear_workspace_size": [_I, _I],
+    "ck_mx4_linear": [_P, _I, _L, _P, _P, _P, _I, _P] + [_I] * 5 + [_P, ctypes.c_size_t, _P],
+    "ck_mx4_cache_append": [_P, _P, _L] + [_I] * 4 + [_P, _P, _I] + [_L] * 4 + [_P, _I, _P],
+    "ck_mx4_cache_read": [_P, _P, _L] + [_I] * 4 + [_P, _I, _P, _P, _I, _P],
+    "ck_mx4_attention_workspace_size": [_I] * 5 + [_L],
+    "ck_mx4_attention": [_P, _I, _L, _L, _L, _P, _P, _L, _I, _P, _L, _I, _P, _P] + [_I] * 6
+                        + [ctypes.c_float, _P, ctypes.c_size_t, _P],
     "ck_convrot_device_status": [_P, ctypes.POINTER(ctypes.c_int)],
     "ck_convrot_selftest_wait_timeout": [ctypes.c_longlong, _P],
     "ck_convrot_last_error": [],
@@ -72,9 +83,8 @@ def _load():
             for name, argtypes in _SIGNATURES.items():
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes
-                fn.restype = {"ck_convrot_last_error": ctypes.c_char_p,
-                              "ck_convrot_w4a4_linear_workspace_size": ctypes.c_size_t,
-                              "ck_convrot_w4a4_linear_unpacked_workspace_size": ctypes.c_size_t}.get(name, ctypes.c_int)
+                fn.restype = (ctypes.c_char_p if name == "ck_convrot_last_error" else
+                              ctypes.c_size_t if name.endswith("_size") else ctypes.c_int)
             _lib = lib
     return _lib
 

@@ -36,7 +36,9 @@
 #include <mutex>
 
 #include "sm100_ptx.cuh"
+#include "hadamard.cuh"
 #include "linear_api.cuh"
+#include "host_launch.cuh"
 
 #define CONVROT_API extern "C" __attribute__((visibility("default")))
 
@@ -86,16 +88,6 @@ template <> struct Act<float> {
     __device__ static float floor_value() { return 1e-10f; }
 };
 
-// Regular Hadamard H4 = J - 2R (ones, minus twice the anti-diagonal):
-// out_i = (v0+v1)+(v2+v3) - 2*v_(3-i), each output rounded once.
-__device__ __forceinline__ void h4(float& v0, float& v1, float& v2, float& v3) {
-    const float s = __fadd_rn(__fadd_rn(v0, v1), __fadd_rn(v2, v3));
-    const float o0 = __fmaf_rn(-2.0f, v3, s);
-    const float o1 = __fmaf_rn(-2.0f, v2, s);
-    const float o2 = __fmaf_rn(-2.0f, v1, s);
-    const float o3 = __fmaf_rn(-2.0f, v0, s);
-    v0 = o0; v1 = o1; v2 = o2; v3 = o3;
-}
 
 // H16 = H4 (x) H4 on v[16] indexed 4*hi + lo: first along lo, then along hi.
 __device__ __forceinline__ void h16(float (&v)[16]) {
@@ -1211,25 +1203,6 @@ int sm_count() {
 }
 
 
-// Launch with programmatic stream serialization: the kernel may start its
-// prologue while the previous kernel in the stream drains; every kernel of this
-// library calls griddep_wait() before touching memory another kernel wrote.
-template <typename... Params, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                       Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
-}
-
 int fail(const char* msg) {
     snprintf(g_last_error, sizeof(g_last_error), "%s", msg);
     return -1;
@@ -1262,11 +1235,6 @@ bool make_packed_tmap(CUtensorMap* map, const void* base, int rows, int K, int b
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
-}
-
-template <typename KernelT>
-cudaError_t ensure_smem(KernelT kernel, int bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 // bf16 output [M, N] for TMA stores of 128-row x 64-column boxes (128 B swizzle).
@@ -2118,11 +2086,14 @@ CONVROT_API int ck_convrot_device_status(void* stream, int* status) {
     cudaError_t e = cudaMemcpyFromSymbolAsync(&host, g_device_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     if (e != cudaSuccess) return static_cast<int>(e);
-    *status = host;
     const int zero = 0;
     e = cudaMemcpyToSymbolAsync(g_device_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    return static_cast<int>(e);
+    int mx4 = 0;                                       // the MX4 kernels' own word (mx4.cu)
+    if (e == cudaSuccess) e = mx4_take_status(s, &mx4);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    *status = host != 0 ? host : mx4;
+    return 0;
 }
 
 // ---------------------------------------------------------------------------

@@ -34,6 +34,9 @@ struct PeerOut {
     int col0;
 };
 
+// Reads and clears the status word of the MX4 kernels (mx4.cu); synchronises `stream`.
+cudaError_t mx4_take_status(cudaStream_t stream, int* status);
+
 // Records `msg` for ck_convrot_last_error() and returns -1.
 int fail(const char* msg);
 

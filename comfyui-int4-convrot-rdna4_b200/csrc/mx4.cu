@@ -1,0 +1,233 @@
+// C entries of the MX4 (microscaled 4-bit float) operators: quantization of
+// rows, the linear on MX4 weights, the paged key/value cache and attention over
+// it. Conventions of include/convrot_b200.h: device pointers, caller-allocated
+// outputs, nothing synchronises; 0, -1 with a message, or a CUDA error.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+
+#include "sm100_ptx.cuh"
+#include "linear_api.cuh"
+#include "host_launch.cuh"
+#include "mx4_common.cuh"
+
+#define CONVROT_API extern "C" __attribute__((visibility("default")))
+
+namespace convrot {
+
+// Status word of this translation unit's kernels (a bounded wait that gave up);
+// ck_convrot_device_status reads and clears it.
+static __device__ int g_mx4_status;
+
+enum : int { kMx4TimeoutProducer = 1, kMx4TimeoutMma = 2, kMx4TimeoutEpilogue = 4 };
+
+__device__ __forceinline__ void mx4_record_status(int code) { atomicCAS(&g_mx4_status, 0, code); }
+
+cudaError_t mx4_take_status(cudaStream_t stream, int* status) {
+    cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_mx4_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    const int zero = 0;
+    if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_mx4_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    return e;
+}
+
+}  // namespace convrot
+
+#include "mx4_quant.cuh"
+#include "mx4_gemm.cuh"
+#include "mx4_cache.cuh"
+#include "mx4_attn.cuh"
+
+namespace convrot {
+
+static size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+static size_t scales_bytes(int rows, int K) {
+    return static_cast<size_t>((rows + 127) / 128) * ((K + 127) / 128) * kMx4TileBytes;
+}
+
+static int check_group(int K, int G) {
+    if (G != 0 && G != 16 && G != 64 && G != 256) return fail("G must be 0, 16, 64 or 256");
+    if (K <= 0 || K % kMx4Block) return fail("K must be a positive multiple of 32");
+    if (G != 0 && K % G) return fail("K must be a multiple of G");
+    return 0;
+}
+
+// Calls f with a null pointer of the C type of dtype code 0 f32, 1 bf16, 2 f16.
+template <typename F>
+static int with_type(int code, F f) {
+    if (code == 0) return f(static_cast<float*>(nullptr));
+    if (code == 1) return f(static_cast<__nv_bfloat16*>(nullptr));
+    return f(static_cast<__half*>(nullptr));
+}
+
+static size_t type_size(int code) { return code == 0 ? 4 : 2; }
+
+static bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+static int check_matrix(const void* x, int dtype, const void* codes, const void* scales, int M, int K, int G) {
+    if (M < 0) return fail("M must not be negative");
+    if (dtype < 0 || dtype > 2) return fail("dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    if (int rc = check_group(K, G)) return rc;
+    if (M == 0) return 0;
+    if (!x || !codes || !scales) return fail("null pointer");
+    if (!aligned_to(x, type_size(dtype))) return fail("values are not aligned to their type");
+    if (!aligned16(codes) || !aligned16(scales)) return fail("codes and scales must be 16-byte aligned");
+    if (static_cast<long long>(M) * ((K + kMx4QuantCols - 1) / kMx4QuantCols) > 0x7FFFFFFFll) return fail("matrix too large");
+    return 0;
+}
+
+static int run_quant(const void* x, int dtype, long long ldx, void* codes, void* scales, int M, int K, int G, cudaStream_t st) {
+    const int grid = M * ((K + kMx4QuantCols - 1) / kMx4QuantCols);
+    return with_type(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return static_cast<int>(launch_pdl(mx4_quant_kernel<T>, dim3(grid), dim3(kMx4QuantThreads), 0, st,
+                                           static_cast<const T*>(x), ldx, static_cast<uint8_t*>(codes),
+                                           static_cast<uint8_t*>(scales), M, K, G));
+    });
+}
+
+}  // namespace convrot
+
+using namespace convrot;
+
+CONVROT_API size_t ck_mx4_scales_size(int rows, int K) {
+    if (rows <= 0 || K <= 0) return 0;
+    return scales_bytes(rows, K);
+}
+
+CONVROT_API int ck_mx4_quant(const void* x, int in_dtype, long long ldx, void* codes, void* scales, int M, int K, int G,
+                             void* stream) {
+    if (int rc = check_matrix(x, in_dtype, codes, scales, M, K, G)) return rc;
+    if (M == 0) return 0;
+    if (ldx < 0 || (M > 1 && ldx < K)) return fail("ldx must be at least K");
+    return run_quant(x, in_dtype, ldx, codes, scales, M, K, G, static_cast<cudaStream_t>(stream));
+}
+
+CONVROT_API int ck_mx4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G,
+                               void* stream) {
+    if (int rc = check_matrix(out, out_dtype, codes, scales, M, K, G)) return rc;
+    if (M == 0) return 0;
+    const int grid = M * ((K + kMx4QuantCols - 1) / kMx4QuantCols);
+    return with_type(out_dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return static_cast<int>(launch_pdl(mx4_dequant_kernel<T>, dim3(grid), dim3(kMx4QuantThreads), 0,
+                                           static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes),
+                                           static_cast<const uint8_t*>(scales), static_cast<T*>(out), K, G));
+    });
+}
+
+CONVROT_API size_t ck_mx4_linear_workspace_size(int M, int K) {
+    if (M <= 0 || K <= 0) return 0;
+    return align256(static_cast<size_t>(M) * K / 2) + align256(scales_bytes(M, K));
+}
+
+CONVROT_API int ck_mx4_linear(const void* x, int in_dtype, long long ldx, const void* Wcodes, const void* Wscales,
+                              const void* bias, int bias_dtype, void* out, int out_dtype, int M, int N, int K, int G,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+    if (N < 0) return fail("N must not be negative");
+    if (N == 0) return 0;
+    if (int rc = check_matrix(x, in_dtype, Wcodes, Wscales, M, K, G)) return rc;
+    if (M == 0) return 0;
+    if (ldx < 0 || (M > 1 && ldx < K)) return fail("ldx must be at least K");
+    if (out_dtype < 0 || out_dtype > 2) return fail("out_dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    if (bias && (bias_dtype < 0 || bias_dtype > 2)) return fail("bias_dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    if (!out || !aligned16(out)) return fail("out must be 16-byte aligned");
+    if (!workspace || !aligned_to(workspace, 256)) return fail("the workspace must be 256-byte aligned");
+    if (workspace_bytes < ck_mx4_linear_workspace_size(M, K)) return fail("workspace smaller than ck_mx4_linear_workspace_size");
+    uint8_t* xc = static_cast<uint8_t*>(workspace);
+    uint8_t* xs = xc + align256(static_cast<size_t>(M) * K / 2);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (int rc = run_quant(x, in_dtype, ldx, xc, xs, M, K, G, st)) return rc;
+    return with_type(out_dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return static_cast<int>(launch_pdl(mx4_gemm_kernel<T>, dim3((N + 31) / 32, (M + 7) / 8), dim3(256), 0, st, xc, xs,
+                                           static_cast<const uint8_t*>(Wcodes), static_cast<const uint8_t*>(Wscales),
+                                           BiasRef{bias, bias_dtype}, static_cast<T*>(out), M, N, K));
+    });
+}
+
+static int check_cache(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G) {
+    if (d != 64 && d != 128 && d != 256) return fail("the head dimension must be 64, 128 or 256");
+    if (int rc = check_group(d, G)) return rc;
+    if (heads <= 0 || page <= 0 || pages < 0) return fail("heads and page must be positive, pages not negative");
+    if (page & (page - 1) || page > 65536) return fail("the page size must be a power of two up to 65536");
+    if (pages > 0x7FFFFFFFll) return fail("too many pages");
+    if (pages && (!codes || !scales)) return fail("null cache pointer");
+    if (!aligned16(codes) || !aligned16(scales)) return fail("the cache must be 16-byte aligned");
+    return 0;
+}
+
+CONVROT_API int ck_mx4_cache_append(void* codes, void* scales, long long pages, int heads, int d, int page, int G,
+                                    const void* k, const void* v, int in_dtype, long long k_token, long long k_head,
+                                    long long v_token, long long v_head, const void* slots, int T, void* stream) {
+    if (int rc = check_cache(codes, scales, pages, heads, d, page, G)) return rc;
+    if (T < 0) return fail("T must not be negative");
+    if (in_dtype < 0 || in_dtype > 2) return fail("dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    if (T == 0) return 0;
+    if (!k || !v || !slots) return fail("null pointer");
+    if (!aligned_to(k, type_size(in_dtype)) || !aligned_to(v, type_size(in_dtype)) || !aligned_to(slots, 8))
+        return fail("keys, values or slots are not aligned to their type");
+    const Mx4CacheShape c{pages * page, heads, d, page, G};
+    return with_type(in_dtype, [&](auto* t) {
+        using E = std::remove_pointer_t<decltype(t)>;
+        return static_cast<int>(launch_pdl(mx4_cache_append_kernel<E>, dim3(T, 2), dim3(256), 0,
+                                           static_cast<cudaStream_t>(stream), static_cast<uint8_t*>(codes),
+                                           static_cast<uint8_t*>(scales), static_cast<const E*>(k), static_cast<const E*>(v),
+                                           k_token, k_head, v_token, v_head, static_cast<const long long*>(slots), c));
+    });
+}
+
+CONVROT_API int ck_mx4_cache_read(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G,
+                                  const void* slots, int T, void* k, void* v, int out_dtype, void* stream) {
+    if (int rc = check_cache(codes, scales, pages, heads, d, page, G)) return rc;
+    if (T < 0) return fail("T must not be negative");
+    if (out_dtype < 0 || out_dtype > 2) return fail("dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    if (T == 0) return 0;
+    if (!k || !v || !slots) return fail("null pointer");
+    if (!aligned16(k) || !aligned16(v) || !aligned_to(slots, 8)) return fail("outputs must be 16-byte, slots 8-byte aligned");
+    const Mx4CacheShape c{pages * page, heads, d, page, G};
+    return with_type(out_dtype, [&](auto* t) {
+        using E = std::remove_pointer_t<decltype(t)>;
+        return static_cast<int>(launch_pdl(mx4_cache_read_kernel<E>, dim3(T, 2), dim3(256), 0,
+                                           static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes),
+                                           static_cast<const uint8_t*>(scales), static_cast<const long long*>(slots),
+                                           static_cast<E*>(k), static_cast<E*>(v), c));
+    });
+}
+
+CONVROT_API size_t ck_mx4_attention_workspace_size(int B, int tq, int hq, int hkv, int d, long long longest) {
+    (void)B; (void)tq; (void)hq; (void)hkv; (void)d; (void)longest;
+    return 0;
+}
+
+CONVROT_API int ck_mx4_attention(const void* q, int dtype, long long q_seq, long long q_token, long long q_head,
+                                 const void* codes, const void* scales, long long pages, int page, const void* table,
+                                 long long table_ld, int table_pages, const void* lens, void* out, int B, int tq, int hq,
+                                 int hkv, int d, int G, float softmax_scale, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+    if (int rc = check_cache(codes, scales, pages, hkv, d, page, G)) return rc;
+    if (dtype != 1 && dtype != 2) return fail("queries must be bf16 (1) or f16 (2)");
+    if (B < 0 || tq <= 0 || hq <= 0 || hq % hkv) return fail("query heads must be a positive multiple of the cache's heads");
+    if (table_pages < 0 || table_ld < table_pages) return fail("bad block table shape");
+    if (static_cast<long long>(table_pages) * page > 0x7FFFFFFFll) return fail("block table longer than 2^31 tokens");
+    if (B == 0) return 0;
+    if (static_cast<long long>(B) * tq * hq > 0x7FFFFFFFll) return fail("too many query rows");
+    if (!q || !lens || !out || (table_pages && !table)) return fail("null pointer");
+    if (!aligned_to(q, 2) || !aligned_to(table, 4) || !aligned_to(lens, 4) || !aligned16(out))
+        return fail("queries, table or lengths not aligned to their type, or out not to 16 bytes");
+    (void)workspace; (void)workspace_bytes;
+    Mx4AttnArgs a{q, q_seq, q_token, q_head, static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
+                  static_cast<const int*>(table), table_ld, table_pages, static_cast<const int*>(lens), out, B, tq, hq, hkv,
+                  d, page, static_cast<int>(pages), G, softmax_scale};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == 1) return static_cast<int>(launch_pdl(mx4_attn_kernel<__nv_bfloat16>, dim3(B * tq * hq), dim3(256), 0, st, a));
+    return static_cast<int>(launch_pdl(mx4_attn_kernel<__half>, dim3(B * tq * hq), dim3(256), 0, st, a));
+}

@@ -296,6 +296,81 @@ int ck_convrot_w4a4_linear_unpacked(const void* x, int in_dtype, const void* Wco
                                     int M, int N, int K, int G, void* workspace, size_t workspace_bytes,
                                     void* stream);
 
+/* ---------------------------------------------------------------------------
+ * MX4: microscaled 4-bit floats (OCP MXFP4) with the ConvRot rotation. No
+ * reference counterpart (the reference's 4-bit format is int4).
+ *
+ * Values e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6; sign in bit 3) in blocks of 32 along
+ * a row, one scale byte E8M0 a block (E stands for 2^(E - 127), 255 for NaN): a
+ * block of amplitude a gets E = max(floor(log2 a) - 2 + 127, 0), codes are
+ * rounded to nearest even and saturate at 6; a block holding an infinity or a
+ * NaN gets 255. Two codes a byte, the even column in the low nibble. Scales of a
+ * matrix [R, K] lie in tiles [ceil(R/128), ceil(K/128), 512]: row r and block b
+ * at byte (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 of tile (r / 128, b / 4).
+ *
+ * dtype codes 0 = f32, 1 = bf16, 2 = f16. G in {0 (not rotated), 16, 64, 256},
+ * K a multiple of 32 and of G. The rotation runs in fp32 in the radix-4 steps of
+ * the int4 quantizers, without an intermediate rounding; it is its own inverse.
+ * -------------------------------------------------------------------------- */
+
+/* Bytes of the scale tiles of a [rows, K] matrix. */
+size_t ck_mx4_scales_size(int rows, int K);
+
+/* x [M, K], row stride ldx elements (>= K) -> codes [M, K/2] and scale tiles
+ * (both 16-byte aligned; every byte of the tiles is written). */
+int ck_mx4_quant(const void* x, int in_dtype, long long ldx, void* codes, void* scales, int M, int K, int G,
+                 void* stream);
+
+/* The values codes and scales stand for -> out [M, K] (16-byte aligned), rotated
+ * back with G != 0; one rounding. */
+int ck_mx4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G, void* stream);
+
+/* Workspace of ck_mx4_linear: the row codes and their scale tiles. */
+size_t ck_mx4_linear_workspace_size(int M, int K);
+
+/* out[m, n] = sum_k x[m, k] W[n, k] + bias[n]: x [M, K] (row stride ldx) is
+ * rotated and quantized into the workspace (256-byte aligned), the weight is
+ * given as codes [N, K/2] and scale tiles from ck_mx4_quant with the same G.
+ * fp32 accumulation, one rounding. bias [N] or NULL in bias_dtype; out [M, N]
+ * 16-byte aligned. Two calls in flight at once need two workspaces. */
+int ck_mx4_linear(const void* x, int in_dtype, long long ldx, const void* Wcodes, const void* Wscales,
+                  const void* bias, int bias_dtype, void* out, int out_dtype, int M, int N, int K, int G,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* Paged key/value cache: codes [pages, 2, heads, page, d/2], scales [pages, 2,
+ * heads, page, d/32] (16-byte aligned), keys at index 0, values at 1, both rotated
+ * along d. d in {64, 128, 256}; page a power of two; slot s (int64) is token
+ * s % page of page s / page.
+ *
+ * append: k, v [T, heads, d] with strides in elements (token, head; d
+ * contiguous) are rotated, quantized and written to their slots; a slot outside
+ * the cache is skipped. Slots of one call must differ. */
+int ck_mx4_cache_append(void* codes, void* scales, long long pages, int heads, int d, int page, int G,
+                        const void* k, const void* v, int in_dtype, long long k_token, long long k_head,
+                        long long v_token, long long v_head, const void* slots, int T, void* stream);
+
+/* read: the slots' keys and values, rotated back, -> k, v [T, heads, d] (16-byte
+ * aligned); a slot outside the cache reads as zeros. */
+int ck_mx4_cache_read(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G,
+                      const void* slots, int T, void* k, void* v, int out_dtype, void* stream);
+
+/* Workspace of ck_mx4_attention for `longest` = table_pages * page (0: none needed). */
+size_t ck_mx4_attention_workspace_size(int B, int tq, int hq, int hkv, int d, long long longest);
+
+/* Causal attention of the newest tq tokens of B sequences over the cache.
+ *   q [B, tq, hq, d] (dtype 1 or 2; strides in elements, d contiguous), hq a
+ *   multiple of hkv (query head h reads cache head h / (hq / hkv));
+ *   table int32 [B, table_pages] (row stride table_ld): token j of sequence b is
+ *   token j % page of page table[b][j / page]; a page outside [0, pages) hides
+ *   its tokens; lens int32 [B] tokens in the cache (cut at table_pages * page);
+ *   query t sees tokens up to position lens[b] - tq + t; one that sees none
+ *   gives zeros; out [B, tq, hq, d] (16-byte aligned) in dtype. */
+int ck_mx4_attention(const void* q, int dtype, long long q_seq, long long q_token, long long q_head,
+                     const void* codes, const void* scales, long long pages, int page, const void* table,
+                     long long table_ld, int table_pages, const void* lens, void* out, int B, int tq, int hq,
+                     int hkv, int d, int G, float softmax_scale, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 /* Reads and clears the device status word that kernels set when a bounded
  * wait gives up (0 = ok). Synchronises `stream`. No reference counterpart:
  * the reference has no device-side timeouts. */
