@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "sm100_ptx.cuh"
 #include "linear_api.cuh"
@@ -94,6 +95,78 @@ static int run_quant(const void* x, int dtype, long long ldx, void* codes, void*
     });
 }
 
+// 2D tensor map of `rows` rows of `cols` elements at a pitch in bytes.
+static bool make_tmap(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, long long cols,
+                      long long pitch, int box_rows, int box_cols, CUtensorMapSwizzle swizzle) {
+    auto enc = get_encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[2] = {1, 1};
+    return enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Codes [rows, K/2] in boxes of 256 values x box_rows; scale tiles as rows of
+// 32-bit words in boxes of two K tiles x box_tiles.
+static bool make_mx4_tmaps(CUtensorMap* codes_map, CUtensorMap* scales_map, const void* codes, const void* scales, int rows,
+                           int K, int box_rows, int box_tiles) {
+    const long long kt = (K + 127) / 128, rt = (rows + 127) / 128;
+    return make_tmap(codes_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, rows, K / 2, K / 2, box_rows, kMx4StageK / 2,
+                     CU_TENSOR_MAP_SWIZZLE_128B) &&
+           make_tmap(scales_map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, rt, kt * 128, kt * kMx4TileBytes, box_tiles, 256,
+                     CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <int BN, typename T>
+static int launch_gemm_pair(const void* xc, const void* xs, const void* wc, const void* ws, BiasRef bias, T* out, int M, int N,
+                            int K, cudaStream_t stream) {
+    using Cfg = Mx4PairCfg<BN>;
+    CUtensorMap tx, tw, txs, tws, to;
+    memset(&to, 0, sizeof(to));
+    if (!make_mx4_tmaps(&tx, &txs, xc, xs, M, K, 128, 1) || !make_mx4_tmaps(&tw, &tws, wc, ws, N, K, BN / 2, BN / 128))
+        return fail("cuTensorMapEncodeTiled failed (operand size out of range or driver entry point missing)");
+    const int staged = (static_cast<size_t>(N) * sizeof(T)) % 16 == 0;
+    if (staged && !make_tmap(&to, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, out, M, N,
+                             static_cast<long long>(N) * sizeof(T), 32, 128 / sizeof(T), CU_TENSOR_MAP_SWIZZLE_128B))
+        return fail("cuTensorMapEncodeTiled failed for the output");
+    auto kernel = mx4_gemm_pair_kernel<BN, T>;
+    cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const int tiles_m = (M + 255) / 256;
+    const long long num_tiles = static_cast<long long>(tiles_m) * ((N + BN - 1) / BN);
+    if (num_tiles > 0x7FFFFFFF) return fail("too many output tiles");
+    const int clusters = static_cast<int>(num_tiles < sm_count() / 2 ? num_tiles : sm_count() / 2);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * clusters, 1, 1);
+    cfg.blockDim = dim3(kMx4PairThreads, 1, 1);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, tx, tw, txs, tws, to, bias, out, M, N, K, tiles_m,
+                                               static_cast<int>(num_tiles), staged));
+}
+
+static int run_gemm(const void* xc, const void* xs, const void* wc, const void* ws, BiasRef bias, void* out, int out_dtype,
+                    int M, int N, int K, cudaStream_t stream) {
+    return with_type(out_dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        // 256-row pairs of weights where their tiles fill the SM pairs
+        const long long tiles256 = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);
+        if (tiles256 * 2 >= sm_count()) return launch_gemm_pair<256>(xc, xs, wc, ws, bias, static_cast<T*>(out), M, N, K, stream);
+        return launch_gemm_pair<128>(xc, xs, wc, ws, bias, static_cast<T*>(out), M, N, K, stream);
+    });
+}
+
 }  // namespace convrot
 
 using namespace convrot;
@@ -146,12 +219,7 @@ CONVROT_API int ck_mx4_linear(const void* x, int in_dtype, long long ldx, const 
     uint8_t* xs = xc + align256(static_cast<size_t>(M) * K / 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (int rc = run_quant(x, in_dtype, ldx, xc, xs, M, K, G, st)) return rc;
-    return with_type(out_dtype, [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        return static_cast<int>(launch_pdl(mx4_gemm_kernel<T>, dim3((N + 31) / 32, (M + 7) / 8), dim3(256), 0, st, xc, xs,
-                                           static_cast<const uint8_t*>(Wcodes), static_cast<const uint8_t*>(Wscales),
-                                           BiasRef{bias, bias_dtype}, static_cast<T*>(out), M, N, K));
-    });
+    return run_gemm(xc, xs, Wcodes, Wscales, BiasRef{bias, bias_dtype}, out, out_dtype, M, N, K, st);
 }
 
 static int check_cache(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G) {

@@ -497,3 +497,53 @@ __device__ __forceinline__ float4 ld_shared_cluster_f4(uint32_t cluster_addr) {
 }
 
 }  // namespace convrot
+
+namespace convrot {
+
+// ---------------------------------------------------------------- block-scaled 4-bit floats
+// Instruction descriptor for kind::mxf4: e2m1 A and B, E8M0 scales, K-major both,
+// fp32 accumulator. `sf` is 0 or 2: which two of the four scale bytes of a TMEM
+// word this K = 64 step takes (the same for A and B).
+__host__ __device__ constexpr uint32_t idesc_mxf4(uint32_t m, uint32_t n, uint32_t sf) {
+    return (sf << 4)             // B scale byte
+         | (1u << 7)             // A: e2m1
+         | (1u << 10)            // B: e2m1
+         | ((n >> 3) << 17)      // N / 8
+         | (1u << 23)            // scales: E8M0
+         | ((m >> 4) << 24)      // M / 16
+         | (sf << 29);           // A scale byte
+}
+
+// D[tmem] (+)= (A * 2^sa) . (B * 2^sb)^T, packed e2m1 operands from shared memory,
+// one scale per 32 values from tensor memory (K = 64: two scales a row).
+template <bool PAIR>
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+            : "memory");
+}
+
+// 32 rows of 16 bytes from shared memory (descriptor without swizzle, 128 bytes
+// between groups of 8 rows) into 4 TMEM columns of every warp's 32 lanes: one
+// scale tile. Runs in order with the MMAs this thread issues. PAIR: in both CTAs.
+template <bool PAIR>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(taddr), "l"(desc) : "memory");
+}
+
+}  // namespace convrot
