@@ -41,12 +41,17 @@ cudaError_t mx4_take_status(cudaStream_t stream, int* status) {
 
 }  // namespace convrot
 
+#include "mx4_unit.cuh"
 #include "mx4_quant.cuh"
 #include "mx4_gemm.cuh"
 #include "mx4_cache.cuh"
 #include "mx4_attn.cuh"
 
 namespace convrot {
+
+// Units (128 values each) of one call: their numbers, and one grid's step beyond,
+// fit 32 bits.
+constexpr long long kMx4MostUnits = 0x7FFFFFFFll - (1 << 20);
 
 static size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
@@ -81,17 +86,39 @@ static int check_matrix(const void* x, int dtype, const void* codes, const void*
     if (!x || !codes || !scales) return fail("null pointer");
     if (!aligned_to(x, type_size(dtype))) return fail("values are not aligned to their type");
     if (!aligned16(codes) || !aligned16(scales)) return fail("codes and scales must be 16-byte aligned");
-    if (static_cast<long long>(M) * ((K + kMx4QuantCols - 1) / kMx4QuantCols) > 0x7FFFFFFFll) return fail("matrix too large");
+    if (static_cast<long long>(M + 127LL) / 128 * 128 * ((K + 127) / 128) > kMx4MostUnits) return fail("matrix too large");
     return 0;
 }
 
+// Calls f with an integral constant for the rotation group.
+template <typename F>
+static int with_group(int G, F f) {
+    if (G == 16) return f(std::integral_constant<int, 16>{});
+    if (G == 64) return f(std::integral_constant<int, 64>{});
+    if (G == 256) return f(std::integral_constant<int, 256>{});
+    return f(std::integral_constant<int, 0>{});
+}
+
+// Blocks of the unit kernels: one wave of three a multiprocessor, a warp's 32
+// units at a time.
+static int unit_blocks(long long units) {
+    const long long want = (units + kMx4QuantWarps * 32 - 1) / (kMx4QuantWarps * 32), most = 3LL * sm_count();
+    return static_cast<int>(want < most ? want : most);
+}
+
 static int run_quant(const void* x, int dtype, long long ldx, void* codes, void* scales, int M, int K, int G, cudaStream_t st) {
-    const int grid = M * ((K + kMx4QuantCols - 1) / kMx4QuantCols);
+    const long long units = static_cast<long long>((M + 127) / 128 * 128) * ((K + 127) / 128);
     return with_type(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return static_cast<int>(launch_pdl(mx4_quant_kernel<T>, dim3(grid), dim3(kMx4QuantThreads), 0, st,
-                                           static_cast<const T*>(x), ldx, static_cast<uint8_t*>(codes),
-                                           static_cast<uint8_t*>(scales), M, K, G));
+        return with_group(G, [&](auto g) {
+            auto kernel = mx4_quant_kernel<T, decltype(g)::value>;
+            cudaError_t e = ensure_smem(kernel, mx4_quant_smem<T>());
+            if (e != cudaSuccess) return static_cast<int>(e);
+            const bool vec = aligned16(x) && ldx * sizeof(T) % 16 == 0;
+            return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<T>(), st,
+                                               static_cast<const T*>(x), ldx, static_cast<uint8_t*>(codes),
+                                               static_cast<uint8_t*>(scales), M, K, static_cast<int>(units), vec));
+        });
     });
 }
 
@@ -188,12 +215,17 @@ CONVROT_API int ck_mx4_dequant(const void* codes, const void* scales, void* out,
                                void* stream) {
     if (int rc = check_matrix(out, out_dtype, codes, scales, M, K, G)) return rc;
     if (M == 0) return 0;
-    const int grid = M * ((K + kMx4QuantCols - 1) / kMx4QuantCols);
+    const long long units = static_cast<long long>(M) * ((K + 127) / 128);
     return with_type(out_dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return static_cast<int>(launch_pdl(mx4_dequant_kernel<T>, dim3(grid), dim3(kMx4QuantThreads), 0,
-                                           static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes),
-                                           static_cast<const uint8_t*>(scales), static_cast<T*>(out), K, G));
+        return with_group(G, [&](auto g) {
+            auto kernel = mx4_dequant_kernel<T, decltype(g)::value>;
+            cudaError_t e = ensure_smem(kernel, mx4_quant_smem<T>() / 2);
+            if (e != cudaSuccess) return static_cast<int>(e);
+            return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<T>() / 2,
+                                               static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes),
+                                               static_cast<const uint8_t*>(scales), static_cast<T*>(out), K, static_cast<int>(units)));
+        });
     });
 }
 
@@ -222,6 +254,23 @@ CONVROT_API int ck_mx4_linear(const void* x, int in_dtype, long long ldx, const 
     return run_gemm(xc, xs, Wcodes, Wscales, BiasRef{bias, bias_dtype}, out, out_dtype, M, N, K, st);
 }
 
+// Calls f with integral constants for the head dimension and the rotation group.
+template <typename F>
+static int with_head(int d, int G, F f) {
+    return with_group(G, [&](auto g) {
+        constexpr int g0 = decltype(g)::value;
+        if (d == 64) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, g0 == 256 ? 0 : g0>{});
+        if (d == 128) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, g0 == 256 ? 0 : g0>{});
+        return f(std::integral_constant<int, 256>{}, g);
+    });
+}
+
+static int page_bits(int page) {
+    int b = 0;
+    while ((1 << b) < page) ++b;
+    return b;
+}
+
 static int check_cache(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G) {
     if (d != 64 && d != 128 && d != 256) return fail("the head dimension must be 64, 128 or 256");
     if (int rc = check_group(d, G)) return rc;
@@ -243,13 +292,22 @@ CONVROT_API int ck_mx4_cache_append(void* codes, void* scales, long long pages, 
     if (!k || !v || !slots) return fail("null pointer");
     if (!aligned_to(k, type_size(in_dtype)) || !aligned_to(v, type_size(in_dtype)) || !aligned_to(slots, 8))
         return fail("keys, values or slots are not aligned to their type");
-    const Mx4CacheShape c{pages * page, heads, d, page, G};
+    const Mx4CacheShape c{pages * page, heads, d, page_bits(page)};
     return with_type(in_dtype, [&](auto* t) {
         using E = std::remove_pointer_t<decltype(t)>;
-        return static_cast<int>(launch_pdl(mx4_cache_append_kernel<E>, dim3(T, 2), dim3(256), 0,
-                                           static_cast<cudaStream_t>(stream), static_cast<uint8_t*>(codes),
-                                           static_cast<uint8_t*>(scales), static_cast<const E*>(k), static_cast<const E*>(v),
-                                           k_token, k_head, v_token, v_head, static_cast<const long long*>(slots), c));
+        return with_head(d, G, [&](auto dim, auto g) {
+            auto kernel = mx4_cache_append_kernel<E, decltype(dim)::value, decltype(g)::value>;
+            cudaError_t e = ensure_smem(kernel, mx4_quant_smem<E>());
+            if (e != cudaSuccess) return static_cast<int>(e);
+            const long long units = static_cast<long long>(T) * 2 * mx4_cache_units<decltype(dim)::value>(heads);
+            if (units > kMx4MostUnits) return fail("too many tokens in one call");
+            const long long strides = k_token | k_head | v_token | v_head;
+            const bool vec = aligned16(k) && aligned16(v) && strides * static_cast<long long>(sizeof(E)) % 16 == 0;
+            return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<E>(),
+                                               static_cast<cudaStream_t>(stream), static_cast<uint8_t*>(codes),
+                                               static_cast<uint8_t*>(scales), static_cast<const E*>(k), static_cast<const E*>(v),
+                                               k_token, k_head, v_token, v_head, static_cast<const long long*>(slots), static_cast<int>(units), c, vec));
+        });
     });
 }
 
@@ -261,13 +319,20 @@ CONVROT_API int ck_mx4_cache_read(const void* codes, const void* scales, long lo
     if (T == 0) return 0;
     if (!k || !v || !slots) return fail("null pointer");
     if (!aligned16(k) || !aligned16(v) || !aligned_to(slots, 8)) return fail("outputs must be 16-byte, slots 8-byte aligned");
-    const Mx4CacheShape c{pages * page, heads, d, page, G};
+    const Mx4CacheShape c{pages * page, heads, d, page_bits(page)};
     return with_type(out_dtype, [&](auto* t) {
         using E = std::remove_pointer_t<decltype(t)>;
-        return static_cast<int>(launch_pdl(mx4_cache_read_kernel<E>, dim3(T, 2), dim3(256), 0,
-                                           static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes),
-                                           static_cast<const uint8_t*>(scales), static_cast<const long long*>(slots),
-                                           static_cast<E*>(k), static_cast<E*>(v), c));
+        return with_head(d, G, [&](auto dim, auto g) {
+            auto kernel = mx4_cache_read_kernel<E, decltype(dim)::value, decltype(g)::value>;
+            cudaError_t e = ensure_smem(kernel, mx4_quant_smem<E>() / 2);
+            if (e != cudaSuccess) return static_cast<int>(e);
+            const long long units = static_cast<long long>(T) * 2 * mx4_cache_units<decltype(dim)::value>(heads);
+            if (units > kMx4MostUnits) return fail("too many tokens in one call");
+            return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<E>() / 2,
+                                               static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes),
+                                               static_cast<const uint8_t*>(scales), static_cast<const long long*>(slots),
+                                               static_cast<E*>(k), static_cast<E*>(v), static_cast<int>(units), c));
+        });
     });
 }
 

@@ -1,71 +1,95 @@
 // MX4 quantization of matrix rows (with the ConvRot rotation) and back.
 //
-// Included by mx4.cu. One block takes 1024 columns of one row: the values go
-// to shared memory in fp32, the radix-4 steps of the rotation run there, then
-// each warp quantizes blocks of 32, a lane a value.
+// Included by mx4.cu. A unit (mx4_unit.cuh) is 128 columns of one row, and the
+// units of the matrix are numbered row after row; a warp takes 32 of them at a
+// time, copying the next 32 while it works on these. Missing columns of a row's
+// last unit read as zeros, which leaves their scale bytes 0.
 #pragma once
 
 namespace convrot {
 
-constexpr int kMx4QuantCols = 1024;           // columns of a block's piece of a row (holds whole groups)
-constexpr int kMx4QuantThreads = 256;
+constexpr int kMx4QuantWarps = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(kMx4QuantThreads)
+template <typename T> constexpr int mx4_quant_smem() { return kMx4QuantWarps * 2 * Mx4Slab<T>::kBytes; }
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kMx4QuantWarps * 32, 3)
 mx4_quant_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                 int M, int K, int group) {
-    __shared__ float v[kMx4QuantCols];
-    const int pieces = (K + kMx4QuantCols - 1) / kMx4QuantCols;
-    const int row = blockIdx.x / pieces, k0 = (blockIdx.x % pieces) * kMx4QuantCols;
-    const int n = min(kMx4QuantCols, K - k0);
+                 int M, int K, int units, bool vec) {
+    using S = Mx4Slab<T>;
+    extern __shared__ __align__(128) unsigned char mx4slabs[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned char* slab = mx4slabs + warp * 2 * S::kBytes;
     const int kt = (K + 127) / 128;
+    const int step = static_cast<int>(gridDim.x) * kMx4QuantWarps * 32;
+    int base = (static_cast<int>(blockIdx.x) * kMx4QuantWarps + warp) * 32;
+    auto place = [&](int u) {
+        const int row = u / kt, c = u - row * kt;
+        const bool held = u < units && row < M;
+        return Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(held ? x + row * ldx + c * kMx4Unit : x),
+                            held ? min(S::kChunks, (K - c * kMx4Unit) / S::kPer) : 0};
+    };
     griddep_wait();
     griddep_launch_dependents();
-    const T* src = x + row * ldx + k0;
-    for (int i = threadIdx.x; i < n; i += kMx4QuantThreads) v[i] = mx4_to_f32(src[i]);
-    __syncthreads();
-    mx4_rotate_shared(v, n, group, threadIdx.x, kMx4QuantThreads);
-    const int lane = threadIdx.x & 31;
-    const int blocks = n / kMx4Block;
-    for (int b = threadIdx.x >> 5; b < blocks; b += kMx4QuantThreads / 32) {
-        const float a = v[b * 32 + lane];
-        uint32_t amax = __float_as_uint(a) & 0x7FFFFFFFu;      // as integers: NaN above inf above every number
-        amax = __reduce_max_sync(0xFFFFFFFFu, amax);
-        const uint32_t e = mx4_scale_byte(__uint_as_float(amax));
-        const float y = a * mx4_inv_scale(e);
-        const float hi = __shfl_down_sync(0xFFFFFFFFu, y, 1);
-        const size_t at = static_cast<size_t>(row) * K + k0 + b * 32 + lane;
-        if (!(lane & 1)) codes[at >> 1] = e == 255u ? 0 : static_cast<uint8_t>(mx4_encode2(y, hi));
-        if (lane == 0) scales[mx4_scale_pos(row, k0 / 32 + b, kt)] = static_cast<uint8_t>(e);
+    if (base < units) slab_load<false>(slab, place(base + lane), 0, vec);
+    cp_async_commit();
+    for (int it = 0; base < units; base += step, ++it) {
+        const unsigned char* cur = slab + (it & 1) * S::kBytes;
+        if (base + step < units) slab_load<false>(slab + ((it + 1) & 1) * S::kBytes, place(base + step + lane), 0, vec);
+        cp_async_commit();
+        cp_async_wait<1>();
+        __syncwarp();
+        float2 v[64];
+        slab_to_unit<T>(cur, v);
+        unit_rotate<G>(v);
+        uint4 q[4];
+        const uint32_t word = unit_quantize(v, unit_factor<G>(), q);
+        const int u = (base + lane) ^ (G == 256 ? 1 : 0);
+        const int row = u / kt, c = u - row * kt;
+        if (u < units) {
+            *reinterpret_cast<uint32_t*>(scales + mx4_scale_pos(row, 4 * c, kt)) = word;
+            if (row < M) {
+                uint4* dst = reinterpret_cast<uint4*>(codes + (static_cast<size_t>(row) * K + c * kMx4Unit) / 2);
+                const int blocks = min(4, (K - c * kMx4Unit) / kMx4Block);
+                #pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (b < blocks) dst[b] = q[b];
+            }
+        }
+        __syncwarp();
     }
-    // the last tile's missing blocks and rows stand for 2^-127 (their codes are never read)
-    const int block_end = k0 + n == K ? kt * 4 : (k0 + n) / 32;
-    if (k0 + n == K && static_cast<int>(threadIdx.x) < kt * 4 - K / 32)
-        scales[mx4_scale_pos(row, K / 32 + threadIdx.x, kt)] = 0;
-    if (row == M - 1)
-        for (int r = M + (threadIdx.x >> 5); r < (M + 127) / 128 * 128; r += kMx4QuantThreads / 32)
-            for (int b = k0 / 32 + lane; b < block_end; b += 32) scales[mx4_scale_pos(r, b, kt)] = 0;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kMx4QuantThreads)
+template <typename T, int G>
+__global__ void __launch_bounds__(kMx4QuantWarps * 32, 3)
 mx4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, int K,
-                   int group) {
-    __shared__ float v[kMx4QuantCols];
-    const int pieces = (K + kMx4QuantCols - 1) / kMx4QuantCols;
-    const int row = blockIdx.x / pieces, k0 = (blockIdx.x % pieces) * kMx4QuantCols;
-    const int n = min(kMx4QuantCols, K - k0);
+                   int units) {
+    using S = Mx4Slab<T>;
+    extern __shared__ __align__(128) unsigned char mx4slabs[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned char* slab = mx4slabs + warp * S::kBytes;
     const int kt = (K + 127) / 128;
+    const int step = static_cast<int>(gridDim.x) * kMx4QuantWarps * 32;
     griddep_wait();
     griddep_launch_dependents();
-    const size_t at = static_cast<size_t>(row) * K + k0;
-    for (int i = threadIdx.x; i < n; i += kMx4QuantThreads) {
-        const uint32_t c = (codes[(at + i) >> 1] >> (4 * (i & 1))) & 15u;
-        v[i] = mx4_code_value(c) * mx4_scale_value(scales[mx4_scale_pos(row, (k0 + i) / 32, kt)]);
+    for (int base = (static_cast<int>(blockIdx.x) * kMx4QuantWarps + warp) * 32; base < units; base += step) {
+        const int u = base + lane;
+        const int row = u / kt, c = u - row * kt;
+        const int blocks = u < units ? min(4, (K - c * kMx4Unit) / kMx4Block) : 0;
+        const uint4* src = reinterpret_cast<const uint4*>(codes + (static_cast<size_t>(row) * K + c * kMx4Unit) / 2);
+        uint4 q[4];
+        #pragma unroll
+        for (int b = 0; b < 4; ++b) q[b] = b < blocks ? src[b] : make_uint4(0, 0, 0, 0);
+        const uint32_t word = blocks ? *reinterpret_cast<const uint32_t*>(scales + mx4_scale_pos(row, 4 * c, kt)) : 0;
+        float2 v[64];
+        unit_decode(q, word, v);
+        unit_rotate<G>(v);
+        unit_to_slab<T>(slab, lane ^ (G == 256 ? 1 : 0), v, unit_factor<G>());
+        __syncwarp();
+        slab_store<T>(slab, Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(out + static_cast<size_t>(row) * K + c * kMx4Unit),
+                                         blocks * (kMx4Block / S::kPer)});
+        __syncwarp();
     }
-    __syncthreads();
-    mx4_rotate_shared(v, n, group, threadIdx.x, kMx4QuantThreads);
-    for (int i = threadIdx.x; i < n; i += kMx4QuantThreads) out[at + i] = mx4_from_f32<T>(v[i]);
 }
 
 }  // namespace convrot
