@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -271,6 +272,47 @@ static int page_bits(int page) {
     return b;
 }
 
+// How an attention call is cut: tiles of query rows (one sequence and cache head
+// each) and splits of the sequences.
+struct AttnPlan {
+    long long tiles;
+    int tile_rows, row_tiles, splits;
+    size_t partials() const { return static_cast<size_t>(tiles) * splits * tile_rows; }
+};
+
+static AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
+    AttnPlan p;
+    const long long rows = static_cast<long long>(tq) * (hq / hkv);
+    p.tile_rows = rows > 16 && d <= 128 ? 32 : 16;
+    p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
+    p.tiles = static_cast<long long>(B) * hkv * p.row_tiles;
+    // splits: enough blocks for two waves of three a multiprocessor, none without
+    // a group of tokens of its own
+    const long long groups = (longest + kMx4AttnGroup - 1) / kMx4AttnGroup;
+    const long long want = (6LL * sm_count() + p.tiles - 1) / (p.tiles > 0 ? p.tiles : 1);
+    p.splits = static_cast<int>(std::max(1LL, std::min({want, groups, 256LL})));
+    return p;
+}
+
+template <typename T, int D, int MT>
+static int launch_attention(const Mx4AttnArgs& a, const AttnPlan& p, cudaStream_t stream) {
+    using Cfg = Mx4AttnCfg<D, MT>;
+    auto kernel = mx4_attn_kernel<T, D, MT>;
+    cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
+    if (e == cudaSuccess)
+        e = launch_pdl(kernel, dim3(static_cast<unsigned>(p.tiles), p.splits), dim3(kMx4AttnWarps * 32), Cfg::kSmemBytes, stream, a);
+    if (e == cudaSuccess && p.splits > 1)
+        e = launch_pdl(mx4_attn_join_kernel<T, D>, dim3(static_cast<unsigned>(a.B * a.tq * a.hq)), dim3(D), 0, stream, a, p.tile_rows);
+    return static_cast<int>(e);
+}
+
+template <typename T>
+static int run_attention(const Mx4AttnArgs& a, int d, const AttnPlan& p, cudaStream_t stream) {
+    if (d == 256) return launch_attention<T, 256, 1>(a, p, stream);
+    if (d == 128) return p.tile_rows == 32 ? launch_attention<T, 128, 2>(a, p, stream) : launch_attention<T, 128, 1>(a, p, stream);
+    return p.tile_rows == 32 ? launch_attention<T, 64, 2>(a, p, stream) : launch_attention<T, 64, 1>(a, p, stream);
+}
+
 static int check_cache(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G) {
     if (d != 64 && d != 128 && d != 256) return fail("the head dimension must be 64, 128 or 256");
     if (int rc = check_group(d, G)) return rc;
@@ -337,8 +379,9 @@ CONVROT_API int ck_mx4_cache_read(const void* codes, const void* scales, long lo
 }
 
 CONVROT_API size_t ck_mx4_attention_workspace_size(int B, int tq, int hq, int hkv, int d, long long longest) {
-    (void)B; (void)tq; (void)hq; (void)hkv; (void)d; (void)longest;
-    return 0;
+    if (B <= 0 || tq <= 0 || hkv <= 0 || hq <= 0 || hq % hkv || d <= 0) return 0;
+    const AttnPlan p = attn_plan(B, tq, hq, hkv, d, longest);
+    return p.splits > 1 ? align256(p.partials() * d * 4) + align256(p.partials() * 8) : 0;
 }
 
 CONVROT_API int ck_mx4_attention(const void* q, int dtype, long long q_seq, long long q_token, long long q_head,
@@ -356,11 +399,20 @@ CONVROT_API int ck_mx4_attention(const void* q, int dtype, long long q_seq, long
     if (!q || !lens || !out || (table_pages && !table)) return fail("null pointer");
     if (!aligned_to(q, 2) || !aligned_to(table, 4) || !aligned_to(lens, 4) || !aligned16(out))
         return fail("queries, table or lengths not aligned to their type, or out not to 16 bytes");
-    (void)workspace; (void)workspace_bytes;
+    if (pages * 2 * hkv * page > 0xFFFFFFFEll) return fail("the cache holds more than 2^32 - 2 rows");
+    const long long longest = static_cast<long long>(table_pages) * page;
+    const AttnPlan p = attn_plan(B, tq, hq, hkv, d, longest);
+    if (static_cast<long long>(p.tiles) > 0x7FFFFFFF || static_cast<long long>(B) * tq * hq > 0x7FFFFFFFll) return fail("too many query rows");
+    const size_t need = ck_mx4_attention_workspace_size(B, tq, hq, hkv, d, longest);
+    if (need && (!workspace || !aligned_to(workspace, 256))) return fail("the workspace must be 256-byte aligned");
+    if (workspace_bytes < need) return fail("workspace smaller than ck_mx4_attention_workspace_size");
     Mx4AttnArgs a{q, q_seq, q_token, q_head, static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
-                  static_cast<const int*>(table), table_ld, table_pages, static_cast<const int*>(lens), out, B, tq, hq, hkv,
-                  d, page, static_cast<int>(pages), G, softmax_scale};
+                  static_cast<const int*>(table), table_ld, longest, static_cast<const int*>(lens), out,
+                  static_cast<float*>(workspace),
+                  need ? reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + align256(p.partials() * d * 4)) : nullptr,
+                  B, tq, hq, hkv, page_bits(page), static_cast<int>(pages), G, p.row_tiles, p.splits,
+                  softmax_scale * 1.4426950408889634f};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == 1) return static_cast<int>(launch_pdl(mx4_attn_kernel<__nv_bfloat16>, dim3(B * tq * hq), dim3(256), 0, st, a));
-    return static_cast<int>(launch_pdl(mx4_attn_kernel<__half>, dim3(B * tq * hq), dim3(256), 0, st, a));
+    if (dtype == 1) return run_attention<__nv_bfloat16>(a, d, p, st);
+    return run_attention<__half>(a, d, p, st);
 }
