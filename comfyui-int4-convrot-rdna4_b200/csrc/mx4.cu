@@ -283,34 +283,45 @@ struct AttnPlan {
 static AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
     AttnPlan p;
     const long long rows = static_cast<long long>(tq) * (hq / hkv);
-    p.tile_rows = rows > 16 && d <= 128 ? 32 : 16;
+    p.tile_rows = rows <= 8 ? 8 : rows <= 16 || d == 256 ? 16 : 32;
     p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     p.tiles = static_cast<long long>(B) * hkv * p.row_tiles;
-    // splits: enough blocks for two waves of three a multiprocessor, none without
-    // a group of tokens of its own
+    // splits: enough blocks for four waves of four a multiprocessor, none without a
+    // group of tokens of its own
     const long long groups = (longest + kMx4AttnGroup - 1) / kMx4AttnGroup;
-    const long long want = (6LL * sm_count() + p.tiles - 1) / (p.tiles > 0 ? p.tiles : 1);
-    p.splits = static_cast<int>(std::max(1LL, std::min({want, groups, 256LL})));
+    const long long want = (16LL * sm_count() + p.tiles - 1) / (p.tiles > 0 ? p.tiles : 1);
+    p.splits = static_cast<int>(std::max(1LL, std::min({want, groups, static_cast<long long>(kMx4MostSplits)})));
     return p;
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int NT>
 static int launch_attention(const Mx4AttnArgs& a, const AttnPlan& p, cudaStream_t stream) {
-    using Cfg = Mx4AttnCfg<D, MT>;
-    auto kernel = mx4_attn_kernel<T, D, MT>;
+    using Cfg = Mx4AttnCfg<D, NT, std::is_same_v<T, __half>>;
+    auto kernel = mx4_attn_kernel<T, D, NT>;
     cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
     if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3(static_cast<unsigned>(p.tiles), p.splits), dim3(kMx4AttnWarps * 32), Cfg::kSmemBytes, stream, a);
-    if (e == cudaSuccess && p.splits > 1)
-        e = launch_pdl(mx4_attn_join_kernel<T, D>, dim3(static_cast<unsigned>(a.B * a.tq * a.hq)), dim3(D), 0, stream, a, p.tile_rows);
+    if (e == cudaSuccess && p.splits > 1) {
+        const unsigned rows = static_cast<unsigned>(a.B * a.tq * a.hq);
+        const int wide = p.splits > 16;
+        e = launch_pdl(mx4_attn_join_kernel<T, D>, dim3(wide ? rows : (rows + 7) / 8), dim3(256), 0, stream, a, p.tile_rows, wide);
+    }
     return static_cast<int>(e);
+}
+
+template <typename T, int D>
+static int launch_attention_rows(const Mx4AttnArgs& a, const AttnPlan& p, cudaStream_t stream) {
+    if (p.tile_rows == 8) return launch_attention<T, D, 1>(a, p, stream);
+    if constexpr (D < 256)
+        if (p.tile_rows == 32) return launch_attention<T, D, 4>(a, p, stream);
+    return launch_attention<T, D, 2>(a, p, stream);
 }
 
 template <typename T>
 static int run_attention(const Mx4AttnArgs& a, int d, const AttnPlan& p, cudaStream_t stream) {
-    if (d == 256) return launch_attention<T, 256, 1>(a, p, stream);
-    if (d == 128) return p.tile_rows == 32 ? launch_attention<T, 128, 2>(a, p, stream) : launch_attention<T, 128, 1>(a, p, stream);
-    return p.tile_rows == 32 ? launch_attention<T, 64, 2>(a, p, stream) : launch_attention<T, 64, 1>(a, p, stream);
+    if (d == 256) return launch_attention_rows<T, 256>(a, p, stream);
+    if (d == 128) return launch_attention_rows<T, 128>(a, p, stream);
+    return launch_attention_rows<T, 64>(a, p, stream);
 }
 
 static int check_cache(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G) {

@@ -1,7 +1,7 @@
 // Attention of the newest tokens' queries over the paged MX4 cache.
 //
 // Included by mx4.cu. For one sequence and cache head, the tq * (hq / hkv) query
-// rows that read it are taken together (16 or 32 a block), so the cache is read
+// rows that read it are taken together (8, 16 or 32 a block), so the cache is read
 // once for all of them; the sequence is split over blocks, and each warp of a
 // block walks its own chunks of 32 tokens with a running maximum and sum. Warps
 // are joined through shared memory, splits by mx4_attn_join_kernel.
@@ -9,22 +9,26 @@
 // Rotated cache: q k = (H q) (H k), so the query rows are rotated once, and the
 // output, a mean of rotated values, is rotated back at the end.
 //
-// Products run on mma.m16n8k16 (f16 operands, fp32 sums; the contraction over a
-// token's channels and the one over tokens are too small a share of the work for
-// more). A code is an f16 value exactly.
-//   Scores: one MMA pair per block of 32 channels, its result times the block's
-//   scale in fp32. Query rows are f16 times a power of two that brings the row's
-//   largest value to 2^8.
+// Products run on mma.m16n8k16 (f16 operands, fp32 sums) with the cache on the
+// side of 16 and the query rows on the side of 8: S^T = K Q^T and O^T = V^T P^T.
+// Few rows then waste nothing, and tcgen05 (128 rows at least) would. A code is an
+// f16 value exactly.
+//   Scores: one pair of MMAs per block of 32 channels, its result times the
+//   block's scale in fp32. Query rows are f16 times a power of two that brings the
+//   row's largest value to 2^8.
 //   Values: a token's codes times 2^(E_b - E), E the token's largest scale
 //   exponent, are f16 values exactly (down to 2^-24 of the token's largest); the
 //   rest, 2^E, goes to the probabilities: the numerator's weights are
 //   2^(s + E - max(s + E)), with a maximum of their own, so that they are f16
 //   values in [0, 1] whatever the values' range. The denominator keeps the usual
 //   weights 2^(s - max s) in fp32.
+// SPLIT (f16 queries): queries and numerator weights as the sum of two f16 values,
+// so that the result is as exact as its own rounding; a bf16 result's rounding is
+// eight times coarser than what one f16 value loses.
 //
 // Columns. The contraction's order is free, so a thread's operands are whole
-// words of codes: in a tile of 8 tokens column c is token (c >> 1) + 4 (c & 1); a
-// thread (g = lane / 4, t = lane % 4) takes word t of each block of its token for
+// words of codes: in a tile of 8 tokens row r is token (r >> 1) + 4 (r & 1); a
+// thread (g = lane / 4, t = lane % 4) takes word t of each block of its tokens for
 // the scores, and word g (8 channels) of tokens t and t + 4 for the values, whose
 // nibbles are interleaved so that one conversion gives both tokens' value of a
 // channel. 16-byte chunks of a token are XORed so that neither read meets a bank
@@ -50,26 +54,30 @@ struct Mx4AttnArgs {
 };
 
 constexpr int kMx4AttnWarps = 4;
+constexpr int kMx4MostSplits = 256;            // of one sequence
 constexpr int kMx4AttnChunk = 32;              // tokens a warp takes at a time
 constexpr int kMx4AttnGroup = kMx4AttnWarps * kMx4AttnChunk;   // tokens a block takes at a time
 
-template <int D, int MT>
+template <int D, int NT, bool SPLIT>
 struct Mx4AttnCfg {
-    static constexpr int kRows = 16 * MT;
+    static constexpr int kRows = 8 * NT;
     static constexpr int kCodeBytes = kMx4AttnChunk * D / 2;
     static constexpr int kScaleSlot = D == 256 ? 8 : 4;           // bytes kept of a token's scales
     static constexpr int kScaleBytes = kMx4AttnChunk * kScaleSlot;
     static constexpr int kStageBytes = 2 * kCodeBytes + 2 * kScaleBytes + kMx4AttnChunk * 4;   // + the tokens' places
-    static constexpr int kStages = 3;
+    static constexpr int kStages = 2;
     static constexpr int kBlocks = D / 32;
     static constexpr int kTableBytes = kMx4AttnChunk * (kBlocks * 4 + kBlocks * 2 + 8);
     static constexpr int kWarpBytes = kStages * kStageBytes + kTableBytes;
     static constexpr int kQStride = D * 2 + 64;                   // bytes; + 64: two rows in distinct banks
-    static constexpr int kQBytes = kRows * kQStride;
+    static constexpr int kQRows = (SPLIT ? 2 : 1) * kRows * kQStride;     // rows, then what their rounding to f16 left
+    static constexpr int kQBytes = kQRows > kRows * D * 4 ? kQRows : kRows * D * 4;   // (first in fp32)
     static constexpr int kPartStride = D + 4;                     // floats of a joined row
     static constexpr int kPartBytes = kMx4AttnWarps * kRows * kPartStride * 4;
     static constexpr int kRing = kMx4AttnWarps * kWarpBytes;
     static constexpr int kSmemBytes = kQBytes + (kRing > kPartBytes ? kRing : kPartBytes);
+    // blocks a multiprocessor holds, by a thread's accumulators (NT D / 4) and operands
+    static constexpr int kResident = NT * D <= 64 ? 5 : NT * D <= 128 ? (NT == 1 ? 5 : 4) : NT * D <= 256 ? 3 : 2;
 };
 
 // Chunk position of a token's 16-byte chunk c.
@@ -128,10 +136,18 @@ __device__ __forceinline__ int mx4_split_groups(int n, int splits) {
     return (groups + splits - 1) / splits;
 }
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kMx4AttnWarps * 32, MT == 1 && D <= 128 ? 3 : 2)
+// Transposes an 8 x 8 tile of 16-bit values held as an MMA fragment.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kMx4AttnWarps * 32, Mx4AttnCfg<D, NT, std::is_same_v<T, __half>>::kResident)
 mx4_attn_kernel(Mx4AttnArgs a) {
-    using Cfg = Mx4AttnCfg<D, MT>;
+    constexpr bool SPLIT = std::is_same_v<T, __half>;
+    using Cfg = Mx4AttnCfg<D, NT, SPLIT>;
     constexpr int kB = Cfg::kBlocks, kR16 = D / 32;               // blocks; 16-byte chunks of a token
     extern __shared__ __align__(128) unsigned char mx4att[];
     __shared__ float row_scale[Cfg::kRows], pm[kMx4AttnWarps][Cfg::kRows], pl[kMx4AttnWarps][Cfg::kRows];
@@ -142,6 +158,16 @@ mx4_attn_kernel(Mx4AttnArgs a) {
     const int rows = min(Cfg::kRows, rows_all - row0);
     griddep_wait();
     griddep_launch_dependents();
+    // this warp's query rows (used after the first chunks' loads are on their way)
+    constexpr int kRw = Cfg::kRows / kMx4AttnWarps;
+    float qv[kRw][D / 32];
+    #pragma unroll
+    for (int k = 0; k < kRw; ++k) {
+        const int r = warp * kRw + k, row = row0 + r;
+        const T* q = static_cast<const T*>(a.q) + b * a.qsb + (row / per_head) * a.qst + (hk * per_head + row % per_head) * a.qsh;
+        #pragma unroll
+        for (int i = 0; i < D / 32; ++i) qv[k][i] = r < rows ? mx4_to_f32(q[lane + 32 * i]) : 0.0f;
+    }
     const int n = max(0, static_cast<int>(min(static_cast<long long>(a.lens[b]), a.cap)));
     const int per_split = mx4_split_groups(n, a.splits) * kMx4AttnWarps;      // chunks
     const int chunks = (n + kMx4AttnChunk - 1) / kMx4AttnChunk;
@@ -150,10 +176,10 @@ mx4_attn_kernel(Mx4AttnArgs a) {
 
     unsigned char* q_smem = mx4att;
     unsigned char* ring = mx4att + Cfg::kQBytes + warp * Cfg::kWarpBytes;
-    float* kf = reinterpret_cast<float*>(ring + Cfg::kStages * Cfg::kStageBytes);          // [blocks][32]
+    float* kf = reinterpret_cast<float*>(ring + Cfg::kStages * Cfg::kStageBytes);          // [32][blocks]
     float2* info = reinterpret_cast<float2*>(kf + kB * kMx4AttnChunk);                     // [32] {0 or -inf, E}
     __half* vf = reinterpret_cast<__half*>(info + kMx4AttnChunk);                          // [blocks][32]
-    // a token's place in the factor tables: columns 2t and 2t + 1 next to each other
+    // a token's place in the value factors: tokens t and t + 4 next to each other
     const int my_pos = (lane & ~7) + 2 * (lane & 3) + ((lane >> 2) & 1);
 
     // ---------------- the pipeline of this warp's chunks
@@ -163,21 +189,49 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         return chunk < c_end && j < n ? __ldg(table + (j >> a.page_bits)) : -1;
     };
     const uint32_t v_off = static_cast<uint32_t>(a.hkv) << a.page_bits;       // from a key's place to its value's
+    const size_t v_bytes = static_cast<size_t>(v_off) * (D / 2);
+    // where this lane's 16 bytes of 512-byte step i go: the swizzle repeats every 8
+    // tokens, in heads of 256 every second step
+    const int copy_at = lane / kR16 * (D / 2) + mx4_chunk_pos<D>(lane / kR16, lane % kR16) * 16;
+    auto copy_dst = [&](int i) { return (D == 256 && (i & 1) ? copy_at ^ 16 : copy_at) + i * 512; };
     auto issue = [&](int stage, int chunk, int page) {
         unsigned char* st = ring + stage * Cfg::kStageBytes;
         const bool held = page >= 0 && page < a.pages;
         const uint32_t off = (chunk * kMx4AttnChunk + lane) & ((1 << a.page_bits) - 1);
         const uint32_t place = held ? (((static_cast<uint32_t>(page) * 2) * a.hkv + hk) << a.page_bits) + off : 0xFFFFFFFFu;
-        #pragma unroll
-        for (int i = 0; i < kR16; ++i) {
-            const int tok = (i * 32 + lane) / kR16, c = (i * 32 + lane) % kR16;
-            const uint32_t p = __shfl_sync(0xFFFFFFFFu, place, tok);
-            const bool h = p != 0xFFFFFFFFu;
-            const uint8_t* src = a.codes + (h ? static_cast<size_t>(p) * (D / 2) + c * 16 : 0);
-            const uint8_t* vsrc = h ? src + static_cast<size_t>(v_off) * (D / 2) : a.codes;
-            unsigned char* dst = st + tok * (D / 2) + mx4_chunk_pos<D>(tok, c) * 16;
-            cp_async16(dst, src, h);
-            cp_async16(dst + Cfg::kCodeBytes, vsrc, h);
+        if (a.page_bits >= 5) {
+            // the chunk lies in one page: its rows are contiguous, and the tokens that
+            // exist come first
+            const int count = __popc(__ballot_sync(0xFFFFFFFFu, held));
+            const uint32_t first = __shfl_sync(0xFFFFFFFFu, place, 0);
+            const uint8_t* src = a.codes + (count ? static_cast<size_t>(first) * (D / 2) + lane * 16 : 0);
+            const uint8_t* vsrc = src + (count ? v_bytes : 0);
+            unsigned char* dst = st;
+            if (count == kMx4AttnChunk) {
+                #pragma unroll
+                for (int i = 0; i < kR16; ++i) {
+                    cp_async16(dst + copy_dst(i), src + i * 512);
+                    cp_async16(dst + copy_dst(i) + Cfg::kCodeBytes, vsrc + i * 512);
+                }
+            } else {
+                #pragma unroll
+                for (int i = 0; i < kR16; ++i) {
+                    const bool h = (i * 32 + lane) / kR16 < count;
+                    cp_async16(dst + copy_dst(i), h ? src + i * 512 : a.codes, h);
+                    cp_async16(dst + copy_dst(i) + Cfg::kCodeBytes, h ? vsrc + i * 512 : a.codes, h);
+                }
+            }
+        } else {
+            #pragma unroll
+            for (int i = 0; i < kR16; ++i) {
+                const int tok = (i * 32 + lane) / kR16, c = (i * 32 + lane) % kR16;
+                const uint32_t p = __shfl_sync(0xFFFFFFFFu, place, tok);
+                const bool h = p != 0xFFFFFFFFu;
+                const uint8_t* src = a.codes + (h ? static_cast<size_t>(p) * (D / 2) + c * 16 : 0);
+                unsigned char* dst = st + copy_dst(i);
+                cp_async16(dst, src, h);
+                cp_async16(dst + Cfg::kCodeBytes, src + (h ? v_bytes : 0), h);
+            }
         }
         // (heads of 64 have two scale bytes: the aligned word that holds them)
         const size_t sp = held ? (D == 64 ? static_cast<size_t>(place & ~1u) * 2 : static_cast<size_t>(place) * kB) : 0;
@@ -197,63 +251,75 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         page = page_of(ahead);
     }
 
-    // ---------------- query rows: rotated, scaled to f16
+    // ---------------- query rows: rotated in fp32, then f16 times a power of two
     {
-        __shared__ float qrow[kMx4AttnWarps][D];                  // (the ring's space is in use: a row at a time)
-        for (int r = warp; r < Cfg::kRows; r += kMx4AttnWarps) {
-            float* v = qrow[warp];
-            const int row = row0 + r;
-            if (r < rows) {
-                const T* q = static_cast<const T*>(a.q) + b * a.qsb + (row / per_head) * a.qst +
-                             (hk * per_head + row % per_head) * a.qsh;
-                for (int i = lane; i < D; i += 32) v[i] = mx4_to_f32(q[i]);
-            } else {
-                for (int i = lane; i < D; i += 32) v[i] = 0.0f;
+        float* v = reinterpret_cast<float*>(q_smem) + warp * kRw * D;
+        #pragma unroll
+        for (int k = 0; k < kRw; ++k)
+            #pragma unroll
+            for (int i = 0; i < D / 32; ++i) v[k * D + lane + 32 * i] = qv[k][i];
+        __syncwarp();
+        for (int st = 1; st < a.group; st *= 4) {
+            #pragma unroll
+            for (int j = 0; j < kRw * D / 128 || j == 0; ++j) {
+                const int i = lane + 32 * j;
+                if (kRw * D < 128 && i >= kRw * D / 4) break;
+                float* p = v + (i / st) * 4 * st + i % st;
+                h4(p[0], p[st], p[2 * st], p[3 * st]);
             }
             __syncwarp();
-            for (int st = 1; st < a.group; st *= 4) {
-                for (int i = lane; i < D / 4; i += 32) {
-                    float* p = v + (i / st) * 4 * st + i % st;
-                    h4(p[0], p[st], p[2 * st], p[3 * st]);
-                }
-                __syncwarp();
-            }
-            const float f = a.group == 16 ? 0.25f : a.group == 64 ? 0.125f : a.group == 256 ? 0.0625f : 1.0f;
+        }
+        const float f = a.group == 16 ? 0.25f : a.group == 64 ? 0.125f : a.group == 256 ? 0.0625f : 1.0f;
+        float to_f16[kRw];
+        #pragma unroll
+        for (int k = 0; k < kRw; ++k) {
             float top = 0.0f;
-            for (int i = lane; i < D; i += 32) top = fmaxf(top, fabsf(v[i]));
+            #pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                qv[k][i] = v[k * D + lane + 32 * i];
+                top = fmaxf(top, fabsf(qv[k][i]));
+            }
             #pragma unroll
             for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
             // 2^(8 - exponent of the row's largest value), within fp32's normal range
             const int e = static_cast<int>(__float_as_uint(top) >> 23);
             const int up = top > 0.0f ? min(max(135 - e, -120), 120) : 0;
-            const float to_f16 = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-            if (lane == 0) row_scale[r] = a.scale * f * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
-            __half* dst = reinterpret_cast<__half*>(q_smem + r * Cfg::kQStride);
-            for (int i = lane; i < D; i += 32) dst[i] = __float2half_rn(v[i] * to_f16);
-            __syncwarp();
+            to_f16[k] = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+            if (lane == 0) row_scale[warp * kRw + k] = a.scale * f * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+        }
+        __syncthreads();                                          // the f16 rows take the place of every warp's fp32 rows
+        #pragma unroll
+        for (int k = 0; k < kRw; ++k) {
+            __half* dst = reinterpret_cast<__half*>(q_smem + (warp * kRw + k) * Cfg::kQStride);
+            #pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                const float x = qv[k][i] * to_f16[k];
+                const __half hi = __float2half_rn(x);
+                dst[lane + 32 * i] = hi;
+                if constexpr (SPLIT) dst[Cfg::kRows * Cfg::kQStride / 2 + lane + 32 * i] = __float2half_rn(x - __half2float(hi));
+            }
         }
     }
     __syncthreads();
 
-    float o[MT][D / 8][4];
-    float m[MT][2], mn[MT][2], l[MT][2], rs[MT][2];
-    int vis[MT][2];                                               // tokens a row sees
+    float o[NT][D / 16][4];                                       // channels g, g + 8 of each 16; rows 2t, 2t + 1
+    float m[NT][2], mn[NT][2], l[NT][2], rs[NT][2];               // rows 2t, 2t + 1 of each 8
     #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < NT; ++i) {
         #pragma unroll
-        for (int j = 0; j < D / 8; ++j)
+        for (int j = 0; j < D / 16; ++j)
             #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][j][e] = 0.0f;
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int r = 16 * i + 8 * h + g;
+            const int r = 8 * i + 2 * t4 + h;
             m[i][h] = mn[i][h] = -INFINITY;
             l[i][h] = 0.0f;
             rs[i][h] = row_scale[r];
-            vis[i][h] = r < rows ? n - a.tq + (row0 + r) / per_head + 1 : 0;
         }
     }
     const int sees_all = n - a.tq + row0 / per_head + 1;          // tokens that every row of the tile sees
+    const int ktok = (g >> 1) + 4 * (g & 1);                      // this thread's token of each tile of 8
 
     for (int it = 0; ci < c_end; ci += kMx4AttnWarps, ++it) {
         if (ahead < c_end) issue((it + Cfg::kStages - 1) % Cfg::kStages, ahead, page);
@@ -280,89 +346,127 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 vs[1] = *reinterpret_cast<const uint32_t*>(sc + Cfg::kScaleBytes + 4);
             }
             int top = 0;
+            float kv[kB];
+            __half vv[kB];
+            bool bad = false;                                     // a block of NaN
             #pragma unroll
             for (int i = 0; i < kB; ++i) {
                 const uint32_t ek = (ks[i / 4] >> (8 * (i % 4))) & 255u;
+                kv[i] = __uint_as_float(ek << 23);                // (2^-127 counts as 0)
                 const int ev = (vs[i / 4] >> (8 * (i % 4))) & 255u;
-                kf[i * 32 + my_pos] = mx4_scale_value(ek);
-                if (ev != 255) top = max(top, ev);
+                top = max(top, ev);
+                bad |= ek == 255u;
             }
+            bad |= top == 255;
             #pragma unroll
             for (int i = 0; i < kB; ++i) {
                 const int ev = (vs[i / 4] >> (8 * (i % 4))) & 255u;
-                const int d = max(ev - top, -126);
-                vf[i * 32 + my_pos] = ev == 255 ? __ushort_as_half(0x7FFF) : __float2half_rn(__uint_as_float(static_cast<uint32_t>(127 + d) << 23));
+                vv[i] = __float2half_rn(__uint_as_float(static_cast<uint32_t>(max(ev - top + 127, 0)) << 23));
             }
-            info[my_pos] = place != 0xFFFFFFFFu ? make_float2(0.0f, static_cast<float>(top - 127)) : make_float2(-INFINITY, 0.0f);
+            if (__any_sync(0xFFFFFFFFu, bad)) {
+                top = 0;
+                #pragma unroll
+                for (int i = 0; i < kB; ++i) {
+                    const int ev = (vs[i / 4] >> (8 * (i % 4))) & 255u;
+                    if (ev != 255) top = max(top, ev);
+                    if (kv[i] == INFINITY) kv[i] = NAN;
+                }
+                #pragma unroll
+                for (int i = 0; i < kB; ++i) {
+                    const int ev = (vs[i / 4] >> (8 * (i % 4))) & 255u;
+                    vv[i] = ev == 255 ? __ushort_as_half(0x7FFF) : __float2half_rn(__uint_as_float(static_cast<uint32_t>(max(ev - top + 127, 0)) << 23));
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < kB; i += 2) *reinterpret_cast<float2*>(kf + lane * kB + i) = make_float2(kv[i], kv[i + 1]);
+            #pragma unroll
+            for (int i = 0; i < kB; ++i) vf[i * 32 + my_pos] = vv[i];
+            info[lane] = place != 0xFFFFFFFFu ? make_float2(0.0f, static_cast<float>(top - 127)) : make_float2(-INFINITY, 0.0f);
         }
         __syncwarp();
 
-        // ---------------- scores
-        float s[MT][4][4];
+        // ---------------- scores: tiles of 16 tokens (rows g, g + 8) by 8 query rows
+        float s[NT][2][4];
         #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < NT; ++i)
             #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 2; ++c)
                 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[i][c][e] = 0.0f;
-        const int ktok = (g >> 1) + 4 * (g & 1);
         #pragma unroll
         for (int blk = 0; blk < kB; ++blk) {
-            uint4 qa[MT][2];
+            uint4 qb[NT], ql[NT];
             #pragma unroll
-            for (int i = 0; i < MT; ++i)
-                #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    qa[i][h] = *reinterpret_cast<const uint4*>(q_smem + (16 * i + 8 * h + g) * Cfg::kQStride + blk * 64 + t4 * 16);
+            for (int i = 0; i < NT; ++i) {
+                const unsigned char* at = q_smem + (8 * i + g) * Cfg::kQStride + blk * 64 + t4 * 16;
+                qb[i] = *reinterpret_cast<const uint4*>(at);
+                if constexpr (SPLIT) ql[i] = *reinterpret_cast<const uint4*>(at + Cfg::kRows * Cfg::kQStride);
+            }
             #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int tok = 8 * c + ktok;
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(st + tok * (D / 2) + mx4_chunk_pos<D>(tok, blk) * 16 + t4 * 4);
-                uint32_t h[4];
-                codes_to_f16(w, h);
-                const float2 f = *reinterpret_cast<const float2*>(kf + blk * 32 + 8 * c + 2 * t4);
+            for (int c = 0; c < 2; ++c) {
+                uint32_t h0[4], h1[4];
+                const int tok = 16 * c + ktok;
+                codes_to_f16(*reinterpret_cast<const uint32_t*>(st + tok * (D / 2) + mx4_chunk_pos<D>(tok, blk) * 16 + t4 * 4), h0);
+                codes_to_f16(*reinterpret_cast<const uint32_t*>(st + (tok + 8) * (D / 2) + mx4_chunk_pos<D>(tok + 8, blk) * 16 + t4 * 4), h1);
+                const float f0 = kf[tok * kB + blk], f1 = kf[(tok + 8) * kB + blk];
                 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
+                for (int i = 0; i < NT; ++i) {
                     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_f16(acc, qa[i][0].x, qa[i][1].x, qa[i][0].y, qa[i][1].y, h[0], h[1]);
-                    mma_f16(acc, qa[i][0].z, qa[i][1].z, qa[i][0].w, qa[i][1].w, h[2], h[3]);
-                    s[i][c][0] = fmaf(acc[0], f.x, s[i][c][0]);
-                    s[i][c][1] = fmaf(acc[1], f.y, s[i][c][1]);
-                    s[i][c][2] = fmaf(acc[2], f.x, s[i][c][2]);
-                    s[i][c][3] = fmaf(acc[3], f.y, s[i][c][3]);
+                    mma_f16(acc, h0[0], h1[0], h0[1], h1[1], qb[i].x, qb[i].y);
+                    mma_f16(acc, h0[2], h1[2], h0[3], h1[3], qb[i].z, qb[i].w);
+                    if constexpr (SPLIT) {
+                        mma_f16(acc, h0[0], h1[0], h0[1], h1[1], ql[i].x, ql[i].y);
+                        mma_f16(acc, h0[2], h1[2], h0[3], h1[3], ql[i].z, ql[i].w);
+                    }
+                    s[i][c][0] = fmaf(acc[0], f0, s[i][c][0]);
+                    s[i][c][1] = fmaf(acc[1], f0, s[i][c][1]);
+                    s[i][c][2] = fmaf(acc[2], f1, s[i][c][2]);
+                    s[i][c][3] = fmaf(acc[3], f1, s[i][c][3]);
                 }
             }
         }
 
         // ---------------- weights
-        float4 tk[4];                                             // {0 or -inf, E} of tokens t and t + 4 of each tile
+        float2 tk[4];                                             // {0 or -inf, E} of this thread's tokens
         #pragma unroll
-        for (int c = 0; c < 4; ++c) tk[c] = *reinterpret_cast<const float4*>(info + 8 * c + 2 * t4);
-        uint32_t p[MT][4][2];                                     // numerator weights, f16 pairs: tile, row half
-        const bool cut = (ci + 1) * kMx4AttnChunk > sees_all;
+        for (int c = 0; c < 4; ++c) tk[c] = info[8 * c + ktok];
+        uint32_t p[NT][4], pr[NT][4];                             // numerator weights as MMA operands, tile by tile of 8 tokens
+        #pragma unroll
+        for (int i = 0; i < NT; ++i)
+            #pragma unroll
+            for (int c = 0; c < 4; ++c)
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) s[i][c >> 1][2 * (c & 1) + h] = fmaf(s[i][c >> 1][2 * (c & 1) + h], rs[i][h], tk[c].x);
+        if ((ci + 1) * kMx4AttnChunk > sees_all) {                // some row's last tokens: hide what a row does not see
+            #pragma unroll
+            for (int i = 0; i < NT; ++i)
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = 8 * i + 2 * t4 + h;
+                    const int sees = r < rows ? n - a.tq + (row0 + r) / per_head + 1 : 0;
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (ci * kMx4AttnChunk + 8 * c + ktok >= sees) s[i][c >> 1][2 * (c & 1) + h] = -INFINITY;
+                }
+        }
         bool moved = false;
-        float fn[MT][2];
+        float fn[NT][2];
         #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < NT; ++i) {
+            float w[2][4];
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float x[8], top = -INFINITY, topn = -INFINITY;
+                float x[4], top = -INFINITY, topn = -INFINITY;
                 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    x[2 * c] = fmaf(s[i][c][2 * h], rs[i][h], tk[c].x);
-                    x[2 * c + 1] = fmaf(s[i][c][2 * h + 1], rs[i][h], tk[c].z);
-                    if (cut) {
-                        const int j = ci * kMx4AttnChunk + 8 * c + t4;
-                        if (j >= vis[i][h]) x[2 * c] = -INFINITY;
-                        if (j + 4 >= vis[i][h]) x[2 * c + 1] = -INFINITY;
-                    }
-                    top = fmaxf(top, fmaxf(x[2 * c], x[2 * c + 1]));
-                    topn = fmaxf(topn, fmaxf(x[2 * c] + tk[c].y, x[2 * c + 1] + tk[c].w));
+                    x[c] = s[i][c >> 1][2 * (c & 1) + h];
+                    top = fmaxf(top, x[c]);
+                    topn = fmaxf(topn, x[c] + tk[c].y);
                 }
                 #pragma unroll
-                for (int w = 1; w < 4; w *= 2) {
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
-                    topn = fmaxf(topn, __shfl_xor_sync(0xFFFFFFFFu, topn, w));
+                for (int z = 4; z < 32; z *= 2) {
+                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
+                    topn = fmaxf(topn, __shfl_xor_sync(0xFFFFFFFFu, topn, z));
                 }
                 const float m2 = fmaxf(m[i][h], top), mn2 = fmaxf(mn[i][h], topn);
                 const float base = m2 == -INFINITY ? 0.0f : m2, basen = mn2 == -INFINITY ? 0.0f : mn2;
@@ -373,23 +477,32 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 mn[i][h] = mn2;
                 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    l[i][h] += ex2(x[2 * c] - base) + ex2(x[2 * c + 1] - base);
-                    p[i][c][h] = f16x2_bits(ex2(x[2 * c] + (tk[c].y - basen)), ex2(x[2 * c + 1] + (tk[c].w - basen)));
+                    l[i][h] += ex2(x[c] - base);
+                    w[h][c] = ex2(x[c] + (tk[c].y - basen));
                 }
             }
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t hi = f16x2_bits(w[0][c], w[1][c]);
+                p[i][c] = movmatrix_trans(hi);
+                if constexpr (SPLIT) {
+                    __half2 r;
+                    memcpy(&r, &hi, 4);
+                    const float2 back = __half22float2(r);
+                    pr[i][c] = movmatrix_trans(f16x2_bits(w[0][c] - back.x, w[1][c] - back.y));
+                }
+            }
+        }
         if (__any_sync(0xFFFFFFFFu, moved)) {
             #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < NT; ++i)
                 #pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
-                    o[i][j][0] *= fn[i][0];
-                    o[i][j][1] *= fn[i][0];
-                    o[i][j][2] *= fn[i][1];
-                    o[i][j][3] *= fn[i][1];
-                }
+                for (int j = 0; j < D / 16; ++j)
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) o[i][j][e] *= fn[i][e & 1];
         }
 
-        // ---------------- values
+        // ---------------- values: tiles of 16 channels by 8 query rows over 16 tokens
         #pragma unroll
         for (int u = 0; u < 2; ++u) {
             #pragma unroll
@@ -407,17 +520,17 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 }
                 uint32_t e0[4], e1[4], d0[4], d1[4];
                 codes_to_f16(lo[0], e0);
-                codes_to_f16(lo[1], e1);
                 codes_to_f16(hi[0], d0);
+                codes_to_f16(lo[1], e1);
                 codes_to_f16(hi[1], d1);
                 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const uint32_t b0 = hmul2_bits(e0[k], f[0]), b1 = hmul2_bits(e1[k], f[1]);
-                    const uint32_t c0 = hmul2_bits(d0[k], f[0]), c1 = hmul2_bits(d1[k], f[1]);
+                    const uint32_t a0 = hmul2_bits(e0[k], f[0]), a1 = hmul2_bits(d0[k], f[0]);
+                    const uint32_t a2 = hmul2_bits(e1[k], f[1]), a3 = hmul2_bits(d1[k], f[1]);
                     #pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        mma_f16(o[i][8 * hf + 2 * k], p[i][2 * u][0], p[i][2 * u][1], p[i][2 * u + 1][0], p[i][2 * u + 1][1], b0, b1);
-                        mma_f16(o[i][8 * hf + 2 * k + 1], p[i][2 * u][0], p[i][2 * u][1], p[i][2 * u + 1][0], p[i][2 * u + 1][1], c0, c1);
+                    for (int i = 0; i < NT; ++i) {
+                        mma_f16(o[i][4 * hf + k], a0, a1, a2, a3, p[i][2 * u], p[i][2 * u + 1]);
+                        if constexpr (SPLIT) mma_f16(o[i][4 * hf + k], a0, a1, a2, a3, pr[i][2 * u], pr[i][2 * u + 1]);
                     }
                 }
             }
@@ -430,45 +543,50 @@ mx4_attn_kernel(Mx4AttnArgs a) {
     // ---------------- join the warps
     float* part = reinterpret_cast<float*>(mx4att + Cfg::kQBytes);
     #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < NT; ++i)
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int r = 16 * i + 8 * h + g;
+            const int r = 8 * i + 2 * t4 + h;
             float sum = l[i][h];
-            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+            #pragma unroll
+            for (int z = 4; z < 32; z *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, z);
             const float f = m[i][h] == -INFINITY ? 0.0f : ex2(mn[i][h] - m[i][h]);
-            if (t4 == 0) {
+            if (g == 0) {
                 pm[warp][r] = m[i][h];
                 pl[warp][r] = sum;
             }
             float* dst = part + (warp * Cfg::kRows + r) * Cfg::kPartStride;
             #pragma unroll
-            for (int j = 0; j < D / 8; ++j)
-                #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    dst[64 * (j / 8) + 8 * (2 * t4 + e) + (j % 8)] = o[i][j][2 * h + e] * f;
+            for (int j = 0; j < D / 16; ++j)                      // channels 8 g + 2 k and the next of each 64
+                *reinterpret_cast<float2*>(dst + 64 * (j / 4) + 8 * g + 2 * (j % 4)) = make_float2(o[i][j][h] * f, o[i][j][2 + h] * f);
         }
     __syncthreads();
     float* joined = part;                                          // warp 0's rows become the block's
-    for (int i = tid; i < rows * D; i += kMx4AttnWarps * 32) {
-        const int r = i / D, c = i % D;
+    for (int i = tid; i < rows * D / 4; i += kMx4AttnWarps * 32) {
+        const int r = i / (D / 4), c = i % (D / 4) * 4;
         float top = -INFINITY;
         #pragma unroll
         for (int w = 0; w < kMx4AttnWarps; ++w) top = fmaxf(top, pm[w][r]);
-        float sum = 0.0f, acc = 0.0f;
+        float sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         #pragma unroll
         for (int w = 0; w < kMx4AttnWarps; ++w) {
             const float f = pm[w][r] == -INFINITY ? 0.0f : ex2(pm[w][r] - top);
+            const float4 x = *reinterpret_cast<const float4*>(part + (w * Cfg::kRows + r) * Cfg::kPartStride + c);
             sum += f * pl[w][r];
-            acc += f * part[(w * Cfg::kRows + r) * Cfg::kPartStride + c];
+            acc.x += f * x.x;
+            acc.y += f * x.y;
+            acc.z += f * x.z;
+            acc.w += f * x.w;
         }
         if (a.splits > 1) {
             const size_t at = (static_cast<size_t>(tile) * a.splits + split) * Cfg::kRows + r;
-            a.part[at * D + c] = acc;
+            *reinterpret_cast<float4*>(a.part + at * D + c) = acc;
             if (c == 0) a.part_ml[at] = make_float2(top, sum);
         } else {
-            joined[r * Cfg::kPartStride + c] = sum == 0.0f ? 0.0f : acc / sum;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            *reinterpret_cast<float4*>(joined + r * Cfg::kPartStride + c) =
+                sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
         }
     }
     if (a.splits > 1) return;
@@ -489,33 +607,70 @@ mx4_attn_kernel(Mx4AttnArgs a) {
     }
 }
 
-// Joins a row's splits, rotates back and rounds. One block a row, a thread a channel.
+// Joins a row's splits, rotates back and rounds. `wide`: a block (eight warps) a
+// row, for many splits of few rows; otherwise a warp a row.
 template <typename T, int D>
-__global__ void __launch_bounds__(D) mx4_attn_join_kernel(Mx4AttnArgs a, int tile_rows) {
-    __shared__ float v[D];
+__global__ void __launch_bounds__(256) mx4_attn_join_kernel(Mx4AttnArgs a, int tile_rows, int wide) {
+    constexpr int kPer = D / 32;
+    __shared__ float v[8][D], weight[kMx4MostSplits];
     griddep_wait();
     griddep_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per_head = a.hq / a.hkv, rows_all = a.tq * per_head;
-    const int row = blockIdx.x % rows_all, hk = blockIdx.x / rows_all % a.hkv, b = blockIdx.x / rows_all / a.hkv;
+    const int index = wide ? blockIdx.x : blockIdx.x * 8 + warp;
+    if (index >= a.B * a.hkv * rows_all) return;                   // (not wide: whole warps leave, no barrier below)
+    const int row = index % rows_all, hk = index / rows_all % a.hkv, b = index / rows_all / a.hkv;
     const int n = max(0, static_cast<int>(min(static_cast<long long>(a.lens[b]), a.cap)));
     const int per_split = mx4_split_groups(n, a.splits) * kMx4AttnGroup;
     const int held = per_split ? (n + per_split - 1) / per_split : 0;          // splits that hold tokens
     const size_t at = ((static_cast<size_t>(b) * a.hkv + hk) * a.row_tiles + row / tile_rows) * a.splits * tile_rows + row % tile_rows;
-    float top = -INFINITY;
-    for (int s = 0; s < held; ++s) top = fmaxf(top, a.part_ml[at + static_cast<size_t>(s) * tile_rows].x);
-    float sum = 0.0f, acc = 0.0f;
-    for (int s = 0; s < held; ++s) {
-        const size_t i = at + static_cast<size_t>(s) * tile_rows;
-        const float2 ml = a.part_ml[i];
-        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-        sum += f * ml.y;
-        acc += f * a.part[i * D + threadIdx.x];
+    const float2* ml = a.part_ml + at;
+    float top = -INFINITY, sum = 0.0f;
+    for (int s = lane; s < held; s += 32) top = fmaxf(top, ml[static_cast<size_t>(s) * tile_rows].x);
+    #pragma unroll
+    for (int z = 16; z; z >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
+    float f = 0.0f;                                                // not wide: at most 32 splits, lane s has split s's
+    for (int s = lane; s < held; s += 32) {
+        const float2 x = ml[static_cast<size_t>(s) * tile_rows];
+        f = x.x == -INFINITY ? 0.0f : ex2(x.x - top);
+        sum += f * x.y;
+        if (wide && warp == 0) weight[s] = f;
     }
-    v[threadIdx.x] = sum == 0.0f ? 0.0f : acc / sum;
-    __syncthreads();
-    mx4_rotate_shared(v, D, a.group, threadIdx.x, D);
+    #pragma unroll
+    for (int z = 16; z; z >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, z);
+    if (wide) __syncthreads();
+    float acc[kPer] = {};
+    const float* src = a.part + at * D + lane;
+    #pragma unroll 4
+    for (int s = wide ? warp : 0; s < held; s += wide ? 8 : 1) {
+        const float w = wide ? weight[s] : __shfl_sync(0xFFFFFFFFu, f, s);
+        #pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] += w * src[static_cast<size_t>(s) * tile_rows * D + 32 * i];
+    }
+    #pragma unroll
+    for (int i = 0; i < kPer; ++i) v[warp][lane + 32 * i] = acc[i];
+    if (wide) {
+        __syncthreads();
+        if (warp != 0) return;
+        #pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            for (int w = 1; w < 8; ++w) acc[i] += v[w][lane + 32 * i];
+            v[0][lane + 32 * i] = acc[i];
+        }
+    }
+    float* r = v[wide ? 0 : warp];
+    __syncwarp();
+    for (int st = 1; st < a.group; st *= 4) {
+        for (int i = lane; i < D / 4; i += 32) {
+            float* p = r + (i / st) * 4 * st + i % st;
+            h4(p[0], p[st], p[2 * st], p[3 * st]);
+        }
+        __syncwarp();
+    }
+    const float g = a.group == 16 ? 0.25f : a.group == 64 ? 0.125f : a.group == 256 ? 0.0625f : 1.0f;
+    const float norm = sum == 0.0f ? 0.0f : g / sum;
     T* out = static_cast<T*>(a.out) + ((static_cast<size_t>(b) * a.tq + row / per_head) * a.hq + hk * per_head + row % per_head) * D;
-    out[threadIdx.x] = mx4_from_f32<T>(v[threadIdx.x]);
+    for (int i = lane; i < D; i += 32) out[i] = mx4_from_f32<T>(r[i] * norm);
 }
 
 }  // namespace convrot

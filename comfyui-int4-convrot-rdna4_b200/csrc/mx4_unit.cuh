@@ -176,6 +176,9 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool held
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
                  :: "r"(smem_u32(dst)), "l"(src), "r"(held ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(dst)), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
