@@ -77,7 +77,7 @@ struct Mx4AttnCfg {
     static constexpr int kRing = kMx4AttnWarps * kWarpBytes;
     static constexpr int kSmemBytes = kQBytes + (kRing > kPartBytes ? kRing : kPartBytes);
     // blocks a multiprocessor holds, by a thread's accumulators (NT D / 4) and operands
-    static constexpr int kResident = NT * D <= 64 ? 5 : NT * D <= 128 ? (NT == 1 ? 5 : 4) : NT * D <= 256 ? 3 : 2;
+    static constexpr int kResident = NT * D <= 64 ? 5 : NT * D <= 128 ? 4 : NT * D <= 256 ? 3 : 2;
 };
 
 // Chunk position of a token's 16-byte chunk c.
@@ -393,6 +393,19 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             for (int c = 0; c < 2; ++c)
                 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[i][c][e] = 0.0f;
+        float fk[4][kB];                                          // the scales of this thread's four tokens
+        #pragma unroll
+        for (int c = 0; c < 4; ++c)
+            #pragma unroll
+            for (int i = 0; i < kB; i += (kB < 4 ? 2 : 4)) {
+                if constexpr (kB < 4) {
+                    const float2 x = *reinterpret_cast<const float2*>(kf + (8 * c + ktok) * kB + i);
+                    fk[c][i] = x.x; fk[c][i + 1] = x.y;
+                } else {
+                    const float4 x = *reinterpret_cast<const float4*>(kf + (8 * c + ktok) * kB + i);
+                    fk[c][i] = x.x; fk[c][i + 1] = x.y; fk[c][i + 2] = x.z; fk[c][i + 3] = x.w;
+                }
+            }
         #pragma unroll
         for (int blk = 0; blk < kB; ++blk) {
             uint4 qb[NT], ql[NT];
@@ -408,7 +421,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 const int tok = 16 * c + ktok;
                 codes_to_f16(*reinterpret_cast<const uint32_t*>(st + tok * (D / 2) + mx4_chunk_pos<D>(tok, blk) * 16 + t4 * 4), h0);
                 codes_to_f16(*reinterpret_cast<const uint32_t*>(st + (tok + 8) * (D / 2) + mx4_chunk_pos<D>(tok + 8, blk) * 16 + t4 * 4), h1);
-                const float f0 = kf[tok * kB + blk], f1 = kf[(tok + 8) * kB + blk];
+                const float f0 = fk[2 * c][blk], f1 = fk[2 * c + 1][blk];
                 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
                     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
