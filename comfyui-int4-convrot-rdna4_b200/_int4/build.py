@@ -15,7 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(os.path.dirname(_HERE), "csrc")
 SOURCES = ["convrot_b200.cu", "noalloc.cu", "mx4.cu"]
 HEADERS = ["sm100_ptx.cuh", "gemm_pair.cuh", "gemm_a8t.cuh", "lora_down.cuh", "linear_api.cuh", "hadamard.cuh",
-           "host_launch.cuh", "mx4_common.cuh", "mx4_unit.cuh", "mx4_quant.cuh", "mx4_gemm.cuh", "mx4_cache.cuh", "mx4_attn.cuh"]
+           "host_launch.cuh", "mx4_common.cuh", "mx4_unit.cuh", "mx4_quant.cuh", "mx4_gemm.cuh", "mx4_few.cuh", "mx4_cache.cuh", "mx4_attn.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

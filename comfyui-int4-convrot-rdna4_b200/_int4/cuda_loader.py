@@ -58,7 +58,7 @@ _SIGNATURES = {
     "ck_mx4_quant": [_P, _I, _L, _P, _P, _I, _I, _I, _P],
     "ck_mx4_dequant": [_P, _P, _P, _I, _I, _I, _I, _P],
     "ck_mx4_linear_workspace_size": [_I, _I],
-    "ck_mx4_linear": [_P, _I, _L, _P, _P, _P, _I, _P] + [_I] * 5 + [_P, ctypes.c_size_t, _P],
+    "ck_mx4_linear": [_P, _I, _L, _P, _P, _P, _I, _P] + [_I] * 4 + [_P, ctypes.c_size_t, _P],
     "ck_mx4_cache_append": [_P, _P, _L] + [_I] * 4 + [_P, _P, _I] + [_L] * 4 + [_P, _I, _P],
     "ck_mx4_cache_read": [_P, _P, _L] + [_I] * 4 + [_P, _I, _P, _P, _I, _P],
     "ck_mx4_attention_workspace_size": [_I] * 5 + [_L],

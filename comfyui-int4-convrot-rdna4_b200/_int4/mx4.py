@@ -40,15 +40,18 @@ def _device_of(*tensors):
     """The one CUDA device of the tensors (None entries skipped); ValueError otherwise."""
     device = None
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("the B200 ConvRot kernels need CUDA tensors")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}")
+        if t is not None:
+            if not t.is_cuda:
+                raise ValueError("the B200 ConvRot kernels need CUDA tensors")
+            if device is None:
+                device = t.device
+            elif t.device != device:
+                raise ValueError(f"tensors on {device} and {t.device}")
     return device
+
+
+# the current stream as a number, without building a Stream object for each call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _call(device, name, *args):
@@ -56,10 +59,10 @@ def _call(device, name, *args):
     fn = getattr(_load(), name)
     index = device.index
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _check(name, rc)
 
@@ -125,8 +128,8 @@ def quantize_convrot_mx4(x: torch.Tensor, convrot_groupsize: int = 256) -> tuple
     code = _dtype_code(x.dtype)
     x2 = _rows(x)
     m = x2.shape[0]
-    codes = torch.empty((*x.shape[:-1], k // 2), dtype=torch.uint8, device=device)
-    scales = torch.empty(_scale_tiles(m, k), dtype=torch.uint8, device=device)
+    codes = x2.new_empty((*x.shape[:-1], k // 2), dtype=torch.uint8)
+    scales = x2.new_empty(_scale_tiles(m, k), dtype=torch.uint8)
     _call(device, "ck_mx4_quant", x2.data_ptr(), code, x2.stride(0), codes.data_ptr(), scales.data_ptr(), m, k, group)
     return codes, scales
 
@@ -142,7 +145,7 @@ def dequantize_convrot_mx4(codes: torch.Tensor, scales: torch.Tensor, convrot_gr
     device = _device_of(codes, scales)
     rows, k = _check_codes(codes, scales, "MX4")
     group = _group(k, convrot_groupsize)
-    out = torch.empty((*codes.shape[:-1], k), dtype=dtype, device=device)
+    out = codes.new_empty((*codes.shape[:-1], k), dtype=dtype)
     _call(device, "ck_mx4_dequant", codes.data_ptr(), scales.data_ptr(), out.data_ptr(), _dtype_code(dtype), rows, k, group)
     return out
 
@@ -192,11 +195,11 @@ def convrot_mx4_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Te
         bias_ptr, bias_code = bias.data_ptr(), _IN_DTYPE_CODE[bias.dtype]
     x2 = _rows(x)
     m = x2.shape[0]
-    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=device)
+    out = x2.new_empty((*x.shape[:-1], n))
     need = _load().ck_mx4_linear_workspace_size(m, k)
-    workspace = torch.empty((need,), dtype=torch.uint8, device=device)
+    workspace = x2.new_empty((need,), dtype=torch.uint8) if need else None
     _call(device, "ck_mx4_linear", x2.data_ptr(), code, x2.stride(0), qweight.data_ptr(), wscales.data_ptr(), bias_ptr,
-          bias_code, out.data_ptr(), code, m, n, k, group, workspace.data_ptr(), need)
+          bias_code, out.data_ptr(), m, n, k, group, workspace.data_ptr() if need else 0, need)
     return out
 
 
@@ -267,8 +270,8 @@ def convrot_mx4_cache_read(codes: torch.Tensor, scales: torch.Tensor, slots: tor
     _check_slots(slots, None)
     t = slots.shape[0]
     code = _dtype_code(dtype)
-    k = torch.empty((t, heads, d), dtype=dtype, device=device)
-    v = torch.empty((t, heads, d), dtype=dtype, device=device)
+    k = codes.new_empty((t, heads, d), dtype=dtype)
+    v = codes.new_empty((t, heads, d), dtype=dtype)
     _call(device, "ck_mx4_cache_read", codes.data_ptr(), scales.data_ptr(), pages, heads, d, page, group, slots.data_ptr(),
           t, k.data_ptr(), v.data_ptr(), code)
     return k, v
@@ -303,9 +306,9 @@ def convrot_mx4_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Te
     if q.stride(3) != 1:
         q = q.contiguous()
     per_seq = block_table.shape[1]
-    out = torch.empty((b, tq, hq, d), dtype=q.dtype, device=device)
+    out = q.new_empty((b, tq, hq, d))
     need = _load().ck_mx4_attention_workspace_size(b, tq, hq, heads, d, per_seq * page)
-    workspace = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
+    workspace = q.new_empty((need,), dtype=torch.uint8) if need else None
     _call(device, "ck_mx4_attention", q.data_ptr(), _IN_DTYPE_CODE[q.dtype], q.stride(0), q.stride(1), q.stride(2),
           codes.data_ptr(), scales.data_ptr(), pages, page, block_table.data_ptr(), max(block_table.stride(0), per_seq),
           per_seq, seq_lens.data_ptr(), out.data_ptr(), b, tq, hq, heads, d, group,

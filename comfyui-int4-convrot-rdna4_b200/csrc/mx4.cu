@@ -45,6 +45,7 @@ cudaError_t mx4_take_status(cudaStream_t stream, int* status) {
 #include "mx4_unit.cuh"
 #include "mx4_quant.cuh"
 #include "mx4_gemm.cuh"
+#include "mx4_few.cuh"
 #include "mx4_cache.cuh"
 #include "mx4_attn.cuh"
 
@@ -184,15 +185,53 @@ static int launch_gemm_pair(const void* xc, const void* xs, const void* wc, cons
                                                static_cast<int>(num_tiles), staged));
 }
 
-static int run_gemm(const void* xc, const void* xs, const void* wc, const void* ws, BiasRef bias, void* out, int out_dtype,
-                    int M, int N, int K, cudaStream_t stream) {
-    return with_type(out_dtype, [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        // 256-row pairs of weights where their tiles fill the SM pairs
-        const long long tiles256 = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);
-        if (tiles256 * 2 >= sm_count()) return launch_gemm_pair<256>(xc, xs, wc, ws, bias, static_cast<T*>(out), M, N, K, stream);
-        return launch_gemm_pair<128>(xc, xs, wc, ws, bias, static_cast<T*>(out), M, N, K, stream);
-    });
+// The few-row kernel: K slices so that the blocks fill two a multiprocessor, at
+// most 8 (a cluster), each with two stages of its own at least.
+template <typename T, int G, int BT, bool FUSED>
+static int launch_gemm_few(const void* x, long long ldx, const void* xc, const void* xs, const void* wc, const void* ws,
+                           BiasRef bias, T* out, int M, int N, int K, cudaStream_t stream) {
+    using Cfg = Mx4FewCfg<T, BT, FUSED>;
+    CUtensorMap tx, tw, txs, tws;
+    memset(&tx, 0, sizeof(tx));
+    memset(&txs, 0, sizeof(txs));
+    if (!make_mx4_tmaps(&tw, &tws, wc, ws, N, K, 128, 1) || (!FUSED && !make_mx4_tmaps(&tx, &txs, xc, xs, M, K, BT, 1)))
+        return fail("cuTensorMapEncodeTiled failed (operand size out of range or driver entry point missing)");
+    auto kernel = mx4_gemm_few_kernel<T, G, BT, FUSED>;
+    cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const int tiles = (N + 127) / 128, num_kt = (K + kMx4StageK - 1) / kMx4StageK;
+    const int splits = std::max(1, std::min({2 * sm_count() / tiles, 8, num_kt / 2}));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles, splits, 1);
+    cfg.blockDim = dim3(kMx4FewThreads, 1, 1);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = splits;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = splits > 1 ? 2 : 1;
+    const bool vec = aligned16(x) && ldx * sizeof(T) % 16 == 0;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, tw, tws, tx, txs, static_cast<const T*>(x), ldx, vec,
+                                               bias, out, M, N, K));
+}
+
+// x [M, K] quantized (xc, xs) times the weight; few rows go through the kernel
+// that is bound by the weight's bytes.
+template <typename T>
+static int run_gemm(const void* xc, const void* xs, const void* wc, const void* ws, BiasRef bias, T* out, int M, int N, int K,
+                    cudaStream_t stream) {
+    if (M <= 32) return launch_gemm_few<T, 0, 32, false>(nullptr, 0, xc, xs, wc, ws, bias, out, M, N, K, stream);
+    if (M <= 64) return launch_gemm_few<T, 0, 64, false>(nullptr, 0, xc, xs, wc, ws, bias, out, M, N, K, stream);
+    if (M <= 128) return launch_gemm_few<T, 0, 128, false>(nullptr, 0, xc, xs, wc, ws, bias, out, M, N, K, stream);
+    // 256-row pairs of weights where their tiles fill the SM pairs
+    const long long tiles256 = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);
+    if (tiles256 * 2 >= sm_count()) return launch_gemm_pair<256>(xc, xs, wc, ws, bias, out, M, N, K, stream);
+    return launch_gemm_pair<128>(xc, xs, wc, ws, bias, out, M, N, K, stream);
 }
 
 }  // namespace convrot
@@ -231,28 +270,36 @@ CONVROT_API int ck_mx4_dequant(const void* codes, const void* scales, void* out,
 }
 
 CONVROT_API size_t ck_mx4_linear_workspace_size(int M, int K) {
-    if (M <= 0 || K <= 0) return 0;
+    if (M <= kMx4FusedRows || K <= 0) return 0;
     return align256(static_cast<size_t>(M) * K / 2) + align256(scales_bytes(M, K));
 }
 
-CONVROT_API int ck_mx4_linear(const void* x, int in_dtype, long long ldx, const void* Wcodes, const void* Wscales,
-                              const void* bias, int bias_dtype, void* out, int out_dtype, int M, int N, int K, int G,
-                              void* workspace, size_t workspace_bytes, void* stream) {
+CONVROT_API int ck_mx4_linear(const void* x, int dtype, long long ldx, const void* Wcodes, const void* Wscales,
+                              const void* bias, int bias_dtype, void* out, int M, int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream) {
     if (N < 0) return fail("N must not be negative");
     if (N == 0) return 0;
-    if (int rc = check_matrix(x, in_dtype, Wcodes, Wscales, M, K, G)) return rc;
+    if (int rc = check_matrix(x, dtype, Wcodes, Wscales, M, K, G)) return rc;
     if (M == 0) return 0;
     if (ldx < 0 || (M > 1 && ldx < K)) return fail("ldx must be at least K");
-    if (out_dtype < 0 || out_dtype > 2) return fail("out_dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
     if (bias && (bias_dtype < 0 || bias_dtype > 2)) return fail("bias_dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
     if (!out || !aligned16(out)) return fail("out must be 16-byte aligned");
-    if (!workspace || !aligned_to(workspace, 256)) return fail("the workspace must be 256-byte aligned");
-    if (workspace_bytes < ck_mx4_linear_workspace_size(M, K)) return fail("workspace smaller than ck_mx4_linear_workspace_size");
+    const size_t need = ck_mx4_linear_workspace_size(M, K);
+    if (need && (!workspace || !aligned_to(workspace, 256))) return fail("the workspace must be 256-byte aligned");
+    if (workspace_bytes < need) return fail("workspace smaller than ck_mx4_linear_workspace_size");
     uint8_t* xc = static_cast<uint8_t*>(workspace);
     uint8_t* xs = xc + align256(static_cast<size_t>(M) * K / 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (int rc = run_quant(x, in_dtype, ldx, xc, xs, M, K, G, st)) return rc;
-    return run_gemm(xc, xs, Wcodes, Wscales, BiasRef{bias, bias_dtype}, out, out_dtype, M, N, K, st);
+    const BiasRef b{bias, bias_dtype};
+    if (M > kMx4FusedRows)
+        if (int rc = run_quant(x, dtype, ldx, xc, xs, M, K, G, st)) return rc;
+    return with_type(dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (M > kMx4FusedRows) return run_gemm(xc, xs, Wcodes, Wscales, b, static_cast<T*>(out), M, N, K, st);
+        return with_group(G, [&](auto g) {
+            return launch_gemm_few<T, decltype(g)::value, kMx4FusedRows, true>(x, ldx, nullptr, nullptr, Wcodes, Wscales, b,
+                                                                               static_cast<T*>(out), M, N, K, st);
+        });
+    });
 }
 
 // Calls f with integral constants for the head dimension and the rotation group.

@@ -325,17 +325,18 @@ int ck_mx4_quant(const void* x, int in_dtype, long long ldx, void* codes, void* 
  * back with G != 0; one rounding. */
 int ck_mx4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G, void* stream);
 
-/* Workspace of ck_mx4_linear: the row codes and their scale tiles. */
+/* Workspace of ck_mx4_linear: the row codes and their scale tiles (0, none needed,
+ * up to 16 rows: one kernel quantizes and multiplies). */
 size_t ck_mx4_linear_workspace_size(int M, int K);
 
 /* out[m, n] = sum_k x[m, k] W[n, k] + bias[n]: x [M, K] (row stride ldx) is
  * rotated and quantized into the workspace (256-byte aligned), the weight is
  * given as codes [N, K/2] and scale tiles from ck_mx4_quant with the same G.
- * fp32 accumulation, one rounding. bias [N] or NULL in bias_dtype; out [M, N]
- * 16-byte aligned. Two calls in flight at once need two workspaces. */
-int ck_mx4_linear(const void* x, int in_dtype, long long ldx, const void* Wcodes, const void* Wscales,
-                  const void* bias, int bias_dtype, void* out, int out_dtype, int M, int N, int K, int G,
-                  void* workspace, size_t workspace_bytes, void* stream);
+ * fp32 accumulation, one rounding. bias [N] or NULL in bias_dtype; out [M, N] in
+ * x's dtype, 16-byte aligned. Two calls in flight at once need two workspaces. */
+int ck_mx4_linear(const void* x, int dtype, long long ldx, const void* Wcodes, const void* Wscales,
+                  const void* bias, int bias_dtype, void* out, int M, int N, int K, int G, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 /* Paged key/value cache: codes [pages, 2, heads, page, d/2], scales [pages, 2,
  * heads, page, d/32] (16-byte aligned), keys at index 0, values at 1, both rotated

@@ -93,14 +93,15 @@ def test_c_entries_refuse_before_any_launch(lib):
     refuse(lib, q(16, 1, 64, 16, 16, -1, 64, 64, None), b"negative")
     assert q(0, 1, 64, 0, 0, 0, 64, 64, None) == 0                                   # nothing to do
     lin = lib.ck_mx4_linear
-    need = lib.ck_mx4_linear_workspace_size(4, 64)
-    assert need == 256 + 512
-    refuse(lib, lin(16, 1, 64, 16, 16, 0, 0, 16, 1, 4, 8, 64, 64, 256, need - 1, None), b"workspace")
-    refuse(lib, lin(16, 1, 64, 16, 16, 0, 0, 16, 1, 4, 8, 64, 64, 128, need, None), b"256-byte")
-    refuse(lib, lin(16, 1, 64, 16, 16, 0, 0, 16, 5, 4, 8, 64, 64, 256, need, None), b"out_dtype")
-    refuse(lib, lin(16, 1, 64, 16, 16, 16, 7, 16, 1, 4, 8, 64, 64, 256, need, None), b"bias_dtype")
-    refuse(lib, lin(16, 1, 64, 16, 16, 0, 0, 8, 1, 4, 8, 64, 64, 256, need, None), b"out must")
-    assert lin(16, 1, 64, 16, 16, 0, 0, 16, 1, 4, 0, 64, 64, 256, need, None) == 0
+    assert lib.ck_mx4_linear_workspace_size(16, 64) == 0
+    need = lib.ck_mx4_linear_workspace_size(20, 64)
+    assert need == 768 + 512
+    refuse(lib, lin(16, 1, 64, 16, 16, 0, 0, 16, 20, 8, 64, 64, 256, need - 1, None), b"workspace")
+    refuse(lib, lin(16, 1, 64, 16, 16, 0, 0, 16, 20, 8, 64, 64, 128, need, None), b"256-byte")
+    refuse(lib, lin(16, 1, 64, 16, 16, 16, 7, 16, 4, 8, 64, 64, 0, 0, None), b"bias_dtype")
+    refuse(lib, lin(16, 1, 64, 16, 16, 0, 0, 8, 4, 8, 64, 64, 0, 0, None), b"out must")
+    refuse(lib, lin(16, 1, 63, 16, 16, 0, 0, 16, 4, 8, 64, 64, 0, 0, None), b"ldx")
+    assert lin(16, 1, 64, 16, 16, 0, 0, 16, 4, 0, 64, 64, 0, 0, None) == 0
     app = lib.ck_mx4_cache_append
     refuse(lib, app(16, 16, 4, 2, 96, 16, 0, 16, 16, 1, 1, 1, 1, 1, 16, 3, None), b"head dimension")
     refuse(lib, app(16, 16, 4, 2, 64, 24, 0, 16, 16, 1, 1, 1, 1, 1, 16, 3, None), b"power of two")
