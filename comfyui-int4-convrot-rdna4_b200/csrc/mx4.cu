@@ -185,8 +185,8 @@ static int launch_gemm_pair(const void* xc, const void* xs, const void* wc, cons
                                                static_cast<int>(num_tiles), staged));
 }
 
-// The few-row kernel: K slices so that the blocks fill two a multiprocessor, at
-// most 8 (a cluster), each with two stages of its own at least.
+// The few-row kernel: 1, 2, 4 or 8 slices of K (a cluster), as many as leave the
+// blocks two a multiprocessor and each slice two stages.
 template <typename T, int G, int BT, bool FUSED>
 static int launch_gemm_few(const void* x, long long ldx, const void* xc, const void* xs, const void* wc, const void* ws,
                            BiasRef bias, T* out, int M, int N, int K, cudaStream_t stream) {
@@ -200,7 +200,8 @@ static int launch_gemm_few(const void* x, long long ldx, const void* xc, const v
     cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int tiles = (N + 127) / 128, num_kt = (K + kMx4StageK - 1) / kMx4StageK;
-    const int splits = std::max(1, std::min({2 * sm_count() / tiles, 8, num_kt / 2}));
+    int splits = 1;
+    while (splits < 8 && 2 * splits * tiles <= 2 * sm_count() && 4 * splits <= num_kt) splits *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles, splits, 1);
     cfg.blockDim = dim3(kMx4FewThreads, 1, 1);

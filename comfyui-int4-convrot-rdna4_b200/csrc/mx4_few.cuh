@@ -27,7 +27,7 @@ struct Mx4FewCfg {
     static constexpr int kBBytes = BT * kMx4StageK / 2;
     static constexpr int kScaleBytes = 2 * kMx4TileBytes;         // of each operand
     static constexpr int kStageBytes = (kABytes + kBBytes + 2 * kScaleBytes + 1023) / 1024 * 1024;
-    static constexpr int kStages = BT == 128 ? 3 : 4;
+    static constexpr int kStages = BT == 128 || FUSED ? 3 : 4;    // two blocks a multiprocessor (fp32 rows: one)
     static constexpr int kSlabBytes = FUSED ? 4 * Mx4Slab<T>::kBytes : 0;
     static constexpr int kSlabOffset = kStages * kStageBytes;
     static constexpr int kBarOffset = kSlabOffset + kSlabBytes;
@@ -38,10 +38,59 @@ struct Mx4FewCfg {
     static_assert(BT * 128 * 4 <= kStages * kStageBytes, "the accumulators fit the ring");
 };
 
-__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-    return v;
+__device__ __forceinline__ void tmem_ld_32x32b_x16_wait(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr) : "memory");
+}
+
+// Adds the S ranks' accumulators [token][128] of this rank's tokens (rank, rank + S,
+// ..), in rank order. A warp a token, a lane four outputs; eight loads are under way
+// before the first is used.
+template <typename T, int S>
+__device__ __forceinline__ void few_reduce(unsigned char* smem, int rank, const BiasRef& bias, T* out, int n0, int M, int N) {
+    constexpr int kBatch = 8 / S;                                 // tokens of a batch
+    const int t = static_cast<int>(threadIdx.x) - 64, n = n0 + (t & 31) * 4;
+    const uint32_t red = smem_u32(smem) + (t & 31) * 16;
+    uint32_t at[S];
+    #pragma unroll
+    for (int r = 0; r < S; ++r) at[r] = mapa_shared(red, r);
+    float b[4];
+    #pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = bias.ptr != nullptr && n + e < N ? bias.at(n + e) : 0.0f;
+    for (int m0 = rank + (t >> 5) * S; m0 < M; m0 += 4 * S * kBatch) {
+        float4 v[kBatch][S];
+        #pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int m = min(m0 + 4 * S * i, M - 1);             // (a token beyond the last: read, not written)
+            #pragma unroll
+            for (int r = 0; r < S; ++r) v[i][r] = ld_shared_cluster_f4(at[r] + m * 512);
+        }
+        #pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int m = m0 + 4 * S * i;
+            float4 sum = v[i][0];
+            #pragma unroll
+            for (int r = 1; r < S; ++r) {
+                sum.x += v[i][r].x;
+                sum.y += v[i][r].y;
+                sum.z += v[i][r].z;
+                sum.w += v[i][r].w;
+            }
+            const T o[4] = {mx4_from_f32<T>(sum.x + b[0]), mx4_from_f32<T>(sum.y + b[1]), mx4_from_f32<T>(sum.z + b[2]), mx4_from_f32<T>(sum.w + b[3])};
+            if (m >= M) break;
+            T* dst = out + static_cast<size_t>(m) * N + n;
+            if (N % 4 == 0 && n < N) {
+                memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), o, 4 * sizeof(T));
+            } else {
+                #pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < N) dst[e] = o[e];
+            }
+        }
+    }
 }
 
 template <typename T, int G, int BT, bool FUSED>
@@ -51,6 +100,7 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     const T* __restrict__ x, long long ldx, bool vec, BiasRef bias,
                     T* __restrict__ out, int M, int N, int K) {
     using Cfg = Mx4FewCfg<T, BT, FUSED>;
+    constexpr int kLd = BT < 32 ? 16 : 32;                        // accumulator columns read at a time
     extern __shared__ __align__(1024) unsigned char mx4few_raw[];
     unsigned char* smem = mx4few_raw + ((1024u - (smem_u32(mx4few_raw) & 1023u)) & 1023u);
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);
@@ -191,23 +241,29 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         tc_fence_after();
         const float b = bias.ptr != nullptr && n < N ? bias.at(n) : 0.0f;
         #pragma unroll 1
-        for (int c = 0; c < BT && c < M; c += 16) {
-            uint32_t v[16];
+        for (int c = 0; c < BT && c < M; c += kLd) {
+            uint32_t v[kLd];
             if (kts > 0) {
-                asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                             "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
-                             : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                               "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                             : "r"(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c) : "memory");
+                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c;
+                if constexpr (kLd == 32) {
+                    tmem_ld_32x32b_x32(at, v);
+                    tmem_ld_wait_regs(v);
+                } else {
+                    tmem_ld_32x32b_x16_wait(at, v);
+                }
             } else {
                 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = 0u;
+                for (int e = 0; e < kLd; ++e) v[e] = 0u;
             }
-            #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                if (c + e >= M) break;
-                if (splits > 1) red[(c + e) * 128 + quarter * 32 + lane] = __uint_as_float(v[e]);
-                else if (n < N) out[static_cast<size_t>(c + e) * N + n] = mx4_from_f32<T>(__uint_as_float(v[e]) + b);
+            if (splits > 1) {
+                // (columns beyond M too: the ring holds all BT)
+                #pragma unroll
+                for (int e = 0; e < kLd; ++e) red[(c + e) * 128 + quarter * 32 + lane] = __uint_as_float(v[e]);
+            } else if (n < N) {
+                T* dst = out + static_cast<size_t>(c) * N + n;
+                #pragma unroll
+                for (int e = 0; e < kLd; ++e)
+                    if (c + e < M) dst[static_cast<size_t>(e) * N] = mx4_from_f32<T>(__uint_as_float(v[e]) + b);
             }
         }
         tc_fence_before();
@@ -215,14 +271,9 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     if (splits > 1) {
         cluster_sync();                                           // every block's accumulators are in its shared memory
         if (warp >= 2) {
-            const int quarter = warp & 3, i = quarter * 32 + lane, n = n0 + i;
-            const float b = bias.ptr != nullptr && n < N ? bias.at(n) : 0.0f;
-            const uint32_t red = smem_u32(smem);
-            for (int m = rank; m < M; m += splits) {
-                float sum = 0.0f;
-                for (int r = 0; r < splits; ++r) sum += ld_shared_cluster_f32(mapa_shared(red + (m * 128 + i) * 4, r));
-                if (n < N) out[static_cast<size_t>(m) * N + n] = mx4_from_f32<T>(sum + b);
-            }
+            if (splits == 2) few_reduce<T, 2>(smem, rank, bias, out, n0, M, N);
+            else if (splits == 4) few_reduce<T, 4>(smem, rank, bias, out, n0, M, N);
+            else few_reduce<T, 8>(smem, rank, bias, out, n0, M, N);
         }
         cluster_sync();                                           // no block leaves while others read its memory
     } else {
