@@ -190,7 +190,7 @@ static int launch_gemm_pair(const void* xc, const void* xs, const void* wc, cons
 template <typename T, int G, int BT, bool FUSED>
 static int launch_gemm_few(const void* x, long long ldx, const void* xc, const void* xs, const void* wc, const void* ws,
                            BiasRef bias, T* out, int M, int N, int K, cudaStream_t stream) {
-    using Cfg = Mx4FewCfg<T, BT, FUSED>;
+    using Cfg = Mx4FewCfg<BT, FUSED>;
     CUtensorMap tx, tw, txs, tws;
     memset(&tx, 0, sizeof(tx));
     memset(&txs, 0, sizeof(txs));
@@ -297,7 +297,7 @@ CONVROT_API int ck_mx4_linear(const void* x, int dtype, long long ldx, const voi
         using T = std::remove_pointer_t<decltype(t)>;
         if (M > kMx4FusedRows) return run_gemm(xc, xs, Wcodes, Wscales, b, static_cast<T*>(out), M, N, K, st);
         return with_group(G, [&](auto g) {
-            return launch_gemm_few<T, decltype(g)::value, kMx4FusedRows, true>(x, ldx, nullptr, nullptr, Wcodes, Wscales, b,
+            return launch_gemm_few<T, decltype(g)::value, 16, true>(x, ldx, nullptr, nullptr, Wcodes, Wscales, b,
                                                                                static_cast<T*>(out), M, N, K, st);
         });
     });

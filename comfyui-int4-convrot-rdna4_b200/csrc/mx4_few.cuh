@@ -3,40 +3,53 @@
 // Included by mx4.cu. The weight takes the tensor core's side of 128 rows and the
 // tokens the other (BT = 16, 32, 64 or 128 columns), so a block streams 128 weight
 // rows and multiplies them with all tokens. The blocks of a cluster take slices of
-// K of one tile (few weight rows then still fill the machine) and add their fp32
-// accumulators over distributed shared memory, in rank order.
+// K of one tile (few weight rows then still fill the machine) and send each other
+// their fp32 accumulators over distributed shared memory: each rank adds those of
+// its own tokens, in rank order.
 //
-// FUSED (up to 16 rows): the activations are rotated and quantized here, by the
-// epilogue's warps while the weight is on its way, a stage (256 columns of 16
-// rows: 32 units, a lane each) by one warp. Every block quantizes its slice of K
-// again, which for 16 rows costs less than a launch and a pass through memory.
+// FUSED (up to 8 rows): the activations are rotated and quantized here, by the
+// epilogue's warps while the weight is on its way, a stage (256 columns) by one
+// warp. Every block quantizes its slice of K again, which for few rows costs less
+// than a launch and a pass through memory (15360 x 3840: 1 row 7.1 us, 8 rows 9.8 us;
+// 16 rows would take 14.6 us, with a kernel of its own 11.0 us). A lane takes 16
+// columns of two rows: short code and a short wait (128 columns a lane, as in
+// mx4_unit.cuh, took 2.8 us to the first stage, most of it the first run through its
+// instructions).
 //
-// Warp roles (6 warps, so that two blocks' registers fit a multiprocessor): w0 TMA
-// producer (one lane), w1 tensor memory and MMA issue, w2..w5 quantizers (FUSED) and
-// epilogue (TMEM lanes 32 * (w % 4) ..).
+// Warp roles (6 warps, so that two blocks fit a multiprocessor): w0 TMA producer
+// (one lane), w1 tensor memory and MMA issue, w2..w5 quantizers (FUSED) and epilogue
+// (TMEM lanes 32 * (w % 4) ..).
 #pragma once
 
 namespace convrot {
 
 constexpr int kMx4FewThreads = 192;
-constexpr int kMx4FusedRows = 16;              // rows up to which the kernel quantizes them itself
+constexpr int kMx4FusedRows = 8;               // rows up to which the kernel quantizes them itself
 
-template <typename T, int BT, bool FUSED>
+template <int BT, bool FUSED>
 struct Mx4FewCfg {
     static constexpr int kABytes = 128 * kMx4StageK / 2;
     static constexpr int kBBytes = BT * kMx4StageK / 2;
     static constexpr int kScaleBytes = 2 * kMx4TileBytes;         // of each operand
-    static constexpr int kStageBytes = (kABytes + kBBytes + 2 * kScaleBytes + 1023) / 1024 * 1024;
-    static constexpr int kStages = BT == 128 || FUSED ? 3 : 4;    // two blocks a multiprocessor (fp32 rows: one)
-    static constexpr int kSlabBytes = FUSED ? 4 * Mx4Slab<T>::kBytes : 0;
-    static constexpr int kSlabOffset = kStages * kStageBytes;
-    static constexpr int kBarOffset = kSlabOffset + kSlabBytes;
+    static constexpr int kStageBytes = kABytes + kBBytes + 2 * kScaleBytes;
+    // the ranks' accumulators of this rank's tokens: memory of its own where it is
+    // small, else the ring's (after a barrier that says the ring is free everywhere)
+    static constexpr bool kOwnInbox = BT <= 32;
+    static constexpr int kInboxBytes = BT * 128 * 4;
+    static constexpr int kStages = BT == 128 ? 3 : 4;             // two blocks a multiprocessor
+    static constexpr int kInboxOffset = kOwnInbox ? kStages * kStageBytes : 0;
+    static constexpr int kBarOffset = kStages * kStageBytes + (kOwnInbox ? kInboxBytes : 0);
     static constexpr int kSmemBytes = kBarOffset + 256 + 1024;
     static constexpr int kScaleCol = BT;                          // two buffers of 8 + 8 columns after the accumulator
-    static constexpr int kTmemCols = BT == 16 ? 64 : BT == 32 ? 64 : BT == 64 ? 128 : 256;
+    static constexpr int kTmemCols = BT <= 32 ? 64 : BT == 64 ? 128 : 256;
+    static_assert(kStageBytes % 1024 == 0, "operand tiles are 1024-byte aligned");
     static_assert(kScaleCol + 32 <= kTmemCols, "tensor memory");
-    static_assert(BT * 128 * 4 <= kStages * kStageBytes, "the accumulators fit the ring");
+    static_assert(kInboxBytes <= kStages * kStageBytes, "the accumulators fit the ring");
 };
+
+__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(cluster_addr), "f"(v) : "memory");
+}
 
 __device__ __forceinline__ void tmem_ld_32x32b_x16_wait(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -46,50 +59,148 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16_wait(uint32_t taddr, uint32_t
                  : "r"(taddr) : "memory");
 }
 
-// Adds the S ranks' accumulators [token][128] of this rank's tokens (rank, rank + S,
-// ..), in rank order. A warp a token, a lane four outputs; eight loads are under way
-// before the first is used.
-template <typename T, int S>
-__device__ __forceinline__ void few_reduce(unsigned char* smem, int rank, const BiasRef& bias, T* out, int n0, int M, int N) {
-    constexpr int kBatch = 8 / S;                                 // tokens of a batch
-    const int t = static_cast<int>(threadIdx.x) - 64, n = n0 + (t & 31) * 4;
-    const uint32_t red = smem_u32(smem) + (t & 31) * 16;
+// 16 accumulator columns from c on (zeros without any stage).
+__device__ __forceinline__ void few_load(uint32_t tmem, int quarter, int c, bool held, uint32_t (&v)[16]) {
+    if (held) {
+        tmem_ld_32x32b_x16_wait(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, v);
+    } else {
+        #pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = 0u;
+    }
+}
+
+// Sends this rank's accumulators to the tokens' owners (token m: rank m % S), into
+// their inboxes [rank][token of the owner][128].
+template <int S, int BT>
+__device__ __forceinline__ void few_send(uint32_t inbox, uint32_t tmem, int rank, int M, bool held) {
+    const int quarter = (threadIdx.x >> 5) & 3, i = quarter * 32 + (threadIdx.x & 31);
     uint32_t at[S];
     #pragma unroll
-    for (int r = 0; r < S; ++r) at[r] = mapa_shared(red, r);
+    for (int r = 0; r < S; ++r) at[r] = mapa_shared(inbox + (rank * (BT / S) * 128 + i) * 4, r);
+    #pragma unroll 1
+    for (int c = 0; c < M; c += 16) {
+        uint32_t v[16];
+        few_load(tmem, quarter, c, held, v);
+        #pragma unroll
+        for (int e = 0; e < 16; ++e)                              // (columns beyond M too: the inbox holds all BT)
+            st_shared_cluster_f32(at[e % S] + (c / S + e / S) * 512, __uint_as_float(v[e]));
+    }
+}
+
+// Adds the ranks' accumulators of this rank's tokens. A warp a token, a lane four
+// outputs.
+template <typename T, int S, int BT>
+__device__ __forceinline__ void few_reduce(const unsigned char* inbox, int rank, const BiasRef& bias, T* out, int n0, int M, int N) {
+    const int t = static_cast<int>(threadIdx.x) - 64, n = n0 + (t & 31) * 4;
     float b[4];
     #pragma unroll
     for (int e = 0; e < 4; ++e) b[e] = bias.ptr != nullptr && n + e < N ? bias.at(n + e) : 0.0f;
-    for (int m0 = rank + (t >> 5) * S; m0 < M; m0 += 4 * S * kBatch) {
-        float4 v[kBatch][S];
+    #pragma unroll 2
+    for (int j = t >> 5; j * S + rank < M; j += 4) {
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int m = min(m0 + 4 * S * i, M - 1);             // (a token beyond the last: read, not written)
-            #pragma unroll
-            for (int r = 0; r < S; ++r) v[i][r] = ld_shared_cluster_f4(at[r] + m * 512);
+        for (int r = 0; r < S; ++r) {
+            const float4 v = *reinterpret_cast<const float4*>(inbox + (r * (BT / S) + j) * 512 + (t & 31) * 16);
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
         }
+        const T o[4] = {mx4_from_f32<T>(sum.x + b[0]), mx4_from_f32<T>(sum.y + b[1]), mx4_from_f32<T>(sum.z + b[2]), mx4_from_f32<T>(sum.w + b[3])};
+        T* dst = out + static_cast<size_t>(j * S + rank) * N + n;
+        if (N % 4 == 0 && n < N) {
+            memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), o, 4 * sizeof(T));
+        } else {
+            #pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < N) dst[e] = o[e];
+        }
+    }
+}
+
+// 16 columns of x as loaded, and as floats.
+template <typename T> struct Few16 { uint4 v[sizeof(T)]; };
+
+template <typename T>
+__device__ __forceinline__ Few16<T> load16(const T* src, bool held, bool vec) {
+    Few16<T> w;
+    #pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) w.v[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (held && vec) {
         #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int m = m0 + 4 * S * i;
-            float4 sum = v[i][0];
-            #pragma unroll
-            for (int r = 1; r < S; ++r) {
-                sum.x += v[i][r].x;
-                sum.y += v[i][r].y;
-                sum.z += v[i][r].z;
-                sum.w += v[i][r].w;
-            }
-            const T o[4] = {mx4_from_f32<T>(sum.x + b[0]), mx4_from_f32<T>(sum.y + b[1]), mx4_from_f32<T>(sum.z + b[2]), mx4_from_f32<T>(sum.w + b[3])};
-            if (m >= M) break;
-            T* dst = out + static_cast<size_t>(m) * N + n;
-            if (N % 4 == 0 && n < N) {
-                memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), o, 4 * sizeof(T));
-            } else {
-                #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n + e < N) dst[e] = o[e];
-            }
+        for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) w.v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    } else if (held) {
+        T e[16];
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) e[i] = src[i];
+        memcpy(&w, e, sizeof(w));
+    }
+    return w;
+}
+
+template <typename T>
+__device__ __forceinline__ void to_floats(const Few16<T>& w, float (&f)[16]) {
+    T e[16];
+    memcpy(e, &w, sizeof(w));
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = mx4_to_f32(e[i]);
+}
+
+// One radix-4 step over lanes whose bits `bit` and 2 * bit number the four values:
+// (v0 + v1) + (v2 + v3) - 2 v_(3-i) in every lane.
+__device__ __forceinline__ float2 h4_lanes(float2 v, int bit) {
+    const float2 o = make_float2(__shfl_xor_sync(0xFFFFFFFFu, v.x, bit), __shfl_xor_sync(0xFFFFFFFFu, v.y, bit));
+    const float2 p = fadd2_rn(v, o);
+    const float2 q = make_float2(__shfl_xor_sync(0xFFFFFFFFu, p.x, 2 * bit), __shfl_xor_sync(0xFFFFFFFFu, p.y, 2 * bit));
+    const float2 w = make_float2(__shfl_xor_sync(0xFFFFFFFFu, v.x, 3 * bit), __shfl_xor_sync(0xFFFFFFFFu, v.y, 3 * bit));
+    return ffma2_rn(make_float2(-2.0f, -2.0f), w, fadd2_rn(p, q));
+}
+
+// Rotates and quantizes rows r and r + 1 (component x and y) of a stage; lane % 16
+// has columns 16 (lane % 16) ... Writes codes (128-byte swizzle) and scale bytes.
+template <int G>
+__device__ __forceinline__ void few_quantize(float2 (&v)[16], int r, unsigned char* codes, unsigned char* scales) {
+    const int a = threadIdx.x & 15;
+    if constexpr (G >= 16) {
+        #pragma unroll
+        for (int i = 0; i < 16; i += 4) h4_pair(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) h4_pair(v[i], v[i + 4], v[i + 8], v[i + 12]);
+    }
+    if constexpr (G >= 64) {
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = h4_lanes(v[i], 1);
+    }
+    if constexpr (G == 256) {
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = h4_lanes(v[i], 4);
+    }
+    float mx = 0.0f, my = 0.0f;
+    #pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        mx = max3_abs_nan(mx, v[i].x, v[i + 1].x);
+        my = max3_abs_nan(my, v[i].y, v[i + 1].y);
+    }
+    // a block is two lanes
+    mx = max3_abs_nan(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1), 0.0f) * unit_factor<G>();
+    my = max3_abs_nan(my, __shfl_xor_sync(0xFFFFFFFFu, my, 1), 0.0f) * unit_factor<G>();
+    const uint32_t ex = mx4_scale_byte(mx), ey = mx4_scale_byte(my);
+    const float2 inv = make_float2(mx4_inv_scale(ex) * unit_factor<G>(), mx4_inv_scale(ey) * unit_factor<G>());
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = fmul2_rn(v[i], inv);
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = r + h;
+        uint2 w;
+        if (h == 0) {
+            w.x = mx4_encode8(v[0].x, v[1].x, v[2].x, v[3].x, v[4].x, v[5].x, v[6].x, v[7].x);
+            w.y = mx4_encode8(v[8].x, v[9].x, v[10].x, v[11].x, v[12].x, v[13].x, v[14].x, v[15].x);
+        } else {
+            w.x = mx4_encode8(v[0].y, v[1].y, v[2].y, v[3].y, v[4].y, v[5].y, v[6].y, v[7].y);
+            w.y = mx4_encode8(v[8].y, v[9].y, v[10].y, v[11].y, v[12].y, v[13].y, v[14].y, v[15].y);
         }
+        *reinterpret_cast<uint2*>(codes + row * 128 + (((a >> 1) ^ (row & 7)) << 4) + (a & 1) * 8) = w;
+        if (!(a & 1)) scales[(a >> 3) * kMx4TileBytes + row * 16 + ((a >> 1) & 3)] = static_cast<uint8_t>(h ? ey : ex);
     }
 }
 
@@ -97,10 +208,8 @@ template <typename T, int G, int BT, bool FUSED>
 __global__ void __launch_bounds__(kMx4FewThreads, 2)
 mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_ws,
                     const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_xs,
-                    const T* __restrict__ x, long long ldx, bool vec, BiasRef bias,
-                    T* __restrict__ out, int M, int N, int K) {
-    using Cfg = Mx4FewCfg<T, BT, FUSED>;
-    constexpr int kLd = BT < 32 ? 16 : 32;                        // accumulator columns read at a time
+                    const T* __restrict__ x, long long ldx, bool vec, BiasRef bias, T* __restrict__ out, int M, int N, int K) {
+    using Cfg = Mx4FewCfg<BT, FUSED>;
     extern __shared__ __align__(1024) unsigned char mx4few_raw[];
     unsigned char* smem = mx4few_raw + ((1024u - (smem_u32(mx4few_raw) & 1023u)) & 1023u);
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);
@@ -128,8 +237,10 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         tmem_alloc(tmem_slot, Cfg::kTmemCols);
         tmem_relinquish();
     }
-    // the first weight boxes into L2 (a hint: safe whatever the previous kernel wrote)
-    if (warp == 2 && lane < Cfg::kStages && lane < kts) tma_prefetch_l2_2d(&tmap_w, (kt0 + lane) * (kMx4StageK / 2), n0);
+    // this block's weights into L2 (a hint: safe whatever the previous kernel wrote), so
+    // that what the ring does not hold yet is nearer when the first tokens are ready
+    if (warp == 2)
+        for (int it = lane; it < kts; it += 32) tma_prefetch_l2_2d(&tmap_w, (kt0 + it) * (kMx4StageK / 2), n0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -196,89 +307,82 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         }
         if (ok && kts > 0 && elect_one()) mma_commit(acc_bar);
         __syncwarp();
-    } else if (FUSED && warp >= 2) {
-        // ---------------- quantizers: stages in turn, a lane a unit (row lane / 2, half lane & 1)
-        unsigned char* slab = smem + Cfg::kSlabOffset + (warp - 2) * Mx4Slab<T>::kBytes;
-        auto load = [&](int it) {
-            const int row = lane >> 1, k = (kt0 + it) * kMx4StageK + (lane & 1) * kMx4Unit;
-            const int cols = row < M ? max(0, min(kMx4Unit, K - k)) : 0;
-            slab_load<false>(slab, Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(cols ? x + row * ldx + k : x), cols / Mx4Slab<T>::kPer}, 0, vec);
-            cp_async_commit();
-        };
-        if (warp - 2 < kts) load(warp - 2);
-        for (int it = warp - 2; it < kts; it += 4) {
-            const int s = it % Cfg::kStages;
-            cp_async_wait<0>();
-            __syncwarp();
-            float2 v[64];
-            slab_to_unit<T>(slab, v);
-            __syncwarp();
-            if (it + 4 < kts) load(it + 4);
-            unit_rotate<G>(v);
-            uint4 q[4];
-            const uint32_t word = unit_quantize(v, unit_factor<G>(), q);
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1))) {
-                if (lane == 0) mx4_record_status(kMx4TimeoutProducer);
-                break;
+    } else {
+        if constexpr (FUSED) {
+            // ---------------- quantizers: stages in turn, four rows a pass; the next pass's
+            // columns are on their way meanwhile
+            const int r0 = 2 * (lane >> 4), col = (lane & 15) * 16;
+            Few16<T> nx, ny;
+            auto fetch = [&](int it, int p) {
+                const int r = p + r0, k = (kt0 + it) * kMx4StageK + col;
+                nx = load16(x + r * ldx + k, it < kts && r < M && k < K, vec);
+                ny = load16(x + (r + 1) * ldx + k, it < kts && r + 1 < M && k < K, vec);
+            };
+            fetch(warp - 2, 0);
+            for (int it = warp - 2; it < kts; it += 4) {
+                const int s = it % Cfg::kStages;
+                unsigned char* b = smem + s * Cfg::kStageBytes + Cfg::kABytes;
+                bool ok = true;
+                #pragma unroll 1
+                for (int p = 0; p < M; p += 4) {
+                    float fx[16], fy[16];
+                    to_floats(nx, fx);
+                    to_floats(ny, fy);
+                    if (p + 4 < M) fetch(it, p + 4);
+                    else fetch(it + 4, 0);
+                    float2 v[16];
+                    #pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = make_float2(fx[i], fy[i]);
+                    // (the slot is free once the MMAs of its last stage are done)
+                    if (p == 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1));
+                    if (!ok) break;
+                    few_quantize<G>(v, p + r0, b, b + Cfg::kBBytes + Cfg::kScaleBytes);
+                }
+                if (!ok) {
+                    if (lane == 0) mx4_record_status(kMx4TimeoutProducer);
+                    break;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ready_bar[s]);
             }
-            const int u = lane ^ (G == 256 ? 1 : 0), row = u >> 1, half = u & 1;
-            unsigned char* b = smem + s * Cfg::kStageBytes + Cfg::kABytes;
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(b + row * 128 + (((4 * half + i) ^ (row & 7)) << 4)) = q[i];
-            *reinterpret_cast<uint32_t*>(b + Cfg::kBBytes + Cfg::kScaleBytes + half * kMx4TileBytes + row * 16) = word;
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ready_bar[s]);
         }
-        cp_async_wait<0>();
-    }
-    if (warp >= 2) {
-        // ---------------- epilogue: lane n0 + 32 q + lane, a column a token
-        const int quarter = warp & 3, n = n0 + quarter * 32 + lane;
-        float* red = reinterpret_cast<float*>(smem);              // [BT][128], in the ring's place
+        // ---------------- accumulators: lane n0 + 32 q + lane, a column a token
         const bool ok = kts == 0 || __all_sync(0xFFFFFFFFu, mbar_wait_bounded(acc_bar, 0));
         if (!ok && lane == 0) mx4_record_status(kMx4TimeoutEpilogue);
         tc_fence_after();
-        const float b = bias.ptr != nullptr && n < N ? bias.at(n) : 0.0f;
-        #pragma unroll 1
-        for (int c = 0; c < BT && c < M; c += kLd) {
-            uint32_t v[kLd];
-            if (kts > 0) {
-                const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c;
-                if constexpr (kLd == 32) {
-                    tmem_ld_32x32b_x32(at, v);
-                    tmem_ld_wait_regs(v);
-                } else {
-                    tmem_ld_32x32b_x16_wait(at, v);
-                }
-            } else {
-                #pragma unroll
-                for (int e = 0; e < kLd; ++e) v[e] = 0u;
-            }
-            if (splits > 1) {
-                // (columns beyond M too: the ring holds all BT)
-                #pragma unroll
-                for (int e = 0; e < kLd; ++e) red[(c + e) * 128 + quarter * 32 + lane] = __uint_as_float(v[e]);
-            } else if (n < N) {
+        if (splits == 1) {
+            const int quarter = warp & 3, n = n0 + quarter * 32 + lane;
+            const float b = bias.ptr != nullptr && n < N ? bias.at(n) : 0.0f;
+            #pragma unroll 1
+            for (int c = 0; c < M; c += 16) {
+                uint32_t v[16];
+                few_load(tmem, quarter, c, kts > 0, v);
                 T* dst = out + static_cast<size_t>(c) * N + n;
                 #pragma unroll
-                for (int e = 0; e < kLd; ++e)
-                    if (c + e < M) dst[static_cast<size_t>(e) * N] = mx4_from_f32<T>(__uint_as_float(v[e]) + b);
+                for (int e = 0; e < 16; ++e)
+                    if (c + e < M && n < N) dst[static_cast<size_t>(e) * N] = mx4_from_f32<T>(__uint_as_float(v[e]) + b);
             }
         }
-        tc_fence_before();
     }
     if (splits > 1) {
-        cluster_sync();                                           // every block's accumulators are in its shared memory
+        unsigned char* inbox = smem + Cfg::kInboxOffset;
+        if (!Cfg::kOwnInbox) cluster_sync();                      // every rank's ring is free
         if (warp >= 2) {
-            if (splits == 2) few_reduce<T, 2>(smem, rank, bias, out, n0, M, N);
-            else if (splits == 4) few_reduce<T, 4>(smem, rank, bias, out, n0, M, N);
-            else few_reduce<T, 8>(smem, rank, bias, out, n0, M, N);
+            const uint32_t to = smem_u32(inbox);
+            if (splits == 2) few_send<2, BT>(to, tmem, rank, M, kts > 0);
+            else if (splits == 4) few_send<4, BT>(to, tmem, rank, M, kts > 0);
+            else few_send<8, BT>(to, tmem, rank, M, kts > 0);
         }
-        cluster_sync();                                           // no block leaves while others read its memory
-    } else {
-        __syncthreads();
+        cluster_sync();                                           // all inboxes are filled
+        if (warp >= 2) {
+            if (splits == 2) few_reduce<T, 2, BT>(inbox, rank, bias, out, n0, M, N);
+            else if (splits == 4) few_reduce<T, 4, BT>(inbox, rank, bias, out, n0, M, N);
+            else few_reduce<T, 8, BT>(inbox, rank, bias, out, n0, M, N);
+        }
     }
+    tc_fence_before();
+    __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, Cfg::kTmemCols);

@@ -160,7 +160,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
                 // the tile before this one shares columns with it (kShared), else the
                 // one before that used this accumulator
                 const int before = Cfg::kShared ? lt - 1 : lt - 2;
-                if (before >= 0 && !__all_sync(0xFFFFFFFFu, mbar_wait_bounded<true>(&acc_free[before & 1], (before >> 1) & 1))) {
+                if (before >= 0 && !__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&acc_free[before & 1], (before >> 1) & 1))) {
                     if (lane == 0) mx4_record_status(kMx4TimeoutMma);
                     break;
                 }
@@ -217,7 +217,7 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
             float* bc = bias_cols + (lt & 1) * BN;
             for (int c = et; c < BN; c += 128) bc[c] = bias.ptr != nullptr && n0 + c < N ? bias.at(n0 + c) : 0.0f;
             named_barrier_sync(1, 128);
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded<true>(&acc_full[lt & 1], (lt >> 1) & 1))) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&acc_full[lt & 1], (lt >> 1) & 1))) {
                 if (lane == 0) mx4_record_status(kMx4TimeoutEpilogue);
                 break;
             }
@@ -237,12 +237,14 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
                 tmem_ld_wait_regs(*reinterpret_cast<uint32_t (*)[32]>(v));
                 if constexpr (kCols == 64) tmem_ld_wait_regs(*reinterpret_cast<uint32_t (*)[32]>(v + 32));
                 if (i == (kSharedSteps ? kSharedSteps : kSteps) - 1) {
-                    // read: hand the shared columns (BN = 128: the accumulator) over
+                    // read: hand the shared columns (BN = 128: the accumulator) over. The values are
+                    // in registers, so the arrival orders nothing in memory: CTA scope, as a
+                    // cluster-scope release waits for the stores under way
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
                         if (cta == 0) mbar_arrive(&acc_free[lt & 1]);
-                        else mbar_arrive_cluster(free_leader + (lt & 1) * 8);
+                        else mbar_arrive_remote_cta(free_leader + (lt & 1) * 8);
                     }
                 }
                 const int n = n0 + col;

@@ -326,7 +326,7 @@ int ck_mx4_quant(const void* x, int in_dtype, long long ldx, void* codes, void* 
 int ck_mx4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G, void* stream);
 
 /* Workspace of ck_mx4_linear: the row codes and their scale tiles (0, none needed,
- * up to 16 rows: one kernel quantizes and multiplies). */
+ * up to 8 rows: one kernel quantizes and multiplies). */
 size_t ck_mx4_linear_workspace_size(int M, int K);
 
 /* out[m, n] = sum_k x[m, k] W[n, k] + bias[n]: x [M, K] (row stride ldx) is

@@ -93,7 +93,7 @@ def test_c_entries_refuse_before_any_launch(lib):
     refuse(lib, q(16, 1, 64, 16, 16, -1, 64, 64, None), b"negative")
     assert q(0, 1, 64, 0, 0, 0, 64, 64, None) == 0                                   # nothing to do
     lin = lib.ck_mx4_linear
-    assert lib.ck_mx4_linear_workspace_size(16, 64) == 0
+    assert lib.ck_mx4_linear_workspace_size(8, 64) == 0
     need = lib.ck_mx4_linear_workspace_size(20, 64)
     assert need == 768 + 512
     refuse(lib, lin(16, 1, 64, 16, 16, 0, 0, 16, 20, 8, 64, 64, 256, need - 1, None), b"workspace")
