@@ -249,17 +249,17 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ---------------- TMA producer
-            for (int it = 0; it < kts; ++it) {
-                const int s = it % Cfg::kStages;
-                if (!mbar_wait_bounded(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1)) {
-                    mx4_record_status(kMx4TimeoutProducer);
-                    break;
-                }
-                unsigned char* st = smem + s * Cfg::kStageBytes;
-                unsigned char* sf = st + Cfg::kABytes + Cfg::kBBytes;
-                const int kt = kt0 + it;
+        // ---------------- TMA producer: the warp runs the loop, one elected lane issues
+        for (int it = 0; it < kts; ++it) {
+            const int s = it % Cfg::kStages;
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1))) {
+                if (lane == 0) mx4_record_status(kMx4TimeoutProducer);
+                break;
+            }
+            unsigned char* st = smem + s * Cfg::kStageBytes;
+            unsigned char* sf = st + Cfg::kABytes + Cfg::kBBytes;
+            const int kt = kt0 + it;
+            if (elect_one()) {
                 mbar_arrive_expect_tx(&full_bar[s], Cfg::kABytes + Cfg::kScaleBytes + (FUSED ? 0 : Cfg::kBBytes + Cfg::kScaleBytes));
                 tma_load_2d(st, &tmap_w, &full_bar[s], kt * (kMx4StageK / 2), n0);
                 tma_load_2d(sf, &tmap_ws, &full_bar[s], kt * 256, n0 / 128);
@@ -268,6 +268,7 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     tma_load_2d(sf + Cfg::kScaleBytes, &tmap_xs, &full_bar[s], kt * 256, 0);
                 }
             }
+            __syncwarp();
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer: the warp runs the loop, one elected lane issues

@@ -11,7 +11,7 @@
 // 128 B | x scales: two tiles | w scales: two tiles for each 128 rows].
 //
 // Warp roles (8 warps, both CTAs alike):
-//   w0       TMA producer (one lane)
+//   w0, w2   TMA producers: codes, scales
 //   w1       TMEM allocation; in the even CTA the MMA issuer
 //   w4..w7   epilogue (TMEM lanes 32 * (w % 4) ..): fp32 + bias, one rounding, a
 //            warp's 32 rows x 128 bytes at a time through shared memory and TMA
@@ -124,31 +124,38 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
     griddep_launch_dependents();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            // ---------------- TMA producer: both CTAs' tiles complete on the even CTA's barrier
-            int it = 0;
-            bool ok = true;
-            for (int t = cluster_id; t < num_tiles && ok; t += num_clusters) {
-                const int m0 = t % tiles_m * 256 + static_cast<int>(cta) * 128;
-                const int n0 = t / tiles_m * BN;
-                for (int kt = 0; kt < num_kt; ++kt, ++it) {
-                    const int s = it % Cfg::kStages;
-                    if (!mbar_wait_bounded<true>(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1)) {
-                        mx4_record_status(kMx4TimeoutProducer);
-                        ok = false;
-                        break;
-                    }
-                    unsigned char* st = smem + s * Cfg::kStageBytes;
-                    const uint32_t full = mapa_shared(smem_u32(&full_bar[s]), 0);
-                    if (cta == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * Cfg::kStageBytes);
-                    tma_load_2d_pair(st, &tmap_x, full, kt * (kMx4StageK / 2), m0);
-                    tma_load_2d_pair(st + Cfg::kABytes, &tmap_w, full, kt * (kMx4StageK / 2),
-                                     n0 + static_cast<int>(cta) * (BN / 2));
-                    unsigned char* sf = st + Cfg::kABytes + Cfg::kBBytes;
-                    tma_load_2d_pair(sf, &tmap_xs, full, kt * 256, m0 / 128);
-                    tma_load_2d_pair(sf + Cfg::kSaBytes, &tmap_ws, full, kt * 256, n0 / 128);
+    if (warp == 0 || warp == 2) {
+        // ---------------- TMA producers: w0 codes, w2 scales; both CTAs' tiles complete on
+        // the even CTA's barrier. The warp runs the loop (uniform addresses), one elected
+        // lane issues: a lane on its own took 600 cycles a stage for its four copies.
+        const uint32_t full0 = mapa_shared(smem_u32(full_bar), 0);
+        int it = 0;
+        bool ok = true;
+        for (int t = cluster_id; t < num_tiles && ok; t += num_clusters) {
+            const int m0 = t % tiles_m * 256 + static_cast<int>(cta) * 128;
+            const int n0 = t / tiles_m * BN;
+            for (int kt = 0; kt < num_kt; ++kt, ++it) {
+                const int s = it % Cfg::kStages;
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1))) {
+                    if (lane == 0) mx4_record_status(kMx4TimeoutProducer);
+                    ok = false;
+                    break;
                 }
+                unsigned char* st = smem + s * Cfg::kStageBytes;
+                const uint32_t full = full0 + s * 8;
+                if (elect_one()) {
+                    if (warp == 0) {
+                        if (cta == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * Cfg::kStageBytes);
+                        tma_load_2d_pair(st, &tmap_x, full, kt * (kMx4StageK / 2), m0);
+                        tma_load_2d_pair(st + Cfg::kABytes, &tmap_w, full, kt * (kMx4StageK / 2),
+                                         n0 + static_cast<int>(cta) * (BN / 2));
+                    } else {
+                        unsigned char* sf = st + Cfg::kABytes + Cfg::kBBytes;
+                        tma_load_2d_pair(sf, &tmap_xs, full, kt * 256, m0 / 128);
+                        tma_load_2d_pair(sf + Cfg::kSaBytes, &tmap_ws, full, kt * 256, n0 / 128);
+                    }
+                }
+                __syncwarp();
             }
         }
     } else if (warp == 1) {
