@@ -250,9 +250,10 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 
     if (warp == 0) {
         // ---------------- TMA producer: the warp runs the loop, one elected lane issues
-        for (int it = 0; it < kts; ++it) {
-            const int s = it % Cfg::kStages;
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1))) {
+        Mx4Ring<Cfg::kStages> ring;
+        for (int it = 0; it < kts; ++it, ring.next()) {
+            const int s = ring.slot;
+            if (!mx4_wait_warp(&empty_bar[s], ring.phase ^ 1, mbar_test_wait(&empty_bar[s], ring.phase ^ 1))) {
                 if (lane == 0) mx4_record_status(kMx4TimeoutProducer);
                 break;
             }
@@ -272,35 +273,42 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer: the warp runs the loop, one elected lane issues
+        const uint32_t base = smem_u32(smem);
+        const uint64_t da0 = smem_desc_kmajor(base, 1024, 2), db0 = smem_desc_kmajor(base + Cfg::kABytes, 1024, 2);
+        const uint64_t dsa0 = smem_desc_kmajor(base + Cfg::kABytes + Cfg::kBBytes, 128, 0);
+        const uint64_t dsb0 = smem_desc_kmajor(base + Cfg::kABytes + Cfg::kBBytes + Cfg::kScaleBytes, 128, 0);
+        const int odd_tail = (K + 127) / 128 & 1;                 // the last stage of K has one 128-value half
+        Mx4Ring<Cfg::kStages> ring;
         bool ok = true;
-        for (int it = 0; it < kts && ok; ++it) {
-            const int s = it % Cfg::kStages;
-            const uint32_t ph = (it / Cfg::kStages) & 1;
-            bool in = mbar_wait_bounded(&full_bar[s], ph);
-            if (FUSED && in) in = mbar_wait_bounded(&ready_bar[s], ph);
-            if (!__all_sync(0xFFFFFFFFu, in)) {
+        for (int it = 0; it < kts && ok; ++it, ring.next()) {
+            const int s = ring.slot;
+            ok = mx4_wait_warp(&full_bar[s], ring.phase, mbar_test_wait(&full_bar[s], ring.phase));
+            if (FUSED && ok) ok = mx4_wait_warp(&ready_bar[s], ring.phase, mbar_test_wait(&ready_bar[s], ring.phase));
+            if (!ok) {
                 if (lane == 0) mx4_record_status(kMx4TimeoutMma);
-                ok = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t a = smem_u32(smem + s * Cfg::kStageBytes), sf = a + Cfg::kABytes + Cfg::kBBytes;
-            const uint64_t da = smem_desc_kmajor(a, 1024, 2), db = smem_desc_kmajor(a + Cfg::kABytes, 1024, 2);
-            const uint64_t dsa = smem_desc_kmajor(sf, 128, 0), dsb = smem_desc_kmajor(sf + Cfg::kScaleBytes, 128, 0);
+            const uint64_t at = static_cast<uint64_t>(s * (Cfg::kStageBytes / 16));
             const uint32_t col = tmem + Cfg::kScaleCol + (it & 1) * 16;
-            const int halves = K - (kt0 + it) * kMx4StageK > 128 ? 2 : 1;
+            const bool both = !(odd_tail && kt0 + it == num_kt - 1);
             if (elect_one()) {
-                #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h >= halves) break;
+                const uint64_t da = da0 + at, db = db0 + at, dsa = dsa0 + at, dsb = dsb0 + at;
+                auto half = [&](int h) {
                     tmem_cp_scales<false>(col + 4 * h, dsa + 32 * h);
                     tmem_cp_scales<false>(col + 8 + 4 * h, dsb + 32 * h);
-                }
-                #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j >= 2 * halves) break;
+                };
+                auto product = [&](int j) {
                     mma_mxf4<false>(tmem, da + 2 * j, db + 2 * j, idesc_mxf4(128, BT, (j & 1) * 2), col + 4 * (j >> 1),
                                     col + 8 + 4 * (j >> 1), (it | j) != 0);
+                };
+                half(0);
+                if (both) half(1);
+                product(0);
+                product(1);
+                if (both) {
+                    product(2);
+                    product(3);
                 }
                 mma_commit(&empty_bar[s]);
             }

@@ -30,6 +30,26 @@ constexpr int kMx4PairThreads = 256;
 constexpr int kMx4StageK = 256;               // values of K a stage
 constexpr int kMx4TmemCols = 512;
 
+// A slot of a ring of N and the parity of its current use.
+template <int N>
+struct Mx4Ring {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == N) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// Whole-warp wait: one look (often taken ahead, by the caller) and a vote when the
+// phase is complete, else the bounded wait.
+__device__ __forceinline__ bool mx4_wait_warp(uint64_t* bar, uint32_t parity, bool seen) {
+    if (__all_sync(0xFFFFFFFFu, seen)) return true;
+    return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, parity));
+}
+
 template <int BN>
 struct Mx4PairCfg {
     static constexpr int kABytes = 128 * kMx4StageK / 2;
@@ -129,14 +149,14 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
         // the even CTA's barrier. The warp runs the loop (uniform addresses), one elected
         // lane issues: a lane on its own took 600 cycles a stage for its four copies.
         const uint32_t full0 = mapa_shared(smem_u32(full_bar), 0);
-        int it = 0;
+        Mx4Ring<Cfg::kStages> ring;
         bool ok = true;
         for (int t = cluster_id; t < num_tiles && ok; t += num_clusters) {
             const int m0 = t % tiles_m * 256 + static_cast<int>(cta) * 128;
             const int n0 = t / tiles_m * BN;
-            for (int kt = 0; kt < num_kt; ++kt, ++it) {
-                const int s = it % Cfg::kStages;
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&empty_bar[s], ((it / Cfg::kStages) & 1) ^ 1))) {
+            for (int kt = 0; kt < num_kt; ++kt, ring.next()) {
+                const int s = ring.slot;
+                if (!mx4_wait_warp(&empty_bar[s], ring.phase ^ 1, mbar_test_wait(&empty_bar[s], ring.phase ^ 1))) {
                     if (lane == 0) mx4_record_status(kMx4TimeoutProducer);
                     ok = false;
                     break;
@@ -160,9 +180,20 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
         }
     } else if (warp == 1) {
         if (cta == 0) {
-            // ---------------- MMA issuer: the warp runs the loop, one elected lane issues
-            int it = 0;
-            bool ok = true;
+            // ---------------- MMA issuer: the warp runs the loop, one elected lane issues.
+            // The loop has to take less than a stage's MMAs (500 cycles at BN = 256): the
+            // next stage's barrier is looked at before this stage's MMAs are issued, and
+            // descriptors are a base and a multiple of the slot.
+            const uint32_t base = smem_u32(smem);
+            const uint64_t da0 = smem_desc_kmajor(base, 1024, 2), db0 = smem_desc_kmajor(base + Cfg::kABytes, 1024, 2);
+            // scale tiles: 512 bytes each, 32 in descriptor units
+            const uint64_t dsa0 = smem_desc_kmajor(base + Cfg::kABytes + Cfg::kBBytes, 128, 0);
+            const uint64_t dsb0 = smem_desc_kmajor(base + Cfg::kABytes + Cfg::kBBytes + Cfg::kSaBytes, 128, 0);
+            const int odd_tail = (K + 127) / 128 & 1;              // the last stage has one 128-value half
+            Mx4Ring<Cfg::kStages> ring;
+            uint32_t sf = tmem + Cfg::kScaleCol;
+            const uint32_t sf_flip = sf ^ (sf + Cfg::kScaleCols);
+            bool ok = true, seen = mbar_test_wait(&full_bar[0], 0);
             for (int lt = 0; lt < my_tiles && ok; ++lt) {
                 // the tile before this one shares columns with it (kShared), else the
                 // one before that used this accumulator
@@ -173,38 +204,41 @@ mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_co
                 }
                 tc_fence_after();
                 const uint32_t acc = tmem + ((lt & 1) ? Cfg::kAcc1 : 0);
-                for (int kt = 0; kt < num_kt; ++kt, ++it) {
-                    const int s = it % Cfg::kStages;
-                    if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&full_bar[s], (it / Cfg::kStages) & 1))) {
+                for (int kt = 0; kt < num_kt; ++kt) {
+                    const int s = ring.slot;
+                    if (!mx4_wait_warp(&full_bar[s], ring.phase, seen)) {
                         if (lane == 0) mx4_record_status(kMx4TimeoutMma);
                         ok = false;
                         break;
                     }
+                    ring.next();
+                    seen = mbar_test_wait(&full_bar[ring.slot], ring.phase);
                     tc_fence_after();
-                    const uint32_t a = smem_u32(smem + s * Cfg::kStageBytes);
-                    const uint64_t da = smem_desc_kmajor(a, 1024, 2), db = smem_desc_kmajor(a + Cfg::kABytes, 1024, 2);
-                    // scale tiles: 512 bytes each, 32 in descriptor units
-                    const uint64_t dsa = smem_desc_kmajor(a + Cfg::kABytes + Cfg::kBBytes, 128, 0);
-                    const uint64_t dsb = smem_desc_kmajor(a + Cfg::kABytes + Cfg::kBBytes + Cfg::kSaBytes, 128, 0);
-                    const uint32_t sf = tmem + Cfg::kScaleCol + (it & 1) * Cfg::kScaleCols;
-                    const int halves = K - kt * kMx4StageK > 128 ? 2 : 1;     // 128-value halves with data
+                    const uint64_t at = static_cast<uint64_t>(s * (Cfg::kStageBytes / 16));
+                    const bool both = !(odd_tail && kt == num_kt - 1);
                     if (elect_one()) {
-                        #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (h >= halves) break;
+                        const uint64_t da = da0 + at, db = db0 + at, dsa = dsa0 + at, dsb = dsb0 + at;
+                        auto half = [&](int h) {
                             tmem_cp_scales<true>(sf + 4 * h, dsa + 32 * h);
                             #pragma unroll
                             for (int j = 0; j < BN / 128; ++j)
                                 tmem_cp_scales<true>(sf + 8 + (BN / 32) * h + 4 * j, dsb + 64 * j + 32 * h);
-                        }
-                        #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if (j >= 2 * halves) break;
+                        };
+                        auto product = [&](int j) {
                             mma_mxf4<true>(acc, da + 2 * j, db + 2 * j, idesc_mxf4(256, BN, (j & 1) * 2), sf + 4 * (j >> 1),
                                            sf + 8 + (BN / 32) * (j >> 1), (kt | j) != 0);
+                        };
+                        half(0);
+                        if (both) half(1);
+                        product(0);
+                        product(1);
+                        if (both) {
+                            product(2);
+                            product(3);
                         }
                         mma_commit_pair_multicast(&empty_bar[s], 0x3);
                     }
+                    sf ^= sf_flip;
                     __syncwarp();
                 }
                 if (ok && elect_one()) mma_commit_pair_multicast(&acc_full[lt & 1], 0x3);
