@@ -117,9 +117,10 @@ static int run_quant(const void* x, int dtype, long long ldx, void* codes, void*
             cudaError_t e = ensure_smem(kernel, mx4_quant_smem<T>());
             if (e != cudaSuccess) return static_cast<int>(e);
             const bool vec = aligned16(x) && ldx * sizeof(T) % 16 == 0;
+            const int linear = vec && (ldx == K || M == 1) && K % kMx4Unit == 0 ? static_cast<int>(static_cast<long long>(M) * K / kMx4Unit) : 0;
             return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<T>(), st,
                                                static_cast<const T*>(x), ldx, static_cast<uint8_t*>(codes),
-                                               static_cast<uint8_t*>(scales), M, K, static_cast<int>(units), vec));
+                                               static_cast<uint8_t*>(scales), M, K, static_cast<int>(units), vec, linear));
         });
     });
 }
@@ -256,11 +257,18 @@ CONVROT_API int ck_mx4_dequant(const void* codes, const void* scales, void* out,
                                void* stream) {
     if (int rc = check_matrix(out, out_dtype, codes, scales, M, K, G)) return rc;
     if (M == 0) return 0;
-    const long long units = static_cast<long long>(M) * ((K + 127) / 128);
+    const long long units = static_cast<long long>(M) * ((K + 127) / 128), words = static_cast<long long>(M) * K / 8;
     return with_type(out_dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
+        if (G == 0) {
+            const long long per = kMx4DecodeThreads * kMx4DecodeWords;
+            return static_cast<int>(launch_pdl(mx4_decode_kernel<T>, dim3(static_cast<unsigned>((words + per - 1) / per)), dim3(kMx4DecodeThreads),
+                                               0, static_cast<cudaStream_t>(stream), static_cast<const uint32_t*>(codes),
+                                               static_cast<const uint8_t*>(scales), static_cast<T*>(out), K, words));
+        }
         return with_group(G, [&](auto g) {
-            auto kernel = mx4_dequant_kernel<T, decltype(g)::value>;
+            constexpr int g0 = decltype(g)::value == 0 ? 16 : decltype(g)::value;
+            auto kernel = mx4_dequant_kernel<T, g0>;
             cudaError_t e = ensure_smem(kernel, mx4_quant_smem<T>() / 2);
             if (e != cudaSuccess) return static_cast<int>(e);
             return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<T>() / 2,
@@ -404,10 +412,12 @@ CONVROT_API int ck_mx4_cache_append(void* codes, void* scales, long long pages, 
             if (units > kMx4MostUnits) return fail("too many tokens in one call");
             const long long strides = k_token | k_head | v_token | v_head;
             const bool vec = aligned16(k) && aligned16(v) && strides * static_cast<long long>(sizeof(E)) % 16 == 0;
+            const bool linear = vec && k_head == d && v_head == d && k_token == static_cast<long long>(heads) * d &&
+                                v_token == k_token && (d != 64 || heads % 2 == 0);
             return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<E>(),
                                                static_cast<cudaStream_t>(stream), static_cast<uint8_t*>(codes),
                                                static_cast<uint8_t*>(scales), static_cast<const E*>(k), static_cast<const E*>(v),
-                                               k_token, k_head, v_token, v_head, static_cast<const long long*>(slots), static_cast<int>(units), c, vec));
+                                               k_token, k_head, v_token, v_head, static_cast<const long long*>(slots), static_cast<int>(units), c, vec, linear));
         });
     });
 }
@@ -425,11 +435,12 @@ CONVROT_API int ck_mx4_cache_read(const void* codes, const void* scales, long lo
         using E = std::remove_pointer_t<decltype(t)>;
         return with_head(d, G, [&](auto dim, auto g) {
             auto kernel = mx4_cache_read_kernel<E, decltype(dim)::value, decltype(g)::value>;
-            cudaError_t e = ensure_smem(kernel, mx4_quant_smem<E>() / 2);
+            const int smem = kMx4QuantWarps * (Mx4Slab<E>::kBytes + kMx4ReadWarpBytes);
+            cudaError_t e = ensure_smem(kernel, smem);
             if (e != cudaSuccess) return static_cast<int>(e);
             const long long units = static_cast<long long>(T) * 2 * mx4_cache_units<decltype(dim)::value>(heads);
             if (units > kMx4MostUnits) return fail("too many tokens in one call");
-            return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<E>() / 2,
+            return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), smem,
                                                static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(codes),
                                                static_cast<const uint8_t*>(scales), static_cast<const long long*>(slots),
                                                static_cast<E*>(k), static_cast<E*>(v), static_cast<int>(units), c));

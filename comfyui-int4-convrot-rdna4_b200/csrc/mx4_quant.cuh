@@ -3,7 +3,8 @@
 // Included by mx4.cu. A unit (mx4_unit.cuh) is 128 columns of one row, and the
 // units of the matrix are numbered row after row; a warp takes 32 of them at a
 // time, copying the next 32 while it works on these. Missing columns of a row's
-// last unit read as zeros, which leaves their scale bytes 0.
+// last unit read as zeros, which leaves their scale bytes 0. The first `linear_units`
+// units lie one after the other in memory (rows without a gap, whole units).
 #pragma once
 
 namespace convrot {
@@ -15,7 +16,7 @@ template <typename T> constexpr int mx4_quant_smem() { return kMx4QuantWarps * 2
 template <typename T, int G>
 __global__ void __launch_bounds__(kMx4QuantWarps * 32, 3)
 mx4_quant_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                 int M, int K, int units, bool vec) {
+                 int M, int K, int units, bool vec, int linear_units) {
     using S = Mx4Slab<T>;
     extern __shared__ __align__(128) unsigned char mx4slabs[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -29,13 +30,17 @@ mx4_quant_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ c
         return Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(held ? x + row * ldx + c * kMx4Unit : x),
                             held ? min(S::kChunks, (K - c * kMx4Unit) / S::kPer) : 0};
     };
+    auto load = [&](unsigned char* to, int first) {
+        if (first + 32 <= linear_units) slab_load_linear<T>(to, x + static_cast<size_t>(first) * kMx4Unit);
+        else slab_load<false>(to, place(first + lane), 0, vec);
+    };
     griddep_wait();
     griddep_launch_dependents();
-    if (base < units) slab_load<false>(slab, place(base + lane), 0, vec);
+    if (base < units) load(slab, base);
     cp_async_commit();
     for (int it = 0; base < units; base += step, ++it) {
         const unsigned char* cur = slab + (it & 1) * S::kBytes;
-        if (base + step < units) slab_load<false>(slab + ((it + 1) & 1) * S::kBytes, place(base + step + lane), 0, vec);
+        if (base + step < units) load(slab + ((it + 1) & 1) * S::kBytes, base + step);
         cp_async_commit();
         cp_async_wait<1>();
         __syncwarp();
@@ -60,6 +65,7 @@ mx4_quant_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ c
     }
 }
 
+// Back, with the rotation: values go out through the warp's slab.
 template <typename T, int G>
 __global__ void __launch_bounds__(kMx4QuantWarps * 32, 3)
 mx4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, int K,
@@ -70,6 +76,7 @@ mx4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict_
     unsigned char* slab = mx4slabs + warp * S::kBytes;
     const int kt = (K + 127) / 128;
     const int step = static_cast<int>(gridDim.x) * kMx4QuantWarps * 32;
+    const bool linear = K % kMx4Unit == 0;
     griddep_wait();
     griddep_launch_dependents();
     for (int base = (static_cast<int>(blockIdx.x) * kMx4QuantWarps + warp) * 32; base < units; base += step) {
@@ -86,9 +93,59 @@ mx4_dequant_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict_
         unit_rotate<G>(v);
         unit_to_slab<T>(slab, lane ^ (G == 256 ? 1 : 0), v, unit_factor<G>());
         __syncwarp();
-        slab_store<T>(slab, Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(out + static_cast<size_t>(row) * K + c * kMx4Unit),
-                                         blocks * (kMx4Block / S::kPer)});
+        if (linear && base + 32 <= units) {
+            slab_store_linear<T>(slab, out + static_cast<size_t>(base) * kMx4Unit);
+        } else {
+            slab_store<T>(slab, Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(out + static_cast<size_t>(row) * K + c * kMx4Unit),
+                                             blocks * (kMx4Block / S::kPer)});
+        }
         __syncwarp();
+    }
+}
+
+// Back, without a rotation: a thread takes words of eight codes, neighbouring
+// threads neighbouring words.
+constexpr int kMx4DecodeThreads = 256, kMx4DecodeWords = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kMx4DecodeThreads)
+mx4_decode_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, int K, long long words) {
+    const int row_words = K / 8, kt = (K + 127) / 128;
+    griddep_wait();
+    griddep_launch_dependents();
+    const long long first = static_cast<long long>(blockIdx.x) * (kMx4DecodeThreads * kMx4DecodeWords) + threadIdx.x;
+    int row = static_cast<int>(first / row_words), col = static_cast<int>(first - static_cast<long long>(row) * row_words);
+    uint32_t w[kMx4DecodeWords], e[kMx4DecodeWords];
+    #pragma unroll
+    for (int i = 0; i < kMx4DecodeWords; ++i) {
+        const long long at = first + i * kMx4DecodeThreads;
+        w[i] = 0;
+        e[i] = 0;
+        if (at < words) {
+            w[i] = __ldg(codes + at);
+            e[i] = __ldg(scales + mx4_scale_pos(row, col >> 2, kt));
+        }
+        row += kMx4DecodeThreads / row_words;
+        col += kMx4DecodeThreads % row_words;
+        if (col >= row_words) {
+            col -= row_words;
+            ++row;
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < kMx4DecodeWords; ++i) {
+        const long long at = first + i * kMx4DecodeThreads;
+        if (at >= words) break;
+        float f[8];
+        mx4_decode8(w[i], f);
+        const float s = mx4_scale_value(e[i]);
+        T v[8];
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = mx4_from_f32<T>(f[j] * s);
+        uint4 p[sizeof(T) / 2];
+        memcpy(p, v, sizeof(v));
+        #pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j) *(reinterpret_cast<uint4*>(out + at * 8) + j) = p[j];
     }
 }
 
