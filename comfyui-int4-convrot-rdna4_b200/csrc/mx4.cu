@@ -342,10 +342,12 @@ static AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longe
     p.tile_rows = rows <= 8 ? 8 : rows <= 16 || d == 256 ? 16 : 32;
     p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     p.tiles = static_cast<long long>(B) * hkv * p.row_tiles;
-    // splits: enough blocks for four waves of four a multiprocessor, none without a
-    // group of tokens of its own
-    const long long groups = (longest + kMx4AttnGroup - 1) / kMx4AttnGroup;
-    const long long want = (16LL * sm_count() + p.tiles - 1) / (p.tiles > 0 ? p.tiles : 1);
+    // splits: one wave (four blocks a multiprocessor) always, as far as every split has
+    // a group of tokens; up to four waves, which even the tail out, while each keeps
+    // eight groups (a block's start and end cost about as much as three)
+    const long long groups = (longest + kMx4AttnGroup - 1) / kMx4AttnGroup, tiles = p.tiles > 0 ? p.tiles : 1;
+    const long long wave = (4LL * sm_count() + tiles - 1) / tiles;
+    const long long want = std::max(wave, std::min(4 * wave, groups / 8));
     p.splits = static_cast<int>(std::max(1LL, std::min({want, groups, static_cast<long long>(kMx4MostSplits)})));
     return p;
 }
