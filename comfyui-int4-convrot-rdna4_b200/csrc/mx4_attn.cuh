@@ -19,9 +19,9 @@
 //   Values: a token's codes times 2^(E_b - E), E the token's largest scale
 //   exponent, are f16 values exactly (down to 2^-24 of the token's largest); the
 //   rest, 2^E, goes to the probabilities: the numerator's weights are
-//   2^(s + E - max(s + E)), with a maximum of their own, so that they are f16
-//   values in [0, 1] whatever the values' range. The denominator keeps the usual
-//   weights 2^(s - max s) in fp32.
+//   2^(s + E - mn), with a running maximum of their own, so that they are f16 values
+//   whatever the values' range. The denominator keeps the usual weights 2^(s - m) in
+//   fp32.
 // SPLIT (f16 queries): queries and numerator weights as the sum of two f16 values,
 // so that the result is as exact as its own rounding; a bf16 result's rounding is
 // eight times coarser than what one f16 value loses.
@@ -97,6 +97,13 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same from a zero accumulator.
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Four bytes of code pairs to four f16 pairs.
@@ -408,6 +415,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             }
         #pragma unroll
         for (int blk = 0; blk < kB; ++blk) {
+            const unsigned char* kc = st + ktok * (D / 2) + mx4_chunk_pos<D>(ktok, blk) * 16 + t4 * 4;
             uint4 qb[NT], ql[NT];
             #pragma unroll
             for (int i = 0; i < NT; ++i) {
@@ -417,15 +425,14 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             }
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t h0[4], h1[4];
-                const int tok = 16 * c + ktok;
-                codes_to_f16(*reinterpret_cast<const uint32_t*>(st + tok * (D / 2) + mx4_chunk_pos<D>(tok, blk) * 16 + t4 * 4), h0);
-                codes_to_f16(*reinterpret_cast<const uint32_t*>(st + (tok + 8) * (D / 2) + mx4_chunk_pos<D>(tok + 8, blk) * 16 + t4 * 4), h1);
+                uint32_t h0[4], h1[4];                            // (a token's swizzle is that of the token 8 on)
+                codes_to_f16(*reinterpret_cast<const uint32_t*>(kc + 16 * c * (D / 2)), h0);
+                codes_to_f16(*reinterpret_cast<const uint32_t*>(kc + (16 * c + 8) * (D / 2)), h1);
                 const float f0 = fk[2 * c][blk], f1 = fk[2 * c + 1][blk];
                 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_f16(acc, h0[0], h1[0], h0[1], h1[1], qb[i].x, qb[i].y);
+                    float acc[4];
+                    mma_f16_zero(acc, h0[0], h1[0], h0[1], h1[1], qb[i].x, qb[i].y);
                     mma_f16(acc, h0[2], h1[2], h0[3], h1[3], qb[i].z, qb[i].w);
                     if constexpr (SPLIT) {
                         mma_f16(acc, h0[0], h1[0], h0[1], h1[1], ql[i].x, ql[i].y);
@@ -462,36 +469,63 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                         if (ci * kMx4AttnChunk + 8 * c + ktok >= sees) s[i][c >> 1][2 * (c & 1) + h] = -INFINITY;
                 }
         }
-        bool moved = false;
-        float fn[NT][2];
+        // The references m and mn need not be the maxima, only near them: they move when
+        // some score is 2^8 above (f16 holds weights up to 2^15), which is rare, and only
+        // then do lanes compare and accumulators get a new scale.
+        bool above = false;
+        #pragma unroll
+        for (int i = 0; i < NT; ++i)
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = -INFINITY, topn = -INFINITY;
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float x = s[i][c >> 1][2 * (c & 1) + h];
+                    top = fmaxf(top, x);
+                    topn = fmaxf(topn, x + tk[c].y);
+                }
+                above |= top > m[i][h] + 8.0f || topn > mn[i][h] + 8.0f;
+            }
+        if (__any_sync(0xFFFFFFFFu, above)) {
+            #pragma unroll
+            for (int i = 0; i < NT; ++i)
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float top = -INFINITY, topn = -INFINITY;
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float x = s[i][c >> 1][2 * (c & 1) + h];
+                        top = fmaxf(top, x);
+                        topn = fmaxf(topn, x + tk[c].y);
+                    }
+                    #pragma unroll
+                    for (int z = 4; z < 32; z *= 2) {
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
+                        topn = fmaxf(topn, __shfl_xor_sync(0xFFFFFFFFu, topn, z));
+                    }
+                    const float m2 = fmaxf(m[i][h], top), mn2 = fmaxf(mn[i][h], topn);
+                    l[i][h] *= m2 == -INFINITY ? 0.0f : ex2(m[i][h] - m2);
+                    const float fn = mn2 == -INFINITY ? 0.0f : ex2(mn[i][h] - mn2);
+                    m[i][h] = m2;
+                    mn[i][h] = mn2;
+                    #pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        o[i][j][h] *= fn;
+                        o[i][j][2 + h] *= fn;
+                    }
+                }
+        }
         #pragma unroll
         for (int i = 0; i < NT; ++i) {
             float w[2][4];
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float x[4], top = -INFINITY, topn = -INFINITY;
+                const float base = m[i][h] == -INFINITY ? 0.0f : m[i][h], basen = mn[i][h] == -INFINITY ? 0.0f : mn[i][h];
                 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    x[c] = s[i][c >> 1][2 * (c & 1) + h];
-                    top = fmaxf(top, x[c]);
-                    topn = fmaxf(topn, x[c] + tk[c].y);
-                }
-                #pragma unroll
-                for (int z = 4; z < 32; z *= 2) {
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
-                    topn = fmaxf(topn, __shfl_xor_sync(0xFFFFFFFFu, topn, z));
-                }
-                const float m2 = fmaxf(m[i][h], top), mn2 = fmaxf(mn[i][h], topn);
-                const float base = m2 == -INFINITY ? 0.0f : m2, basen = mn2 == -INFINITY ? 0.0f : mn2;
-                l[i][h] *= ex2(m[i][h] - base);
-                fn[i][h] = ex2(mn[i][h] - basen);
-                moved |= mn2 != mn[i][h];
-                m[i][h] = m2;
-                mn[i][h] = mn2;
-                #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    l[i][h] += ex2(x[c] - base);
-                    w[h][c] = ex2(x[c] + (tk[c].y - basen));
+                    const float x = s[i][c >> 1][2 * (c & 1) + h];
+                    l[i][h] += ex2(x - base);
+                    w[h][c] = ex2(x + (tk[c].y - basen));
                 }
             }
             #pragma unroll
@@ -506,30 +540,28 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 }
             }
         }
-        if (__any_sync(0xFFFFFFFFu, moved)) {
-            #pragma unroll
-            for (int i = 0; i < NT; ++i)
-                #pragma unroll
-                for (int j = 0; j < D / 16; ++j)
-                    #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[i][j][e] *= fn[i][e & 1];
-        }
 
         // ---------------- values: tiles of 16 channels by 8 query rows over 16 tokens
+        const unsigned char *va[D / 64], *vb[D / 64];             // this thread's word of tokens t and t + 4
+        #pragma unroll
+        for (int hf = 0; hf < D / 64; ++hf) {
+            const int blk = 2 * hf + (g >> 2);
+            va[hf] = vcodes + t4 * (D / 2) + mx4_chunk_pos<D>(t4, blk) * 16 + (g & 3) * 4;
+            vb[hf] = vcodes + (t4 + 4) * (D / 2) + mx4_chunk_pos<D>(t4 + 4, blk) * 16 + (g & 3) * 4;
+        }
+        const __half* vfac = vf + (g >> 2) * 32 + 2 * t4;
         #pragma unroll
         for (int u = 0; u < 2; ++u) {
             #pragma unroll
             for (int hf = 0; hf < D / 64; ++hf) {
-                const int blk = 2 * hf + (g >> 2);
                 uint32_t lo[2], hi[2], f[2];
                 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const int tok = 8 * (2 * u + x) + t4;
-                    const uint32_t wa = *reinterpret_cast<const uint32_t*>(vcodes + tok * (D / 2) + mx4_chunk_pos<D>(tok, blk) * 16 + (g & 3) * 4);
-                    const uint32_t wb = *reinterpret_cast<const uint32_t*>(vcodes + (tok + 4) * (D / 2) + mx4_chunk_pos<D>(tok + 4, blk) * 16 + (g & 3) * 4);
+                    const uint32_t wa = *reinterpret_cast<const uint32_t*>(va[hf] + 8 * (2 * u + x) * (D / 2));
+                    const uint32_t wb = *reinterpret_cast<const uint32_t*>(vb[hf] + 8 * (2 * u + x) * (D / 2));
                     lo[x] = (wa & 0x0F0F0F0Fu) | ((wb << 4) & 0xF0F0F0F0u);
                     hi[x] = ((wa >> 4) & 0x0F0F0F0Fu) | (wb & 0xF0F0F0F0u);
-                    f[x] = *reinterpret_cast<const uint32_t*>(vf + blk * 32 + 8 * (2 * u + x) + 2 * t4);
+                    f[x] = *reinterpret_cast<const uint32_t*>(vfac + 64 * hf + 8 * (2 * u + x));
                 }
                 uint32_t e0[4], e1[4], d0[4], d1[4];
                 codes_to_f16(lo[0], e0);
