@@ -230,9 +230,15 @@ static int run_gemm(const void* xc, const void* xs, const void* wc, const void* 
     if (M <= 32) return launch_gemm_few<T, 0, 32, false>(nullptr, 0, xc, xs, wc, ws, bias, out, M, N, K, stream);
     if (M <= 64) return launch_gemm_few<T, 0, 64, false>(nullptr, 0, xc, xs, wc, ws, bias, out, M, N, K, stream);
     if (M <= 128) return launch_gemm_few<T, 0, 128, false>(nullptr, 0, xc, xs, wc, ws, bias, out, M, N, K, stream);
-    // 256-row pairs of weights where their tiles fill the SM pairs
-    const long long tiles256 = static_cast<long long>((M + 255) / 256) * ((N + 255) / 256);
-    if (tiles256 * 2 >= sm_count()) return launch_gemm_pair<256>(xc, xs, wc, ws, bias, out, M, N, K, stream);
+    // Tile width by the waves of tiles over the SM pairs: a stage of 256 values of K
+    // takes 560 cycles in a 256-wide tile and 400 in a 128-wide one (measured), a tile's
+    // start about 500.
+    const long long tiles_m = (M + 255) / 256, pairs = sm_count() / 2, stages = (K + kMx4StageK - 1) / kMx4StageK;
+    auto cost = [&](int width, int cycles) {
+        const long long tiles = tiles_m * ((N + width - 1) / width);
+        return (tiles + pairs - 1) / pairs * (stages * cycles + 500);
+    };
+    if (cost(256, 560) <= cost(128, 400)) return launch_gemm_pair<256>(xc, xs, wc, ws, bias, out, M, N, K, stream);
     return launch_gemm_pair<128>(xc, xs, wc, ws, bias, out, M, N, K, stream);
 }
 
