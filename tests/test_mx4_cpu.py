@@ -124,3 +124,32 @@ def test_c_entries_refuse_before_any_launch(lib):
     refuse(lib, attention(table=0), b"null")
     refuse(lib, attention(ld=3), b"block table")
     assert attention(b=0) == 0
+
+
+def test_cache_pages_of_sequences():
+    from _int4.mx4_layers import Mx4KVCache
+    c = Mx4KVCache(5, 1, 64, page=16, device="cpu")
+    a, b = c.add(), c.add()
+    assert c.extend(a, 17) == list(range(16)) + [16]
+    assert c.extend(b, 1) == [32]
+    assert c.extend(a, 1) == [17] and c.length(a) == 18
+    assert c.slots(a) == list(range(18))
+    table, lens = c.tables([b, a])
+    assert table.tolist() == [[2, -1], [0, 1]] and lens.tolist() == [1, 18]
+    with pytest.raises(RuntimeError, match="free pages"):
+        c.extend(b, 48)
+    assert c.length(b) == 1
+    c.free(a)
+    assert c.extend(b, 63) == list(range(33, 48)) + list(range(0, 32)) + list(range(48, 64))
+    assert c.tables([b])[0].tolist() == [[2, 0, 1, 3]]
+
+
+def test_linear_module_refuses_and_shapes():
+    from _int4.mx4_layers import Mx4ConvRotLinear, Mx4SelfAttention
+    with pytest.raises(ValueError):
+        Mx4ConvRotLinear(48, 8)
+    m = Mx4ConvRotLinear(320, 24, convrot_groupsize=0)
+    assert m.weight.shape == (24, 160) and m.weight_scale.shape == (1, 3, 512) and m.groupsize == 0
+    assert Mx4ConvRotLinear(320, 24).groupsize == 64
+    with pytest.raises(ValueError):
+        Mx4SelfAttention(64, 5, 2, 64)
