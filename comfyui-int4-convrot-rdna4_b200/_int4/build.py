@@ -1,9 +1,9 @@
 """Build the B200 ConvRot library (libconvrot_b200.so) with nvcc for sm_100a.
 
 Counterpart of the reference's hipcc build (_int4/build.py:73-86): one nvcc
-call on the package's CUDA sources, output next to this file. It is run by
-``__graft_entry__.build()`` and, when the library is missing, once by the
-loader.
+call on the package's CUDA sources, output next to this file, and one g++ call for
+the Python binding of the MX4 entries, which links against it. It is run by
+``__graft_entry__.build()`` and, when a file is missing, once by the loaders.
 """
 from __future__ import annotations
 
@@ -40,6 +40,14 @@ def is_stale() -> bool:
     return newest > os.path.getmtime(out)
 
 
+def binding_name() -> str:
+    return "_mx4_binding.so"
+
+
+def binding_path() -> str:
+    return os.path.join(_HERE, binding_name())
+
+
 def find_nvcc() -> str | None:
     cand = shutil.which("nvcc")
     if cand:
@@ -67,5 +75,31 @@ def build(verbose: bool = False) -> str:
     return out
 
 
+def build_binding(verbose: bool = False) -> str:
+    """The Python module of the MX4 entries (needs the built library and torch's headers)."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    out = binding_path()
+    tmp = out + ".tmp"
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               os.path.join(home, "include"), sysconfig.get_paths()["include"],
+               os.path.join(os.path.dirname(os.path.dirname(_HERE)), "include")]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in include],
+           os.path.join(_CSRC, "mx4_binding.cpp"), "-o", tmp, f"-L{os.path.join(root, 'lib')}", f"-L{_HERE}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-l:{lib_name()}", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print("building:", " ".join(cmd))
+    cp = subprocess.run(cmd, capture_output=True, text=True)
+    if cp.returncode != 0 or not os.path.exists(tmp):
+        raise RuntimeError(f"the binding's build failed:\n{cp.stderr}")
+    os.replace(tmp, out)
+    return out
+
+
 if __name__ == "__main__":
     print("built:", build(verbose=True))
+    print("built:", build_binding(verbose=True))

@@ -27,89 +27,42 @@ stream; bad arguments raise ValueError, a refused or failed launch RuntimeError.
 """
 from __future__ import annotations
 
+import importlib.machinery
+import importlib.util
+import os
+import threading
+
 import torch
 
-from .cuda_loader import _check, _IN_DTYPE_CODE, _load
+from . import build as _build
 
 BLOCK = 32
-_GROUPS = (0, 16, 64, 256)
 _HEAD_DIMS = (64, 128, 256)
 
-
-def _device_of(*tensors):
-    """The one CUDA device of the tensors (None entries skipped); ValueError otherwise."""
-    device = None
-    for t in tensors:
-        if t is not None:
-            if not t.is_cuda:
-                raise ValueError("the B200 ConvRot kernels need CUDA tensors")
-            if device is None:
-                device = t.device
-            elif t.device != device:
-                raise ValueError(f"tensors on {device} and {t.device}")
-    return device
+_native = None
+_lock = threading.Lock()
 
 
-# the current stream as a number, without building a Stream object for each call
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-
-
-def _call(device, name, *args):
-    """Calls a C entry with the device current and its current stream as the last argument."""
-    fn = getattr(_load(), name)
-    index = device.index
-    if index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        _check(name, rc)
-
-
-def _group(k: int, group) -> int:
-    group = 0 if group is None else group
-    if group not in _GROUPS:
-        raise ValueError(f"convrot_groupsize must be 16, 64, 256 or 0 (not rotated), got {group!r}")
-    if k <= 0 or k % BLOCK:
-        raise ValueError(f"MX4 needs a last dimension that is a positive multiple of {BLOCK}, got {k}")
-    if group and k % group:
-        raise ValueError(f"K={k} not divisible by convrot_groupsize {group}")
-    return group
-
-
-def _dtype_code(dtype) -> int:
-    code = _IN_DTYPE_CODE.get(dtype)
-    if code is None:
-        raise ValueError(f"unsupported dtype {dtype}: float32, bfloat16 or float16")
-    return code
-
-
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x [..., K] as a matrix whose rows are contiguous (a view where strides allow it)."""
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        x = x.contiguous()
-    return x
+def native():
+    """The binding module (_mx4_binding.so, built first when missing)."""
+    global _native
+    if _native is None:
+        with _lock:
+            if _native is None:
+                if not os.path.exists(_build.lib_path()):
+                    _build.build()
+                if not os.path.exists(_build.binding_path()):
+                    _build.build_binding()
+                loader = importlib.machinery.ExtensionFileLoader("_mx4_binding", _build.binding_path())
+                spec = importlib.util.spec_from_loader("_mx4_binding", loader)
+                module = importlib.util.module_from_spec(spec)
+                loader.exec_module(module)
+                _native = module
+    return _native
 
 
 def _scale_tiles(rows: int, k: int) -> tuple[int, int, int]:
     return (rows + 127) // 128, (k + 127) // 128, 512
-
-
-def _check_codes(codes: torch.Tensor, scales: torch.Tensor, what: str) -> tuple[int, int]:
-    """(rows, K) of packed codes [..., K/2] and their tiled scales."""
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise ValueError(f"{what} codes and scales must be uint8")
-    if codes.dim() < 1 or not codes.is_contiguous() or not scales.is_contiguous():
-        raise ValueError(f"{what} codes and scales must be contiguous")
-    k = codes.shape[-1] * 2
-    rows = codes.numel() // codes.shape[-1] if k else 0
-    if tuple(scales.shape) != _scale_tiles(rows, k):
-        raise ValueError(f"{what} scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}: "
-                         f"expected {_scale_tiles(rows, k)}")
-    return rows, k
 
 
 def quantize_convrot_mx4(x: torch.Tensor, convrot_groupsize: int = 256) -> tuple[torch.Tensor, torch.Tensor]:
@@ -120,18 +73,7 @@ def quantize_convrot_mx4(x: torch.Tensor, convrot_groupsize: int = 256) -> tuple
     [ceil(R/128), ceil(K/128), 512] for the R rows. Weights are quantized with the
     same call. A block holding an infinity or a NaN stands for NaN as a whole.
     """
-    device = _device_of(x)
-    if x.dim() < 1:
-        raise ValueError("quantize_convrot_mx4 needs at least one dimension")
-    k = x.shape[-1]
-    group = _group(k, convrot_groupsize)
-    code = _dtype_code(x.dtype)
-    x2 = _rows(x)
-    m = x2.shape[0]
-    codes = x2.new_empty((*x.shape[:-1], k // 2), dtype=torch.uint8)
-    scales = x2.new_empty(_scale_tiles(m, k), dtype=torch.uint8)
-    _call(device, "ck_mx4_quant", x2.data_ptr(), code, x2.stride(0), codes.data_ptr(), scales.data_ptr(), m, k, group)
-    return codes, scales
+    return (_native or native()).quantize(x, convrot_groupsize)
 
 
 def dequantize_convrot_mx4(codes: torch.Tensor, scales: torch.Tensor, convrot_groupsize: int = 0,
@@ -142,12 +84,7 @@ def dequantize_convrot_mx4(codes: torch.Tensor, scales: torch.Tensor, convrot_gr
     ``dtype``; with 0, the default, the values of the rotated rows come back: exact
     in bfloat16 and float32.
     """
-    device = _device_of(codes, scales)
-    rows, k = _check_codes(codes, scales, "MX4")
-    group = _group(k, convrot_groupsize)
-    out = codes.new_empty((*codes.shape[:-1], k), dtype=dtype)
-    _call(device, "ck_mx4_dequant", codes.data_ptr(), scales.data_ptr(), out.data_ptr(), _dtype_code(dtype), rows, k, group)
-    return out
+    return (_native or native()).dequantize(codes, scales, convrot_groupsize, dtype)
 
 
 def mx4_scales_to_rows(scales: torch.Tensor, rows: int, k: int) -> torch.Tensor:
@@ -179,28 +116,7 @@ def convrot_mx4_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Te
     any of the three dtypes or None. fp32 accumulation, one rounding; returns
     [..., N] in x.dtype.
     """
-    device = _device_of(x, qweight, wscales, bias)
-    if qweight.dim() != 2:
-        raise ValueError(f"qweight must be [N, K/2], got {tuple(qweight.shape)}")
-    n, k = _check_codes(qweight, wscales, "weight")
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"Input K={x.shape[-1] if x.dim() else 0} does not match qweight K={k}")
-    group = _group(k, convrot_groupsize)
-    code = _dtype_code(x.dtype)
-    bias_ptr = bias_code = 0
-    if bias is not None:
-        if bias.shape != (n,) or bias.dtype not in _IN_DTYPE_CODE:
-            raise ValueError(f"bias must be [{n}] in float32, bfloat16 or float16")
-        bias = bias.contiguous()
-        bias_ptr, bias_code = bias.data_ptr(), _IN_DTYPE_CODE[bias.dtype]
-    x2 = _rows(x)
-    m = x2.shape[0]
-    out = x2.new_empty((*x.shape[:-1], n))
-    need = _load().ck_mx4_linear_workspace_size(m, k)
-    workspace = x2.new_empty((need,), dtype=torch.uint8) if need else None
-    _call(device, "ck_mx4_linear", x2.data_ptr(), code, x2.stride(0), qweight.data_ptr(), wscales.data_ptr(), bias_ptr,
-          bias_code, out.data_ptr(), m, n, k, group, workspace.data_ptr() if need else 0, need)
-    return out
+    return (_native or native()).linear(x, qweight, wscales, bias, convrot_groupsize)
 
 
 # --------------------------------------------------------------------- paged cache
@@ -217,26 +133,6 @@ def mx4_cache_empty(pages: int, page: int, heads: int, head_dim: int, device="cu
     return codes, scales
 
 
-def _check_cache(codes, scales, convrot_groupsize):
-    """(pages, heads, D, page, group) of a cache."""
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise ValueError("cache codes and scales must be uint8")
-    if codes.dim() != 5 or codes.shape[1] != 2 or not codes.is_contiguous() or not scales.is_contiguous():
-        raise ValueError("cache codes must be contiguous [pages, 2, heads, page, D/2]")
-    pages, _, heads, page, half = codes.shape
-    d = 2 * half
-    if d not in _HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {_HEAD_DIMS}, got {d}")
-    if scales.shape != (pages, 2, heads, page, d // BLOCK):
-        raise ValueError(f"cache scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}")
-    return pages, heads, d, page, _group(d, convrot_groupsize)
-
-
-def _check_slots(slots, t):
-    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous() or (t is not None and slots.shape[0] != t):
-        raise ValueError("slots must be a contiguous int64 vector, one a token")
-
-
 def convrot_mx4_cache_append(codes: torch.Tensor, scales: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                              slots: torch.Tensor, convrot_groupsize: int = 64) -> None:
     """Rotates and quantizes new keys and values and writes them to their slots.
@@ -245,19 +141,7 @@ def convrot_mx4_cache_append(codes: torch.Tensor, scales: torch.Tensor, k: torch
     contiguous), slots int64 [T]. A slot outside the cache (-1, say) is skipped;
     two tokens of one call must not share a slot.
     """
-    device = _device_of(codes, scales, k, v, slots)
-    pages, heads, d, page, group = _check_cache(codes, scales, convrot_groupsize)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (heads, d) or k.dtype != v.dtype:
-        raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} must both be [T, {heads}, {d}] of one dtype")
-    t = k.shape[0]
-    _check_slots(slots, t)
-    code = _dtype_code(k.dtype)
-    if k.stride(2) != 1:
-        k = k.contiguous()
-    if v.stride(2) != 1:
-        v = v.contiguous()
-    _call(device, "ck_mx4_cache_append", codes.data_ptr(), scales.data_ptr(), pages, heads, d, page, group, k.data_ptr(),
-          v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), t)
+    (_native or native()).cache_append(codes, scales, k, v, slots, convrot_groupsize)
 
 
 def convrot_mx4_cache_read(codes: torch.Tensor, scales: torch.Tensor, slots: torch.Tensor,
@@ -265,16 +149,7 @@ def convrot_mx4_cache_read(codes: torch.Tensor, scales: torch.Tensor, slots: tor
                            ) -> tuple[torch.Tensor, torch.Tensor]:
     """Keys and values [T, heads, D] held at ``slots`` (int64 [T]), rotated back, in ``dtype``;
     a slot outside the cache reads as zeros."""
-    device = _device_of(codes, scales, slots)
-    pages, heads, d, page, group = _check_cache(codes, scales, convrot_groupsize)
-    _check_slots(slots, None)
-    t = slots.shape[0]
-    code = _dtype_code(dtype)
-    k = codes.new_empty((t, heads, d), dtype=dtype)
-    v = codes.new_empty((t, heads, d), dtype=dtype)
-    _call(device, "ck_mx4_cache_read", codes.data_ptr(), scales.data_ptr(), pages, heads, d, page, group, slots.data_ptr(),
-          t, k.data_ptr(), v.data_ptr(), code)
-    return k, v
+    return (_native or native()).cache_read(codes, scales, slots, dtype, convrot_groupsize)
 
 
 def convrot_mx4_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
@@ -291,26 +166,4 @@ def convrot_mx4_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Te
     Query t sees the tokens up to position seq_len - Tq + t; a query that sees none
     gives zeros. Returns [B, Tq, Hq, D] in q.dtype.
     """
-    device = _device_of(q, codes, scales, block_table, seq_lens)
-    pages, heads, d, page, group = _check_cache(codes, scales, convrot_groupsize)
-    if q.dim() != 4 or q.shape[3] != d or q.shape[1] == 0 or q.shape[2] == 0 or q.shape[2] % heads:
-        raise ValueError(f"q {tuple(q.shape)} must be [B, Tq, a multiple of {heads}, {d}]")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"queries must be bfloat16 or float16, got {q.dtype}")
-    b, tq, hq, _ = q.shape
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b or \
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 [B, pages of a sequence] with contiguous rows")
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != (b,) or not seq_lens.is_contiguous():
-        raise ValueError("seq_lens must be a contiguous int32 vector [B]")
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    per_seq = block_table.shape[1]
-    out = q.new_empty((b, tq, hq, d))
-    need = _load().ck_mx4_attention_workspace_size(b, tq, hq, heads, d, per_seq * page)
-    workspace = q.new_empty((need,), dtype=torch.uint8) if need else None
-    _call(device, "ck_mx4_attention", q.data_ptr(), _IN_DTYPE_CODE[q.dtype], q.stride(0), q.stride(1), q.stride(2),
-          codes.data_ptr(), scales.data_ptr(), pages, page, block_table.data_ptr(), max(block_table.stride(0), per_seq),
-          per_seq, seq_lens.data_ptr(), out.data_ptr(), b, tq, hq, heads, d, group,
-          d ** -0.5 if softmax_scale is None else float(softmax_scale), workspace.data_ptr() if need else 0, need)
-    return out
+    return (_native or native()).attention(q, codes, scales, block_table, seq_lens, softmax_scale, convrot_groupsize)

@@ -59,14 +59,23 @@ def test_python_entries_refuse_cpu_tensors_and_bad_arguments():
     x = torch.zeros(2, 64)
     with pytest.raises(ValueError, match="CUDA"):
         _int4.quantize_convrot_mx4(x, 64)
-    with pytest.raises(ValueError, match="CUDA"):
-        _int4.convrot_mx4_linear(x, x, x)
-    with pytest.raises(ValueError, match="multiple of 32"):
-        mx4._group(48, 16)
-    with pytest.raises(ValueError, match="convrot_groupsize"):
-        mx4._group(64, 32)
-    with pytest.raises(ValueError, match="not divisible"):
-        mx4._group(96, 64)
+    for bad, group, text in ((torch.zeros(2, 48), 16, "multiple of 32"), (x, 32, "convrot_groupsize"), (torch.zeros(2, 96), 64, "not divisible"),
+                             (x.double(), 64, "unsupported dtype")):
+        with pytest.raises(ValueError, match=text):
+            _int4.quantize_convrot_mx4(bad, group)
+    with pytest.raises(TypeError):
+        _int4.quantize_convrot_mx4(None, 64)
+    with pytest.raises(TypeError):
+        _int4.quantize_convrot_mx4(x, "64")
+    codes = torch.zeros(3, 64, dtype=torch.uint8)
+    scales = torch.zeros(1, 1, 512, dtype=torch.uint8)
+    for call, text in ((lambda: _int4.dequantize_convrot_mx4(codes, scales), "CUDA"),
+                       (lambda: _int4.dequantize_convrot_mx4(codes, scales[:, :, :8].contiguous()), "do not match"),
+                       (lambda: _int4.convrot_mx4_linear(torch.zeros(2, 128), codes, scales, torch.zeros(3), 64), "CUDA"),
+                       (lambda: _int4.convrot_mx4_linear(torch.zeros(2, 128), codes, scales, torch.zeros(4), 64), "bias"),
+                       (lambda: _int4.convrot_mx4_linear(torch.zeros(2, 64), codes, scales), "does not match")):
+        with pytest.raises(ValueError, match=text):
+            call()
     with pytest.raises(ValueError, match="power of two"):
         _int4.mx4_cache_empty(1, 48, 1, 64, device="cpu")
     with pytest.raises(ValueError, match="head_dim"):
