@@ -4,7 +4,8 @@
 // rows that read it are taken together (8, 16 or 32 a block), so the cache is read
 // once for all of them; the sequence is split over blocks, and each warp of a
 // block walks its own chunks of 32 tokens with a running maximum and sum. Warps
-// are joined through shared memory, splits by mx4_attn_join_kernel.
+// are joined through shared memory; up to 8 splits of a sequence are a cluster and
+// join over distributed shared memory, more by mx4_attn_join_kernel.
 //
 // Rotated cache: q k = (H q) (H k), so the query rows are rotated once, and the
 // output, a mean of rotated values, is rotated back at the end.
@@ -50,6 +51,7 @@ struct Mx4AttnArgs {
     float* part;                   // per (tile, split, row): D floats ...
     float2* part_ml;               // ... and {maximum, sum}
     int B, tq, hq, hkv, page_bits, pages, group, row_tiles, splits;
+    int clustered;                 // a sequence's splits are one cluster and join themselves
     float scale;                   // softmax scale times log2(e)
 };
 
@@ -130,6 +132,12 @@ __device__ __forceinline__ uint32_t f16x2_bits(float lo, float hi) {
     return r;
 }
 
+__device__ __forceinline__ float2 ld_shared_cluster_f2(uint32_t cluster_addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
 template <int BYTES>
 __device__ __forceinline__ void cp_async_small(void* dst, const void* src, bool held) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;"
@@ -158,6 +166,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
     constexpr int kB = Cfg::kBlocks, kR16 = D / 32;               // blocks; 16-byte chunks of a token
     extern __shared__ __align__(128) unsigned char mx4att[];
     __shared__ float row_scale[Cfg::kRows], pm[kMx4AttnWarps][Cfg::kRows], pl[kMx4AttnWarps][Cfg::kRows];
+    __shared__ float2 block_ml[Cfg::kRows];                       // {m, sum} of the block's rows
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int tile = blockIdx.x, split = blockIdx.y;
     const int rt = tile % a.row_tiles, hk = tile / a.row_tiles % a.hkv, b = tile / a.row_tiles / a.hkv;
@@ -179,7 +188,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
     const int per_split = mx4_split_groups(n, a.splits) * kMx4AttnWarps;      // chunks
     const int chunks = (n + kMx4AttnChunk - 1) / kMx4AttnChunk;
     const int c_begin = split * per_split, c_end = min(chunks, c_begin + per_split);
-    if (a.splits > 1 && c_begin >= c_end) return;                 // (the join knows how many splits hold tokens)
+    if (a.splits > 1 && !a.clustered && c_begin >= c_end) return; // (the join knows how many splits hold tokens)
 
     unsigned char* q_smem = mx4att;
     unsigned char* ring = mx4att + Cfg::kQBytes + warp * Cfg::kWarpBytes;
@@ -624,7 +633,10 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             acc.z += f * x.z;
             acc.w += f * x.w;
         }
-        if (a.splits > 1) {
+        if (a.clustered) {
+            *reinterpret_cast<float4*>(joined + r * Cfg::kPartStride + c) = acc;
+            if (c == 0) block_ml[r] = make_float2(top, sum);
+        } else if (a.splits > 1) {
             const size_t at = (static_cast<size_t>(tile) * a.splits + split) * Cfg::kRows + r;
             *reinterpret_cast<float4*>(a.part + at * D + c) = acc;
             if (c == 0) a.part_ml[at] = make_float2(top, sum);
@@ -634,10 +646,48 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
         }
     }
-    if (a.splits > 1) return;
-    __syncthreads();
-    for (int r = warp; r < rows; r += kMx4AttnWarps) {
+    if (a.splits > 1 && !a.clustered) return;
+    if (a.clustered) cluster_sync(); else __syncthreads();
+    // rows in turn over the warps, and over the cluster's blocks
+    const int first = a.clustered ? split + a.splits * warp : warp, step = a.clustered ? a.splits * kMx4AttnWarps : kMx4AttnWarps;
+    for (int r = first; r < rows; r += step) {
         float* v = joined + r * Cfg::kPartStride;
+        if (a.clustered) {
+            // the splits' sums of this row, each from its block's memory
+            constexpr int kPer = D / 32;
+            float2 ml[8];
+            float x[8][kPer];
+            const uint32_t ml_at = smem_u32(&block_ml[r]), row_at = smem_u32(v + lane * kPer);
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                ml[k] = make_float2(-INFINITY, 0.0f);
+                if (k >= a.splits) continue;
+                const uint32_t from = mapa_shared(row_at, k);
+                ml[k] = ld_shared_cluster_f2(mapa_shared(ml_at, k));
+                #pragma unroll
+                for (int i = 0; i < kPer; i += 2) {
+                    const float2 y = ld_shared_cluster_f2(from + i * 4);
+                    x[k][i] = y.x;
+                    x[k][i + 1] = y.y;
+                }
+            }
+            float top = -INFINITY, sum = 0.0f, acc[kPer] = {};
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (ml[k].x == -INFINITY) continue;
+                const float w = ex2(ml[k].x - top);
+                sum += w * ml[k].y;
+                #pragma unroll
+                for (int i = 0; i < kPer; ++i) acc[i] += w * x[k][i];
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            v = reinterpret_cast<float*>(q_smem) + warp * D;      // (the joined rows are still read by other blocks)
+            #pragma unroll
+            for (int i = 0; i < kPer; ++i) v[lane * kPer + i] = acc[i] * inv;
+            __syncwarp();
+        }
         for (int st = 1; st < a.group; st *= 4) {
             for (int i = lane; i < D / 4; i += 32) {
                 float* p = v + (i / st) * 4 * st + i % st;
@@ -649,7 +699,9 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         const int row = row0 + r;
         T* out = static_cast<T*>(a.out) + ((static_cast<size_t>(b) * a.tq + row / per_head) * a.hq + hk * per_head + row % per_head) * D;
         for (int i = lane; i < D; i += 32) out[i] = mx4_from_f32<T>(v[i] * f);
+        __syncwarp();
     }
+    if (a.clustered) cluster_sync();                              // no block leaves while others read its memory
 }
 
 // Joins a row's splits, rotates back and rounds. `wide`: a block (eight warps) a
