@@ -57,6 +57,8 @@ struct Mx4AttnArgs {
 
 constexpr int kMx4AttnWarps = 4;
 constexpr int kMx4MostSplits = 256;            // of one sequence
+constexpr float kMx4NoScore = -1e30f;          // a row's reference before its first score (finite: -inf less it is -inf);
+                                               // scores below it count as hidden
 constexpr int kMx4AttnChunk = 32;              // tokens a warp takes at a time
 constexpr int kMx4AttnGroup = kMx4AttnWarps * kMx4AttnChunk;   // tokens a block takes at a time
 
@@ -329,7 +331,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = 8 * i + 2 * t4 + h;
-            m[i][h] = mn[i][h] = -INFINITY;
+            m[i][h] = mn[i][h] = kMx4NoScore;
             l[i][h] = 0.0f;
             rs[i][h] = row_scale[r];
         }
@@ -482,25 +484,20 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         // some score is 2^8 above (f16 holds weights up to 2^15), which is rare, and only
         // then do lanes compare and accumulators get a new scale.
         bool above = false;
+        const float most = fmaxf(fmaxf(tk[0].y, tk[1].y), fmaxf(tk[2].y, tk[3].y));   // (s + E is at most max s + max E)
         #pragma unroll
         for (int i = 0; i < NT; ++i)
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float top = -INFINITY, topn = -INFINITY;
-                #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float x = s[i][c >> 1][2 * (c & 1) + h];
-                    top = fmaxf(top, x);
-                    topn = fmaxf(topn, x + tk[c].y);
-                }
-                above |= top > m[i][h] + 8.0f || topn > mn[i][h] + 8.0f;
+                const float top = fmaxf(fmaxf(s[i][0][h], s[i][0][2 + h]), fmaxf(s[i][1][h], s[i][1][2 + h]));
+                above |= top > m[i][h] + 8.0f || top + most > mn[i][h] + 8.0f;
             }
         if (__any_sync(0xFFFFFFFFu, above)) {
             #pragma unroll
             for (int i = 0; i < NT; ++i)
                 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float top = -INFINITY, topn = -INFINITY;
+                    float top = kMx4NoScore, topn = kMx4NoScore;
                     #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const float x = s[i][c >> 1][2 * (c & 1) + h];
@@ -513,8 +510,8 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                         topn = fmaxf(topn, __shfl_xor_sync(0xFFFFFFFFu, topn, z));
                     }
                     const float m2 = fmaxf(m[i][h], top), mn2 = fmaxf(mn[i][h], topn);
-                    l[i][h] *= m2 == -INFINITY ? 0.0f : ex2(m[i][h] - m2);
-                    const float fn = mn2 == -INFINITY ? 0.0f : ex2(mn[i][h] - mn2);
+                    l[i][h] *= ex2(m[i][h] - m2);
+                    const float fn = ex2(mn[i][h] - mn2);
                     m[i][h] = m2;
                     mn[i][h] = mn2;
                     #pragma unroll
@@ -529,12 +526,11 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             float w[2][4];
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float base = m[i][h] == -INFINITY ? 0.0f : m[i][h], basen = mn[i][h] == -INFINITY ? 0.0f : mn[i][h];
                 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const float x = s[i][c >> 1][2 * (c & 1) + h];
-                    l[i][h] += ex2(x - base);
-                    w[h][c] = ex2(x + (tk[c].y - basen));
+                    l[i][h] += ex2(x - m[i][h]);
+                    w[h][c] = ex2(x + (tk[c].y - mn[i][h]));
                 }
             }
             #pragma unroll
@@ -604,9 +600,10 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             float sum = l[i][h];
             #pragma unroll
             for (int z = 4; z < 32; z *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, z);
-            const float f = m[i][h] == -INFINITY ? 0.0f : ex2(mn[i][h] - m[i][h]);
+            const bool none = m[i][h] == kMx4NoScore;
+            const float f = none ? 0.0f : ex2(mn[i][h] - m[i][h]);
             if (g == 0) {
-                pm[warp][r] = m[i][h];
+                pm[warp][r] = none ? -INFINITY : m[i][h];
                 pl[warp][r] = sum;
             }
             float* dst = part + (warp * Cfg::kRows + r) * Cfg::kPartStride;
