@@ -470,3 +470,14 @@ def test_refusals(mx):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"refusal {i} was accepted")
+
+
+@pytest.mark.parametrize("m,n,k,group,dtype,bias", [
+    (333, 3840, 4096, 256, "bf16", "bf16"), (130, 520, 2080, 16, "f16", None), (257, 255, 4128, 0, "f32", "f32"), (500, 2049, 7680, 64, "bf16", "f16")])
+def test_linear_few_tiles_long_k(mx, m, n, k, group, dtype, bias):
+    """Sizes with few output tiles and a long K (the product may be split along K)."""
+    check_linear(mx, m, n, k, group, dtype, bias, seed=m + n)
+    w, ws = mx.quantize_convrot_mx4(torch.randn(n, k, device="cuda") * 0.02, group)
+    x = rows(m, k, dtype, 1)
+    want = mx.convrot_mx4_linear(x, w, ws, None, group)
+    assert all(torch.equal(mx.convrot_mx4_linear(x, w, ws, None, group), want) for _ in range(3))
