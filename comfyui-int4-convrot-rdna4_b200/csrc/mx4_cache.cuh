@@ -9,6 +9,10 @@
 // 128, half a head of 256 or two heads of 64 (the second may be missing). Units
 // are numbered key or value, token, position, so a warp's units are neighbours on
 // the side of the [T, heads, D] tensors (`linear`: without a gap).
+//
+// Bound by memory. 8 heads of 128, pages of 64, groups of 64: 32768 tokens written in
+// 40 us from a view of a QKV projection (4.2 TB/s), 32 us from contiguous tensors;
+// 65536 tokens read back in 66 us (5.2 TB/s, four fifths of it writing bf16).
 #pragma once
 
 namespace convrot {

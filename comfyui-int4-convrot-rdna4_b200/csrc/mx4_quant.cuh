@@ -5,6 +5,11 @@
 // time, copying the next 32 while it works on these. Missing columns of a row's
 // last unit read as zeros, which leaves their scale bytes 0. The first `linear_units`
 // units lie one after the other in memory (rows without a gap, whole units).
+//
+// Bound by memory, in groups of 256 as much by issue (10 instructions a value, the
+// exchanged step alone 2.5). 4608 x 15360 bf16: 37 us in groups of 256 (4.8 TB/s), 33 us
+// in groups of 64, 31 us not rotated (5.8 TB/s); fp32 56 us (5.8 TB/s). Back: 30 us not
+// rotated (5.9 TB/s), 44 / 36 / 34 us in groups of 256 / 64 / 16.
 #pragma once
 
 namespace convrot {
