@@ -68,6 +68,10 @@ constexpr float kMx4NoScore = -1e30f;          // a row's reference before its f
 constexpr int kMx4AttnChunk = 32;              // tokens a warp takes at a time
 constexpr int kMx4AttnGroup = kMx4AttnWarps * kMx4AttnChunk;   // tokens a block takes at a time
 
+// Blocks a multiprocessor holds, by a thread's accumulators (rows * D / 32 of them) and
+// operands; `size` is rows / 8 * D.
+__host__ __device__ constexpr int mx4_attn_resident(int size) { return size <= 64 ? 5 : size <= 128 ? 4 : size <= 256 ? 3 : 2; }
+
 template <int D, int NT, bool SPLIT>
 struct Mx4AttnCfg {
     static constexpr int kRows = 8 * NT;
@@ -86,8 +90,7 @@ struct Mx4AttnCfg {
     static constexpr int kPartBytes = kMx4AttnWarps * kRows * kPartStride * 4;
     static constexpr int kRing = kMx4AttnWarps * kWarpBytes;
     static constexpr int kSmemBytes = kQBytes + (kRing > kPartBytes ? kRing : kPartBytes);
-    // blocks a multiprocessor holds, by a thread's accumulators (NT D / 4) and operands
-    static constexpr int kResident = NT * D <= 64 ? 5 : NT * D <= 128 ? 4 : NT * D <= 256 ? 3 : 2;
+    static constexpr int kResident = mx4_attn_resident(NT * D);
 };
 
 // Chunk position of a token's 16-byte chunk c.
