@@ -609,7 +609,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             float sum = l[i][h];
             #pragma unroll
             for (int z = 4; z < 32; z *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, z);
-            const bool none = m[i][h] == kMx4NoScore;
+            const bool none = m[i][h] == kMx4NoScore && sum == 0.0f;      // (scores that are all NaN move no reference)
             const float f = none ? 0.0f : ex2(mn[i][h] - m[i][h]);
             if (g == 0) {
                 pm[warp][r] = none ? -INFINITY : m[i][h];

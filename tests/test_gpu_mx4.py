@@ -481,3 +481,30 @@ def test_linear_few_tiles_long_k(mx, m, n, k, group, dtype, bias):
     x = rows(m, k, dtype, 1)
     want = mx.convrot_mx4_linear(x, w, ws, None, group)
     assert all(torch.equal(mx.convrot_mx4_linear(x, w, ws, None, group), want) for _ in range(3))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,nan_at", [([1, 1], 0), ([129, 129], 128), ([40, 40], 39), ([3000, 3000], 2999), ([1500, 1500], 7)])
+def test_attention_visible_nan_key_spoils_its_sequence(mx, lens, nan_at, dtype):
+    """Also where the key is the only one that a warp or a block meets."""
+    codes, scales, table, _, _ = make_cache(mx, lens, 16, 1, 128, 64, 11)
+    q = torch.randn(2, 1, 2, 128, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = mx.convrot_mx4_attention(q, codes, scales, table, n, convrot_groupsize=64)
+    scales[table[1, nan_at // 16].long(), 0, 0, nan_at % 16, 2] = 255
+    out = mx.convrot_mx4_attention(q, codes, scales, table, n, convrot_groupsize=64)
+    assert torch.equal(out[0], want[0]) and bool(want.isfinite().all())
+    assert bool(out[1].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 40, 1500])
+def test_attention_nan_query_spoils_its_row(mx, n, dtype):
+    codes, scales, table, _, _ = make_cache(mx, [n], 16, 2, 128, 64, 12)
+    q = torch.randn(1, 1, 4, 128, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    want = mx.convrot_mx4_attention(q, codes, scales, table, lens, convrot_groupsize=0)
+    q[0, 0, 2, 70] = math.nan
+    out = mx.convrot_mx4_attention(q, codes, scales, table, lens, convrot_groupsize=0)
+    assert bool(out[0, 0, 2].isnan().all())
+    assert all(torch.equal(out[0, 0, h], want[0, 0, h]) for h in (0, 1, 3))
