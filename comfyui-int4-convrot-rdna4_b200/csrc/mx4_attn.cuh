@@ -488,6 +488,28 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                     for (int c = 0; c < 4; ++c)
                         if (ci * kMx4AttnChunk + 8 * c + ktok >= sees) s[i][c >> 1][2 * (c & 1) + h] = -INFINITY;
                 }
+            // a value's block of NaN: straight to the accumulators of the rows that see its
+            // token, which are those that see the first such (a product with the weight 0 would
+            // give it to all)
+            #pragma unroll
+            for (int hf = 0; hf < D / 64; ++hf) {
+                __half* mine = vf + 64 * hf + my_pos;
+                const uint32_t nan0 = __ballot_sync(0xFFFFFFFFu, __hisnan(mine[0])), nan1 = __ballot_sync(0xFFFFFFFFu, __hisnan(mine[32]));
+                if ((nan0 | nan1) == 0) continue;
+                const uint32_t nan = g >> 2 ? nan1 : nan0;        // of this thread's channels
+                const int first = nan ? ci * kMx4AttnChunk + __ffs(nan) - 1 : n;
+                #pragma unroll
+                for (int i = 0; i < NT; ++i)
+                    #pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (first <= n - a.tq + (row0 + 8 * i + 2 * t4 + h) / per_head) {
+                            #pragma unroll
+                            for (int j = 4 * hf; j < 4 * hf + 4; ++j) o[i][j][h] = o[i][j][2 + h] = NAN;
+                        }
+                if (nan0 >> lane & 1) mine[0] = __ushort_as_half(0);
+                if (nan1 >> lane & 1) mine[32] = __ushort_as_half(0);
+                __syncwarp();
+            }
         }
         // The references m and mn need not be the maxima, only near them: they move when
         // some score is 2^8 above (f16 holds weights up to 2^15), which is rare, and only

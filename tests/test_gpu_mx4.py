@@ -508,3 +508,17 @@ def test_attention_nan_query_spoils_its_row(mx, n, dtype):
     out = mx.convrot_mx4_attention(q, codes, scales, table, lens, convrot_groupsize=0)
     assert bool(out[0, 0, 2].isnan().all())
     assert all(torch.equal(out[0, 0, h], want[0, 0, h]) for h in (0, 1, 3))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,tq,d", [(3, 3, 64), (40, 3, 128), (33, 4, 128), (300, 2, 256), (1500, 5, 64)])
+def test_attention_nan_of_the_newest_token_stays_hidden(mx, n, tq, d, dtype, which):
+    """The newest token's key or value block is NaN: only the last row sees it."""
+    codes, scales, table, ks, vs = make_cache(mx, [n], 16, 1, d, 64, 13)
+    q = torch.randn(1, tq, 2, d, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    scales[table[0, (n - 1) // 16].long(), which, 0, (n - 1) % 16, 1] = 255
+    out = mx.convrot_mx4_attention(q, codes, scales, table, lens, convrot_groupsize=64)
+    assert bool(out[0, -1, :, 0:64].isnan().all())
+    check_attention(q[:, :-1], out[:, :-1], [ks[0][:-1]], [vs[0][:-1]], [n - 1], 64, 1 / math.sqrt(d), "bf16" if dtype == torch.bfloat16 else "f16")
