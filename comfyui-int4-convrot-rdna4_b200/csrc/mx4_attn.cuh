@@ -38,8 +38,8 @@
 // Bound by issue: some 820 instructions a warp for 32 tokens of 128 (keys 160, values
 // 270, weights 200, loads and tables 110), 2.7 a cycle, half of them on the ALU pipe that
 // converts codes; the tensor pipe is busy 21 % and memory 59 %. 16 sequences of 32768,
-// 64 heads on 8 of 128: 146 us (3.9 TB/s of the cache); 32 heads on 32: 4.0 TB/s; 128 x
-// 2048: 3.3 TB/s; one of 777: 6.8 us. f16 queries cost about a fifth more (SPLIT).
+// 64 heads on 8 of 128: 146 us (3.9 TB/s of the cache); 64 of 4096, 32 heads on 32: 252 us
+// (4.5 TB/s); 128 x 2048: 3.3 TB/s; one of 777: 7.4 us. f16 queries cost about a fifth more (SPLIT).
 #pragma once
 
 namespace convrot {
