@@ -371,7 +371,7 @@ static AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longe
 
 template <typename T, int D, int NT>
 static int launch_attention(const Mx4AttnArgs& a, const AttnPlan& p, cudaStream_t stream) {
-    using Cfg = Mx4AttnCfg<D, NT, std::is_same_v<T, __half>>;
+    using Cfg = Mx4AttnCfg<D, NT>;
     auto kernel = mx4_attn_kernel<T, D, NT>;
     cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
     if (e != cudaSuccess) return static_cast<int>(e);

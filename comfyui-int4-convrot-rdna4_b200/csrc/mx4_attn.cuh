@@ -14,18 +14,18 @@
 // side of 16 and the query rows on the side of 8: S^T = K Q^T and O^T = V^T P^T.
 // Few rows then waste nothing, and tcgen05 (128 rows at least) would. A code is an
 // f16 value exactly.
-//   Scores: one pair of MMAs per block of 32 channels, its result times the
-//   block's scale in fp32. Query rows are f16 times a power of two that brings the
-//   row's largest value to 2^8.
+//   Scores: two pairs of MMAs per block of 32 channels, their result times the
+//   block's scale in fp32. Query rows are times a power of two that brings the row's
+//   largest value to 2^8.
 //   Values: a token's codes times 2^(E_b - E), E the token's largest scale
 //   exponent, are f16 values exactly (down to 2^-24 of the token's largest); the
 //   rest, 2^E, goes to the probabilities: the numerator's weights are
 //   2^(s + E - mn), with a running maximum of their own, so that they are f16 values
 //   whatever the values' range. The denominator keeps the usual weights 2^(s - m) in
 //   fp32.
-// SPLIT (f16 queries): queries and numerator weights as the sum of two f16 values,
-// so that the result is as exact as its own rounding; a bf16 result's rounding is
-// eight times coarser than what one f16 value loses.
+// Rotated queries and numerator weights are the sum of two f16 values each (22 bits):
+// with one, a seventh of the bf16 outputs and half of the f16 ones were rounded to
+// a neighbour of the nearest value.
 //
 // Columns. The contraction's order is free, so a thread's operands are whole
 // words of codes: in a tile of 8 tokens row r is token (r >> 1) + 4 (r & 1); a
@@ -35,11 +35,10 @@
 // channel. 16-byte chunks of a token are XORed so that neither read meets a bank
 // conflict.
 //
-// Bound by issue: some 820 instructions a warp for 32 tokens of 128 (keys 160, values
-// 270, weights 200, loads and tables 110), 2.7 a cycle, half of them on the ALU pipe that
-// converts codes; the tensor pipe is busy 21 % and memory 59 %. 16 sequences of 32768,
-// 64 heads on 8 of 128: 146 us (3.9 TB/s of the cache); 64 of 4096, 32 heads on 32: 252 us
-// (4.5 TB/s); 128 x 2048: 3.3 TB/s; one of 777: 7.4 us. f16 queries cost about a fifth more (SPLIT).
+// Bound by issue: the conversions of codes (ALU pipe), scales, weights and their second
+// terms, page look-ups. 16 sequences of 32768, 64 heads on 8 of 128: 177 us (3.2 TB/s of the
+// cache; 146 us with one f16 term an operand); 64 of 4096, 32 heads on 32: 314 us (3.6 TB/s);
+// 128 x 2048: 2.8 TB/s; one of 777: 7.8 us.
 #pragma once
 
 namespace convrot {
@@ -72,7 +71,7 @@ constexpr int kMx4AttnGroup = kMx4AttnWarps * kMx4AttnChunk;   // tokens a block
 // operands; `size` is rows / 8 * D.
 __host__ __device__ constexpr int mx4_attn_resident(int size) { return size <= 64 ? 5 : size <= 128 ? 4 : size <= 256 ? 3 : 2; }
 
-template <int D, int NT, bool SPLIT>
+template <int D, int NT>
 struct Mx4AttnCfg {
     static constexpr int kRows = 8 * NT;
     static constexpr int kCodeBytes = kMx4AttnChunk * D / 2;
@@ -84,8 +83,7 @@ struct Mx4AttnCfg {
     static constexpr int kTableBytes = kMx4AttnChunk * (kBlocks * 4 + kBlocks * 2 + 8);
     static constexpr int kWarpBytes = kStages * kStageBytes + kTableBytes;
     static constexpr int kQStride = D * 2 + 64;                   // bytes; + 64: two rows in distinct banks
-    static constexpr int kQRows = (SPLIT ? 2 : 1) * kRows * kQStride;     // rows, then what their rounding to f16 left
-    static constexpr int kQBytes = kQRows > kRows * D * 4 ? kQRows : kRows * D * 4;   // (first in fp32)
+    static constexpr int kQBytes = 2 * kRows * kQStride;          // rows, then what their rounding to f16 left (first in fp32)
     static constexpr int kPartStride = D + 4;                     // floats of a joined row
     static constexpr int kPartBytes = kMx4AttnWarps * kRows * kPartStride * 4;
     static constexpr int kRing = kMx4AttnWarps * kWarpBytes;
@@ -170,10 +168,9 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kMx4AttnWarps * 32, Mx4AttnCfg<D, NT, std::is_same_v<T, __half>>::kResident)
+__global__ void __launch_bounds__(kMx4AttnWarps * 32, Mx4AttnCfg<D, NT>::kResident)
 mx4_attn_kernel(Mx4AttnArgs a) {
-    constexpr bool SPLIT = std::is_same_v<T, __half>;
-    using Cfg = Mx4AttnCfg<D, NT, SPLIT>;
+    using Cfg = Mx4AttnCfg<D, NT>;
     constexpr int kB = Cfg::kBlocks, kR16 = D / 32;               // blocks; 16-byte chunks of a token
     extern __shared__ __align__(128) unsigned char mx4att[];
     __shared__ float row_scale[Cfg::kRows], pm[kMx4AttnWarps][Cfg::kRows], pl[kMx4AttnWarps][Cfg::kRows];
@@ -323,7 +320,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 const float x = qv[k][i] * to_f16[k];
                 const __half hi = __float2half_rn(x);
                 dst[lane + 32 * i] = hi;
-                if constexpr (SPLIT) dst[Cfg::kRows * Cfg::kQStride / 2 + lane + 32 * i] = __float2half_rn(x - __half2float(hi));
+                dst[Cfg::kRows * Cfg::kQStride / 2 + lane + 32 * i] = __float2half_rn(x - __half2float(hi));
             }
         }
     }
@@ -441,7 +438,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             for (int i = 0; i < NT; ++i) {
                 const unsigned char* at = q_smem + (8 * i + g) * Cfg::kQStride + blk * 64 + t4 * 16;
                 qb[i] = *reinterpret_cast<const uint4*>(at);
-                if constexpr (SPLIT) ql[i] = *reinterpret_cast<const uint4*>(at + Cfg::kRows * Cfg::kQStride);
+                ql[i] = *reinterpret_cast<const uint4*>(at + Cfg::kRows * Cfg::kQStride);
             }
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -454,10 +451,8 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                     float acc[4];
                     mma_f16_zero(acc, h0[0], h1[0], h0[1], h1[1], qb[i].x, qb[i].y);
                     mma_f16(acc, h0[2], h1[2], h0[3], h1[3], qb[i].z, qb[i].w);
-                    if constexpr (SPLIT) {
-                        mma_f16(acc, h0[0], h1[0], h0[1], h1[1], ql[i].x, ql[i].y);
-                        mma_f16(acc, h0[2], h1[2], h0[3], h1[3], ql[i].z, ql[i].w);
-                    }
+                    mma_f16(acc, h0[0], h1[0], h0[1], h1[1], ql[i].x, ql[i].y);
+                    mma_f16(acc, h0[2], h1[2], h0[3], h1[3], ql[i].z, ql[i].w);
                     s[i][c][0] = fmaf(acc[0], f0, s[i][c][0]);
                     s[i][c][1] = fmaf(acc[1], f0, s[i][c][1]);
                     s[i][c][2] = fmaf(acc[2], f1, s[i][c][2]);
@@ -568,12 +563,10 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             for (int c = 0; c < 4; ++c) {
                 const uint32_t hi = f16x2_bits(w[0][c], w[1][c]);
                 p[i][c] = movmatrix_trans(hi);
-                if constexpr (SPLIT) {
-                    __half2 r;
-                    memcpy(&r, &hi, 4);
-                    const float2 back = __half22float2(r);
-                    pr[i][c] = movmatrix_trans(f16x2_bits(w[0][c] - back.x, w[1][c] - back.y));
-                }
+                __half2 r;
+                memcpy(&r, &hi, 4);
+                const float2 back = __half22float2(r);
+                pr[i][c] = movmatrix_trans(f16x2_bits(w[0][c] - back.x, w[1][c] - back.y));
             }
         }
 
@@ -611,7 +604,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                     #pragma unroll
                     for (int i = 0; i < NT; ++i) {
                         mma_f16(o[i][4 * hf + k], a0, a1, a2, a3, p[i][2 * u], p[i][2 * u + 1]);
-                        if constexpr (SPLIT) mma_f16(o[i][4 * hf + k], a0, a1, a2, a3, pr[i][2 * u], pr[i][2 * u + 1]);
+                        mma_f16(o[i][4 * hf + k], a0, a1, a2, a3, pr[i][2 * u], pr[i][2 * u + 1]);
                     }
                 }
             }

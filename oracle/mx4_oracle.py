@@ -110,3 +110,32 @@ def attention64(q, k, v, lens, scale):
                 spread[i, t, h] = p @ np.abs(vv)
                 reach[i, t, h] = (np.abs(kk) @ np.abs(q[i, t, h])).max() * abs(scale)
     return out, spread, reach
+
+
+def rounded_apart(got, ref, dtype):
+    """Share of the outputs that are not the nearest value of their type ("bf16" or "f16") to ``ref``."""
+    import torch
+    near = torch.from_numpy(np.ascontiguousarray(ref)).to({"bf16": torch.bfloat16, "f16": torch.float16}[dtype])
+    return float((near.double() != torch.from_numpy(np.ascontiguousarray(got, np.float64))).double().mean())
+
+
+# Operands of attention as the sum of f16 values leave a relative error of at most 2^-22 a
+# factor; a score sums up to some 2^5 in magnitude, so weights and outputs are within 2^-17.
+# An output is then rounded to another value than the nearest only where it lies that near
+# to the middle of two: 2^-17 over the spacing, which is at least 2^-8 (bf16) or 2^-11 (f16)
+# of the output. Shares of the outputs:
+MOST_APART = {"bf16": 2.0 ** -9, "f16": 2.0 ** -6}
+
+
+def attention_f16_terms(q, k, v, scale, terms):
+    """One head's attention q [R, D], k, v [N, D] with queries and weights as sums of ``terms`` f16 values."""
+    def cut(x):
+        left, held = x, np.zeros_like(x)
+        for _ in range(terms):
+            part = left.astype(np.float16).astype(np.float64)
+            held, left = held + part, left - part
+        return held
+    up = np.exp2(8 - np.floor(np.log2(np.abs(q).max(-1, keepdims=True))))
+    s = cut(q * up) / up @ k.T * scale
+    p = np.exp(s - s.max(-1, keepdims=True))
+    return cut(p) @ v / p.sum(-1, keepdims=True)
