@@ -37,7 +37,8 @@ struct Mx4FewCfg {
     static constexpr int kScaleBytes = 2 * kMx4TileBytes;         // of each operand
     static constexpr int kStageBytes = kABytes + kBBytes + 2 * kScaleBytes;
     // the ranks' accumulators of this rank's tokens: memory of its own where it is
-    // small, else the ring's (after a barrier that says the ring is free everywhere)
+    // small (after a barrier that says every rank has started), else the ring's (after one
+    // that says the ring is free everywhere)
     static constexpr bool kOwnInbox = BT <= 32;
     static constexpr int kInboxBytes = BT * 128 * 4;
     static constexpr int kStages = BT == 128 ? 3 : 4;             // two blocks a multiprocessor
@@ -248,6 +249,9 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // (waited for ahead of the first store to another rank: its block has to have started,
+    // and a rank without any stage would be there at once)
+    if (Cfg::kOwnInbox && splits > 1) cluster_arrive_started();
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t tmem = *tmem_slot;
@@ -380,7 +384,8 @@ mx4_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     }
     if (splits > 1) {
         unsigned char* inbox = smem + Cfg::kInboxOffset;
-        if (!Cfg::kOwnInbox) cluster_sync();                      // every rank's ring is free
+        if constexpr (Cfg::kOwnInbox) cluster_wait_started();
+        else cluster_sync();                                      // every rank's ring is free
         if (warp >= 2) {
             const uint32_t to = smem_u32(inbox);
             if (splits == 2) few_send<2, BT>(to, tmem, rank, M, kts > 0);
