@@ -33,7 +33,7 @@ struct Mx4CacheUnit {
     int t, kv, head, part;           // part: which half of a head of 256
     int halves;                      // 64-value halves of the unit that exist
     __device__ __forceinline__ Mx4CacheUnit(int u, int per, int heads, int units) {
-        kv = 2 * u >= units;
+        kv = u >= units / 2;         // (units is even)
         const int r = kv ? u - units / 2 : u;
         t = r / per;
         const int p = r - t * per;
