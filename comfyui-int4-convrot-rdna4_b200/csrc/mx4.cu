@@ -264,6 +264,7 @@ CONVROT_API int ck_mx4_dequant(const void* codes, const void* scales, void* out,
                                void* stream) {
     if (int rc = check_matrix(out, out_dtype, codes, scales, M, K, G)) return rc;
     if (M == 0) return 0;
+    if (!aligned16(out)) return fail("out must be 16-byte aligned");
     const long long units = static_cast<long long>(M) * ((K + 127) / 128), words = static_cast<long long>(M) * K / 8;
     return with_type(out_dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -1,0 +1,23 @@
+"""What the MX4 C entries refuse before any launch (no GPU needed)."""
+import pytest
+
+from _int4 import cuda_loader
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return cuda_loader.library()
+
+
+def refuse(lib, rc, text):
+    assert rc == -1
+    assert text in lib.ck_convrot_last_error()
+
+
+@pytest.mark.parametrize("group", [0, 64])
+@pytest.mark.parametrize("dtype,size", [(0, 4), (1, 2), (2, 2)])
+def test_dequant_refuses_an_unaligned_output(lib, group, dtype, size):
+    """Values are stored 16 bytes at a time."""
+    for at in (size, 8, 24):
+        refuse(lib, lib.ck_mx4_dequant(16, 16, at, dtype, 3, 64, group, None), b"out must be 16-byte aligned")
+    assert lib.ck_mx4_dequant(16, 16, 2, dtype, 0, 64, group, None) == 0             # nothing to do
