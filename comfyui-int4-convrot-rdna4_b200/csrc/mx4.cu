@@ -299,6 +299,7 @@ CONVROT_API int ck_mx4_linear(const void* x, int dtype, long long ldx, const voi
     if (M == 0) return 0;
     if (ldx < 0 || (M > 1 && ldx < K)) return fail("ldx must be at least K");
     if (bias && (bias_dtype < 0 || bias_dtype > 2)) return fail("bias_dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    if (bias && !aligned_to(bias, type_size(bias_dtype))) return fail("bias is not aligned to its type");
     if (!out || !aligned16(out)) return fail("out must be 16-byte aligned");
     const size_t need = ck_mx4_linear_workspace_size(M, K);
     if (need && (!workspace || !aligned_to(workspace, 256))) return fail("the workspace must be 256-byte aligned");

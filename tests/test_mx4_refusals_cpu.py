@@ -21,3 +21,9 @@ def test_dequant_refuses_an_unaligned_output(lib, group, dtype, size):
     for at in (size, 8, 24):
         refuse(lib, lib.ck_mx4_dequant(16, 16, at, dtype, 3, 64, group, None), b"out must be 16-byte aligned")
     assert lib.ck_mx4_dequant(16, 16, 2, dtype, 0, 64, group, None) == 0             # nothing to do
+
+
+@pytest.mark.parametrize("m", [4, 20])
+def test_linear_refuses_a_bias_that_is_not_aligned_to_its_type(lib, m):
+    for kind, at in ((0, 18), (1, 17), (2, 33)):
+        refuse(lib, lib.ck_mx4_linear(16, 1, 64, 16, 16, at, kind, 16, m, 8, 64, 64, 256, 1 << 20, None), b"bias is not aligned")
