@@ -498,7 +498,7 @@ CONVROT_API int ck_mx4_attention(const void* q, int dtype, long long q_seq, long
     if (dtype != 1 && dtype != 2) return fail("queries must be bf16 (1) or f16 (2)");
     if (B < 0 || tq <= 0 || hq <= 0 || hq % hkv) return fail("query heads must be a positive multiple of the cache's heads");
     if (table_pages < 0 || table_ld < table_pages) return fail("bad block table shape");
-    if (static_cast<long long>(table_pages) * page > 0x7FFFFFFFll) return fail("block table longer than 2^31 tokens");
+    if (static_cast<long long>(table_pages) * page > kMx4MostTokens) return fail("block table longer than 2^31 - 1024 tokens");
     if (B == 0) return 0;
     if (static_cast<long long>(B) * tq * hq > 0x7FFFFFFFll) return fail("too many query rows");
     if (!q || !lens || !out || (table_pages && !table)) return fail("null pointer");

@@ -62,6 +62,8 @@ struct Mx4AttnArgs {
 
 constexpr int kMx4AttnWarps = 4;
 constexpr int kMx4MostSplits = 256;            // of one sequence
+constexpr long long kMx4MostTokens = 0x7FFFFFFFll - 1023;      // of one sequence: positions, and the chunks and groups
+                                                               // looked at beyond the last, fit 32 bits
 constexpr float kMx4NoScore = -1e30f;          // a row's reference before its first score (finite: -inf less it is -inf);
                                                // scores below it count as hidden
 constexpr int kMx4AttnChunk = 32;              // tokens a warp takes at a time
@@ -153,12 +155,9 @@ __device__ __forceinline__ void cp_async_small(void* dst, const void* src, bool 
                  :: "r"(smem_u32(dst)), "l"(src), "n"(BYTES), "r"(held ? BYTES : 0) : "memory");
 }
 
-// Chunks [first, end) of 32 tokens of a sequence of `n` tokens that `split` of
-// `splits` takes: whole groups of a block, evenly.
-__device__ __forceinline__ int mx4_split_groups(int n, int splits) {
-    const int groups = (n + kMx4AttnGroup - 1) / kMx4AttnGroup;
-    return (groups + splits - 1) / splits;
-}
+// Groups of tokens of a sequence of `n` tokens, and those that each of `splits` takes.
+__device__ __forceinline__ int mx4_groups(int n) { return (n + kMx4AttnGroup - 1) / kMx4AttnGroup; }
+__device__ __forceinline__ int mx4_split_groups(int n, int splits) { return (mx4_groups(n) + splits - 1) / splits; }
 
 // Transposes an 8 x 8 tile of 16-bit values held as an MMA fragment.
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
@@ -739,8 +738,8 @@ __global__ void __launch_bounds__(256) mx4_attn_join_kernel(Mx4AttnArgs a, int t
     if (index >= a.B * a.hkv * rows_all) return;                   // (not wide: whole warps leave, no barrier below)
     const int row = index % rows_all, hk = index / rows_all % a.hkv, b = index / rows_all / a.hkv;
     const int n = max(0, static_cast<int>(min(static_cast<long long>(a.lens[b]), a.cap)));
-    const int per_split = mx4_split_groups(n, a.splits) * kMx4AttnGroup;
-    const int held = per_split ? (n + per_split - 1) / per_split : 0;          // splits that hold tokens
+    const int per_split = mx4_split_groups(n, a.splits);
+    const int held = per_split ? (mx4_groups(n) + per_split - 1) / per_split : 0;          // splits that hold tokens
     const size_t at = ((static_cast<size_t>(b) * a.hkv + hk) * a.row_tiles + row / tile_rows) * a.splits * tile_rows + row % tile_rows;
     const float2* ml = a.part_ml + at;
     float top = -INFINITY, sum = 0.0f;

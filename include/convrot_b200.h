@@ -363,7 +363,8 @@ size_t ck_mx4_attention_workspace_size(int B, int tq, int hq, int hkv, int d, lo
  *   multiple of hkv (query head h reads cache head h / (hq / hkv));
  *   table int32 [B, table_pages] (row stride table_ld): token j of sequence b is
  *   token j % page of page table[b][j / page]; a page outside [0, pages) hides
- *   its tokens; lens int32 [B] tokens in the cache (cut at table_pages * page);
+ *   its tokens; lens int32 [B] tokens in the cache (cut at table_pages * page,
+ *   which may be 2^31 - 1024 at most);
  *   query t sees tokens up to position lens[b] - tq + t; one that sees none
  *   gives zeros; out [B, tq, hq, d] (16-byte aligned) in dtype. */
 int ck_mx4_attention(const void* q, int dtype, long long q_seq, long long q_token, long long q_head,

@@ -27,3 +27,15 @@ def test_dequant_refuses_an_unaligned_output(lib, group, dtype, size):
 def test_linear_refuses_a_bias_that_is_not_aligned_to_its_type(lib, m):
     for kind, at in ((0, 18), (1, 17), (2, 33)):
         refuse(lib, lib.ck_mx4_linear(16, 1, 64, 16, 16, at, kind, 16, m, 8, 64, 64, 256, 1 << 20, None), b"bias is not aligned")
+
+
+def test_attention_refuses_tables_at_the_end_of_32_bit_positions(lib):
+    """Token positions, and those of the chunks and groups that end behind the last token, are 32-bit numbers."""
+    import ctypes
+
+    def attention(per, page):
+        return lib.ck_mx4_attention(16, 1, 1, 1, 1, 16, 16, 8, page, 16, per, per, 16, 16, 1, 1, 4, 2, 64, 64,
+                                    ctypes.c_float(1.0), 0, 0, None)
+    for per, page in ((2 ** 31 - 1, 1), (2 ** 27 - 1, 16), (2 ** 31 - 1000, 1), (2 ** 25, 64)):
+        refuse(lib, attention(per, page), b"block table longer")
+    refuse(lib, attention(2 ** 26 - 64, 32), b"workspace")                          # accepted as a length
