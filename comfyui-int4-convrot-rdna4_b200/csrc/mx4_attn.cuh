@@ -18,11 +18,14 @@
 //   block's scale in fp32. Query rows are times a power of two that brings the row's
 //   largest value to 2^8.
 //   Values: a token's codes times 2^(E_b - E), E the token's largest scale
-//   exponent, are f16 values exactly (down to 2^-24 of the token's largest); the
-//   rest, 2^E, goes to the probabilities: the numerator's weights are
-//   2^(s + E - mn), with a running maximum of their own, so that they are f16 values
-//   whatever the values' range. The denominator keeps the usual weights 2^(s - m) in
-//   fp32.
+//   exponent, are f16 values exactly; the rest, 2^E, goes to the probabilities: the
+//   numerator's weights are 2^(s + E - mn), with a reference of their own, so that
+//   they are f16 values whatever the values' range. The denominator keeps the usual
+//   weights 2^(s - m) in fp32.
+//   A weight is off by 2^-25 at most where the row's largest is 2^8 to 2^15. That is
+//   relative to the token with the largest values: a channel block whose values are far
+//   smaller would lose its own precision, so chunks with a block more than 2^8 below the
+//   largest seen so far take fp32 products instead (three to four times as long).
 // Rotated queries and numerator weights are the sum of two f16 values each (22 bits):
 // with one, a seventh of the bf16 outputs and half of the f16 ones were rounded to
 // a neighbour of the nearest value.
@@ -36,9 +39,9 @@
 // conflict.
 //
 // Bound by issue: the conversions of codes (ALU pipe), scales, weights and their second
-// terms, page look-ups. 16 sequences of 32768, 64 heads on 8 of 128: 177 us (3.2 TB/s of the
-// cache; 146 us with one f16 term an operand); 64 of 4096, 32 heads on 32: 314 us (3.6 TB/s);
-// 128 x 2048: 2.8 TB/s; one of 777: 7.8 us.
+// terms, page look-ups. 16 sequences of 32768, 64 heads on 8 of 128: 179 us (3.2 TB/s of the
+// cache; 146 us with one f16 term an operand); 64 of 4096, 32 heads on 32: 317 us (3.6 TB/s);
+// 128 x 2048: 2.8 TB/s; one of 777: 7.9 us.
 #pragma once
 
 namespace convrot {
@@ -66,6 +69,7 @@ constexpr long long kMx4MostTokens = 0x7FFFFFFFll - 1023;      // of one sequenc
                                                                // looked at beyond the last, fit 32 bits
 constexpr float kMx4NoScore = -1e30f;          // a row's reference before its first score (finite: -inf less it is -inf);
                                                // scores below it count as hidden
+constexpr int kMx4NarrowBits = 8;              // blocks of values this many powers of two apart share f16 weights
 constexpr int kMx4AttnChunk = 32;              // tokens a warp takes at a time
 constexpr int kMx4AttnGroup = kMx4AttnWarps * kMx4AttnChunk;   // tokens a block takes at a time
 
@@ -343,6 +347,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
     }
     const int sees_all = n - a.tq + row0 / per_head + 1;          // tokens that every row of the tile sees
     const int ktok = (g >> 1) + 4 * (g & 1);                      // this thread's token of each tile of 8
+    int most_seen = 0;                                            // largest scale byte of the warp's values so far
 
     for (int it = 0; ci < c_end; ci += kMx4AttnWarps, ++it) {
         if (ahead < c_end) issue((it + Cfg::kStages - 1) % Cfg::kStages, ahead, page);
@@ -353,6 +358,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         __syncwarp();
         const unsigned char* st = ring + (it % Cfg::kStages) * Cfg::kStageBytes;
         const unsigned char* vcodes = st + Cfg::kCodeBytes;
+        bool narrow = true;                                       // the chunk's blocks of values are near the largest
         // this lane's token: factors of its keys and values
         {
             const unsigned char* sc = st + 2 * Cfg::kCodeBytes + lane * Cfg::kScaleSlot;
@@ -368,7 +374,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 ks[1] = *reinterpret_cast<const uint32_t*>(sc + 4);
                 vs[1] = *reinterpret_cast<const uint32_t*>(sc + Cfg::kScaleBytes + 4);
             }
-            int top = 0;
+            int top = 0, low = 255;                               // (blocks of zeros have 0)
             float kv[kB];
             __half vv[kB];
             bool bad = false;                                     // a block of NaN
@@ -378,6 +384,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 kv[i] = __uint_as_float(ek << 23);                // (2^-127 counts as 0)
                 const int ev = (vs[i / 4] >> (8 * (i % 4))) & 255u;
                 top = max(top, ev);
+                low = min(low, ev ? ev : 255);
                 bad |= ek == 255u;
             }
             bad |= top == 255;
@@ -386,7 +393,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 const int ev = (vs[i / 4] >> (8 * (i % 4))) & 255u;
                 vv[i] = __float2half_rn(__uint_as_float(static_cast<uint32_t>(max(ev - top + 127, 0)) << 23));
             }
-            if (__any_sync(0xFFFFFFFFu, bad)) {
+            if (__any_sync(0xFFFFFFFFu, bad || top > most_seen || low < most_seen - kMx4NarrowBits)) {
                 top = 0;
                 #pragma unroll
                 for (int i = 0; i < kB; ++i) {
@@ -399,6 +406,8 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                     const int ev = (vs[i / 4] >> (8 * (i % 4))) & 255u;
                     vv[i] = ev == 255 ? __ushort_as_half(0x7FFF) : __float2half_rn(__uint_as_float(static_cast<uint32_t>(max(ev - top + 127, 0)) << 23));
                 }
+                most_seen = max(most_seen, __reduce_max_sync(0xFFFFFFFFu, top));
+                narrow = __reduce_min_sync(0xFFFFFFFFu, low) >= most_seen - kMx4NarrowBits;
             }
             #pragma unroll
             for (int i = 0; i < kB; i += 2) *reinterpret_cast<float2*>(kf + lane * kB + i) = make_float2(kv[i], kv[i + 1]);
@@ -464,7 +473,6 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         float2 tk[4];                                             // {0 or -inf, E} of this thread's tokens
         #pragma unroll
         for (int c = 0; c < 4; ++c) tk[c] = info[8 * c + ktok];
-        uint32_t p[NT][4], pr[NT][4];                             // numerator weights as MMA operands, tile by tile of 8 tokens
         #pragma unroll
         for (int i = 0; i < NT; ++i)
             #pragma unroll
@@ -506,8 +514,10 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             }
         }
         // The references m and mn need not be the maxima, only near them: they move when
-        // some score is 2^8 above (f16 holds weights up to 2^15), which is rare, and only
-        // then do lanes compare and accumulators get a new scale.
+        // some weight is above 2^8 in the denominator or 2^15 in the numerator (f16 holds it),
+        // which is rare, and only then do lanes compare and accumulators get a new scale. mn
+        // moves to 2^8 below the maximum, so that f16 holds small weights too (2^12 below moves
+        // more often: 37 sequences up to 4096 of heads of 64, 4 tokens: 62.6 against 60.2 us).
         bool above = false;
         const float most = fmaxf(fmaxf(tk[0].y, tk[1].y), fmaxf(tk[2].y, tk[3].y));   // (s + E is at most max s + max E)
         #pragma unroll
@@ -515,7 +525,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float top = fmaxf(fmaxf(s[i][0][h], s[i][0][2 + h]), fmaxf(s[i][1][h], s[i][1][2 + h]));
-                above |= top > m[i][h] + 8.0f || top + most > mn[i][h] + 8.0f;
+                above |= top > m[i][h] + 8.0f || top + most > mn[i][h] + 15.0f;
             }
         if (__any_sync(0xFFFFFFFFu, above)) {
             #pragma unroll
@@ -534,7 +544,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
                         topn = fmaxf(topn, __shfl_xor_sync(0xFFFFFFFFu, topn, z));
                     }
-                    const float m2 = fmaxf(m[i][h], top), mn2 = fmaxf(mn[i][h], topn);
+                    const float m2 = fmaxf(m[i][h], top), mn2 = fmaxf(mn[i][h], topn - 8.0f);
                     l[i][h] *= ex2(m[i][h] - m2);
                     const float fn = ex2(mn[i][h] - mn2);
                     m[i][h] = m2;
@@ -546,6 +556,54 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                     }
                 }
         }
+        if (!narrow) {
+            #pragma unroll
+            for (int i = 0; i < NT; ++i)
+                #pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float& x = s[i][c >> 1][2 * (c & 1) + h];
+                        l[i][h] += ex2(x - m[i][h]);
+                        x = ex2(x + (tk[c].y - mn[i][h]));
+                    }
+            // blocks of values far apart: fp32 products, token by token, with the block's own
+            // scale (NaN and its masking as in the table of factors)
+            #pragma unroll
+            for (int c = 0; c < 4; ++c)
+                #pragma unroll 1
+                for (int j = 0; j < 8; ++j) {
+                    const int tok = 8 * c + j, from = (2 * (j & 3) + (j >> 2)) * 4 + t4;
+                    float x[NT][2];
+                    #pragma unroll
+                    for (int i = 0; i < NT; ++i)
+                        #pragma unroll
+                        for (int h = 0; h < 2; ++h) x[i][h] = __shfl_sync(0xFFFFFFFFu, s[i][c >> 1][2 * (c & 1) + h], from);
+                    const uint32_t place = reinterpret_cast<const uint32_t*>(st + 2 * Cfg::kCodeBytes + 2 * Cfg::kScaleBytes)[tok];
+                    const unsigned char* sc = st + 2 * Cfg::kCodeBytes + Cfg::kScaleBytes + tok * Cfg::kScaleSlot + (D == 64 ? 2 * ((place + v_off) & 1) : 0);
+                    const int top = static_cast<int>(info[tok].y) + 127;
+                    #pragma unroll
+                    for (int hf = 0; hf < D / 64; ++hf) {
+                        const int blk = 2 * hf + (g >> 2), ev = sc[blk];
+                        const float f = ev == 255 ? __half2float(vf[blk * 32 + (tok & ~7) + 2 * (tok & 3) + ((tok >> 2) & 1)])
+                                                  : __uint_as_float(static_cast<uint32_t>(max(ev - top + 127, 0)) << 23);
+                        float v[8];
+                        mx4_decode8(*reinterpret_cast<const uint32_t*>(vcodes + tok * (D / 2) + mx4_chunk_pos<D>(tok, blk) * 16 + (g & 3) * 4), v);
+                        #pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            #pragma unroll
+                            for (int i = 0; i < NT; ++i)
+                                #pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    o[i][4 * hf + k][h] = fmaf(x[i][h], v[2 * k] * f, o[i][4 * hf + k][h]);
+                                    o[i][4 * hf + k][2 + h] = fmaf(x[i][h], v[2 * k + 1] * f, o[i][4 * hf + k][2 + h]);
+                                }
+                    }
+                }
+            __syncwarp();
+            continue;
+        }
+        uint32_t p[NT][4], pr[NT][4];                             // numerator weights as MMA operands, tile by tile of 8 tokens
         #pragma unroll
         for (int i = 0; i < NT; ++i) {
             float w[2][4];

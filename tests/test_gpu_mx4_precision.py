@@ -30,3 +30,59 @@ def test_attention_outputs_are_the_nearest_values(mx, lens, tq, hq, hkv, d, grou
     out = mx.convrot_mx4_attention(q, codes, scales, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), convrot_groupsize=group)
     apart = orc.rounded_apart(f64(out), expected(q, ks, vs, lens, group, 1 / math.sqrt(d)), dtype)
     assert apart <= orc.MOST_APART[dtype], apart
+
+
+def set_values(codes, scales, table, at, v):
+    """Writes values v [N, heads, D] (64 bits), unrotated, as the cache's tokens 0 .. of its only sequence."""
+    c, e = orc.encode(v)
+    page = codes.shape[3]
+    j = torch.arange(v.shape[0])
+    pages, off = table[0].cpu().long()[j // page], j % page
+    codes[pages.cuda(), at, :, off.cuda()] = torch.from_numpy(orc.pack(c)).cuda()
+    scales[pages.cuda(), at, :, off.cuda()] = torch.from_numpy(e).cuda()
+    return orc.decode(c, e)
+
+
+@pytest.mark.parametrize("dtype,ratio", [("bf16", 2.0 ** 6), ("bf16", 2.0 ** 9), ("bf16", 2.0 ** 14), ("bf16", 2.0 ** 20), ("bf16", 2.0 ** 40), ("bf16", 2.0 ** 100),
+                                         ("f16", 2.0 ** 6), ("f16", 2.0 ** 9), ("f16", 2.0 ** 12)])
+@pytest.mark.parametrize("each", [True, False])
+@pytest.mark.parametrize("n,tq,hq,d", [(70, 1, 16, 64), (300, 2, 8, 128), (1500, 1, 32, 128), (300, 16, 2, 128), (200, 8, 2, 256), (500, 32, 1, 64)])
+def test_attention_channels_of_different_magnitudes(mx, n, tq, hq, d, each, ratio, dtype):  # noqa: F811
+    """Channel blocks whose values differ by a ratio, in every token or (not ``each``) with the
+    large block in the even tokens and the others in the odd ones only: every channel keeps
+    the precision of its own values."""
+    codes, scales, table, ks, vs = make_cache(mx, [n], 16, 1, d, 0, 21)
+    v = np.random.default_rng(3).standard_normal((n, 1, d))
+    v[..., 32:64] *= ratio
+    if not each:
+        v[::2, :, :32] = v[::2, :, 64:] = 0
+        v[1::2, :, 32:64] = 0
+    vs = [set_values(codes, scales, table, 1, v)]
+    q = torch.randn(1, tq, hq, d, generator=torch.Generator().manual_seed(6)).to(DT[dtype]).cuda()
+    out = f64(mx.convrot_mx4_attention(q, codes, scales, table, torch.tensor([n], dtype=torch.int32, device="cuda"), convrot_groupsize=0))
+    ref = expected(q, ks, vs, [n], 0, 1 / math.sqrt(d))
+    for part in (slice(0, 32), slice(32, 64), slice(64, d)):
+        apart = orc.rounded_apart(out[..., part], ref[..., part], dtype) if part.stop > part.start else 0.0
+        assert apart <= 2 * orc.MOST_APART[dtype], (part, apart)               # (twice: down to 512 outputs a part)
+
+
+@pytest.mark.parametrize("d,bits", [(64, 16), (128, 24), (128, 27), (256, 20)])
+def test_attention_of_many_small_weights(mx, d, bits):  # noqa: F811
+    """One token outweighs thousands by 2^bits and has no values in a block that they have. A
+    weight is off by 2^-25 where the largest product of weight and values is 2^8 at
+    least, so an output by 2^-33 of that product for each token, beside the 2^-17 of every operand."""
+    n = 4000
+    codes, scales, table, _, _ = make_cache(mx, [n], 64, 1, d, 0, 22)
+    k = np.zeros((n, 1, d))
+    k[0, 0, 0] = 4.0
+    v = np.full((n, 1, d), 1.5)
+    v[0, :, :32] = 0
+    ks, vs = [set_values(codes, scales, table, 0, k)], [set_values(codes, scales, table, 1, v)]
+    q = torch.zeros(1, 1, 8, d, dtype=torch.bfloat16, device="cuda")
+    q[0, 0, :, 0] = torch.linspace(0.9, 1.1, 8)
+    scale = bits * math.log(2) / 4
+    out = f64(mx.convrot_mx4_attention(q, codes, scales, table, torch.tensor([n], dtype=torch.int32, device="cuda"), scale, 0))
+    ref = expected(q, ks, vs, [n], 0, scale)
+    tol = 2.0 ** -8 * np.abs(ref) + 2.0 ** -17 * np.abs(ref) + n * 2.0 ** -33 * 1.5
+    err = np.abs(out - ref)
+    assert (err <= tol).all(), (err / tol).max()
