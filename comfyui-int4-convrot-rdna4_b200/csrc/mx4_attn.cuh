@@ -381,7 +381,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             #pragma unroll
             for (int i = 0; i < kB; ++i) {
                 const uint32_t ek = (ks[i / 4] >> (8 * (i % 4))) & 255u;
-                kv[i] = __uint_as_float(ek << 23);                // (2^-127 counts as 0)
+                kv[i] = __uint_as_float(max(ek << 23, 0x00400000u));          // (0: the subnormal 2^-127)
                 const int ev = (vs[i / 4] >> (8 * (i % 4))) & 255u;
                 top = max(top, ev);
                 low = min(low, ev ? ev : 255);

@@ -86,3 +86,34 @@ def test_attention_of_many_small_weights(mx, d, bits):  # noqa: F811
     tol = 2.0 ** -8 * np.abs(ref) + 2.0 ** -17 * np.abs(ref) + n * 2.0 ** -33 * 1.5
     err = np.abs(out - ref)
     assert (err <= tol).all(), (err / tol).max()
+
+
+def test_attention_of_far_blocks_and_a_hidden_nan(mx):  # noqa: F811
+    """Values far apart and a NaN block in the newest token: rows that do not see it keep their result."""
+    n, tq, d = 75, 3, 128
+    codes, scales, table, ks, _ = make_cache(mx, [n], 16, 1, d, 0, 26)
+    v = np.random.default_rng(4).standard_normal((n, 1, d))
+    v[:, :, 64:96] *= 2.0 ** 30
+    vs = [set_values(codes, scales, table, 1, v)]
+    scales[table[0, (n - 1) // 16].long(), 1, 0, (n - 1) % 16, 1] = 255
+    q = torch.randn(1, tq, 4, d, generator=torch.Generator().manual_seed(9)).bfloat16().cuda()
+    out = f64(mx.convrot_mx4_attention(q, codes, scales, table, torch.tensor([n], dtype=torch.int32, device="cuda"), convrot_groupsize=0))
+    ref = expected(q, ks, vs, [n], 0, d ** -0.5)
+    seen = np.zeros((tq, 1, d), bool)
+    seen[-1, :, 32:64] = True
+    assert np.array_equal(np.isnan(out[0]), np.broadcast_to(seen, out[0].shape))
+    apart = orc.rounded_apart(np.where(seen, 0, out[0]), np.where(seen, 0, ref[0]), "bf16")
+    assert apart <= 2 * orc.MOST_APART["bf16"], apart
+
+
+def test_attention_keys_of_the_smallest_scale(mx):  # noqa: F811
+    """Keys whose scale byte is 0 (2^-127) are not zeros: queries of 2^120 bring the scores near 1."""
+    n, d = 60, 128
+    codes, scales, table, _, vs = make_cache(mx, [n], 16, 1, d, 0, 23)
+    rng = np.random.default_rng(1)
+    ks = [set_values(codes, scales, table, 0, rng.standard_normal((n, 1, d)) * 2.0 ** -126)]
+    assert ks[0].any() and not scales[table[0].long(), 0, 0].reshape(-1, d // 32)[:n].any()
+    q = (torch.randn(1, 1, 64, d, generator=torch.Generator().manual_seed(7)) * 2.0 ** 120).bfloat16().cuda()
+    out = mx.convrot_mx4_attention(q, codes, scales, table, torch.tensor([n], dtype=torch.int32, device="cuda"), 8.0, 0)
+    apart = orc.rounded_apart(f64(out), expected(q, ks, vs, [n], 0, 8.0), "bf16")
+    assert apart <= orc.MOST_APART["bf16"], apart
