@@ -19,9 +19,10 @@
 //   largest value to 2^8.
 //   Values: a token's codes times 2^(E_b - E), E the token's largest scale
 //   exponent, are f16 values exactly; the rest, 2^E, goes to the probabilities: the
-//   numerator's weights are 2^(s + E - mn), with a reference of their own, so that
-//   they are f16 values whatever the values' range. The denominator keeps the usual
-//   weights 2^(s - m) in fp32.
+//   numerator's weights are 2^((s - m) + (E - dn)), with a reference dn of their own, so
+//   that they are f16 values whatever the values' range. The denominator keeps the
+//   usual weights 2^(s - m) in fp32. (dn is relative to m: large scores would take the
+//   bits of an E added to them.)
 //   A weight is off by 2^-25 at most where the row's largest is 2^8 to 2^15. That is
 //   relative to the token with the largest values: a channel block whose values are far
 //   smaller would lose its own precision, so chunks with a block more than 2^8 below the
@@ -330,7 +331,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
     __syncthreads();
 
     float o[NT][D / 16][4];                                       // channels g, g + 8 of each 16; rows 2t, 2t + 1
-    float m[NT][2], mn[NT][2], l[NT][2], rs[NT][2];               // rows 2t, 2t + 1 of each 8
+    float m[NT][2], dn[NT][2], l[NT][2], rs[NT][2];               // rows 2t, 2t + 1 of each 8
     #pragma unroll
     for (int i = 0; i < NT; ++i) {
         #pragma unroll
@@ -340,7 +341,8 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = 8 * i + 2 * t4 + h;
-            m[i][h] = mn[i][h] = kMx4NoScore;
+            m[i][h] = kMx4NoScore;
+            dn[i][h] = 0.0f;
             l[i][h] = 0.0f;
             rs[i][h] = row_scale[r];
         }
@@ -513,9 +515,9 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 __syncwarp();
             }
         }
-        // The references m and mn need not be the maxima, only near them: they move when
+        // The references m and dn need not be the maxima, only near them: they move when
         // some weight is above 2^8 in the denominator or 2^15 in the numerator (f16 holds it),
-        // which is rare, and only then do lanes compare and accumulators get a new scale. mn
+        // which is rare, and only then do lanes compare and accumulators get a new scale. dn
         // moves to 2^8 below the maximum, so that f16 holds small weights too (2^12 below moves
         // more often: 37 sequences up to 4096 of heads of 64, 4 tokens: 62.6 against 60.2 us).
         bool above = false;
@@ -525,30 +527,27 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float top = fmaxf(fmaxf(s[i][0][h], s[i][0][2 + h]), fmaxf(s[i][1][h], s[i][1][2 + h]));
-                above |= top > m[i][h] + 8.0f || top + most > mn[i][h] + 15.0f;
+                above |= top > m[i][h] + 8.0f || (top - m[i][h]) + most > dn[i][h] + 15.0f;
             }
         if (__any_sync(0xFFFFFFFFu, above)) {
             #pragma unroll
             for (int i = 0; i < NT; ++i)
                 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float top = kMx4NoScore, topn = kMx4NoScore;
+                    float top = m[i][h], topn = -INFINITY;
                     #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float x = s[i][c >> 1][2 * (c & 1) + h];
-                        top = fmaxf(top, x);
-                        topn = fmaxf(topn, x + tk[c].y);
-                    }
+                    for (int c = 0; c < 4; ++c) top = fmaxf(top, s[i][c >> 1][2 * (c & 1) + h]);
                     #pragma unroll
-                    for (int z = 4; z < 32; z *= 2) {
-                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
-                        topn = fmaxf(topn, __shfl_xor_sync(0xFFFFFFFFu, topn, z));
-                    }
-                    const float m2 = fmaxf(m[i][h], top), mn2 = fmaxf(mn[i][h], topn - 8.0f);
-                    l[i][h] *= ex2(m[i][h] - m2);
-                    const float fn = ex2(mn[i][h] - mn2);
-                    m[i][h] = m2;
-                    mn[i][h] = mn2;
+                    for (int z = 4; z < 32; z *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, z));
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) topn = fmaxf(topn, (s[i][c >> 1][2 * (c & 1) + h] - top) + tk[c].y);
+                    #pragma unroll
+                    for (int z = 4; z < 32; z *= 2) topn = fmaxf(topn, __shfl_xor_sync(0xFFFFFFFFu, topn, z));
+                    const float down = m[i][h] - top, was = dn[i][h] + down;
+                    l[i][h] *= ex2(down);
+                    m[i][h] = top;
+                    dn[i][h] = fmaxf(was, topn - 8.0f);
+                    const float fn = ex2(was - dn[i][h]);
                     #pragma unroll
                     for (int j = 0; j < D / 16; ++j) {
                         o[i][j][h] *= fn;
@@ -565,7 +564,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                     for (int c = 0; c < 4; ++c) {
                         float& x = s[i][c >> 1][2 * (c & 1) + h];
                         l[i][h] += ex2(x - m[i][h]);
-                        x = ex2(x + (tk[c].y - mn[i][h]));
+                        x = ex2((x - m[i][h]) + (tk[c].y - dn[i][h]));
                     }
             // blocks of values far apart: fp32 products, token by token, with the block's own
             // scale (NaN and its masking as in the table of factors)
@@ -613,7 +612,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 for (int c = 0; c < 4; ++c) {
                     const float x = s[i][c >> 1][2 * (c & 1) + h];
                     l[i][h] += ex2(x - m[i][h]);
-                    w[h][c] = ex2(x + (tk[c].y - mn[i][h]));
+                    w[h][c] = ex2((x - m[i][h]) + (tk[c].y - dn[i][h]));
                 }
             }
             #pragma unroll
@@ -682,7 +681,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             #pragma unroll
             for (int z = 4; z < 32; z *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, z);
             const bool none = m[i][h] == kMx4NoScore && sum == 0.0f;      // (scores that are all NaN move no reference)
-            const float f = none ? 0.0f : ex2(mn[i][h] - m[i][h]);
+            const float f = none ? 0.0f : ex2(dn[i][h]);
             if (g == 0) {
                 pm[warp][r] = none ? -INFINITY : m[i][h];
                 pl[warp][r] = sum;

@@ -117,3 +117,21 @@ def test_attention_keys_of_the_smallest_scale(mx):  # noqa: F811
     out = mx.convrot_mx4_attention(q, codes, scales, table, torch.tensor([n], dtype=torch.int32, device="cuda"), 8.0, 0)
     apart = orc.rounded_apart(f64(out), expected(q, ks, vs, [n], 0, 8.0), "bf16")
     assert apart <= orc.MOST_APART["bf16"], apart
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("size", [3e2, 1e4, 1e6, -1e4, -1e6, -1e9, 1e12])
+@pytest.mark.parametrize("n,d", [(1, 64), (40, 128), (3000, 64)])
+def test_attention_of_large_scores(mx, n, d, size, dtype):  # noqa: F811
+    """Two tokens share the highest score, all others are far below it: the result is the
+    mean of their values, however large the scores are."""
+    codes, scales, table, _, vs = make_cache(mx, [n], 16, 1, d, 0, 27)
+    k = np.full((n, 1, d), 0.5 if size > 0 else 1.0)
+    best = sorted({n // 3, n - 1})
+    k[best] = 1.0 if size > 0 else 0.5
+    set_values(codes, scales, table, 0, k)
+    q = torch.ones(1, 1, 2, d, dtype=DT[dtype], device="cuda") * math.copysign(1.0, size)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    out = mx.convrot_mx4_attention(q, codes, scales, table, lens, abs(size) / d, 0)
+    want = torch.from_numpy(vs[0][best].mean(0)).to(DT[dtype])
+    assert torch.equal(out[0, 0].cpu().float(), want.repeat(2, 1).float())
