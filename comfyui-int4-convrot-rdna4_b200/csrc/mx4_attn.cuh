@@ -68,8 +68,8 @@ constexpr int kMx4AttnWarps = 4;
 constexpr int kMx4MostSplits = 256;            // of one sequence
 constexpr long long kMx4MostTokens = 0x7FFFFFFFll - 1023;      // of one sequence: positions, and the chunks and groups
                                                                // looked at beyond the last, fit 32 bits
-constexpr float kMx4NoScore = -1e30f;          // a row's reference before its first score (finite: -inf less it is -inf);
-                                               // scores below it count as hidden
+constexpr float kMx4NoScore = -3.402823466e38f;        // a row's reference before its first score: the lowest finite
+                                                       // value (-inf less it is -inf)
 constexpr int kMx4NarrowBits = 8;              // blocks of values this many powers of two apart share f16 weights
 constexpr int kMx4AttnChunk = 32;              // tokens a warp takes at a time
 constexpr int kMx4AttnGroup = kMx4AttnWarps * kMx4AttnChunk;   // tokens a block takes at a time

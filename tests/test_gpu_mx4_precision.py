@@ -135,3 +135,18 @@ def test_attention_of_large_scores(mx, n, d, size, dtype):  # noqa: F811
     out = mx.convrot_mx4_attention(q, codes, scales, table, lens, abs(size) / d, 0)
     want = torch.from_numpy(vs[0][best].mean(0)).to(DT[dtype])
     assert torch.equal(out[0, 0].cpu().float(), want.repeat(2, 1).float())
+
+
+@pytest.mark.parametrize("n", [1, 40, 3000])
+def test_attention_of_very_low_scores(mx, n):  # noqa: F811
+    """All of a row's scores lie below -1e30: the highest one's values are the result."""
+    d = 64
+    codes, scales, table, _, vs = make_cache(mx, [n], 16, 1, d, 0, 24)
+    k = np.full((n, 1, d), 1.5e17)
+    k[n // 2] = 1e17
+    set_values(codes, scales, table, 0, k)
+    q = torch.full((1, 1, 2, d), -2e18, dtype=torch.bfloat16, device="cuda")
+    out = mx.convrot_mx4_attention(q, codes, scales, table, torch.tensor([n], dtype=torch.int32, device="cuda"), 0.25, 0)
+    assert np.array_equal(f64(out)[0, 0], np.repeat(vs[0][n // 2], 2, 0))
+    none = mx.convrot_mx4_attention(q, codes, scales, table, torch.zeros(1, dtype=torch.int32, device="cuda"), 0.25, 0)
+    assert not none.any()
