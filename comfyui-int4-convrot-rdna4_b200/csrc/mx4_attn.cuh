@@ -57,8 +57,8 @@ struct Mx4AttnArgs {
     long long cap;                 // tokens a table row holds
     const int* lens;
     void* out;
-    float* part;                   // per (tile, split, row): D floats ...
-    float2* part_ml;               // ... and {maximum, sum}
+    float* part;                   // per (tile, split, row): the mean of the split's values, D floats ...
+    float2* part_ml;               // ... and {reference, sum of weights}
     int B, tq, hq, hkv, page_bits, pages, group, row_tiles, splits;
     int clustered;                 // a sequence's splits are one cluster and join themselves
     float scale;                   // softmax scale times log2(e)
@@ -109,6 +109,13 @@ __device__ __forceinline__ int mx4_chunk_pos(int tok, int c) {
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 1 / x to about 2^-23, x a sum of weights (1 at least, unless none).
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -681,7 +688,9 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             #pragma unroll
             for (int z = 4; z < 32; z *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, z);
             const bool none = m[i][h] == kMx4NoScore && sum == 0.0f;      // (scores that are all NaN move no reference)
-            const float f = none ? 0.0f : ex2(dn[i][h]);
+            // the mean of the warp's values (their sum could leave fp32's range), by two factors:
+            // 2^dn alone could be below it
+            const float half = none ? 0.0f : ex2(0.5f * dn[i][h]), f = none ? 0.0f : half * rcp(sum);
             if (g == 0) {
                 pm[warp][r] = none ? -INFINITY : m[i][h];
                 pl[warp][r] = sum;
@@ -689,7 +698,7 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             float* dst = part + (warp * Cfg::kRows + r) * Cfg::kPartStride;
             #pragma unroll
             for (int j = 0; j < D / 16; ++j)                      // channels 8 g + 2 k and the next of each 64
-                *reinterpret_cast<float2*>(dst + 64 * (j / 4) + 8 * g + 2 * (j % 4)) = make_float2(o[i][j][h] * f, o[i][j][2 + h] * f);
+                *reinterpret_cast<float2*>(dst + 64 * (j / 4) + 8 * g + 2 * (j % 4)) = make_float2(o[i][j][h] * half * f, o[i][j][2 + h] * half * f);
         }
     __syncthreads();
     float* joined = part;                                          // warp 0's rows become the block's
@@ -698,29 +707,30 @@ mx4_attn_kernel(Mx4AttnArgs a) {
         float top = -INFINITY;
         #pragma unroll
         for (int w = 0; w < kMx4AttnWarps; ++w) top = fmaxf(top, pm[w][r]);
-        float sum = 0.0f;
+        float sum = 0.0f, f[kMx4AttnWarps];
+        #pragma unroll
+        for (int w = 0; w < kMx4AttnWarps; ++w) {
+            f[w] = pm[w][r] == -INFINITY ? 0.0f : ex2(pm[w][r] - top) * pl[w][r];
+            sum += f[w];
+        }
+        const float inv = sum == 0.0f ? 0.0f : rcp(sum);
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         #pragma unroll
         for (int w = 0; w < kMx4AttnWarps; ++w) {
-            const float f = pm[w][r] == -INFINITY ? 0.0f : ex2(pm[w][r] - top);
+            const float share = f[w] * inv;
             const float4 x = *reinterpret_cast<const float4*>(part + (w * Cfg::kRows + r) * Cfg::kPartStride + c);
-            sum += f * pl[w][r];
-            acc.x += f * x.x;
-            acc.y += f * x.y;
-            acc.z += f * x.z;
-            acc.w += f * x.w;
+            acc.x += share * x.x;
+            acc.y += share * x.y;
+            acc.z += share * x.z;
+            acc.w += share * x.w;
         }
-        if (a.clustered) {
+        if (a.clustered || a.splits == 1) {
             *reinterpret_cast<float4*>(joined + r * Cfg::kPartStride + c) = acc;
             if (c == 0) block_ml[r] = make_float2(top, sum);
-        } else if (a.splits > 1) {
+        } else {
             const size_t at = (static_cast<size_t>(tile) * a.splits + split) * Cfg::kRows + r;
             *reinterpret_cast<float4*>(a.part + at * D + c) = acc;
             if (c == 0) a.part_ml[at] = make_float2(top, sum);
-        } else {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            *reinterpret_cast<float4*>(joined + r * Cfg::kPartStride + c) =
-                sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
         }
     }
     if (a.splits > 1 && !a.clustered) return;
@@ -753,16 +763,20 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
             #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                if (ml[k].x == -INFINITY) continue;
-                const float w = ex2(ml[k].x - top);
-                sum += w * ml[k].y;
-                #pragma unroll
-                for (int i = 0; i < kPer; ++i) acc[i] += w * x[k][i];
+                ml[k].y = ml[k].x == -INFINITY ? 0.0f : ex2(ml[k].x - top) * ml[k].y;
+                sum += ml[k].y;
             }
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float inv = sum == 0.0f ? 0.0f : rcp(sum);
+            #pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (ml[k].x == -INFINITY) continue;
+                const float share = ml[k].y * inv;
+                #pragma unroll
+                for (int i = 0; i < kPer; ++i) acc[i] += share * x[k][i];
+            }
             v = reinterpret_cast<float*>(q_smem) + warp * D;      // (the joined rows are still read by other blocks)
             #pragma unroll
-            for (int i = 0; i < kPer; ++i) v[lane * kPer + i] = acc[i] * inv;
+            for (int i = 0; i < kPer; ++i) v[lane * kPer + i] = acc[i];
             __syncwarp();
         }
         for (int st = 1; st < a.group; st *= 4) {
@@ -806,18 +820,19 @@ __global__ void __launch_bounds__(256) mx4_attn_join_kernel(Mx4AttnArgs a, int t
     float f = 0.0f;                                                // not wide: at most 32 splits, lane s has split s's
     for (int s = lane; s < held; s += 32) {
         const float2 x = ml[static_cast<size_t>(s) * tile_rows];
-        f = x.x == -INFINITY ? 0.0f : ex2(x.x - top);
-        sum += f * x.y;
+        f = x.x == -INFINITY ? 0.0f : ex2(x.x - top) * x.y;
+        sum += f;
         if (wide && warp == 0) weight[s] = f;
     }
     #pragma unroll
     for (int z = 16; z; z >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, z);
+    const float inv = sum == 0.0f ? 0.0f : rcp(sum);
     if (wide) __syncthreads();
     float acc[kPer] = {};
     const float* src = a.part + at * D + lane;
     #pragma unroll 4
     for (int s = wide ? warp : 0; s < held; s += wide ? 8 : 1) {
-        const float w = wide ? weight[s] : __shfl_sync(0xFFFFFFFFu, f, s);
+        const float w = (wide ? weight[s] : __shfl_sync(0xFFFFFFFFu, f, s)) * inv;
         #pragma unroll
         for (int i = 0; i < kPer; ++i) acc[i] += w * src[static_cast<size_t>(s) * tile_rows * D + 32 * i];
     }
@@ -842,9 +857,8 @@ __global__ void __launch_bounds__(256) mx4_attn_join_kernel(Mx4AttnArgs a, int t
         __syncwarp();
     }
     const float g = a.group == 16 ? 0.25f : a.group == 64 ? 0.125f : a.group == 256 ? 0.0625f : 1.0f;
-    const float norm = sum == 0.0f ? 0.0f : g / sum;
     T* out = static_cast<T*>(a.out) + ((static_cast<size_t>(b) * a.tq + row / per_head) * a.hq + hk * per_head + row % per_head) * D;
-    for (int i = lane; i < D; i += 32) out[i] = mx4_from_f32<T>(r[i] * norm);
+    for (int i = lane; i < D; i += 32) out[i] = mx4_from_f32<T>(r[i] * g);
 }
 
 }  // namespace convrot

@@ -150,3 +150,21 @@ def test_attention_of_very_low_scores(mx, n):  # noqa: F811
     assert np.array_equal(f64(out)[0, 0], np.repeat(vs[0][n // 2], 2, 0))
     none = mx.convrot_mx4_attention(q, codes, scales, table, torch.zeros(1, dtype=torch.int32, device="cuda"), 0.25, 0)
     assert not none.any()
+
+
+@pytest.mark.parametrize("vscale", [2.0 ** 124, 2.0 ** 110, 2.0 ** -124])
+@pytest.mark.parametrize("b,n", [(1, 30), (1, 500), (3, 4000), (40, 6000)])
+def test_attention_values_at_the_ends_of_the_range(mx, b, n, vscale):  # noqa: F811
+    """Sums of many values stay in fp32's range, and tiny ones are not flushed (one block,
+    a cluster, and the separate join, whose sequences share their pages)."""
+    d = 64
+    codes, scales, table, ks, _ = make_cache(mx, [n], 64, 1, d, 0, 25)
+    v = np.clip(np.random.default_rng(2).standard_normal((n, 1, d)), -3, 3) + 1
+    v = [set_values(codes, scales, table, 1, v * vscale)]
+    q = torch.randn(1, 1, 8, d, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    lens = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    out = f64(mx.convrot_mx4_attention(q.repeat(b, 1, 1, 1), codes, scales, table.repeat(b, 1), lens, convrot_groupsize=0))
+    ref = np.repeat(expected(q, ks, v, [n], 0, d ** -0.5), b, 0)
+    err = np.abs(out - ref)
+    # half a spacing, 2^-17 of the operands; fp32 sums below its normal range: 2^-149 each
+    assert (err <= (2.0 ** -8 + 2.0 ** -16) * np.abs(ref) + 2.0 ** -134).all(), (err / np.abs(ref)).max()
