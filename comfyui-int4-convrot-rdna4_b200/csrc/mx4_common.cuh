@@ -42,24 +42,6 @@ __device__ __forceinline__ float mx4_scale_value(uint32_t e) {
     return __uint_as_float(bits);
 }
 
-// Two values on the code grid to one byte (lo in the low nibble): round to
-// nearest even, saturating at 6.
-__device__ __forceinline__ uint32_t mx4_encode2(float lo, float hi) {
-    uint16_t r;
-    asm("{\n\t.reg .b8 c;\n\tcvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\n\tcvt.u16.u8 %0, c;\n\t}"
-        : "=h"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-
-// Code 0..15 as the float it stands for (without its block's scale): e2m1's
-// magnitude is 0, 1, 2, 3 halves below 2 and m * 2^(e - 1) above.
-__device__ __forceinline__ float mx4_code_value(uint32_t c) {
-    // bits e e m placed at the top of an fp32 exponent offset by 126, as a
-    // product with 2^126: covers the subnormal code 0.5 too
-    const float v = __uint_as_float(((c & 7u) << 22) | ((c & 8u) << 28));
-    return v * __uint_as_float((127u + 126u) << 23);
-}
-
 __device__ __forceinline__ float mx4_to_f32(float v) { return v; }
 __device__ __forceinline__ float mx4_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float mx4_to_f32(__half v) { return __half2float(v); }
@@ -75,26 +57,6 @@ template <> __device__ __forceinline__ __half mx4_from_f32<__half>(float v) { re
 __device__ __forceinline__ size_t mx4_scale_pos(int row, int block, int kt) {
     return (static_cast<size_t>(row >> 7) * kt + (block >> 2)) * kMx4TileBytes +
            (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
-}
-
-// Regular-Hadamard rotation, in place, of `n` floats in shared memory in groups
-// of `group` (16, 64 or 256; 0: none), by all `nthreads` threads of the block
-// (n a multiple of the group): radix-4 steps at strides 1, 4, 16, 64, then
-// 1 / sqrt(group). The matrix is symmetric and orthogonal, so the same call
-// rotates back. Ends with a barrier.
-__device__ __forceinline__ void mx4_rotate_shared(float* v, int n, int group, int tid, int nthreads) {
-    for (int st = 1; st < group; st *= 4) {
-        for (int i = tid; i < n / 4; i += nthreads) {
-            float* p = v + (i / st) * 4 * st + i % st;
-            h4(p[0], p[st], p[2 * st], p[3 * st]);
-        }
-        __syncthreads();
-    }
-    if (group) {
-        const float f = group == 16 ? 0.25f : group == 64 ? 0.125f : 0.0625f;
-        for (int i = tid; i < n; i += nthreads) v[i] *= f;
-        __syncthreads();
-    }
 }
 
 }  // namespace convrot
