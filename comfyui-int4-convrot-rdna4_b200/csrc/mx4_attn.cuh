@@ -74,9 +74,14 @@ constexpr int kMx4NarrowBits = 8;              // blocks of values this many pow
 constexpr int kMx4AttnChunk = 32;              // tokens a warp takes at a time
 constexpr int kMx4AttnGroup = kMx4AttnWarps * kMx4AttnChunk;   // tokens a block takes at a time
 
-// Blocks a multiprocessor holds, by a thread's accumulators (rows * D / 32 of them) and
-// operands; `size` is rows / 8 * D.
-__host__ __device__ constexpr int mx4_attn_resident(int size) { return size <= 64 ? 5 : size <= 128 ? 4 : size <= 256 ? 3 : 2; }
+// Blocks a multiprocessor holds, for the launch bound (registers) and the plan alike; `size`
+// is rows / 8 * D. Two leave a thread 255 registers, four 128. Heads of 128, 8 rows: 180 us
+// with four, 183 with three, 199 with five (16 x 32768); heads of 64, 8 rows: 119.5 with four,
+// 121.8 with five (64 x 8192), 16 rows: 61 with four, 66 with three (37 up to 4096), 32 rows: 187
+// with two, 197 with three, which spill (64 x 4096, 8 tokens); heads of 128, 16 rows: 154 with two, 156 with
+// three (32 x 8192, 4 tokens); heads of 256, 8 rows: 176 with two, which is what shared memory
+// holds, 195 planned for three (32 x 8192).
+__host__ __device__ constexpr int mx4_attn_resident(int size) { return size <= 128 ? 4 : 2; }
 
 template <int D, int NT>
 struct Mx4AttnCfg {
@@ -96,6 +101,8 @@ struct Mx4AttnCfg {
     static constexpr int kRing = kMx4AttnWarps * kWarpBytes;
     static constexpr int kSmemBytes = kQBytes + (kRing > kPartBytes ? kRing : kPartBytes);
     static constexpr int kResident = mx4_attn_resident(NT * D);
+    // (with up to 2 KB of static memory and the 1 KB that the system takes a block)
+    static_assert(kResident * (kSmemBytes + 3072) <= 228 * 1024, "the blocks that are planned for fit");
 };
 
 // Chunk position of a token's 16-byte chunk c.
