@@ -47,6 +47,12 @@ class Mx4ConvRotLinear(torch.nn.Module):
             mod.bias = linear.bias.detach().to(device)
         return mod
 
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        bias = state_dict.get(prefix + "bias")
+        if self.bias is not None and bias is not None:
+            self.bias = self.bias.to(bias.dtype)                  # (copied into; a checkpoint's type is kept)
+        super()._load_from_state_dict(state_dict, prefix, *args)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return convrot_mx4_linear(x, self.weight, self.weight_scale, self.bias, self.groupsize)
 
