@@ -24,7 +24,11 @@ from .mx4 import (
 
 
 class Mx4ConvRotLinear(torch.nn.Module):
-    """``x @ W.T + bias`` with W held in MX4 (rotated in groups of ``convrot_groupsize``, 0: not rotated)."""
+    """``x @ W.T + bias`` with W held in MX4 (rotated in groups of ``convrot_groupsize``, 0: not rotated).
+
+    State dict: ``weight`` (codes), ``weight_scale`` (tiles), ``bias`` and ``convrot_groupsize``,
+    the group that the codes belong to; a dict without the last keeps the module's.
+    """
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None,
                  convrot_groupsize: int | None = None):
@@ -47,11 +51,24 @@ class Mx4ConvRotLinear(torch.nn.Module):
             mod.bias = linear.bias.detach().to(device)
         return mod
 
-    def _load_from_state_dict(self, state_dict, prefix, *args):
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "convrot_groupsize"] = torch.tensor(self.groupsize)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        key = prefix + "convrot_groupsize"
+        if key in state_dict:
+            g = int(state_dict[key])
+            if g not in (0, 16, 64, 256) or (g and self.in_features % g):
+                error_msgs.append(f"{key}: {g} is no rotation group of in_features={self.in_features}")
+                return
+            self.groupsize = g
         bias = state_dict.get(prefix + "bias")
         if self.bias is not None and bias is not None:
             self.bias = self.bias.to(bias.dtype)                  # (copied into; a checkpoint's type is kept)
-        super()._load_from_state_dict(state_dict, prefix, *args)
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if key in unexpected_keys:
+            unexpected_keys.remove(key)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return convrot_mx4_linear(x, self.weight, self.weight_scale, self.bias, self.groupsize)
