@@ -243,6 +243,9 @@ PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
           ck_mx4_cache_append(codes.data_ptr(), scales.data_ptr(), c.pages, c.heads, c.d, c.page, c.group, k.const_data_ptr(),
                               v.const_data_ptr(), code, k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.const_data_ptr(),
                               small(k.size(0), "tokens"), stream_of(codes.device())));
+    // written in place: what autograd saved of them is out of date (inference tensors have no version)
+    for (const Tensor* t : {&codes, &scales})
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
