@@ -7,9 +7,12 @@ the Python binding of the MX4 entries, which links against it. It is run by
 """
 from __future__ import annotations
 
+import glob
+import hashlib
 import os
 import shutil
 import subprocess
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(os.path.dirname(_HERE), "csrc")
@@ -40,12 +43,20 @@ def is_stale() -> bool:
     return newest > os.path.getmtime(out)
 
 
-def binding_name() -> str:
-    return "_mx4_binding.so"
+def binding_sources() -> list[str]:
+    return [os.path.join(_CSRC, "mx4_binding.cpp"),
+            os.path.join(os.path.dirname(os.path.dirname(_HERE)), "include", "convrot_b200.h")]
 
 
 def binding_path() -> str:
-    return os.path.join(_HERE, binding_name())
+    """The binding's file, named after its sources and the torch and Python it is built for:
+    one that does not fit is not found."""
+    import torch
+    key = hashlib.sha1(f"{torch.__version__} {sys.implementation.cache_tag}".encode())
+    for path in binding_sources():
+        with open(path, "rb") as f:
+            key.update(f.read())
+    return os.path.join(_HERE, f"_mx4_binding_{key.hexdigest()[:12]}.so")
 
 
 def find_nvcc() -> str | None:
@@ -62,7 +73,7 @@ def build(verbose: bool = False) -> str:
     if not nvcc:
         raise RuntimeError("nvcc not found; cannot build libconvrot_b200.so")
     out = lib_path()
-    tmp = out + ".tmp"
+    tmp = f"{out}.{os.getpid()}.tmp"
     cmd = [nvcc, *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared", "--threads", "0",
            "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
            "-o", tmp, *src_paths()]
@@ -83,13 +94,13 @@ def build_binding(verbose: bool = False) -> str:
     root = os.path.dirname(torch.__file__)
     home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     out = binding_path()
-    tmp = out + ".tmp"
+    tmp = f"{out}.{os.getpid()}.tmp"
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                os.path.join(home, "include"), sysconfig.get_paths()["include"],
                os.path.join(os.path.dirname(os.path.dirname(_HERE)), "include")]
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in include],
-           os.path.join(_CSRC, "mx4_binding.cpp"), "-o", tmp, f"-L{os.path.join(root, 'lib')}", f"-L{_HERE}",
+           binding_sources()[0], "-o", tmp, f"-L{os.path.join(root, 'lib')}", f"-L{_HERE}",
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-l:{lib_name()}", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print("building:", " ".join(cmd))
@@ -97,6 +108,9 @@ def build_binding(verbose: bool = False) -> str:
     if cp.returncode != 0 or not os.path.exists(tmp):
         raise RuntimeError(f"the binding's build failed:\n{cp.stderr}")
     os.replace(tmp, out)
+    for old in glob.glob(os.path.join(os.path.dirname(out), "_mx4_binding*.so")):
+        if old != out:
+            os.remove(old)
     return out
 
 

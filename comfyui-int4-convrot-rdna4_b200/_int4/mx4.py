@@ -35,6 +35,7 @@ import threading
 import torch
 
 from . import build as _build
+from . import cuda_loader
 
 BLOCK = 32
 _HEAD_DIMS = (64, 128, 256)
@@ -44,16 +45,16 @@ _lock = threading.Lock()
 
 
 def native():
-    """The binding module (_mx4_binding.so, built first when missing)."""
+    """The binding module (built first when there is none for these sources and this torch)."""
     global _native
     if _native is None:
         with _lock:
             if _native is None:
-                if not os.path.exists(_build.lib_path()):
-                    _build.build()
-                if not os.path.exists(_build.binding_path()):
+                cuda_loader.library()
+                path = _build.binding_path()
+                if not os.path.exists(path):
                     _build.build_binding()
-                loader = importlib.machinery.ExtensionFileLoader("_mx4_binding", _build.binding_path())
+                loader = importlib.machinery.ExtensionFileLoader("_mx4_binding", path)
                 spec = importlib.util.spec_from_loader("_mx4_binding", loader)
                 module = importlib.util.module_from_spec(spec)
                 loader.exec_module(module)
