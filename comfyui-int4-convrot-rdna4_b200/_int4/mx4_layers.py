@@ -167,8 +167,8 @@ class Mx4SelfAttention(torch.nn.Module):
         so far are read back once and torch's attention runs on them."""
         t = x.shape[0]
         device = x.device
-        new = torch.tensor(cache.extend(seq, t), dtype=torch.int64, device=device)
         q, k, v = self.project(x)
+        new = torch.tensor(cache.extend(seq, t), dtype=torch.int64, device=device)
         cache.append(k, v, new)
         ks, vs = cache.read(torch.tensor(cache.slots(seq), dtype=torch.int64, device=device), x.dtype)
         n = ks.shape[0]

@@ -33,3 +33,13 @@ def test_linear_state_dict_carries_the_rotation_group():
     for bad in (32, 256):
         with pytest.raises(RuntimeError, match="convrot_groupsize"):
             Mx4ConvRotLinear(64, 2, device="cpu").load_state_dict({**block[0].state_dict(), "convrot_groupsize": torch.tensor(bad)})
+
+
+def test_prefill_that_fails_reserves_no_tokens():
+    from _int4.mx4_layers import Mx4KVCache, Mx4SelfAttention
+    block = Mx4SelfAttention(64, 2, 1, 64, device="cpu")
+    cache = Mx4KVCache(4, 1, 64, page=16, device="cpu")
+    seq = cache.add()
+    with pytest.raises(ValueError):
+        block.prefill(torch.zeros(5, 64), cache, seq)             # (not on a CUDA device)
+    assert cache.length(seq) == 0 and cache.slots(seq) == []
