@@ -127,8 +127,10 @@ def mx4_cache_empty(pages: int, page: int, heads: int, head_dim: int, device="cu
     """A zeroed paged cache: codes [pages, 2, heads, page, D/2] and scales [pages, 2, heads, page, D/32]."""
     if head_dim not in _HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {_HEAD_DIMS}, got {head_dim}")
-    if page <= 0 or page & (page - 1):
-        raise ValueError(f"the page size must be a power of two, got {page}")
+    if page <= 0 or page & (page - 1) or page > 65536:
+        raise ValueError(f"the page size must be a power of two up to 65536, got {page}")
+    if heads <= 0:
+        raise ValueError("the cache has no heads")
     codes = torch.zeros(pages, 2, heads, page, head_dim // 2, dtype=torch.uint8, device=device)
     scales = torch.zeros(pages, 2, heads, page, head_dim // BLOCK, dtype=torch.uint8, device=device)
     return codes, scales

@@ -216,7 +216,10 @@ Cache cache_of(const Tensor& codes, const Tensor& scales, PyObject* group) {
     TORCH_CHECK_VALUE(scales.dim() == 5 && scales.size(0) == codes.size(0) && scales.size(1) == 2 && scales.size(2) == codes.size(2) &&
                           scales.size(3) == codes.size(3) && scales.size(4) == d / kBlock,
                       "cache scales ", scales.sizes(), " do not match codes ", codes.sizes());
-    return {codes.size(0), small(codes.size(2), "heads"), static_cast<int>(d), small(codes.size(3), "page"), group_of(d, group)};
+    const int64_t page = codes.size(3);
+    TORCH_CHECK_VALUE(page > 0 && page <= 65536 && (page & (page - 1)) == 0, "the page size must be a power of two up to 65536, got ", page);
+    TORCH_CHECK_VALUE(codes.size(2) > 0, "the cache has no heads");
+    return {codes.size(0), small(codes.size(2), "heads"), static_cast<int>(d), static_cast<int>(page), group_of(d, group)};
 }
 
 void check_slots(const Tensor& slots, int64_t t) {

@@ -39,3 +39,20 @@ def test_attention_refuses_tables_at_the_end_of_32_bit_positions(lib):
     for per, page in ((2 ** 31 - 1, 1), (2 ** 27 - 1, 16), (2 ** 31 - 1000, 1), (2 ** 25, 64)):
         refuse(lib, attention(per, page), b"block table longer")
     refuse(lib, attention(2 ** 26 - 64, 32), b"workspace")                          # accepted as a length
+
+
+def test_cache_shapes_that_the_kernels_do_not_take_are_value_errors():
+    import torch
+
+    import _int4
+    slots = torch.zeros(1, dtype=torch.int64)
+    for page, heads, text in ((48, 1, "power of two"), (1 << 17, 1, "power of two"), (16, 0, "heads")):
+        codes = torch.empty(0, 2, heads, page, 32, dtype=torch.uint8)
+        scales = torch.empty(0, 2, heads, page, 2, dtype=torch.uint8)
+        kv = torch.zeros(1, heads, 64)
+        with pytest.raises(ValueError, match=text):
+            _int4.convrot_mx4_cache_read(codes, scales, slots)
+        with pytest.raises(ValueError, match=text):
+            _int4.convrot_mx4_cache_append(codes, scales, kv, kv, slots)
+        with pytest.raises(ValueError, match=text):
+            _int4.mx4_cache_empty(0, page, heads, 64, device="cpu")
