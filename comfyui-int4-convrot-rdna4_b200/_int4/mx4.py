@@ -24,6 +24,8 @@ D; slot s is token s % page of page s / page.
 
 All tensors are CUDA tensors of one device; calls run on that device's current
 stream; bad arguments raise ValueError, a refused or failed launch RuntimeError.
+Forward only, like the int4 operators: no result carries a gradient, whether the
+inputs require one or not.
 """
 from __future__ import annotations
 
@@ -167,6 +169,7 @@ def convrot_mx4_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Te
     block_table[b, j / page]; a page number outside the cache hides its tokens.
     seq_lens int32 [B]: tokens in the cache, new ones included (cut at P * page).
     Query t sees the tokens up to position seq_len - Tq + t; a query that sees none
-    gives zeros. Returns [B, Tq, Hq, D] in q.dtype.
+    gives zeros. Returns [B, Tq, Hq, D] in q.dtype. Keys of a magnitude beyond 2^111
+    may overflow the scores' partial sums.
     """
     return (_native or native()).attention(q, codes, scales, block_table, seq_lens, softmax_scale, convrot_groupsize)

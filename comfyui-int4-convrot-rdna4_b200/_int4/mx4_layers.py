@@ -5,7 +5,7 @@ self-attention block that uses both.
 scale byte per 32) and runs ``convrot_mx4_linear``. ``Mx4KVCache`` owns the
 cache's tensors and hands out pages. ``Mx4SelfAttention`` is the path of one
 transformer block from hidden states to hidden states: QKV projection, new keys
-and values into the cache, attention over it, output projection.
+and values into the cache, attention over it, output projection. Forward only.
 """
 from __future__ import annotations
 
@@ -137,7 +137,11 @@ class Mx4KVCache:
 
 
 class Mx4SelfAttention(torch.nn.Module):
-    """Causal self-attention of new tokens over a paged MX4 cache, with MX4 projections."""
+    """Causal self-attention of new tokens over a paged MX4 cache, with MX4 projections.
+
+    No position embedding. A model that has one calls the parts itself: ``project``,
+    its embedding of q and k, ``cache.append``, ``cache.attend``, ``out``.
+    """
 
     def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, bias: bool = False, device=None):
         super().__init__()

@@ -188,7 +188,7 @@ static int launch_gemm_pair(const void* xc, const void* xs, const void* wc, cons
 
 // The few-row kernel: 1, 2, 4 or 8 slices of K (a cluster), as many as leave the
 // blocks two a multiprocessor and each slice four stages (4 x 4096 x 4096: 4.5 us in four
-// slices, 5.2 in eight; 1 x 15360 x 3840: 8.0 us in two, 9.6 in one, weights beyond L2).
+// slices, 5.3 in eight, 7.9 in one; 1 x 15360 x 3840: 7.7 us in two, 9.4 in one; weights beyond L2).
 template <typename T, int G, int BT, bool FUSED>
 static int launch_gemm_few(const void* x, long long ldx, const void* xc, const void* xs, const void* wc, const void* ws,
                            BiasRef bias, T* out, int M, int N, int K, cudaStream_t stream) {
@@ -355,18 +355,17 @@ static AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longe
     // splits: one full wave of blocks always, as far as every split has a group of
     // tokens; up to four waves, which even the tail out, while each split keeps eight
     // groups (a block's start and end cost about as much as three). Waves counted by the
-    // blocks a multiprocessor really holds, and whole ones: against four blocks for every
-    // shape and any part of a wave, 64 x 4096 tokens of 32 heads 283 -> 248 us, 8 x 16384 of
-    // 16 query heads on one 25.8 -> 21.4 us
+    // blocks a multiprocessor really holds, and whole ones: 64 x 4096 tokens of 32 heads 320 us,
+    // 355 with a part of a wave; 64 x 1024 of 32 heads on 8: 30.4 against 35.5
     const long long groups = (longest + kMx4AttnGroup - 1) / kMx4AttnGroup, tiles = p.tiles > 0 ? p.tiles : 1;
     const long long places = static_cast<long long>(mx4_attn_resident(p.tile_rows / 8 * d)) * sm_count();
     long long waves = 4;
     while (waves > 1 && waves * places / tiles > groups / 8) --waves;
     const long long want = waves * places / tiles;
     p.splits = static_cast<int>(std::max(1LL, std::min({want, groups, static_cast<long long>(kMx4MostSplits)})));
-    // one launch instead of two (1 x 777 tokens: 7.3 against 9.4 us), where every block is
+    // one launch instead of two (1 x 777 tokens: 7.8 against 9.9 us), where every block is
     // resident at once; with more, a cluster's blocks wait for each other and for places
-    // (64 x 4096 tokens, 4 splits: 89 against 84 us)
+    // (64 x 4096 tokens, 4 splits: 106 against 99 us)
     p.clustered = p.splits > 1 && p.splits <= 8 && tiles * p.splits <= 2LL * sm_count();
     return p;
 }

@@ -5,7 +5,8 @@
 // once for all of them; the sequence is split over blocks, and each warp of a
 // block walks its own chunks of 32 tokens with a running maximum and sum. Warps
 // are joined through shared memory; up to 8 splits of a sequence are a cluster and
-// join over distributed shared memory, more by mx4_attn_join_kernel.
+// join over distributed shared memory where all blocks are resident at once, others
+// by mx4_attn_join_kernel.
 //
 // Rotated cache: q k = (H q) (H k), so the query rows are rotated once, and the
 // output, a mean of rotated values, is rotated back at the end.
@@ -39,10 +40,11 @@
 // channel. 16-byte chunks of a token are XORed so that neither read meets a bank
 // conflict.
 //
-// Bound by issue: the conversions of codes (ALU pipe), scales, weights and their second
-// terms, page look-ups. 16 sequences of 32768, 64 heads on 8 of 128: 179 us (3.2 TB/s of the
-// cache; 146 us with one f16 term an operand); 64 of 4096, 32 heads on 32: 317 us (3.6 TB/s);
-// 128 x 2048: 2.8 TB/s; one of 777: 7.9 us.
+// Bound by issue: some 910 instructions a warp for 32 tokens of 128, 2.5 a cycle, half of
+// them on the ALU pipe that converts codes (busy 51 %; tensor pipe 35 %). 16 sequences of
+// 32768, 64 heads on 8 of 128: 181 us (3.2 TB/s of the cache; 146 us with one f16 term an
+// operand); 64 of 4096, 32 heads on 32: 320 us (3.6 TB/s); 128 x 2048: 104 us (2.7 TB/s); one of
+// 777: 7.8 us.
 #pragma once
 
 namespace convrot {

@@ -10,15 +10,15 @@
 // FUSED (up to 8 rows): the activations are rotated and quantized here, by the
 // epilogue's warps while the weight is on its way, a stage (256 columns) by one
 // warp. Every block quantizes its slice of K again, which for few rows costs less
-// than a launch and a pass through memory (15360 x 3840: 1 row 7.1 us, 8 rows 9.8 us;
-// 16 rows would take 14.6 us, with a kernel of its own 11.0 us). A lane takes 16
+// than a launch and a pass through memory (15360 x 3840: 1 row 7.7 us, 8 rows 9.4 us;
+// 16 rows would take 14.3 us, with a kernel of its own 10.5 us). A lane takes 16
 // columns of two rows: short code and a short wait (128 columns a lane, as in
 // mx4_unit.cuh, took 2.8 us to the first stage, most of it the first run through its
 // instructions).
 //
-// Measured, weights beyond what L2 keeps: 1 x 15360 x 3840 7.3 us (31 MB, 4.3 TB/s), of
+// Measured, weights beyond what L2 keeps: 1 x 15360 x 3840 7.7 us (31 MB, 4.1 TB/s), of
 // it about 2 us to the first MMA and 2 us from the last one to the end of the output; with
-// the quantizer's launch, 64 x 4096 x 4096 8.9 us and 128 x 15360 x 3840 14 us.
+// the quantizer's launch, 64 x 4096 x 4096 9.1 us and 128 x 15360 x 3840 13.8 us.
 //
 // Warp roles (6 warps, so that two blocks fit a multiprocessor): w0 TMA producer
 // (one lane), w1 tensor memory and MMA issue, w2..w5 quantizers (FUSED) and epilogue
