@@ -33,14 +33,19 @@ from .int8_eager import quantize_signed_int8_rowwise as _quantize_int8_rowwise
 from .mx4 import (
     convrot_mx4_attention,
     convrot_mx4_cache_append,
+    convrot_mx4_cache_append_rope,
     convrot_mx4_cache_read,
     convrot_mx4_linear,
+    convrot_mx4_tree_attention,
     dequantize_convrot_mx4,
     mx4_cache_empty,
     mx4_scales_from_rows,
     mx4_scales_to_rows,
+    native as _native,
     quantize_convrot_mx4,
+    tree_mask,
 )
+from .rope import apply_rope, rope_freqs
 
 __all__ = [
     "quantize_convrot_w4a4_weight",
@@ -58,6 +63,12 @@ __all__ = [
     "convrot_mx4_cache_append",
     "convrot_mx4_cache_read",
     "convrot_mx4_attention",
+    "convrot_mx4_cache_append_rope",
+    "convrot_mx4_tree_attention",
+    "tree_mask",
+    "rope_freqs",
+    "apply_rope",
+    "convrot_w8a8_linear_rmsnorm",
     "is_available",
     "pick_groupsize",
 ]
@@ -317,3 +328,28 @@ def convrot_w8a8_linear_lora(x, qweight, wscales, bias, adapters, convrot_groups
     if out.dtype != x.dtype:
         out = out.to(x.dtype)
     return out.reshape(*shape[:-1], qweight.shape[0])
+
+
+def convrot_w8a8_linear_rmsnorm(
+    x: torch.Tensor,
+    qweight: torch.Tensor,
+    wscales: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    norm_weight: torch.Tensor | None = None,
+    residual: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    convrot_groupsize: int = 256,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``convrot_w8a8_linear`` of the root-mean-square norm of x + residual; returns (out, x + residual).
+
+    h = x + residual, y = h / sqrt(mean(h^2) + eps) * norm_weight, out = y @ W.T + bias
+    with y rotated and quantized to int8 (scale max|y| / 127 a row, ties to even) and
+    W held in int8. One kernel adds, normalises, rotates and quantizes, in fp32 without
+    an intermediate rounding (the norm is taken of the unrounded sum; the sum that is
+    returned is rounded to x's dtype). x, residual [..., K] of one dtype (float32,
+    bfloat16 or float16), K a multiple of the group (16, 64 or 256) and at most 16384;
+    qweight int8 [N, K], wscales [N], norm_weight [K] and bias [N] in any of the three
+    types or None. Without a residual the second value is x itself. out is in x's dtype;
+    a row with an infinity or a NaN gives NaN. Forward only.
+    """
+    return _native().linear_rmsnorm(x, qweight, wscales, bias, norm_weight, residual, eps, convrot_groupsize)

@@ -64,6 +64,15 @@ _SIGNATURES = {
     "ck_mx4_attention_workspace_size": [_I] * 5 + [_L],
     "ck_mx4_attention": [_P, _I, _L, _L, _L, _P, _P, _L, _I, _P, _L, _I, _P, _P] + [_I] * 6
                         + [ctypes.c_float, _P, ctypes.c_size_t, _P],
+    "ck_rope": [_P, _I, _L, _L, _L, _P] + [_I] * 4 + [_P, _I, _L, _L, _L, _P, ctypes.POINTER(_I), _I, _I, _I, _P],
+    "ck_mx4_cache_append_rope": [_P, _P, _L] + [_I] * 4 + [_P, _P, _P, _I, _I] + [_L] * 6 + [_P, _P, _I, _P, _I, _L, _L, _P,
+                                 ctypes.POINTER(_I), _I, _I, _P],
+    "ck_mx4_tree_attention_workspace_size": [_I] * 5 + [_L],
+    "ck_mx4_tree_attention": [_P, _I, _L, _L, _L, _P, _P, _L, _I, _P, _L, _I, _P, _P, _P, _L, _L, _P] + [_I] * 6
+                             + [ctypes.c_float, _P, ctypes.c_size_t, _P],
+    "ck_convrot_w8a8_linear_rmsnorm_workspace_size": [_I, _I],
+    "ck_convrot_w8a8_linear_rmsnorm": [_P, _P, _I, _L, _L, _P, _I, ctypes.c_float, _P, _P, _P, _I, _P, _P] + [_I] * 5
+                                      + [_P, ctypes.c_size_t, _P],
     "ck_convrot_device_status": [_P, ctypes.POINTER(ctypes.c_int)],
     "ck_convrot_selftest_wait_timeout": [ctypes.c_longlong, _P],
     "ck_convrot_last_error": [],

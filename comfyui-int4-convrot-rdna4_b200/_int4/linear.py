@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import (checkpoint, convrot_w4a4_linear, convrot_w4a4_linear_lnmod, convrot_w4a4_linear_lora,
-               convrot_w8a8_linear_lora, cuda_loader, pick_groupsize)
+               convrot_w8a8_linear_lora, convrot_w8a8_linear_rmsnorm, cuda_loader, pick_groupsize)
 from .eager import quantize_convrot_w4a4_weight
 
 _CKPT_KEYS = ("weight", "weight_scale", "comfy_quant", "bias")
@@ -112,6 +112,20 @@ class Int4ConvRotLinear(torch.nn.Module):
         if shift is not None:
             xn = xn + shift
         return self(xn)
+
+    def forward_rmsnorm(self, x: torch.Tensor, norm_weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                        eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+        """``self(rms_norm(x + residual) * norm_weight)`` and x + residual, as a transformer block takes
+        them. Plain int8 layers run it in one pass over x (``_int4.convrot_w8a8_linear_rmsnorm``);
+        int4 layers and layers with Dynamic-LoRA adapters, whose down projection needs the
+        normalised rows, add and normalise in torch first."""
+        if self._qmode == "int8" and not self._dyn_lora:
+            return convrot_w8a8_linear_rmsnorm(x, self._q, self._qs, self.bias, norm_weight, residual, eps, self._qgs)
+        h = x.float() if residual is None else x.float() + residual.float()
+        y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps)
+        if norm_weight is not None:
+            y = y * norm_weight.float()
+        return self(y.to(x.dtype)), x if residual is None else h.to(x.dtype)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self._qmode == "int8":

@@ -12,6 +12,8 @@ intermediate rounding.
     convrot_mx4_cache_append(codes, scales, k, v, slots, G)
     convrot_mx4_cache_read(codes, scales, slots, dtype, G) -> (k, v)
     convrot_mx4_attention(q, codes, scales, block_table, seq_lens, ...) -> out
+    convrot_mx4_cache_append_rope(codes, scales, q, k, v, slots, positions, freqs, ...) -> q turned
+    convrot_mx4_tree_attention(q, codes, scales, block_table, seq_lens, tree_mask, ...) -> out
 
 Layouts. Codes: two a byte, the even column in the low nibble. Scales of a
 matrix [R, K] are held in tiles [ceil(R/128), ceil(K/128), 512] (the order in
@@ -173,3 +175,59 @@ def convrot_mx4_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Te
     may overflow the scores' partial sums.
     """
     return (_native or native()).attention(q, codes, scales, block_table, seq_lens, softmax_scale, convrot_groupsize)
+
+
+def convrot_mx4_cache_append_rope(codes: torch.Tensor, scales: torch.Tensor, q: torch.Tensor | None, k: torch.Tensor,
+                                  v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,
+                                  sections: tuple[int, ...] | None = None, interleaved: bool = False,
+                                  convrot_groupsize: int = 64) -> torch.Tensor | None:
+    """``convrot_mx4_cache_append`` of keys that are turned by their tokens' positions on the way.
+
+    One launch for a token's queries, keys and values: q [T, Hq, D] (or None) is turned
+    and returned in its dtype, k is turned in fp32 and goes on to the cache without a
+    rounding between, v is written as by ``convrot_mx4_cache_append``. q, k and v have one
+    dtype and any token and head strides; positions [T] or, with several sections,
+    [T, axes], freqs, sections and interleaved as in ``apply_rope``. A slot outside the
+    cache writes nothing (its query is turned all the same); two tokens of one call must
+    not share a slot.
+    """
+    return (_native or native()).cache_append_rope(codes, scales, q, k, v, slots, positions, freqs, sections, interleaved, convrot_groupsize)
+
+
+def tree_mask(parents) -> tuple[torch.Tensor, torch.Tensor]:
+    """(mask bool [.., T, T], depths int64 [.., T]) of trees of drafted tokens.
+
+    parents [T] or [B, T] (a list or a whole-number tensor): the node that each node
+    follows, one before it, or -1 for the sequence's last token. A node's row names its
+    ancestors and itself; its depth is the number of ancestors, so that it stands at
+    position context + depth. Worked out on the host and given back on the parents' device.
+    """
+    given = torch.as_tensor(parents)
+    if given.dim() not in (1, 2) or given.is_floating_point() or given.dtype == torch.bool:
+        raise ValueError("parents must be whole numbers [T] or [B, T]")
+    p = given.cpu().long().reshape(-1, given.shape[-1])
+    b, t = p.shape
+    if bool(((p >= torch.arange(t)) | (p < -1)).any()):
+        raise ValueError("a node's parent must be a node before it, or -1")
+    mask = torch.eye(t, dtype=torch.bool).repeat(b, 1, 1)
+    rows = torch.arange(b)
+    for j in range(1, t):
+        mask[:, j] |= mask[rows, p[:, j].clamp(min=0)] & (p[:, j] >= 0)[:, None]
+    depths = mask.sum(-1) - 1
+    return mask.reshape(*given.shape, t).to(given.device), depths.reshape(given.shape).to(given.device)
+
+
+def convrot_mx4_tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
+                               seq_lens: torch.Tensor, tree_mask: torch.Tensor, tree_lens: torch.Tensor | None = None,
+                               softmax_scale: float | None = None, convrot_groupsize: int = 64) -> torch.Tensor:
+    """Attention of drafted tokens that form a tree, over the paged cache that holds them.
+
+    As ``convrot_mx4_attention``, but the T newest tokens of a sequence are the nodes of a
+    tree: node t sees all tokens before the nodes, and of the nodes those whose entry
+    tree_mask[t, j] is true (``tree_mask`` makes such a mask from parents; a node sees
+    itself only if named). tree_mask bool [T, T] for all sequences or [B, T, T].
+    tree_lens int32 [B]: nodes of each sequence, its newest tokens (cut to 0 .. T; None: T
+    each); the rows behind them are zeros. q [B, T, Hq, D], block_table and seq_lens (nodes
+    included) as there; a node that sees nothing gives zeros.
+    """
+    return (_native or native()).tree_attention(q, codes, scales, block_table, seq_lens, tree_mask, tree_lens, softmax_scale, convrot_groupsize)

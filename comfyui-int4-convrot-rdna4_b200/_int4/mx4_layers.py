@@ -4,10 +4,13 @@ self-attention block that uses both.
 ``Mx4ConvRotLinear`` holds a weight as MX4 codes (half a byte a value plus one
 scale byte per 32) and runs ``convrot_mx4_linear``. ``Mx4KVCache`` owns the
 cache's tensors and hands out pages. ``Mx4SelfAttention`` is the path of one
-transformer block from hidden states to hidden states: QKV projection, new keys
-and values into the cache, attention over it, output projection. Forward only.
+transformer block from hidden states to hidden states: QKV projection, positions, new
+keys and values into the cache, attention over it (of a chain of tokens or of a tree of
+drafted ones), output projection. Forward only.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -16,8 +19,10 @@ from .mx4 import (
     _scale_tiles,
     convrot_mx4_attention,
     convrot_mx4_cache_append,
+    convrot_mx4_cache_append_rope,
     convrot_mx4_cache_read,
     convrot_mx4_linear,
+    convrot_mx4_tree_attention,
     mx4_cache_empty,
     quantize_convrot_mx4,
 )
@@ -128,6 +133,10 @@ class Mx4KVCache:
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         convrot_mx4_cache_append(self.codes, self.scales, k, v, slots, self.groupsize)
 
+    def append_rope(self, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
+                    freqs: torch.Tensor, sections: tuple[int, ...] | None = None, interleaved: bool = False) -> torch.Tensor | None:
+        return convrot_mx4_cache_append_rope(self.codes, self.scales, q, k, v, slots, positions, freqs, sections, interleaved, self.groupsize)
+
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
         return convrot_mx4_cache_read(self.codes, self.scales, slots, dtype, self.groupsize)
 
@@ -135,45 +144,108 @@ class Mx4KVCache:
                softmax_scale: float | None = None) -> torch.Tensor:
         return convrot_mx4_attention(q, self.codes, self.scales, block_table, seq_lens, softmax_scale, self.groupsize)
 
+    def attend_tree(self, q: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, tree_mask: torch.Tensor,
+                    tree_lens: torch.Tensor | None = None, softmax_scale: float | None = None) -> torch.Tensor:
+        return convrot_mx4_tree_attention(q, self.codes, self.scales, block_table, seq_lens, tree_mask, tree_lens, softmax_scale, self.groupsize)
+
+    def accept(self, seq: int, nodes: int, kept) -> None:
+        """Ends a tree's verification: of the sequence's ``nodes`` newest tokens those numbered
+        ``kept`` stay (in rising order, a path from the root), the others' tokens and the pages
+        behind the last are given back. Keys carry their positions already: a node's depth must
+        be its place on the path."""
+        kept = [int(i) for i in kept]
+        start = self._len[seq] - nodes
+        if nodes < 0 or start < 0 or any(not 0 <= i < nodes for i in kept) or any(b <= a for a, b in zip(kept, kept[1:])):
+            raise ValueError(f"kept nodes {kept} of the newest {nodes} of {self._len[seq]} tokens")
+        slots = self.slots(seq)
+        moved = [(slots[start + i], slots[start + to]) for to, i in enumerate(kept) if i != to]
+        if moved:
+            src, dst = torch.tensor(moved, dtype=torch.int64, device=self.codes.device).unbind(1)
+            for t in (self.codes, self.scales):                   # (read as a whole before it is written)
+                t[dst // self.page, :, :, dst % self.page] = t[src // self.page, :, :, src % self.page]
+        self._len[seq] = start + len(kept)
+        pages = self._pages[seq]
+        while len(pages) > -(-self._len[seq] // self.page):
+            self._free.append(pages.pop())
+
 
 class Mx4SelfAttention(torch.nn.Module):
     """Causal self-attention of new tokens over a paged MX4 cache, with MX4 projections.
 
-    No position embedding. A model that has one calls the parts itself: ``project``,
-    its embedding of q and k, ``cache.append``, ``cache.attend``, ``out``.
+    freqs (float64 [pairs], ``rope_freqs``): rotary positions for queries and keys, with
+    sections and interleaved as in ``apply_rope``; None: no position embedding. A model that
+    has another one calls the parts itself: ``project``, its embedding of q and k,
+    ``cache.append``, ``cache.attend``, ``out``.
     """
 
-    def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, bias: bool = False, device=None):
+    def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, bias: bool = False, device=None,
+                 freqs: torch.Tensor | None = None, sections: tuple[int, ...] | None = None, interleaved: bool = False):
         super().__init__()
         if heads % kv_heads:
             raise ValueError(f"{heads} query heads are no multiple of {kv_heads} key/value heads")
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.sections, self.interleaved = sections, interleaved
         self.qkv = Mx4ConvRotLinear(hidden, (heads + 2 * kv_heads) * head_dim, bias, device)
         self.out = Mx4ConvRotLinear(heads * head_dim, hidden, bias, device)
+        self.register_buffer("freqs", None if freqs is None else freqs.to(device), persistent=False)
 
     def project(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """q [..., heads, D], k and v [..., kv_heads, D] of x [..., hidden]: views of one projection."""
         y = self.qkv(x).unflatten(-1, (self.heads + 2 * self.kv_heads, self.head_dim))
         return y.split((self.heads, self.kv_heads, self.kv_heads), dim=-2)
 
-    def forward(self, x: torch.Tensor, cache: Mx4KVCache, slots: torch.Tensor, block_table: torch.Tensor,
-                seq_lens: torch.Tensor) -> torch.Tensor:
-        """x [B, T, hidden]: the newest T tokens of B sequences, whose slots (int64 [B * T]),
-        pages and lengths (the new tokens included) are given. Few tokens a sequence (decoding,
-        drafts to verify): every query row is read against the cache as it is stored."""
-        b, t, _ = x.shape
-        q, k, v = self.project(x)
-        cache.append(k.flatten(0, 1), v.flatten(0, 1), slots)
-        return self.out(cache.attend(q, block_table, seq_lens).reshape(b, t, self.heads * self.head_dim))
+    def _positions(self, positions: torch.Tensor | None, tokens: int) -> torch.Tensor | None:
+        """The tokens' positions as the cache takes them; ValueError where they do not fit the block."""
+        if (positions is None) != (self.freqs is None):
+            raise ValueError("a block with frequencies needs its tokens' positions" if positions is None
+                             else "positions were given to a block without frequencies")
+        if positions is None:
+            return None
+        shape = (tokens,) if self.sections is None or len(self.sections) == 1 else (tokens, len(self.sections))
+        if positions.numel() != math.prod(shape) or positions.dtype not in (torch.int32, torch.int64, torch.float32):
+            raise ValueError(f"positions {tuple(positions.shape)} of {positions.dtype}: int32, int64 or float32 {shape} expected")
+        return positions.reshape(shape)
 
-    def prefill(self, x: torch.Tensor, cache: Mx4KVCache, seq: int) -> torch.Tensor:
+    def _store(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Mx4KVCache, slots: torch.Tensor,
+               positions: torch.Tensor | None) -> torch.Tensor:
+        """Keys and values [T, kv_heads, D] into the cache; the queries [T, heads, D] to attend with."""
+        if positions is None:
+            cache.append(k, v, slots)
+            return q
+        return cache.append_rope(q, k, v, slots, positions, self.freqs, self.sections, self.interleaved)
+
+    def forward(self, x: torch.Tensor, cache: Mx4KVCache, slots: torch.Tensor, block_table: torch.Tensor,
+                seq_lens: torch.Tensor, positions: torch.Tensor | None = None, tree_mask: torch.Tensor | None = None,
+                tree_lens: torch.Tensor | None = None) -> torch.Tensor:
+        """x [B, T, hidden]: the newest T tokens of B sequences, whose slots (int64 [B * T]),
+        pages and lengths (the new tokens included) are given, and with frequencies their
+        positions [B, T] (several sections: [B, T, axes]). Few tokens a sequence (decoding,
+        drafts to verify): every query row is read against the cache as it is stored. With
+        tree_mask (and tree_lens) the tokens are a tree's nodes, as in
+        ``convrot_mx4_tree_attention``; slots of padding behind them are -1."""
+        b, t, _ = x.shape
+        positions = self._positions(positions, b * t)
+        q = self._store(*self.project(x.flatten(0, 1)), cache, slots, positions).unflatten(0, (b, t))
+        if tree_mask is not None:
+            y = cache.attend_tree(q, block_table, seq_lens, tree_mask, tree_lens)
+        elif tree_lens is not None:
+            raise ValueError("tree_lens were given without a tree_mask")
+        else:
+            y = cache.attend(q, block_table, seq_lens)
+        return self.out(y.reshape(b, t, self.heads * self.head_dim))
+
+    def prefill(self, x: torch.Tensor, cache: Mx4KVCache, seq: int, positions: torch.Tensor | None = None) -> torch.Tensor:
         """x [T, hidden]: the next T tokens of one sequence. Many query rows: the keys and values
-        so far are read back once and torch's attention runs on them."""
+        so far are read back once and torch's attention runs on them. Positions of a block with
+        frequencies: [T(, axes)], or None for the tokens' places in the sequence on one axis."""
         t = x.shape[0]
         device = x.device
+        if positions is None and self.freqs is not None and (self.sections is None or len(self.sections) == 1):
+            positions = torch.arange(cache.length(seq), cache.length(seq) + t, device=device)
+        positions = self._positions(positions, t)
         q, k, v = self.project(x)
         new = torch.tensor(cache.extend(seq, t), dtype=torch.int64, device=device)
-        cache.append(k, v, new)
+        q = self._store(q, k, v, cache, new, positions)
         ks, vs = cache.read(torch.tensor(cache.slots(seq), dtype=torch.int64, device=device), x.dtype)
         n = ks.shape[0]
         seen = torch.ones(t, n, dtype=torch.bool, device=device).tril(n - t)

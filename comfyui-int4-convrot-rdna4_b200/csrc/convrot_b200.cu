@@ -1433,6 +1433,12 @@ int dispatch_gemm_i8(const void* X, const void* W, const float* xs, const float*
     return launch_pair_impl<256, false, OUT, false, false, true>(X, W, xs, ws, bias, out, M, N, K, LoraArgs(), stream);
 }
 
+int run_gemm_i8(const void* X, const void* W, const float* xs, const float* ws, BiasRef bias, void* out, int out_dtype,
+                int M, int N, int K, cudaStream_t stream) {
+    if (out_dtype == 1) return dispatch_gemm_i8<kOutBF16>(X, W, xs, ws, bias, out, M, N, K, stream);
+    return dispatch_gemm_i8<kOutF32>(X, W, xs, ws, bias, out, M, N, K, stream);
+}
+
 // Packed int4 weights [rows, K/2] in boxes of 128 rows x 64 bytes (128 codes), 64-byte swizzle.
 bool make_w64_tmap(CUtensorMap* map, const void* base, int rows, int K) {
     auto enc = get_encode_fn();
@@ -1932,8 +1938,7 @@ CONVROT_API int ck_int8_convrot_gemm(const void* X, const void* W, const void* x
     const float* ws = static_cast<const float*>(wscale);
     const BiasRef b{bias, 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (out_dtype == 1) return dispatch_gemm_i8<kOutBF16>(X, W, xs, ws, b, out, M, N, K, s);
-    return dispatch_gemm_i8<kOutF32>(X, W, xs, ws, b, out, M, N, K, s);
+    return run_gemm_i8(X, W, xs, ws, b, out, out_dtype, M, N, K, s);
 }
 
 CONVROT_API int ck_int8_gemm_s32(const void* X, const void* W, void* acc, int M, int N, int K, void* stream) {

@@ -58,4 +58,9 @@ int run_linear(const void* x, int in_dtype, const void* Wp, const float* ws, Bia
                int out_dtype, int M, int N, int K, int G, unsigned char* workspace, cudaStream_t stream,
                bool allow_a8);
 
+// out[m, n] = ((float(D) * xs[m]) * ws[n]) + bias[n], D the exact product of int8 X [M, K] and
+// W [N, K] (both 16-byte aligned, K a multiple of 16); out_dtype 0 f32, 1 bf16.
+int run_gemm_i8(const void* X, const void* W, const float* xs, const float* ws, BiasRef bias, void* out, int out_dtype,
+                int M, int N, int K, cudaStream_t stream);
+
 }  // namespace convrot

@@ -48,37 +48,14 @@ cudaError_t mx4_take_status(cudaStream_t stream, int* status) {
 #include "mx4_few.cuh"
 #include "mx4_cache.cuh"
 #include "mx4_attn.cuh"
+#include "mx4_host.cuh"
+#include "mx4_attn_host.cuh"
 
 namespace convrot {
-
-// Units (128 values each) of one call: their numbers, and one grid's step beyond,
-// fit 32 bits.
-constexpr long long kMx4MostUnits = 0x7FFFFFFFll - (1 << 20);
-
-static size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 static size_t scales_bytes(int rows, int K) {
     return static_cast<size_t>((rows + 127) / 128) * ((K + 127) / 128) * kMx4TileBytes;
 }
-
-static int check_group(int K, int G) {
-    if (G != 0 && G != 16 && G != 64 && G != 256) return fail("G must be 0, 16, 64 or 256");
-    if (K <= 0 || K % kMx4Block) return fail("K must be a positive multiple of 32");
-    if (G != 0 && K % G) return fail("K must be a multiple of G");
-    return 0;
-}
-
-// Calls f with a null pointer of the C type of dtype code 0 f32, 1 bf16, 2 f16.
-template <typename F>
-static int with_type(int code, F f) {
-    if (code == 0) return f(static_cast<float*>(nullptr));
-    if (code == 1) return f(static_cast<__nv_bfloat16*>(nullptr));
-    return f(static_cast<__half*>(nullptr));
-}
-
-static size_t type_size(int code) { return code == 0 ? 4 : 2; }
-
-static bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 static int check_matrix(const void* x, int dtype, const void* codes, const void* scales, int M, int K, int G) {
     if (M < 0) return fail("M must not be negative");
@@ -90,22 +67,6 @@ static int check_matrix(const void* x, int dtype, const void* codes, const void*
     if (!aligned16(codes) || !aligned16(scales)) return fail("codes and scales must be 16-byte aligned");
     if (static_cast<long long>(M + 127LL) / 128 * 128 * ((K + 127) / 128) > kMx4MostUnits) return fail("matrix too large");
     return 0;
-}
-
-// Calls f with an integral constant for the rotation group.
-template <typename F>
-static int with_group(int G, F f) {
-    if (G == 16) return f(std::integral_constant<int, 16>{});
-    if (G == 64) return f(std::integral_constant<int, 64>{});
-    if (G == 256) return f(std::integral_constant<int, 256>{});
-    return f(std::integral_constant<int, 0>{});
-}
-
-// Blocks of the unit kernels: one wave of three a multiprocessor, a warp's 32
-// units at a time.
-static int unit_blocks(long long units) {
-    const long long want = (units + kMx4QuantWarps * 32 - 1) / (kMx4QuantWarps * 32), most = 3LL * sm_count();
-    return static_cast<int>(want < most ? want : most);
 }
 
 static int run_quant(const void* x, int dtype, long long ldx, void* codes, void* scales, int M, int K, int G, cudaStream_t st) {
@@ -320,111 +281,6 @@ CONVROT_API int ck_mx4_linear(const void* x, int dtype, long long ldx, const voi
     });
 }
 
-// Calls f with integral constants for the head dimension and the rotation group.
-template <typename F>
-static int with_head(int d, int G, F f) {
-    return with_group(G, [&](auto g) {
-        constexpr int g0 = decltype(g)::value;
-        if (d == 64) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, g0 == 256 ? 0 : g0>{});
-        if (d == 128) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, g0 == 256 ? 0 : g0>{});
-        return f(std::integral_constant<int, 256>{}, g);
-    });
-}
-
-static int page_bits(int page) {
-    int b = 0;
-    while ((1 << b) < page) ++b;
-    return b;
-}
-
-// How an attention call is cut: tiles of query rows (one sequence and cache head
-// each) and splits of the sequences.
-struct AttnPlan {
-    long long tiles;
-    int tile_rows, row_tiles, splits;
-    bool clustered;                // a sequence's splits are one cluster and join themselves
-    size_t partials() const { return splits > 1 && !clustered ? static_cast<size_t>(tiles) * splits * tile_rows : 0; }
-};
-
-static AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
-    AttnPlan p;
-    const long long rows = static_cast<long long>(tq) * (hq / hkv);
-    p.tile_rows = rows <= 8 ? 8 : rows <= 16 || d == 256 ? 16 : 32;
-    p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
-    p.tiles = static_cast<long long>(B) * hkv * p.row_tiles;
-    // splits: one full wave of blocks always, as far as every split has a group of
-    // tokens; up to four waves, which even the tail out, while each split keeps eight
-    // groups (a block's start and end cost about as much as three). Waves counted by the
-    // blocks a multiprocessor really holds, and whole ones: 64 x 4096 tokens of 32 heads 320 us,
-    // 355 with a part of a wave; 64 x 1024 of 32 heads on 8: 30.4 against 35.5
-    const long long groups = (longest + kMx4AttnGroup - 1) / kMx4AttnGroup, tiles = p.tiles > 0 ? p.tiles : 1;
-    const long long places = static_cast<long long>(mx4_attn_resident(p.tile_rows / 8 * d)) * sm_count();
-    long long waves = 4;
-    while (waves > 1 && waves * places / tiles > groups / 8) --waves;
-    const long long want = waves * places / tiles;
-    p.splits = static_cast<int>(std::max(1LL, std::min({want, groups, static_cast<long long>(kMx4MostSplits)})));
-    // one launch instead of two (1 x 777 tokens: 7.8 against 9.9 us), where every block is
-    // resident at once; with more, a cluster's blocks wait for each other and for places
-    // (64 x 4096 tokens, 4 splits: 106 against 99 us)
-    p.clustered = p.splits > 1 && p.splits <= 8 && tiles * p.splits <= 2LL * sm_count();
-    return p;
-}
-
-template <typename T, int D, int NT>
-static int launch_attention(const Mx4AttnArgs& a, const AttnPlan& p, cudaStream_t stream) {
-    using Cfg = Mx4AttnCfg<D, NT>;
-    auto kernel = mx4_attn_kernel<T, D, NT>;
-    cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.tiles), p.splits, 1);
-    cfg.blockDim = dim3(kMx4AttnWarps * 32, 1, 1);
-    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 1;
-    attr[1].val.clusterDim.y = p.splits;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.clustered ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e == cudaSuccess && p.splits > 1 && !p.clustered) {
-        const unsigned rows = static_cast<unsigned>(a.B * a.tq * a.hq);
-        const int wide = p.splits > 16;
-        e = launch_pdl(mx4_attn_join_kernel<T, D>, dim3(wide ? rows : (rows + 7) / 8), dim3(256), 0, stream, a, p.tile_rows, wide);
-    }
-    return static_cast<int>(e);
-}
-
-template <typename T, int D>
-static int launch_attention_rows(const Mx4AttnArgs& a, const AttnPlan& p, cudaStream_t stream) {
-    if (p.tile_rows == 8) return launch_attention<T, D, 1>(a, p, stream);
-    if constexpr (D < 256)
-        if (p.tile_rows == 32) return launch_attention<T, D, 4>(a, p, stream);
-    return launch_attention<T, D, 2>(a, p, stream);
-}
-
-template <typename T>
-static int run_attention(const Mx4AttnArgs& a, int d, const AttnPlan& p, cudaStream_t stream) {
-    if (d == 256) return launch_attention_rows<T, 256>(a, p, stream);
-    if (d == 128) return launch_attention_rows<T, 128>(a, p, stream);
-    return launch_attention_rows<T, 64>(a, p, stream);
-}
-
-static int check_cache(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G) {
-    if (d != 64 && d != 128 && d != 256) return fail("the head dimension must be 64, 128 or 256");
-    if (int rc = check_group(d, G)) return rc;
-    if (heads <= 0 || page <= 0 || pages < 0) return fail("heads and page must be positive, pages not negative");
-    if (page & (page - 1) || page > 65536) return fail("the page size must be a power of two up to 65536");
-    if (pages > 0x7FFFFFFFll) return fail("too many pages");
-    if (pages && (!codes || !scales)) return fail("null cache pointer");
-    if (!aligned16(codes) || !aligned16(scales)) return fail("the cache must be 16-byte aligned");
-    return 0;
-}
-
 CONVROT_API int ck_mx4_cache_append(void* codes, void* scales, long long pages, int heads, int d, int page, int G,
                                     const void* k, const void* v, int in_dtype, long long k_token, long long k_head,
                                     long long v_token, long long v_head, const void* slots, int T, void* stream) {
@@ -517,6 +373,6 @@ CONVROT_API int ck_mx4_attention(const void* q, int dtype, long long q_seq, long
                   B, tq, hq, hkv, page_bits(page), static_cast<int>(pages), G, p.row_tiles, p.splits, p.clustered,
                   softmax_scale * 1.4426950408889634f};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == 1) return run_attention<__nv_bfloat16>(a, d, p, st);
-    return run_attention<__half>(a, d, p, st);
+    if (dtype == 1) return run_attention<__nv_bfloat16, false>(a, d, p, st);
+    return run_attention<__half, false>(a, d, p, st);
 }

@@ -64,6 +64,27 @@ struct Mx4AttnArgs {
     int B, tq, hq, hkv, page_bits, pages, group, row_tiles, splits;
     int clustered;                 // a sequence's splits are one cluster and join themselves
     float scale;                   // softmax scale times log2(e)
+    // a tree of drafted tokens (TREE): node t of a sequence, one of its last nodes[b] tokens
+    // (null: tq), sees those before them and the nodes that mask[b][t] names
+    const uint8_t* mask;
+    const int* nodes;
+    long long mask_seq, mask_row;  // strides in bytes
+};
+
+// A sequence's nodes and the tokens before them (negative: nodes -context .. 0 do not exist).
+struct Mx4Tree {
+    int nodes, context;
+    const uint8_t* mask;
+    long long row;
+    Mx4Tree() = default;
+    __device__ __forceinline__ Mx4Tree(const Mx4AttnArgs& a, int b, int n) {
+        nodes = a.nodes ? max(0, min(a.nodes[b], a.tq)) : a.tq;
+        context = n - nodes;
+        mask = a.mask + b * a.mask_seq;
+        row = a.mask_row;
+    }
+    // Whether node t, one of the tree's, sees token j, one of the cache's.
+    __device__ __forceinline__ bool sees(int t, int j) const { return j < context || mask[t * row + (j - context)] != 0; }
 };
 
 constexpr int kMx4AttnWarps = 4;
@@ -187,7 +208,7 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
     return d;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool TREE = false>
 __global__ void __launch_bounds__(kMx4AttnWarps * 32, Mx4AttnCfg<D, NT>::kResident)
 mx4_attn_kernel(Mx4AttnArgs a) {
     using Cfg = Mx4AttnCfg<D, NT>;
@@ -363,7 +384,9 @@ mx4_attn_kernel(Mx4AttnArgs a) {
             rs[i][h] = row_scale[r];
         }
     }
-    const int sees_all = n - a.tq + row0 / per_head + 1;          // tokens that every row of the tile sees
+    int sees_all = n - a.tq + row0 / per_head + 1;                // tokens that every row of the tile sees
+    const Mx4Tree tree = TREE ? Mx4Tree(a, b, n) : Mx4Tree{};
+    if constexpr (TREE) sees_all = (row0 + rows - 1) / per_head < tree.nodes ? tree.context : 0;   // (padding sees nothing)
     const int ktok = (g >> 1) + 4 * (g & 1);                      // this thread's token of each tile of 8
     int most_seen = 0;                                            // largest scale byte of the warp's values so far
 
@@ -503,10 +526,13 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int r = 8 * i + 2 * t4 + h;
-                    const int sees = r < rows ? n - a.tq + (row0 + r) / per_head + 1 : 0;
+                    const int t = (row0 + r) / per_head;
+                    const int sees = r >= rows ? 0 : !TREE ? n - a.tq + t + 1 : t < tree.nodes ? n : 0;
                     #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (ci * kMx4AttnChunk + 8 * c + ktok >= sees) s[i][c >> 1][2 * (c & 1) + h] = -INFINITY;
+                    for (int c = 0; c < 4; ++c) {
+                        const int j = ci * kMx4AttnChunk + 8 * c + ktok;
+                        if (j >= sees || (TREE && !tree.sees(t, j))) s[i][c >> 1][2 * (c & 1) + h] = -INFINITY;
+                    }
                 }
             // a value's block of NaN: straight to the accumulators of the rows that see its
             // token, which are those that see the first such (a product with the weight 0 would
@@ -521,11 +547,22 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 #pragma unroll
                 for (int i = 0; i < NT; ++i)
                     #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (first <= n - a.tq + (row0 + 8 * i + 2 * t4 + h) / per_head) {
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = 8 * i + 2 * t4 + h, t = (row0 + r) / per_head;
+                        bool seen = first <= n - a.tq + t;
+                        if constexpr (TREE) {                     // any of them, not the first alone
+                            seen = false;
+                            if (r < rows && t < tree.nodes)
+                                for (uint32_t left = nan; left; left &= left - 1) {
+                                    const int j = ci * kMx4AttnChunk + __ffs(left) - 1;
+                                    seen |= j < n && tree.sees(t, j);
+                                }
+                        }
+                        if (seen) {
                             #pragma unroll
                             for (int j = 4 * hf; j < 4 * hf + 4; ++j) o[i][j][h] = o[i][j][2 + h] = NAN;
                         }
+                    }
                 if (nan0 >> lane & 1) mine[0] = __ushort_as_half(0);
                 if (nan1 >> lane & 1) mine[32] = __ushort_as_half(0);
                 __syncwarp();

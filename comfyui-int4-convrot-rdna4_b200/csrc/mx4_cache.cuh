@@ -47,6 +47,30 @@ struct Mx4CacheUnit {
 template <int D>
 __host__ __device__ constexpr int mx4_cache_units(int heads) { return D == 64 ? (heads + 1) / 2 : D == 128 ? heads : 2 * heads; }
 
+// Writes a unit's codes and scale bytes to its place in a slot (outside the cache: nowhere).
+template <int D>
+__device__ __forceinline__ void cache_store_unit(uint8_t* codes, uint8_t* scales, const Mx4CacheShape& c, long long slot,
+                                                 const Mx4CacheUnit<D>& at, const uint4 (&q)[4], uint32_t word) {
+    if (slot < 0 || slot >= c.slots) return;
+    const size_t tok = c.token(slot, at.kv, at.head);
+    if constexpr (D == 64) {
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h >= at.halves) break;
+            const size_t to = tok + (static_cast<size_t>(h) << c.page_bits);
+            uint4* dst = reinterpret_cast<uint4*>(codes + to * 32);
+            dst[0] = q[2 * h];
+            dst[1] = q[2 * h + 1];
+            *reinterpret_cast<uint16_t*>(scales + to * 2) = static_cast<uint16_t>(word >> (16 * h));
+        }
+    } else {
+        uint4* dst = reinterpret_cast<uint4*>(codes + tok * (D / 2) + at.part * 64);
+        #pragma unroll
+        for (int b = 0; b < 4; ++b) dst[b] = q[b];
+        *reinterpret_cast<uint32_t*>(scales + tok * (D / 32) + at.part * 4) = word;
+    }
+}
+
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(kMx4QuantWarps * 32, 3)
 mx4_cache_append_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ k,
@@ -91,26 +115,7 @@ mx4_cache_append_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scale
         const uint32_t word = unit_quantize(val, unit_factor<G>(), q);
         const int u = (base + lane) ^ (G == 256 ? 1 : 0);
         const Mx4CacheUnit<D> at(u, per, c.heads, units);
-        const long long slot = u < units ? slots[at.t] : -1;
-        if (slot >= 0 && slot < c.slots) {
-            const size_t tok = c.token(slot, at.kv, at.head);
-            if constexpr (D == 64) {
-                #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (h >= at.halves) break;
-                    const size_t to = tok + (static_cast<size_t>(h) << c.page_bits);
-                    uint4* dst = reinterpret_cast<uint4*>(codes + to * 32);
-                    dst[0] = q[2 * h];
-                    dst[1] = q[2 * h + 1];
-                    *reinterpret_cast<uint16_t*>(scales + to * 2) = static_cast<uint16_t>(word >> (16 * h));
-                }
-            } else {
-                uint4* dst = reinterpret_cast<uint4*>(codes + tok * (D / 2) + at.part * 64);
-                #pragma unroll
-                for (int b = 0; b < 4; ++b) dst[b] = q[b];
-                *reinterpret_cast<uint32_t*>(scales + tok * (D / 32) + at.part * 4) = word;
-            }
-        }
+        cache_store_unit<D>(codes, scales, c, u < units ? slots[at.t] : -1, at, q, word);
         __syncwarp();
     }
 }

@@ -1,0 +1,139 @@
+// C entries of the rotary positions: on their own, and on the way into the paged MX4
+// cache. Conventions of include/convrot_b200.h.
+#include <algorithm>
+
+#include "mx4_host.cuh"
+#include "mx4_cache.cuh"
+#include "rope.cuh"
+#include "mx4_cache_rope.cuh"
+
+#define CONVROT_API extern "C" __attribute__((visibility("default")))
+
+using namespace convrot;
+
+namespace {
+
+// Fills `r`; `rot` pairs must fit a head of D channels.
+int rope_args(RopeArgs& r, const void* positions, int pos_type, long long p_batch, long long p_token, long long p_axis, const void* freqs,
+              const int* sections, int axes, int interleaved, int inverse, int D) {
+    if (axes <= 0 || axes > kRopeMostAxes) return fail("positions must have 1 to 8 axes");
+    if (!sections) return fail("null sections");
+    if (pos_type < 0 || pos_type > 2) return fail("positions must be int32 (0), int64 (1) or f32 (2)");
+    long long pairs = 0;
+    for (int i = 0; i < axes; ++i) {
+        if (sections[i] < 0) return fail("sections must not be negative");
+        pairs += sections[i];
+        if (2 * pairs > D) return fail("the sections hold more pairs than a head");
+        r.ends[i] = static_cast<int>(pairs);
+    }
+    r.pos = positions;
+    r.freqs = static_cast<const double*>(freqs);
+    r.pb = p_batch;
+    r.pt = p_token;
+    r.pa = p_axis;
+    r.pos_type = pos_type;
+    r.pairs = static_cast<int>(pairs);
+    r.axes = axes;
+    r.interleaved = interleaved != 0;
+    r.sign = inverse ? -1.0f : 1.0f;
+    return 0;
+}
+
+int rope_pointers(const RopeArgs& r) {
+    if (r.pairs && (!r.pos || !r.freqs)) return fail("null positions or frequencies");
+    if (!aligned_to(r.pos, r.pos_type == 1 ? 8 : 4) || !aligned_to(r.freqs, 8)) return fail("positions or frequencies not aligned to their type");
+    return 0;
+}
+
+// Chunks of 16 bytes: sections of whole chunks, every row on a 16-byte boundary.
+bool whole_chunks(const RopeArgs& r, int D, size_t size, long long strides) {
+    const int vp = static_cast<int>(16 / size);
+    return r.pairs % vp == 0 && D % (2 * vp) == 0 && strides * static_cast<long long>(size) % 16 == 0;
+}
+
+template <typename T, int VP>
+int launch_rope(const void* x, void* out, RopeShape s, long long tokens, const RopeArgs& r, cudaStream_t stream) {
+    const long long chunks = s.D / (2 * VP);
+    // heads a thread: as many as leave every multiprocessor `kFull` threads
+    constexpr long long kFull = 1024;
+    s.heads = static_cast<int>(std::max(1LL, std::min(static_cast<long long>(s.H), tokens * chunks * s.H / (kFull * sm_count()))));
+    s.runs = (s.H + s.heads - 1) / s.heads;
+    s.threads = tokens * chunks * s.runs;
+    const long long blocks = (s.threads + kRopeThreads - 1) / kRopeThreads;
+    if (blocks > 0x7FFFFFFFll) return fail("tensor too large");
+    return static_cast<int>(launch_pdl(rope_kernel<T, VP>, dim3(static_cast<unsigned>(blocks)), dim3(kRopeThreads), 0, stream,
+                                       static_cast<const T*>(x), static_cast<T*>(out), s, r));
+}
+
+}  // namespace
+
+CONVROT_API int ck_rope(const void* x, int dtype, long long x_batch, long long x_token, long long x_head, void* out, int B, int T, int H,
+                        int D, const void* positions, int pos_type, long long p_batch, long long p_token, long long p_axis, const void* freqs,
+                        const int* sections, int axes, int interleaved, int inverse, void* stream) {
+    if (dtype < 0 || dtype > 2) return fail("dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    if (B < 0 || T < 0 || H < 0 || D <= 0 || D % 2) return fail("sizes must not be negative, D even");
+    RopeArgs r;
+    if (int rc = rope_args(r, positions, pos_type, p_batch, p_token, p_axis, freqs, sections, axes, interleaved, inverse, D)) return rc;
+    const long long tokens = static_cast<long long>(B) * T;
+    if (tokens == 0 || H == 0) return 0;
+    if (tokens > (1ll << 62) / (static_cast<long long>(H) * D)) return fail("tensor too large");
+    if (!x || !out) return fail("null pointer");
+    if (int rc = rope_pointers(r)) return rc;
+    if (!aligned_to(x, type_size(dtype)) || !aligned_to(out, type_size(dtype))) return fail("x or out is not aligned to its type");
+    const RopeShape s{x_batch, x_token, x_head, T, H, D, 0, 0, 0};
+    return with_type(dtype, [&](auto* t) {
+        using E = std::remove_pointer_t<decltype(t)>;
+        const bool wide = aligned16(x) && aligned16(out) && whole_chunks(r, D, sizeof(E), x_batch | x_token | x_head);
+        if (wide) return launch_rope<E, 16 / sizeof(E)>(x, out, s, tokens, r, static_cast<cudaStream_t>(stream));
+        return launch_rope<E, 1>(x, out, s, tokens, r, static_cast<cudaStream_t>(stream));
+    });
+}
+
+CONVROT_API int ck_mx4_cache_append_rope(void* codes, void* scales, long long pages, int heads, int d, int page, int G, const void* q,
+                                         const void* k, const void* v, int dtype, int q_heads, long long q_token, long long q_head,
+                                         long long k_token, long long k_head, long long v_token, long long v_head, void* q_out,
+                                         const void* slots, int T, const void* positions, int pos_type, long long p_token, long long p_axis,
+                                         const void* freqs, const int* sections, int axes, int interleaved, void* stream) {
+    if (int rc = check_cache(codes, scales, pages, heads, d, page, G)) return rc;
+    if (T < 0 || q_heads < 0) return fail("T and the query heads must not be negative");
+    if (dtype < 0 || dtype > 2) return fail("dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    RopeArgs r;
+    if (int rc = rope_args(r, positions, pos_type, 0, p_token, p_axis, freqs, sections, axes, interleaved, 0, d)) return rc;
+    if (T == 0) return 0;
+    if (!k || !v || !slots || (q_heads && (!q || !q_out))) return fail("null pointer");
+    if (int rc = rope_pointers(r)) return rc;
+    const size_t size = type_size(dtype);
+    if (!aligned_to(k, size) || !aligned_to(v, size) || !aligned_to(slots, 8)) return fail("keys, values or slots are not aligned to their type");
+    if (q_heads && (!aligned_to(q, size) || !aligned_to(q_out, size))) return fail("queries are not aligned to their type");
+    const Mx4CacheShape c{pages * page, heads, d, page_bits(page)};
+    return with_type(dtype, [&](auto* t) {
+        using E = std::remove_pointer_t<decltype(t)>;
+        return with_head(d, G, [&](auto dim, auto g) {
+            constexpr int D = decltype(dim)::value;
+            const long long units = static_cast<long long>(T) * mx4_cache_units<D>(heads), q_items = static_cast<long long>(T) * q_heads;
+            if (2 * units > kMx4MostUnits || q_items > 0x7FFFFFFFll - 4096) return fail("too many tokens in one call");
+            Mx4AppendRope a{};
+            a.q = q;
+            a.k = k;
+            a.v = v;
+            a.q_out = q_out;
+            a.qst = q_token; a.qsh = q_head; a.kst = k_token; a.ksh = k_head; a.vst = v_token; a.vsh = v_head;
+            a.slots = static_cast<const long long*>(slots);
+            a.codes = static_cast<uint8_t*>(codes);
+            a.scales = static_cast<uint8_t*>(scales);
+            a.tokens = T;
+            a.hq = q_heads;
+            a.units = static_cast<int>(units);
+            a.kv_tasks = static_cast<int>((units + 31) / 32);
+            a.tasks = 2 * a.kv_tasks + static_cast<int>((q_items * D + 4095) / 4096);
+            const long long strides = k_token | k_head | v_token | v_head | (q_heads ? q_token | q_head : 0);
+            a.wide = aligned16(k) && aligned16(v) && (!q_heads || (aligned16(q) && aligned16(q_out))) && whole_chunks(r, d, sizeof(E), strides);
+            auto kernel = mx4_cache_append_rope_kernel<E, D, decltype(g)::value>;
+            const int smem = kMx4QuantWarps * Mx4Slab<float>::kBytes;
+            cudaError_t e = ensure_smem(kernel, smem);
+            if (e != cudaSuccess) return static_cast<int>(e);
+            const int blocks = std::min((a.tasks + kMx4QuantWarps - 1) / kMx4QuantWarps, 3 * sm_count());
+            return static_cast<int>(launch_pdl(kernel, dim3(blocks), dim3(kMx4QuantWarps * 32), smem, static_cast<cudaStream_t>(stream), a, c, r));
+        });
+    });
+}

@@ -1,0 +1,207 @@
+// Rotary positions: pair i of a head is turned by the angle p f_i, p the token's
+// position on the pair's axis.
+//
+// Pairs are channels (2i, 2i + 1) (interleaved) or (i, i + P) of P pairs; the
+// channels behind the 2P first stay as they are. The pairs are cut into sections, one an
+// axis (text: one; images and video: index, height, width).
+//
+// The angle is taken in turns and in 64 bits, t = p (f / 2 pi), and only its fraction
+// t - round(t) goes to fp32: at position 10^6 an fp32 product would be 0.06 radians
+// off, this is 2^-24 turns off wherever the token stands. (64-bit products run at half
+// the fp32 rate here, and a token's angles serve all of its heads.)
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+#include <type_traits>
+
+#include "mx4_common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace convrot {
+
+constexpr int kRopeMostAxes = 8;
+
+struct RopeArgs {
+    const void* pos;               // [B, T, axes] by strides
+    const double* freqs;           // [pairs], radians a position
+    long long pb, pt, pa;
+    int pos_type;                  // 0 int32, 1 int64, 2 f32
+    int pairs, axes, interleaved;
+    float sign;                    // -1: the rotation back
+    int ends[kRopeMostAxes];       // where each axis's section ends
+
+    __device__ __forceinline__ double position(long long b, long long t, int axis) const {
+        const long long at = b * pb + t * pt + axis * pa;
+        if (pos_type == 0) return static_cast<double>(static_cast<const int*>(pos)[at]);
+        if (pos_type == 1) return static_cast<double>(static_cast<const long long*>(pos)[at]);
+        return static_cast<double>(static_cast<const float*>(pos)[at]);
+    }
+};
+
+// Cosine and sine of VP pairs of a token in a row.
+template <int VP>
+struct RopeCoef {
+    float c[VP], s[VP];
+    __device__ __forceinline__ void none() {
+        #pragma unroll
+        for (int i = 0; i < VP; ++i) { c[i] = 1.0f; s[i] = 0.0f; }
+    }
+    __device__ __forceinline__ void load(const RopeArgs& r, long long b, long long t, int pair) {
+        int axis = 0;
+        while (axis < r.axes - 1 && pair >= r.ends[axis]) ++axis;
+        double p = r.position(b, t, axis);
+        #pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            if (axis < r.axes - 1 && pair + i >= r.ends[axis]) {
+                do ++axis; while (axis < r.axes - 1 && pair + i >= r.ends[axis]);
+                p = r.position(b, t, axis);
+            }
+            const double turns = p * (r.freqs[pair + i] * 0.15915494309189533577);
+            sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s[i], &c[i]);
+            s[i] *= r.sign;
+        }
+    }
+};
+
+// Where a thread's 2 VP channels lie: VP from a and VP from b, which are pairs (halves)
+// or hold pairs of neighbours (interleaved); behind the rotated channels, plain copies.
+template <int VP>
+struct RopePlace {
+    int a, b, pair;                // pair < 0: no pairs here
+    __device__ __forceinline__ RopePlace(const RopeArgs& r, int u) {
+        const int turned = r.pairs / VP;
+        if (u >= turned || r.interleaved) {
+            a = 2 * VP * u;
+            b = a + VP;
+            pair = u < turned ? VP * u : -1;
+        } else {
+            a = pair = VP * u;
+            b = r.pairs + VP * u;
+        }
+    }
+};
+
+template <int VP>
+__device__ __forceinline__ void rope_turn(float (&a)[VP], float (&b)[VP], const RopeCoef<VP>& w, bool interleaved) {
+    if (VP > 1 && interleaved) {
+        #pragma unroll
+        for (int i = 0; i + 1 < VP; i += 2) {
+            const float x = a[i], y = a[i + 1], z = b[i], t = b[i + 1];
+            a[i] = fmaf(x, w.c[i / 2], -y * w.s[i / 2]);
+            a[i + 1] = fmaf(x, w.s[i / 2], y * w.c[i / 2]);
+            b[i] = fmaf(z, w.c[(VP + i) / 2], -t * w.s[(VP + i) / 2]);
+            b[i + 1] = fmaf(z, w.s[(VP + i) / 2], t * w.c[(VP + i) / 2]);
+        }
+    } else {
+        #pragma unroll
+        for (int i = 0; i < VP; ++i) {
+            const float x = a[i], y = b[i];
+            a[i] = fmaf(x, w.c[i], -y * w.s[i]);
+            b[i] = fmaf(x, w.s[i], y * w.c[i]);
+        }
+    }
+}
+
+// VP values from memory as they are: 16 bytes where VP is more than one.
+template <typename T, int VP>
+struct RopeRaw {
+    static_assert(VP == 1 || VP * sizeof(T) == 16, "a chunk is 16 bytes or one value");
+    std::conditional_t<VP == 1, T, uint4> v;
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VP == 1) v = *p;
+        else v = __ldg(reinterpret_cast<const uint4*>(p));
+    }
+    __device__ __forceinline__ void zero() {
+        if constexpr (VP == 1) v = mx4_from_f32<T>(0.0f);
+        else v = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void get(float (&f)[VP]) const {
+        if constexpr (VP == 1) {
+            f[0] = mx4_to_f32(v);
+        } else {
+            T e[VP];
+            memcpy(e, &v, 16);
+            #pragma unroll
+            for (int i = 0; i < VP; ++i) f[i] = mx4_to_f32(e[i]);
+        }
+    }
+    __device__ __forceinline__ void put(const float (&f)[VP]) {
+        if constexpr (VP == 1) {
+            v = mx4_from_f32<T>(f[0]);
+        } else {
+            T e[VP];
+            #pragma unroll
+            for (int i = 0; i < VP; ++i) e[i] = mx4_from_f32<T>(f[i]);
+            memcpy(&v, e, 16);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (VP == 1) *p = v;
+        else *reinterpret_cast<uint4*>(p) = v;
+    }
+};
+
+struct RopeShape {
+    long long xb, xt, xh;          // strides of the input in elements: batch, token, head
+    int T, H, D;
+    int heads, runs;               // heads a thread takes, threads a chunk of a token needs
+    long long threads;
+};
+
+constexpr int kRopeThreads = 256;
+
+// x [B, T, H, D] by strides -> out [B, T, H, D] without gaps. A thread has 2 VP channels
+// of one token and goes through its heads.
+template <typename T, int VP>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const T* __restrict__ x, T* __restrict__ out, RopeShape s, RopeArgs r) {
+    constexpr int kAhead = 4;
+    griddep_wait();
+    griddep_launch_dependents();
+    const long long id = static_cast<long long>(blockIdx.x) * kRopeThreads + threadIdx.x;
+    if (id >= s.threads) return;
+    const int chunks = s.D / (2 * VP);
+    const int u = static_cast<int>(id % chunks);
+    const long long rest = id / chunks, token = rest / s.runs;
+    const int h0 = static_cast<int>(rest % s.runs) * s.heads, h1 = min(s.H, h0 + s.heads);
+    const long long b = token / s.T, t = token % s.T;
+    const RopePlace<VP> at(r, u);
+    const T* src = x + b * s.xb + t * s.xt;
+    T* dst = out + token * s.H * s.D;
+    RopeCoef<VP> w;
+    bool known = false;
+    for (int h = h0; h < h1; h += kAhead) {
+        RopeRaw<T, VP> ra[kAhead], rb[kAhead];
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (h + i < h1) {
+                ra[i].load(src + (h + i) * s.xh + at.a);
+                rb[i].load(src + (h + i) * s.xh + at.b);
+            }
+        if (!known) {                                             // (the first loads are on their way)
+            if (at.pair >= 0) w.load(r, b, t, at.pair);
+            known = true;
+        }
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (h + i < h1) {
+                T* to = dst + static_cast<long long>(h + i) * s.D;
+                if (at.pair >= 0) {
+                    float fa[VP], fb[VP];
+                    ra[i].get(fa);
+                    rb[i].get(fb);
+                    rope_turn<VP>(fa, fb, w, r.interleaved);
+                    ra[i].put(fa);
+                    rb[i].put(fb);
+                }
+                ra[i].store(to + at.a);
+                rb[i].store(to + at.b);
+            }
+    }
+}
+
+}  // namespace convrot

@@ -373,6 +373,60 @@ int ck_mx4_attention(const void* q, int dtype, long long q_seq, long long q_toke
                      int hkv, int d, int G, float softmax_scale, void* workspace, size_t workspace_bytes,
                      void* stream);
 
+/* Rotary positions. x [B, T, H, D] (dtype, strides in elements, D contiguous and even) -> out [B, T,
+ * H, D] without gaps: pair i of a head, channels (2i, 2i + 1) where `interleaved`, else (i, i + P), is
+ * turned by the angle p freqs[i], p the token's position on the axis whose section holds i; the channels
+ * behind the 2P first are copied. positions [B, T, axes] by strides (pos_type 0 int32, 1 int64, 2 f32),
+ * freqs [P] f64 radians a position, both on the device; sections [axes] (host): pairs of each axis, P in
+ * all, 1 to 8 axes. inverse != 0 turns back. Angles are taken in 64 bits, one rounding. */
+int ck_rope(const void* x, int dtype, long long x_batch, long long x_token, long long x_head, void* out,
+            int B, int T, int H, int D, const void* positions, int pos_type, long long p_batch,
+            long long p_token, long long p_axis, const void* freqs, const int* sections, int axes,
+            int interleaved, int inverse, void* stream);
+
+/* ck_mx4_cache_append with positions (as ck_rope, [T, axes]): keys are turned before they are rotated
+ * and quantized, without a rounding between; values as in ck_mx4_cache_append. q [T, q_heads, d] turned
+ * -> q_out [T, q_heads, d] in the same dtype (q_heads 0: none, q and q_out may be NULL). Tokens whose slot
+ * lies outside the cache write no key and no value; their queries are turned. Slots of one call must
+ * differ. */
+int ck_mx4_cache_append_rope(void* codes, void* scales, long long pages, int heads, int d, int page, int G,
+                             const void* q, const void* k, const void* v, int dtype, int q_heads,
+                             long long q_token, long long q_head, long long k_token, long long k_head,
+                             long long v_token, long long v_head, void* q_out, const void* slots, int T,
+                             const void* positions, int pos_type, long long p_token, long long p_axis,
+                             const void* freqs, const int* sections, int axes, int interleaved, void* stream);
+
+/* Workspace of ck_mx4_tree_attention for `longest` = table_pages * page (0: none needed). */
+size_t ck_mx4_tree_attention_workspace_size(int B, int tq, int hq, int hkv, int d, long long longest);
+
+/* ck_mx4_attention for drafted tokens that form a tree: sequence b's nodes are its nodes[b] newest tokens
+ * (int32 [B], cut to 0 .. tq; NULL: tq each). Node t sees the tokens before the nodes and those nodes j
+ * whose byte mask[b * mask_seq + t * mask_row + j] is not zero (itself only if named); one that sees none
+ * gives zeros, and so do the rows behind a sequence's nodes. mask_seq 0: one mask for all sequences. */
+int ck_mx4_tree_attention(const void* q, int dtype, long long q_seq, long long q_token, long long q_head,
+                          const void* codes, const void* scales, long long pages, int page, const void* table,
+                          long long table_ld, int table_pages, const void* lens, const void* nodes,
+                          const void* mask, long long mask_seq, long long mask_row, void* out, int B, int tq,
+                          int hq, int hkv, int d, int G, float softmax_scale, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Workspace of ck_convrot_w8a8_linear_rmsnorm: the int8 codes and the row scales. */
+size_t ck_convrot_w8a8_linear_rmsnorm_workspace_size(int M, int K);
+
+/* The W8A8 linear behind a root-mean-square norm: hidden = x + residual (rounded to dtype; residual NULL:
+ * hidden is not written), y = R(h / sqrt(mean h^2 + eps) * norm_weight), xs = max(max |y|, 1e-10) / 127,
+ * codes = y / xs to nearest even, out = ((float(D) * xs[m]) * wscale[n]) + bias[n] with the exact product
+ * D. fp32 throughout, h unrounded; a row with an infinity or a NaN gives NaN.
+ *   x, residual [M, K] (row strides ldx, ldr >= K), hidden [M, K] (16-byte aligned) in dtype;
+ *   norm_weight [K] in norm_dtype or NULL (ones); W [N, K] int8 and out [M, N] 16-byte aligned, wscale [N]
+ *   f32, bias [N] in bias_dtype or NULL; out_dtype 0 f32, 1 bf16; G in {16, 64, 256}, K a multiple of G and
+ *   at most 16384; workspace 256-byte aligned. */
+int ck_convrot_w8a8_linear_rmsnorm(const void* x, const void* residual, int dtype, long long ldx, long long ldr,
+                                   const void* norm_weight, int norm_dtype, float eps, const void* W,
+                                   const void* wscale, const void* bias, int bias_dtype, void* hidden, void* out,
+                                   int out_dtype, int M, int N, int K, int G, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
 /* Reads and clears the device status word that kernels set when a bounded
  * wait gives up (0 = ok). Synchronises `stream`. No reference counterpart:
  * the reference has no device-side timeouts. */
