@@ -19,7 +19,7 @@ _CSRC = os.path.join(os.path.dirname(_HERE), "csrc")
 SOURCES = ["convrot_b200.cu", "noalloc.cu", "mx4.cu", "rope.cu", "mx4_tree.cu", "rms_linear.cu"]
 HEADERS = ["sm100_ptx.cuh", "gemm_pair.cuh", "gemm_a8t.cuh", "lora_down.cuh", "linear_api.cuh", "hadamard.cuh",
            "host_launch.cuh", "mx4_common.cuh", "mx4_unit.cuh", "mx4_quant.cuh", "mx4_gemm.cuh", "mx4_few.cuh", "mx4_cache.cuh", "mx4_attn.cuh",
-           "mx4_host.cuh", "mx4_attn_host.cuh", "rope.cuh", "mx4_cache_rope.cuh", "rms_quant.cuh"]
+           "mx4_host.cuh", "mx4_attn_host.cuh", "rope.cuh", "mx4_cache_rope.cuh", "mx4_tree.cuh", "rms_quant.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -2096,7 +2096,10 @@ CONVROT_API int ck_convrot_device_status(void* stream, int* status) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     int mx4 = 0;                                       // the MX4 kernels' own word (mx4.cu)
     if (e == cudaSuccess) e = mx4_take_status(s, &mx4);
+    int tree = 0;
+    if (e == cudaSuccess) e = tree_take_status(s, &tree);
     if (e != cudaSuccess) return static_cast<int>(e);
+    if (mx4 == 0) mx4 = tree;
     *status = host != 0 ? host : mx4;
     return 0;
 }

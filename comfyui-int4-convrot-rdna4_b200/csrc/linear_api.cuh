@@ -37,6 +37,9 @@ struct PeerOut {
 // Reads and clears the status word of the MX4 kernels (mx4.cu); synchronises `stream`.
 cudaError_t mx4_take_status(cudaStream_t stream, int* status);
 
+// The same for the kernels of mx4_tree.cu.
+cudaError_t tree_take_status(cudaStream_t stream, int* status);
+
 // Records `msg` for ck_convrot_last_error() and returns -1.
 int fail(const char* msg);
 

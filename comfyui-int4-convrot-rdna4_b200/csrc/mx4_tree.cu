@@ -7,13 +7,96 @@
 #include "mx4_attn.cuh"
 #include "mx4_attn_host.cuh"
 
+namespace convrot {
+
+// Status word of the kernels of this file (a bounded wait that gave up).
+static __device__ int g_tree_status;
+
+enum : int { kMx4TimeoutProducer = 1, kMx4TimeoutMma = 2, kMx4TimeoutEpilogue = 4 };
+
+__device__ __forceinline__ void tree_record_status(int code) { atomicCAS(&g_tree_status, 0, code); }
+
+cudaError_t tree_take_status(cudaStream_t stream, int* status) {
+    cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_tree_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    const int zero = 0;
+    if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_tree_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    return e;
+}
+
+}  // namespace convrot
+
+#include "mx4_tree.cuh"
+
 #define CONVROT_API extern "C" __attribute__((visibility("default")))
 
 using namespace convrot;
 
+namespace {
+
+// How a call is cut. `tensor`: the kernel of this file's header, with 256 rows of a cache head a
+// block (pair) or 128; otherwise the one for few rows.
+struct TreePlan {
+    AttnPlan p;
+    bool tensor, pair;
+};
+
+TreePlan tree_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
+    TreePlan t{};
+    const long long rows = static_cast<long long>(tq) * (hq / hkv);
+    t.tensor = d <= 128 && rows > 32;
+    if (!t.tensor) {
+        t.p = attn_plan(B, tq, hq, hkv, d, longest);
+        return t;
+    }
+    t.pair = rows > kTreeTile;
+    t.p.tile_rows = t.pair ? 2 * kTreeTile : kTreeTile;
+    t.p.row_tiles = static_cast<int>((rows + t.p.tile_rows - 1) / t.p.tile_rows);
+    t.p.tiles = static_cast<long long>(B) * hkv * t.p.row_tiles;
+    // as many splits as give the least waves of blocks times tiles of a block, a block's start and
+    // end counted as two tiles
+    const long long groups = std::max(1LL, (longest + kTreeTile - 1) / kTreeTile), sms = sm_count();
+    long long best = -1;
+    t.p.splits = 1;
+    for (long long s = 1; s <= std::min(groups, 64LL) && t.p.tiles * s <= 16 * sms + t.p.tiles; ++s) {
+        const long long cost = (t.p.tiles * s + sms - 1) / sms * ((groups + s - 1) / s + 2 + (s > 1));
+        if (best < 0 || cost < best) {
+            best = cost;
+            t.p.splits = static_cast<int>(s);
+        }
+    }
+    return t;
+}
+
+template <typename T, int D, bool PAIR>
+int launch_tree(const Mx4AttnArgs& a, const AttnPlan& p, int vec_q, cudaStream_t stream) {
+    using Cfg = Mx4TreeCfg<D>;
+    auto kernel = mx4_tree_kernel<T, D, PAIR>;
+    cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    e = launch_pdl(kernel, dim3(static_cast<unsigned>(p.tiles), p.splits), dim3(kTreeThreads), Cfg::kSmemBytes, stream, a, vec_q);
+    if (e == cudaSuccess && p.splits > 1) {
+        const unsigned rows = static_cast<unsigned>(a.B * a.tq * a.hq);
+        const int wide = p.splits > 16;
+        e = launch_pdl(mx4_attn_join_kernel<T, D>, dim3(wide ? rows : (rows + 7) / 8), dim3(256), 0, stream, a, p.tile_rows, wide);
+    }
+    return static_cast<int>(e);
+}
+
+template <typename T>
+int run_tree(const Mx4AttnArgs& a, int d, const TreePlan& t, cudaStream_t stream) {
+    if (!t.tensor) return run_attention<T, true>(a, d, t.p, stream);
+    const int vec_q = aligned16(a.q) && (a.qsb | a.qst | a.qsh) % 8 == 0;
+    if (d == 128) return t.pair ? launch_tree<T, 128, true>(a, t.p, vec_q, stream) : launch_tree<T, 128, false>(a, t.p, vec_q, stream);
+    return t.pair ? launch_tree<T, 64, true>(a, t.p, vec_q, stream) : launch_tree<T, 64, false>(a, t.p, vec_q, stream);
+}
+
+}  // namespace
+
 CONVROT_API size_t ck_mx4_tree_attention_workspace_size(int B, int tq, int hq, int hkv, int d, long long longest) {
     if (B <= 0 || tq <= 0 || hkv <= 0 || hq <= 0 || hq % hkv || d <= 0) return 0;
-    const AttnPlan p = attn_plan(B, tq, hq, hkv, d, longest);
+    const AttnPlan p = tree_plan(B, tq, hq, hkv, d, longest).p;
     return align256(p.partials() * d * 4) + align256(p.partials() * 8);
 }
 
@@ -35,7 +118,8 @@ CONVROT_API int ck_mx4_tree_attention(const void* q, int dtype, long long q_seq,
         return fail("queries, table or lengths not aligned to their type, or out not to 16 bytes");
     if (pages * 2 * hkv * page > 0xFFFFFFFEll) return fail("the cache holds more than 2^32 - 2 rows");
     const long long longest = static_cast<long long>(table_pages) * page;
-    const AttnPlan p = attn_plan(B, tq, hq, hkv, d, longest);
+    const TreePlan t = tree_plan(B, tq, hq, hkv, d, longest);
+    const AttnPlan& p = t.p;
     if (p.tiles > 0x7FFFFFFF) return fail("too many query rows");
     const size_t need = ck_mx4_tree_attention_workspace_size(B, tq, hq, hkv, d, longest);
     if (need && (!workspace || !aligned_to(workspace, 256))) return fail("the workspace must be 256-byte aligned");
@@ -46,6 +130,6 @@ CONVROT_API int ck_mx4_tree_attention(const void* q, int dtype, long long q_seq,
                   B, tq, hq, hkv, page_bits(page), static_cast<int>(pages), G, p.row_tiles, p.splits, p.clustered,
                   softmax_scale * 1.4426950408889634f, static_cast<const uint8_t*>(mask), static_cast<const int*>(nodes), mask_seq, mask_row};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == 1) return run_attention<__nv_bfloat16, true>(a, d, p, st);
-    return run_attention<__half, true>(a, d, p, st);
+    if (dtype == 1) return run_tree<__nv_bfloat16>(a, d, t, st);
+    return run_tree<__half>(a, d, t, st);
 }

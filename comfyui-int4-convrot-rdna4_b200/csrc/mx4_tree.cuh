@@ -1,0 +1,665 @@
+// Attention of a tree of drafted tokens over the paged MX4 cache, many query rows
+// of a cache head: both products on tcgen05 (mx4_attn.cuh has the kernel for few rows).
+//
+// A block takes two streams of 128 query rows each. Where a cache head has more than 128 rows
+// (nodes times query heads), the streams are two row tiles that share each tile of 128
+// tokens; otherwise they are the same rows over two halves of the block's tokens, joined at
+// the end. Warps 0 - 3 and 4 - 7 are the streams' softmax (a thread a row), 8 - 11 turn codes
+// into operands, 12 issues the MMAs.
+//
+//   S = Q K^T   queries rotated in fp32, then two f16 terms (22 bits) of the row times a power of two;
+//               a key's codes times 2^(E_b - E), E its largest scale exponent, are f16 values, and
+//               2^E goes to its column of S in fp32
+//   O = P V     values are bf16 exactly, whatever their scale; weights two bf16 terms (16 bits)
+//
+// S lies in tensor memory, the weights take its place (32 columns of S: 16 of the first terms, 16 of
+// the second), O beside it. The order of the MMAs is P_A V, Q_A K, P_B V, Q_B K, ..., so that
+// one stream's softmax runs under the other's products, and single buffers of K and V
+// (32 KB each at heads of 128) are refilled under the products that do not read them.
+// Codes come in by 16-byte asynchronous copies two tiles ahead.
+//
+// Weights are 2^(s - m - 24), m near the row's maximum: sums of up to 2^24 of them stay
+// below one, so that O does not leave fp32's range where the mean does not. m moves when a score
+// is 2^8 above it.
+#pragma once
+
+namespace convrot {
+
+constexpr int kTreeTile = 128;                 // tokens of a tile, rows of a stream
+constexpr int kTreeThreads = 13 * 32;
+constexpr int kTreeStages = 3;                 // tiles of codes on their way
+constexpr float kTreeDown = 24.0f;
+
+template <int D>
+struct Mx4TreeCfg {
+    static constexpr int kOperand = kTreeTile * D * 2;            // a term of a stream's queries, a tile of K or V
+    static constexpr int kAtom = kTreeTile * 128;                 // 128 rows of 64 16-bit columns, 128-byte swizzle
+    static constexpr int kVAtom = D * 128;                        // D rows (channels) of 64 tokens
+    static constexpr int kBlocks = D / 32;
+    static constexpr int kRaw = kTreeTile * D / 2;
+    static constexpr int kRawOffset = 6 * kOperand;               // four terms of queries, or two and the second K and V; K, V
+    static constexpr int kScaleOffset = kRawOffset + kTreeStages * kRaw;          // [stage][128] words of scale bytes
+    static constexpr int kPlaceOffset = kScaleOffset + kTreeStages * 512;         // [stage][128] places
+    static constexpr int kVfacOffset = kPlaceOffset + kTreeStages * 512;          // [2][block][128] bf16
+    static constexpr int kFacOffset = kVfacOffset + 2 * kBlocks * 256;            // [buffer][parity][128] fp32
+    static constexpr int kHidOffset = kFacOffset + 2048;                          // [buffer][parity][4] bits
+    static constexpr int kRowOffset = kHidOffset + 64;                            // [256] fp32: the rows' scales
+    static constexpr int kBarOffset = kRowOffset + 1024;
+    static constexpr int kBars = 2 * 4 + 2 * 2 + 2 * 3 + 2;
+    static constexpr int kEnd = kBarOffset + kBars * 8 + 16;
+    // (all of the tensor memory is taken: one block a multiprocessor, by shared memory too)
+    static constexpr int kSmemBytes = (kEnd > 116 * 1024 ? kEnd : 116 * 1024) + 1024;
+    static_assert(kSmemBytes <= 227 * 1024, "fits a multiprocessor");
+    static constexpr uint32_t kIdescS = idesc_f16(kTreeTile, kTreeTile), kIdescO = idesc_bf16(kTreeTile, D);
+};
+
+// D (+)= A B^T, kind::f16, A from tensor memory.
+__device__ __forceinline__ void mma_f16kind_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Eight codes as bf16, in pairs of neighbours: the two bytes of a value are looked up by its
+// three low bits, the sign byte comes from bit 3.
+__device__ __forceinline__ void codes_to_bf16(uint32_t x, uint32_t (&h)[4]) {
+    const uint32_t mag = x & 0x77777777u, low = x << 4;           // low: bit 3 of the even nibbles at their byte's end
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t sel = i ? mag >> 16 : mag;
+        const uint32_t lb = __byte_perm(0xC0800000u, 0xC0804000u, sel);           // 0, .5, 1, 1.5, 2, 3, 4, 6: low bytes
+        uint32_t hb = __byte_perm(0x3F3F3F00u, 0x40404040u, sel);                 // and high bytes
+        hb |= __byte_perm(low, x, i ? 0xFBEAu : 0xD9C8u) & 0x80808080u;
+        h[2 * i] = __byte_perm(lb, hb, 0x5140);
+        h[2 * i + 1] = __byte_perm(lb, hb, 0x7362);
+    }
+}
+
+// The tiles of a stream in the order in which the MMAs take them: for each i, the values of
+// tile i - 1, then the keys of tile i, stream after stream.
+struct TreeOrder {
+    int n0, n1, streams, i, s, value;
+    __device__ __forceinline__ TreeOrder(int a, int b, int of) : n0(a), n1(b), streams(of), i(0), s(0), value(1) { settle(); }
+    __device__ __forceinline__ bool done() const { return i > max(n0, n1); }
+    __device__ __forceinline__ int tile() const { return value ? i - 1 : i; }
+    __device__ __forceinline__ void step() {
+        if (value) { value = 0; return; }
+        value = 1;
+        if (++s == streams) { s = 0; ++i; }
+    }
+    __device__ __forceinline__ void settle() {
+        while (!done()) {
+            const int t = tile();
+            if (t >= 0 && t < (s ? n1 : n0)) return;
+            step();
+        }
+    }
+    __device__ __forceinline__ void next() { step(); settle(); }
+};
+
+// The rotation of 64 channels of a row without its factor (groups of 16 or 64), in the order of the
+// other kernels.
+__device__ __forceinline__ void tree_rotate(float (&v)[64], int group) {
+    constexpr int D = 64;
+    if (group >= 16) {
+        #pragma unroll
+        for (int i = 0; i < D; i += 4) h4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        #pragma unroll
+        for (int i = 0; i < D; i += 16)
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) h4(v[i + j], v[i + j + 4], v[i + j + 8], v[i + j + 12]);
+    }
+    if (group >= 64) {
+        #pragma unroll
+        for (int i = 0; i < D; i += 64)
+            #pragma unroll
+            for (int j = 0; j < 16; ++j) h4(v[i + j], v[i + j + 16], v[i + j + 32], v[i + j + 48]);
+    }
+}
+
+__device__ __forceinline__ float tree_factor(int group) { return group == 16 ? 0.25f : group == 64 ? 0.125f : 1.0f; }
+
+template <typename T, int D, bool PAIR>
+__global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a, int vec_q) {
+    using Cfg = Mx4TreeCfg<D>;
+    constexpr int kB = Cfg::kBlocks;
+    extern __shared__ __align__(1024) unsigned char tree_smem_raw[];
+    unsigned char* smem = tree_smem_raw + ((1024u - (smem_u32(tree_smem_raw) & 1023u)) & 1023u);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);
+    uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;       // [buffer]
+    uint64_t* f_full = bars + 8;                                  // [buffer][parity]: the columns' factors
+    uint64_t *s_full = bars + 12, *p_full = bars + 14, *o_done = bars + 16;                      // [stream]
+    uint64_t *q_full = bars + 18, *drain = bars + 19;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
+    int* nan_nodes = reinterpret_cast<int*>(tmem_slot + 1);       // a node's values hold a block of NaN
+    float* row_scale = reinterpret_cast<float*>(smem + Cfg::kRowOffset);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tile = blockIdx.x, split = blockIdx.y;
+    const int rt = tile % a.row_tiles, hk = tile / a.row_tiles % a.hkv, b = tile / a.row_tiles / a.hkv;
+    const int per_head = a.hq / a.hkv, rows_all = a.tq * per_head;
+    constexpr int kTileRows = PAIR ? 2 * kTreeTile : kTreeTile;
+    const int row0 = rt * kTileRows, rows = min(kTileRows, rows_all - row0);
+    griddep_wait();
+    griddep_launch_dependents();
+    const int n = max(0, static_cast<int>(min(static_cast<long long>(a.lens[b]), a.cap)));
+    const Mx4Tree tree(a, b, n);
+    const int per_split = mx4_split_groups(n, a.splits), groups = mx4_groups(n);
+    const int c0 = min(groups, split * per_split), count = min(groups, c0 + per_split) - c0;
+    if (a.splits > 1 && count == 0) return;                       // (the join knows how many splits hold tokens)
+    // tiles of each stream, and where the second starts
+    const int n0 = PAIR ? count : (count + 1) / 2, n1 = PAIR ? (rows > kTreeTile ? count : 0) : count - n0;
+    const int c1 = PAIR ? c0 : c0 + n0;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 128);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 128);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&f_full[2 * i], 128);
+            mbar_init(&f_full[2 * i + 1], 128);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_init(q_full, PAIR ? 256 : 128);
+        mbar_init(drain, 1);
+        *nan_nodes = 0;
+        fence_mbar_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto tmem_s = [&](int s) { return tmem + s * kTreeTile; };
+    auto tmem_o = [&](int s) { return tmem + 2 * kTreeTile + s * D; };
+    auto k_buf = [&](int i) { return smem + (PAIR || i == 0 ? 4 : 2) * Cfg::kOperand; };
+    auto v_buf = [&](int i) { return smem + (PAIR || i == 0 ? 5 : 3) * Cfg::kOperand; };
+    float* fac = reinterpret_cast<float*>(smem + Cfg::kFacOffset);
+    uint32_t* hid = reinterpret_cast<uint32_t*>(smem + Cfg::kHidOffset);
+
+    if (warp == 12) {
+        // ---------------- MMAs
+        const int streams = PAIR ? (n1 ? 2 : 1) : 2;
+        bool ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(q_full, 0));
+        for (int i = 0; ok && i <= n0; ++i) {
+            for (int s = 0; ok && s < streams; ++s) {
+                const int ns = s ? n1 : n0, buf = PAIR ? 0 : s;
+                const bool last = !PAIR || s == streams - 1;      // of those that read the buffers
+                if (i > 0 && i - 1 < ns) {
+                    const int t = i - 1;
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&v_full[buf], t & 1) && mbar_wait_bounded(&p_full[s], t & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t vd = smem_desc_kmajor(smem_u32(v_buf(buf)), 1024, 2);
+                    if (elect_one()) {
+                        #pragma unroll
+                        for (int j = 0; j < kTreeTile / 16; ++j)
+                            #pragma unroll
+                            for (int term = 0; term < 2; ++term)
+                                mma_f16kind_ts(tmem_o(s), tmem_s(s) + 32 * (j / 2) + 8 * (j % 2) + 16 * term,
+                                               vd + (j / 4) * (Cfg::kVAtom / 16) + 2 * (j % 4), Cfg::kIdescO, t > 0 || j > 0 || term > 0);
+                        if (last) mma_commit(&v_empty[buf]);
+                        if (t == ns - 1) mma_commit(&o_done[s]);
+                    }
+                    __syncwarp();
+                }
+                if (i < ns) {
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&k_full[buf], i & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t kd = smem_desc_kmajor(smem_u32(k_buf(buf)), 1024, 2);
+                    const uint64_t qd = smem_desc_kmajor(smem_u32(smem + (PAIR ? 2 * s : 0) * Cfg::kOperand), 1024, 2);
+                    if (elect_one()) {
+                        #pragma unroll
+                        for (int term = 0; term < 2; ++term)
+                            #pragma unroll
+                            for (int j = 0; j < D / 16; ++j) {
+                                const int at = (j / 4) * (Cfg::kAtom / 16) + 2 * (j % 4);
+                                mma_f16kind_ss(tmem_s(s), qd + term * (Cfg::kOperand / 16) + at, kd + at, Cfg::kIdescS, term > 0 || j > 0);
+                            }
+                        mma_commit(&s_full[s]);
+                        if (last) mma_commit(&k_empty[buf]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (!ok && lane == 0) tree_record_status(kMx4TimeoutMma);
+        if (elect_one()) mma_commit(drain);
+        __syncwarp();
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(drain, 0)) && lane == 0) tree_record_status(kMx4TimeoutMma);
+    } else if (warp >= 8) {
+        // ---------------- codes to operands: a thread a token, except for the values' transposition
+        const int t128 = tid - 256;
+        const int* table = a.table + b * a.table_ld;
+        const uint32_t v_off = static_cast<uint32_t>(a.hkv) << a.page_bits;
+        uint32_t* scale_words = reinterpret_cast<uint32_t*>(smem + Cfg::kScaleOffset);
+        uint32_t* places = reinterpret_cast<uint32_t*>(smem + Cfg::kPlaceOffset);
+        uint16_t* vfac = reinterpret_cast<uint16_t*>(smem + Cfg::kVfacOffset);
+        auto token_of = [&](const TreeOrder& o) { return ((o.s ? c1 : c0) + o.tile()) * kTreeTile + t128; };
+        auto page_of = [&](const TreeOrder& o) -> int {
+            if (o.done()) return -1;
+            const int j = token_of(o);
+            return j < n ? __ldg(table + (j >> a.page_bits)) : -1;
+        };
+        // a token's 16-byte chunk c lies where neither reader meets a bank conflict
+        auto raw_at = [&](int value, int t, int c) {
+            const int unit = t * kB + c;
+            return (value ? unit ^ ((t >> 3) & 7) : kB == 4 ? unit ^ ((t >> 1) & 3) : unit ^ ((t >> 2) & 1)) * 16;
+        };
+        auto issue = [&](const TreeOrder& o, int page, int stage) {
+            const bool held = page >= 0 && page < a.pages;
+            const uint32_t off = static_cast<uint32_t>(token_of(o)) & ((1u << a.page_bits) - 1);
+            const uint32_t place = held ? (((static_cast<uint32_t>(page) * 2) * a.hkv + hk) << a.page_bits) + off + (o.value ? v_off : 0u) : 0xFFFFFFFFu;
+            unsigned char* raw = smem + Cfg::kRawOffset + stage * Cfg::kRaw;
+            #pragma unroll
+            for (int i = 0; i < kB; ++i) {
+                const int tok = (i * 32 + lane) / kB, c = (i * 32 + lane) % kB;
+                const uint32_t p = __shfl_sync(0xFFFFFFFFu, place, tok);
+                const bool h = p != 0xFFFFFFFFu;
+                cp_async16(raw + raw_at(o.value, (warp - 8) * 32 + tok, c), a.codes + (h ? static_cast<size_t>(p) * (D / 2) + c * 16 : 0), h);
+            }
+            // (heads of 64 have two scale bytes: the aligned word that holds them)
+            const size_t sp = held ? (D == 64 ? static_cast<size_t>(place & ~1u) * 2 : static_cast<size_t>(place) * kB) : 0;
+            cp_async_small<4>(scale_words + stage * 128 + t128, a.scales + sp, held);
+            places[stage * 128 + t128] = place;
+        };
+        TreeOrder ahead(n0, n1, PAIR ? 1 : 2), at(n0, n1, PAIR ? 1 : 2);
+        int page = page_of(ahead);
+        #pragma unroll
+        for (int i = 0; i < kTreeStages - 1; ++i) {
+            if (!ahead.done()) {
+                issue(ahead, page, i);
+                ahead.next();
+                page = page_of(ahead);
+            }
+            cp_async_commit();
+        }
+        bool ok = true;
+        for (int u = 0; !at.done(); ++u, at.next()) {
+            const int stage = u % kTreeStages, buf = at.s, i = at.tile();
+            cp_async_wait<kTreeStages - 2>();
+            const uint32_t place = places[stage * 128 + t128];
+            uint32_t word = scale_words[stage * 128 + t128];
+            if constexpr (D == 64) word = place == 0xFFFFFFFFu ? 0u : word >> (16 * (place & 1));
+            const int j = token_of(at);
+            if (at.value) {
+                #pragma unroll
+                for (int k = 0; k < kB; ++k) {
+                    const uint32_t e = (word >> (8 * k)) & 255u;
+                    uint32_t f = e == 0u ? 0x0040u : e << 7;
+                    if (e == 255u) {
+                        // NaN: straight to the weighted sums where every row sees the token, at the end to
+                        // those rows that do where it is a node (a product with the weight 0 would give it to all)
+                        f = j < tree.context ? 0x7FC0u : 0u;
+                        if (j >= tree.context) *nan_nodes = 1;
+                    }
+                    vfac[((u & 1) * kB + k) * 128 + t128] = static_cast<uint16_t>(f);
+                }
+            } else {
+                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, place == 0xFFFFFFFFu);
+                if (lane == 0) hid[(buf * 2 + (i & 1)) * 4 + warp - 8] = gone;
+            }
+            named_barrier_sync(1, 128);                           // every warp's codes are there
+            // the next tile but one takes the stage that was read before the barrier
+            if (!ahead.done()) {
+                issue(ahead, page, (u + kTreeStages - 1) % kTreeStages);
+                ahead.next();
+                page = page_of(ahead);
+            }
+            cp_async_commit();
+            const unsigned char* raw = smem + Cfg::kRawOffset + stage * Cfg::kRaw;
+            if (at.value) {
+                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&v_empty[buf], (i & 1) ^ 1));
+                if (!ok) continue;                                // (the barriers go on: no warp waits for one that left)
+                // groups of 8 tokens by 8 channels: word w of the tokens' codes
+                constexpr int kItems = kTreeTile / 8 * (D / 8) / 128;
+                #pragma unroll
+                for (int k = 0; k < kItems; ++k) {
+                    const int g = t128 & 7, w = (t128 >> 3) % (D / 8), half = D == 128 ? k : t128 >> 6;
+                    uint32_t words[8];
+                    #pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        words[e] = *reinterpret_cast<const uint32_t*>(raw + raw_at(1, 64 * half + 8 * g + e, w >> 2) + (w & 3) * 4);
+                    const uint4 f4 = *reinterpret_cast<const uint4*>(vfac + ((u & 1) * kB + (w >> 2)) * 128 + 64 * half + 8 * g);
+                    const uint32_t f[4] = {f4.x, f4.y, f4.z, f4.w};
+                    uint32_t out[8][4];                           // [channel][pair of tokens]
+                    #pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        const uint32_t x = words[2 * p], y = words[2 * p + 1];
+                        uint32_t even[4], odd[4];
+                        codes_to_bf16((x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u), even);
+                        codes_to_bf16(((x >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u), odd);
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            out[2 * c][p] = mul_bf16x2(even[c], f[p]);
+                            out[2 * c + 1][p] = mul_bf16x2(odd[c], f[p]);
+                        }
+                    }
+                    unsigned char* to = v_buf(buf) + half * Cfg::kVAtom + w * 1024;
+                    #pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        *reinterpret_cast<uint4*>(to + c * 128 + ((g ^ c) << 4)) = make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&v_full[buf]);
+            } else {
+                uint32_t top = 0, f[kB];
+                #pragma unroll
+                for (int k = 0; k < kB; ++k) {
+                    const uint32_t e = (word >> (8 * k)) & 255u;
+                    if (e != 255u) top = max(top, e);
+                }
+                #pragma unroll
+                for (int k = 0; k < kB; ++k) {
+                    const int e = static_cast<int>((word >> (8 * k)) & 255u);
+                    const float x = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(max(e - static_cast<int>(top) + 127, 0)) << 23);
+                    f[k] = f16x2_bits(x, x);
+                }
+                fac[(buf * 2 + (i & 1)) * 128 + t128] = __uint_as_float(max(top << 23, 0x00400000u));
+                mbar_arrive(&f_full[buf * 2 + (i & 1)]);
+                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&k_empty[buf], (i & 1) ^ 1));
+                if (!ok) continue;
+                #pragma unroll
+                for (int k = 0; k < kB; ++k) {
+                    const uint4 codes = *reinterpret_cast<const uint4*>(raw + raw_at(0, t128, k));
+                    const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+                    unsigned char* to = k_buf(buf) + (k / 2) * Cfg::kAtom + t128 * 128;
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t h[4];
+                        codes_to_f16(words[c], h);
+                        *reinterpret_cast<uint4*>(to + ((((k & 1) * 4 + c) ^ (t128 & 7)) << 4)) =
+                            make_uint4(hmul2_bits(h[0], f[k]), hmul2_bits(h[1], f[k]), hmul2_bits(h[2], f[k]), hmul2_bits(h[3], f[k]));
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&k_full[buf]);
+            }
+        }
+        if (!ok && lane == 0) tree_record_status(kMx4TimeoutProducer);
+        cp_async_wait<0>();
+    } else {
+        // ---------------- a stream's softmax, a thread a row
+        const int s = warp >> 2, r = tid & 127;
+        const int row = row0 + (PAIR ? s * kTreeTile : 0) + r, t = row / per_head;
+        const bool real = row < rows_all && (PAIR || r < rows);
+        if (PAIR || s == 0) {
+            const T* q = static_cast<const T*>(a.q) + b * a.qsb + t * a.qst + (hk * per_head + row % per_head) * a.qsh;
+            // 64 channels at a time, rotated (twice: for the largest value, then as operands; a whole
+            // row of 128 does not fit the registers)
+            auto channels = [&](int from, float (&v)[64]) {
+                if (!real) {
+                    #pragma unroll
+                    for (int i = 0; i < 64; ++i) v[i] = 0.0f;
+                } else if (vec_q) {
+                    #pragma unroll
+                    for (int i = 0; i < 64; i += 8) {
+                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(q + from + i));
+                        T e[8];
+                        memcpy(e, &x, 16);
+                        #pragma unroll
+                        for (int k = 0; k < 8; ++k) v[i + k] = mx4_to_f32(e[k]);
+                    }
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < 64; ++i) v[i] = mx4_to_f32(q[from + i]);
+                }
+                tree_rotate(v, a.group);
+            };
+            float top = 0.0f;
+            #pragma unroll 1
+            for (int from = 0; from < D; from += 64) {
+                float v[64];
+                channels(from, v);
+                #pragma unroll
+                for (int i = 0; i < 64; ++i) top = fmaxf(top, fabsf(v[i]));
+            }
+            // 2^(8 - exponent of the row's largest value), within fp32's normal range
+            const int e = static_cast<int>(__float_as_uint(top) >> 23);
+            const int up = top > 0.0f ? min(max(135 - e, -120), 120) : 0;
+            // (the scale's sign goes to the queries, and 0 to the smallest number: a hidden score stays -inf)
+            const float to_f16 = copysignf(__uint_as_float(static_cast<uint32_t>(127 + up) << 23), a.scale);
+            row_scale[s * 128 + r] = fmaxf(fabsf(a.scale) * tree_factor(a.group) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
+            #pragma unroll 1
+            for (int from = 0; from < D; from += 64) {
+                float v[64];
+                channels(from, v);
+                unsigned char* base = smem + (PAIR ? 2 * s : 0) * Cfg::kOperand + from / 64 * Cfg::kAtom + r * 128;
+                #pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t hi[4], lo[4];
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float x = v[8 * c + 2 * k] * to_f16, y = v[8 * c + 2 * k + 1] * to_f16;
+                        hi[k] = f16x2_bits(x, y);
+                        __half2 h;
+                        memcpy(&h, &hi[k], 4);
+                        const float2 back = __half22float2(h);
+                        lo[k] = f16x2_bits(x - back.x, y - back.y);
+                    }
+                    unsigned char* to = base + ((c ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(to + Cfg::kOperand) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(q_full);
+        }
+        const int ns = s ? n1 : n0, first = s ? c1 : c0, buf = PAIR ? 0 : s;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem_s(s) + lanes, to = tmem_o(s) + lanes;
+        float m = kMx4NoScore, l = 0.0f, rs = 0.0f;
+        bool ok = true;
+        if (!PAIR && ns) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(q_full, 0));      // (both streams' rows are scaled by one of them)
+        if (ns) rs = row_scale[(PAIR ? s * 128 : 0) + r];
+        const bool node = real && t < tree.nodes;                 // (what other rows compute is not kept)
+        for (int i = 0; ok && i < ns; ++i) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&s_full[s], i & 1) && mbar_wait_bounded(&f_full[buf * 2 + (i & 1)], (i >> 1) & 1));
+            if (!ok) break;
+            tc_fence_after();
+            const float* f = fac + (buf * 2 + (i & 1)) * 128;
+            const uint32_t* gone = hid + (buf * 2 + (i & 1)) * 4;
+            const int j0 = (first + i) * kTreeTile;
+            const bool hides = !__all_sync(0xFFFFFFFFu, !node || (j0 + kTreeTile <= tree.context && (gone[0] | gone[1] | gone[2] | gone[3]) == 0));
+            uint32_t seen[4];                                     // columns that this row sees
+            if (hides) {
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int from = j0 + 32 * c, known = min(max(tree.context - from, 0), 32);
+                    uint32_t bits = known == 32 ? 0xFFFFFFFFu : (1u << known) - 1u;
+                    const int end = min(32, n - from);
+                    if (node)
+                        for (int k = known; k < end; ++k)
+                            if (tree.sees(t, from + k)) bits |= 1u << k;
+                    seen[c] = bits & ~gone[c];
+                }
+            }
+            // x: scores without the row's scale
+            float2 x[16];
+            auto scores = [&](int c, bool masked) {
+                uint32_t sr[32];
+                tmem_ld_32x32b_x32(ts + 32 * c, sr);
+                tmem_ld_wait_regs(sr);
+                #pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float4 f4 = *reinterpret_cast<const float4*>(f + 32 * c + 4 * k);
+                    x[2 * k] = fmul2_rn(make_float2(__uint_as_float(sr[4 * k]), __uint_as_float(sr[4 * k + 1])), make_float2(f4.x, f4.y));
+                    x[2 * k + 1] = fmul2_rn(make_float2(__uint_as_float(sr[4 * k + 2]), __uint_as_float(sr[4 * k + 3])), make_float2(f4.z, f4.w));
+                }
+                if (masked) {
+                    #pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        if (!(seen[c] >> (2 * k) & 1u)) x[k].x = -INFINITY;
+                        if (!(seen[c] >> (2 * k + 1) & 1u)) x[k].y = -INFINITY;
+                    }
+                }
+            };
+            float top = -INFINITY;
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                scores(c, hides);
+                #pragma unroll
+                for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(x[k].x, x[k].y));
+            }
+            top *= rs;
+            if (__any_sync(0xFFFFFFFFu, top > m + 8.0f)) {
+                const float was = m;
+                m = fmaxf(m, top);
+                const float down = ex2(was - m);
+                l *= down;
+                if (i > 0) {
+                    #pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(to + 32 * c, o);
+                        tmem_ld_wait_regs(o);
+                        #pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+                        tmem_st_32x32b_x32(to + 32 * c, o);
+                    }
+                }
+            }
+            const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), rs2 = make_float2(rs, rs);
+            float2 sum = make_float2(0.0f, 0.0f);
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                scores(c, hides);
+                uint32_t p[32];
+                #pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const float2 y = ffma2_rn(x[k], rs2, less);
+                    const float2 w = make_float2(ex2(y.x), ex2(y.y));
+                    sum = fadd2_rn(sum, w);
+                    const uint32_t hi = bf16x2_bits(w.x, w.y);
+                    p[k] = hi;
+                    p[16 + k] = bf16x2_bits(w.x - __uint_as_float(hi << 16), w.y - __uint_as_float(hi & 0xFFFF0000u));
+                }
+                tmem_st_32x32b_x32(ts + 32 * c, p);
+            }
+            l += sum.x + sum.y;
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&p_full[s]);
+        }
+        // ---------------- the row's mean
+        if (ok && ns) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&o_done[s], 0));
+        if (!ok && lane == 0) tree_record_status(kMx4TimeoutEpilogue);
+        tc_fence_after();
+        const bool none = !ok || !node || (m == kMx4NoScore && l == 0.0f);        // (scores that are all NaN move no reference)
+        if (none) { m = -INFINITY; l = 0.0f; }
+        float* part = reinterpret_cast<float*>(smem);             // the operands' place, which nothing reads any more
+        constexpr int kLd = 64 + 4;                               // floats of a row: rows in distinct banks
+        float2* ml = reinterpret_cast<float2*>(smem + 128 * kLd * 4);
+        static_assert(128 * (kLd * 4 + 8) <= 4 * Cfg::kOperand, "fits the first operands");
+        float2 other = make_float2(-INFINITY, 0.0f);              // of the same rows in the second stream
+        float mine_share = 1.0f, other_share = 0.0f;
+        if constexpr (!PAIR) {
+            named_barrier_sync(2, 256);                           // both streams' products are done
+            if (s == 1) ml[r] = make_float2(m, l);
+            named_barrier_sync(2, 256);
+            other = ml[r];
+        }
+        const float own_m = m, own_l = l;
+        if (!PAIR && s == 0) {
+            m = fmaxf(own_m, other.x);
+            const float w0 = own_m == -INFINITY ? 0.0f : ex2(own_m - m) * own_l, w1 = other.x == -INFINITY ? 0.0f : ex2(other.x - m) * other.y;
+            l = w0 + w1;
+            mine_share = w0 == 0.0f ? 0.0f : w0 / l;
+            other_share = w1 == 0.0f ? 0.0f : w1 / l;
+        }
+        #pragma unroll 1
+        for (int from = 0; from < D; from += 64) {
+            float v[64];
+            #pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t o[32];
+                if (ns) {                                         // (of the whole warp)
+                    tmem_ld_32x32b_x32(to + from + 32 * c, o);
+                    tmem_ld_wait_regs(o);
+                }
+                const float inv = none ? 0.0f : 1.0f / own_l;
+                #pragma unroll
+                for (int k = 0; k < 32; ++k) v[32 * c + k] = none ? 0.0f : __uint_as_float(o[k]) * inv;
+            }
+            if constexpr (!PAIR) {
+                named_barrier_sync(2, 256);
+                if (s == 1) {
+                    #pragma unroll
+                    for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4*>(part + r * kLd + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+                named_barrier_sync(2, 256);
+                if (s == 0) {
+                    #pragma unroll
+                    for (int i = 0; i < 64; i += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(part + r * kLd + i);
+                        v[i] = mine_share * v[i] + other_share * x.x;
+                        v[i + 1] = mine_share * v[i + 1] + other_share * x.y;
+                        v[i + 2] = mine_share * v[i + 2] + other_share * x.z;
+                        v[i + 3] = mine_share * v[i + 3] + other_share * x.w;
+                    }
+                }
+            }
+            if (!real || (!PAIR && s == 1)) continue;
+            if (*nan_nodes && node) {
+                for (int j = max(tree.context, c0 * kTreeTile); j < min(n, (c0 + count) * kTreeTile); ++j) {
+                    const int page = a.table[b * a.table_ld + (j >> a.page_bits)];
+                    if (page < 0 || page >= a.pages || !tree.sees(t, j)) continue;
+                    const size_t place = (((static_cast<size_t>(page) * 2 + 1) * a.hkv + hk) << a.page_bits) + (j & ((1 << a.page_bits) - 1));
+                    #pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (a.scales[place * kB + from / 32 + k] == 255) {
+                            #pragma unroll
+                            for (int i = 0; i < 32; ++i) v[32 * k + i] = NAN;
+                        }
+                }
+            }
+            if (a.splits > 1) {
+                const size_t at = (static_cast<size_t>(tile) * a.splits + split) * kTileRows + (row - row0);
+                #pragma unroll
+                for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4*>(a.part + at * D + from + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                if (from == 0) a.part_ml[at] = make_float2(m, l);
+            } else {
+                tree_rotate(v, a.group);
+                const float f = tree_factor(a.group);
+                T* out = static_cast<T*>(a.out) + ((static_cast<size_t>(b) * a.tq + t) * a.hq + hk * per_head + row % per_head) * D + from;
+                #pragma unroll
+                for (int i = 0; i < 64; i += 8) {
+                    T e[8];
+                    #pragma unroll
+                    for (int k = 0; k < 8; ++k) e[k] = mx4_from_f32<T>(v[i + k] * f);
+                    uint4 x;
+                    memcpy(&x, e, 16);
+                    *reinterpret_cast<uint4*>(out + i) = x;
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace convrot
