@@ -42,8 +42,9 @@ struct Mx4TreeCfg {
     static constexpr int kPlaceOffset = kScaleOffset + kTreeStages * 512;         // [stage][128] places
     static constexpr int kVfacOffset = kPlaceOffset + kTreeStages * 512;          // [2][block][128] bf16
     static constexpr int kFacOffset = kVfacOffset + 2 * kBlocks * 256;            // [buffer][parity][128] fp32
-    static constexpr int kHidOffset = kFacOffset + 2048;                          // [buffer][parity][4] bits
-    static constexpr int kRowOffset = kHidOffset + 64;                            // [256] fp32: the rows' scales
+    static constexpr int kHidOffset = kFacOffset + 2048;                          // [buffer][parity][8]: hidden tokens' bits, far apart
+    static constexpr int kRangeOffset = kHidOffset + 128;                         // [2][4] largest and least exponents of a tile's keys
+    static constexpr int kRowOffset = kRangeOffset + 64;                            // [256] fp32: the rows' scales
     static constexpr int kBarOffset = kRowOffset + 1024;
     static constexpr int kBars = 2 * 4 + 2 * 2 + 2 * 3 + 2;
     static constexpr int kEnd = kBarOffset + kBars * 8 + 16;
@@ -72,6 +73,14 @@ __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+
+// Two weights as the sum of two bf16 terms each: the upper halves as they are, and what they leave out.
+__device__ __forceinline__ void split_bf16(float2 w, uint32_t& hi, uint32_t& lo) {
+    const uint32_t x = __float_as_uint(w.x), y = __float_as_uint(w.y);
+    hi = __byte_perm(x, y, 0x7632);
+    const float2 left = ffma2_rn(make_float2(__uint_as_float(x & 0xFFFF0000u), __uint_as_float(y & 0xFFFF0000u)), make_float2(-1.0f, -1.0f), w);
+    lo = bf16x2_bits(left.x, left.y);
 }
 
 // Eight codes as bf16, in pairs of neighbours: the two bytes of a value are looked up by its
@@ -254,6 +263,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
         const uint32_t v_off = static_cast<uint32_t>(a.hkv) << a.page_bits;
         uint32_t* scale_words = reinterpret_cast<uint32_t*>(smem + Cfg::kScaleOffset);
         uint32_t* places = reinterpret_cast<uint32_t*>(smem + Cfg::kPlaceOffset);
+        short2* range = reinterpret_cast<short2*>(smem + Cfg::kRangeOffset);
         uint16_t* vfac = reinterpret_cast<uint16_t*>(smem + Cfg::kVfacOffset);
         auto token_of = [&](const TreeOrder& o) { return ((o.s ? c1 : c0) + o.tile()) * kTreeTile + t128; };
         auto page_of = [&](const TreeOrder& o) -> int {
@@ -302,6 +312,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             uint32_t word = scale_words[stage * 128 + t128];
             if constexpr (D == 64) word = place == 0xFFFFFFFFu ? 0u : word >> (16 * (place & 1));
             const int j = token_of(at);
+            int top = 0, low = 255;                               // of the token's scale exponents
             if (at.value) {
                 #pragma unroll
                 for (int k = 0; k < kB; ++k) {
@@ -317,7 +328,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 }
             } else {
                 const uint32_t gone = __ballot_sync(0xFFFFFFFFu, place == 0xFFFFFFFFu);
-                if (lane == 0) hid[(buf * 2 + (i & 1)) * 4 + warp - 8] = gone;
+                low = 255;
+                #pragma unroll
+                for (int k = 0; k < kB; ++k) {
+                    const int e = static_cast<int>((word >> (8 * k)) & 255u);
+                    if (e != 255) top = max(top, e);
+                    if (e != 255 && e != 0) low = min(low, e);    // (0: blocks of zeros, or the least there is)
+                }
+                const int most = __reduce_max_sync(0xFFFFFFFFu, top), least = __reduce_min_sync(0xFFFFFFFFu, low);
+                if (lane == 0) {
+                    hid[(buf * 2 + (i & 1)) * 8 + warp - 8] = gone;
+                    range[(u & 1) * 4 + warp - 8] = make_short2(static_cast<short>(most), static_cast<short>(least));
+                }
             }
             named_barrier_sync(1, 128);                           // every warp's codes are there
             // the next tile but one takes the stage that was read before the barrier
@@ -363,19 +385,26 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 fence_proxy_async_smem();
                 mbar_arrive(&v_full[buf]);
             } else {
-                uint32_t top = 0, f[kB];
+                // A code times 2^-23 is an f16 value exactly: where the tile's exponents lie no further apart
+                // one factor serves all columns.
+                uint32_t f[kB];
+                int most = 0, least = 255;
                 #pragma unroll
-                for (int k = 0; k < kB; ++k) {
-                    const uint32_t e = (word >> (8 * k)) & 255u;
-                    if (e != 255u) top = max(top, e);
+                for (int k = 0; k < 4; ++k) {
+                    const short2 x = range[(u & 1) * 4 + k];
+                    most = max(most, static_cast<int>(x.x));
+                    least = min(least, static_cast<int>(x.y));
                 }
+                const bool apart = most - least > 23;
+                if (!apart) top = most;
                 #pragma unroll
                 for (int k = 0; k < kB; ++k) {
                     const int e = static_cast<int>((word >> (8 * k)) & 255u);
-                    const float x = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(max(e - static_cast<int>(top) + 127, 0)) << 23);
+                    const float x = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(max(e - top + 127, 0)) << 23);
                     f[k] = f16x2_bits(x, x);
                 }
-                fac[(buf * 2 + (i & 1)) * 128 + t128] = __uint_as_float(max(top << 23, 0x00400000u));
+                fac[(buf * 2 + (i & 1)) * 128 + t128] = __uint_as_float(max(static_cast<uint32_t>(top) << 23, 0x00400000u));
+                if (t128 == 0) hid[(buf * 2 + (i & 1)) * 8 + 4] = apart;
                 mbar_arrive(&f_full[buf * 2 + (i & 1)]);
                 ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&k_empty[buf], (i & 1) ^ 1));
                 if (!ok) continue;
@@ -478,7 +507,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             if (!ok) break;
             tc_fence_after();
             const float* f = fac + (buf * 2 + (i & 1)) * 128;
-            const uint32_t* gone = hid + (buf * 2 + (i & 1)) * 4;
+            const uint32_t* gone = hid + (buf * 2 + (i & 1)) * 8;
             const int j0 = (first + i) * kTreeTile;
             const bool hides = !__all_sync(0xFFFFFFFFu, !node || (j0 + kTreeTile <= tree.context && (gone[0] | gone[1] | gone[2] | gone[3]) == 0));
             uint32_t seen[4];                                     // columns that this row sees
@@ -494,67 +523,97 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                     seen[c] = bits & ~gone[c];
                 }
             }
-            // x: scores without the row's scale
-            float2 x[16];
-            auto scores = [&](int c, bool masked) {
-                uint32_t sr[32];
-                tmem_ld_32x32b_x32(ts + 32 * c, sr);
-                tmem_ld_wait_regs(sr);
+            // Scores x and the factor sc to m's scale: what the products gave and the tile's own factor, or
+            // with columns that are hidden or keys far apart, column by column.
+            const bool slow = hides || gone[4] != 0u;
+            const float sc = slow ? rs : rs * f[0];
+            auto columns = [&](int c, uint32_t (&sr)[32]) {
+                if (!slow) return;
+                const uint32_t bits = hides ? seen[c] : 0xFFFFFFFFu;
                 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float4 f4 = *reinterpret_cast<const float4*>(f + 32 * c + 4 * k);
-                    x[2 * k] = fmul2_rn(make_float2(__uint_as_float(sr[4 * k]), __uint_as_float(sr[4 * k + 1])), make_float2(f4.x, f4.y));
-                    x[2 * k + 1] = fmul2_rn(make_float2(__uint_as_float(sr[4 * k + 2]), __uint_as_float(sr[4 * k + 3])), make_float2(f4.z, f4.w));
-                }
-                if (masked) {
-                    #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        if (!(seen[c] >> (2 * k) & 1u)) x[k].x = -INFINITY;
-                        if (!(seen[c] >> (2 * k + 1) & 1u)) x[k].y = -INFINITY;
-                    }
+                for (int k = 0; k < 32; ++k) {
+                    const float x = __uint_as_float(sr[k]) * f[32 * c + k];
+                    sr[k] = bits >> k & 1u ? __float_as_uint(x) : 0xFF800000u;
                 }
             };
-            float top = -INFINITY;
-            #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                scores(c, hides);
-                #pragma unroll
-                for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(x[k].x, x[k].y));
-            }
-            top *= rs;
-            if (__any_sync(0xFFFFFFFFu, top > m + 8.0f)) {
+            // The reference is one of earlier tiles as long as the weights stay below 2^-14 (their sum tells);
+            // where they do not, it moves to the largest of the scores from chunk `from` on, and what was
+            // summed and laid down gets the new scale.
+            float2 sum = make_float2(0.0f, 0.0f);
+            auto move = [&](int from) {
+                float top = -INFINITY;
+                #pragma unroll 1
+                for (int c = from; c < 4; ++c) {
+                    uint32_t sr[32];
+                    tmem_ld_32x32b_x32(ts + 32 * c, sr);
+                    tmem_ld_wait_regs(sr);
+                    columns(c, sr);
+                    #pragma unroll
+                    for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(sr[k]));
+                }
                 const float was = m;
-                m = fmaxf(m, top);
+                m = fmaxf(m, top * sc);
                 const float down = ex2(was - m);
                 l *= down;
-                if (i > 0) {
-                    #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32x32b_x32(to + 32 * c, o);
-                        tmem_ld_wait_regs(o);
-                        #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
-                        tmem_st_32x32b_x32(to + 32 * c, o);
-                    }
+                sum = fmul2_rn(sum, make_float2(down, down));
+                #pragma unroll 1
+                for (int c = 0; i > 0 && c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld_32x32b_x32(to + 32 * c, o);
+                    tmem_ld_wait_regs(o);
+                    #pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+                    tmem_st_32x32b_x32(to + 32 * c, o);
                 }
-            }
-            const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), rs2 = make_float2(rs, rs);
-            float2 sum = make_float2(0.0f, 0.0f);
-            #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                scores(c, hides);
-                uint32_t p[32];
+                #pragma unroll 1
+                for (int c = 0; c < from; ++c) {
+                    uint32_t w[32];
+                    tmem_ld_32x32b_x32(ts + 32 * c, w);
+                    tmem_ld_wait_regs(w);
+                    #pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float x = (__uint_as_float(w[k] << 16) + __uint_as_float(w[16 + k] << 16)) * down;
+                        const float y = (__uint_as_float(w[k] & 0xFFFF0000u) + __uint_as_float(w[16 + k] & 0xFFFF0000u)) * down;
+                        split_bf16(make_float2(x, y), w[k], w[16 + k]);
+                    }
+                    tmem_st_32x32b_x32(ts + 32 * c, w);
+                }
+            };
+            // a chunk's weights, in place; their sum
+            auto weights = [&](uint32_t (&sr)[32]) {
+                const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), by = make_float2(sc, sc);
+                float2 part[2] = {};
+                uint32_t lo[16];
                 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const float2 y = ffma2_rn(x[k], rs2, less);
+                    const float2 y = ffma2_rn(make_float2(__uint_as_float(sr[2 * k]), __uint_as_float(sr[2 * k + 1])), by, less);
                     const float2 w = make_float2(ex2(y.x), ex2(y.y));
-                    sum = fadd2_rn(sum, w);
-                    const uint32_t hi = bf16x2_bits(w.x, w.y);
-                    p[k] = hi;
-                    p[16 + k] = bf16x2_bits(w.x - __uint_as_float(hi << 16), w.y - __uint_as_float(hi & 0xFFFF0000u));
+                    part[k & 1] = fadd2_rn(part[k & 1], w);
+                    split_bf16(w, sr[k], lo[k]);
                 }
-                tmem_st_32x32b_x32(ts + 32 * c, p);
+                #pragma unroll
+                for (int k = 0; k < 16; ++k) sr[16 + k] = lo[k];
+                return fadd2_rn(part[0], part[1]);
+            };
+            uint32_t sr[2][32];
+            tmem_ld_32x32b_x32(ts, sr[0]);
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t (&cur)[32] = sr[c & 1];
+                tmem_ld_wait_regs(cur);
+                if (c < 3) tmem_ld_32x32b_x32(ts + 32 * (c + 1), sr[(c + 1) & 1]);
+                columns(c, cur);
+                float2 here = weights(cur);
+                if (__any_sync(0xFFFFFFFFu, here.x + here.y > 6.1035156e-5f)) {
+                    tmem_ld_wait();
+                    move(c);
+                    tmem_ld_32x32b_x32(ts + 32 * c, cur);
+                    tmem_ld_wait_regs(cur);
+                    columns(c, cur);
+                    here = weights(cur);
+                }
+                sum = fadd2_rn(sum, here);
+                tmem_st_32x32b_x32(ts + 32 * c, cur);
             }
             l += sum.x + sum.y;
             tmem_st_wait();
