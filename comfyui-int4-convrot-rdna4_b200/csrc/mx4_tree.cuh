@@ -4,8 +4,8 @@
 // A block takes two streams of 128 query rows each. Where a cache head has more than 128 rows
 // (nodes times query heads), the streams are two row tiles that share each tile of 128
 // tokens; otherwise they are the same rows over two halves of the block's tokens, joined at
-// the end. Warps 0 - 3 and 4 - 7 are the streams' softmax (a thread a row), 8 - 11 turn codes
-// into operands, 12 issues the MMAs.
+// the end. Warps 0 - 3 and 4 - 7 are the streams' softmax (a thread a row), 8 - 11 turn the
+// values' codes into operands, 12 and 13 the keys', 14 issues the MMAs.
 //
 //   S = Q K^T   queries rotated in fp32, then two f16 terms (22 bits) of the row times a power of two;
 //               a key's codes times 2^(E_b - E), E its largest scale exponent, are f16 values, and
@@ -16,7 +16,6 @@
 // the second), O beside it. The order of the MMAs is P_A V, Q_A K, P_B V, Q_B K, ..., so that
 // one stream's softmax runs under the other's products, and single buffers of K and V
 // (32 KB each at heads of 128) are refilled under the products that do not read them.
-// Codes come in by 16-byte asynchronous copies two tiles ahead.
 //
 // Weights are 2^(s - m - 24), m near the row's maximum: sums of up to 2^24 of them stay
 // below one, so that O does not leave fp32's range where the mean does not. m moves when a score
@@ -26,8 +25,7 @@
 namespace convrot {
 
 constexpr int kTreeTile = 128;                 // tokens of a tile, rows of a stream
-constexpr int kTreeThreads = 13 * 32;
-constexpr int kTreeStages = 3;                 // tiles of codes on their way
+constexpr int kTreeThreads = 15 * 32;
 constexpr float kTreeDown = 24.0f;
 
 template <int D>
@@ -36,15 +34,11 @@ struct Mx4TreeCfg {
     static constexpr int kAtom = kTreeTile * 128;                 // 128 rows of 64 16-bit columns, 128-byte swizzle
     static constexpr int kVAtom = D * 128;                        // D rows (channels) of 64 tokens
     static constexpr int kBlocks = D / 32;
-    static constexpr int kRaw = kTreeTile * D / 2;
-    static constexpr int kRawOffset = 6 * kOperand;               // four terms of queries, or two and the second K and V; K, V
-    static constexpr int kScaleOffset = kRawOffset + kTreeStages * kRaw;          // [stage][128] words of scale bytes
-    static constexpr int kPlaceOffset = kScaleOffset + kTreeStages * 512;         // [stage][128] places
-    static constexpr int kVfacOffset = kPlaceOffset + kTreeStages * 512;          // [2][block][128] bf16
-    static constexpr int kFacOffset = kVfacOffset + 2 * kBlocks * 256;            // [buffer][parity][128] fp32
-    static constexpr int kHidOffset = kFacOffset + 2048;                          // [buffer][parity][8]: hidden tokens' bits, far apart
-    static constexpr int kRangeOffset = kHidOffset + 128;                         // [2][4] largest and least exponents of a tile's keys
-    static constexpr int kRowOffset = kRangeOffset + 64;                            // [256] fp32: the rows' scales
+    static constexpr int kFacOffset = 6 * kOperand;               // (four terms of queries, or two and the second K and V; K, V)
+                                                                  // [buffer][parity][128] fp32: factors of a tile's keys
+    static constexpr int kHidOffset = kFacOffset + 2048;          // [buffer][parity][8]: hidden tokens' bits, keys far apart
+    static constexpr int kRangeOffset = kHidOffset + 128;         // [2][2] largest and least exponents of a tile's keys
+    static constexpr int kRowOffset = kRangeOffset + 32;                            // [256] fp32: the rows' scales
     static constexpr int kBarOffset = kRowOffset + 1024;
     static constexpr int kBars = 2 * 4 + 2 * 2 + 2 * 3 + 2;
     static constexpr int kEnd = kBarOffset + kBars * 8 + 16;
@@ -97,28 +91,6 @@ __device__ __forceinline__ void codes_to_bf16(uint32_t x, uint32_t (&h)[4]) {
         h[2 * i + 1] = __byte_perm(lb, hb, 0x7362);
     }
 }
-
-// The tiles of a stream in the order in which the MMAs take them: for each i, the values of
-// tile i - 1, then the keys of tile i, stream after stream.
-struct TreeOrder {
-    int n0, n1, streams, i, s, value;
-    __device__ __forceinline__ TreeOrder(int a, int b, int of) : n0(a), n1(b), streams(of), i(0), s(0), value(1) { settle(); }
-    __device__ __forceinline__ bool done() const { return i > max(n0, n1); }
-    __device__ __forceinline__ int tile() const { return value ? i - 1 : i; }
-    __device__ __forceinline__ void step() {
-        if (value) { value = 0; return; }
-        value = 1;
-        if (++s == streams) { s = 0; ++i; }
-    }
-    __device__ __forceinline__ void settle() {
-        while (!done()) {
-            const int t = tile();
-            if (t >= 0 && t < (s ? n1 : n0)) return;
-            step();
-        }
-    }
-    __device__ __forceinline__ void next() { step(); settle(); }
-};
 
 // The rotation of 64 channels of a row without its factor (groups of 16 or 64), in the order of the
 // other kernels.
@@ -175,12 +147,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 128);
+            mbar_init(&k_full[i], 64);
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_full[i], 128);
             mbar_init(&v_empty[i], 1);
-            mbar_init(&f_full[2 * i], 128);
-            mbar_init(&f_full[2 * i + 1], 128);
+            mbar_init(&f_full[2 * i], 64);
+            mbar_init(&f_full[2 * i + 1], 64);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
             mbar_init(&o_done[i], 1);
@@ -190,7 +162,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
         *nan_nodes = 0;
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 14) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -205,7 +177,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
     float* fac = reinterpret_cast<float*>(smem + Cfg::kFacOffset);
     uint32_t* hid = reinterpret_cast<uint32_t*>(smem + Cfg::kHidOffset);
 
-    if (warp == 12) {
+    if (warp == 14) {
         // ---------------- MMAs
         const int streams = PAIR ? (n1 ? 2 : 1) : 2;
         bool ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(q_full, 0));
@@ -257,117 +229,111 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
         __syncwarp();
         if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(drain, 0)) && lane == 0) tree_record_status(kMx4TimeoutMma);
     } else if (warp >= 8) {
-        // ---------------- codes to operands: a thread a token, except for the values' transposition
-        const int t128 = tid - 256;
+        // ---------------- codes to operands. The next tile's codes are loaded into registers when this
+        // one's are laid down, and are there when its place gets free; page numbers a tile earlier.
         const int* table = a.table + b * a.table_ld;
-        const uint32_t v_off = static_cast<uint32_t>(a.hkv) << a.page_bits;
-        uint32_t* scale_words = reinterpret_cast<uint32_t*>(smem + Cfg::kScaleOffset);
-        uint32_t* places = reinterpret_cast<uint32_t*>(smem + Cfg::kPlaceOffset);
-        short2* range = reinterpret_cast<short2*>(smem + Cfg::kRangeOffset);
-        uint16_t* vfac = reinterpret_cast<uint16_t*>(smem + Cfg::kVfacOffset);
-        auto token_of = [&](const TreeOrder& o) { return ((o.s ? c1 : c0) + o.tile()) * kTreeTile + t128; };
-        auto page_of = [&](const TreeOrder& o) -> int {
-            if (o.done()) return -1;
-            const int j = token_of(o);
-            return j < n ? __ldg(table + (j >> a.page_bits)) : -1;
+        const uint32_t in_page = (1u << a.page_bits) - 1;
+        const int streams = PAIR ? 1 : 2;
+        // tiles in the order of the MMAs: stream after stream (the second may have one less)
+        const int units = PAIR ? n0 : n0 + n1;
+        auto first_of = [&](int u) { return ((PAIR || u % 2 == 0 ? c0 : c1) + u / streams) * kTreeTile; };
+        auto page_at = [&](int j) { return j < n ? __ldg(table + (j >> a.page_bits)) : -1; };
+        auto place_of = [&](int page, int j, int value) {         // in tokens of a head, the highest number: none
+            return page >= 0 && page < a.pages ? (((static_cast<uint32_t>(page) * 2 + value) * a.hkv + hk) << a.page_bits) + (static_cast<uint32_t>(j) & in_page)
+                                               : 0xFFFFFFFFu;
         };
-        // a token's 16-byte chunk c lies where neither reader meets a bank conflict
-        auto raw_at = [&](int value, int t, int c) {
-            const int unit = t * kB + c;
-            return (value ? unit ^ ((t >> 3) & 7) : kB == 4 ? unit ^ ((t >> 1) & 3) : unit ^ ((t >> 2) & 1)) * 16;
-        };
-        auto issue = [&](const TreeOrder& o, int page, int stage) {
-            const bool held = page >= 0 && page < a.pages;
-            const uint32_t off = static_cast<uint32_t>(token_of(o)) & ((1u << a.page_bits) - 1);
-            const uint32_t place = held ? (((static_cast<uint32_t>(page) * 2) * a.hkv + hk) << a.page_bits) + off + (o.value ? v_off : 0u) : 0xFFFFFFFFu;
-            unsigned char* raw = smem + Cfg::kRawOffset + stage * Cfg::kRaw;
-            #pragma unroll
-            for (int i = 0; i < kB; ++i) {
-                const int tok = (i * 32 + lane) / kB, c = (i * 32 + lane) % kB;
-                const uint32_t p = __shfl_sync(0xFFFFFFFFu, place, tok);
-                const bool h = p != 0xFFFFFFFFu;
-                cp_async16(raw + raw_at(o.value, (warp - 8) * 32 + tok, c), a.codes + (h ? static_cast<size_t>(p) * (D / 2) + c * 16 : 0), h);
-            }
-            // (heads of 64 have two scale bytes: the aligned word that holds them)
-            const size_t sp = held ? (D == 64 ? static_cast<size_t>(place & ~1u) * 2 : static_cast<size_t>(place) * kB) : 0;
-            cp_async_small<4>(scale_words + stage * 128 + t128, a.scales + sp, held);
-            places[stage * 128 + t128] = place;
-        };
-        TreeOrder ahead(n0, n1, PAIR ? 1 : 2), at(n0, n1, PAIR ? 1 : 2);
-        int page = page_of(ahead);
-        #pragma unroll
-        for (int i = 0; i < kTreeStages - 1; ++i) {
-            if (!ahead.done()) {
-                issue(ahead, page, i);
-                ahead.next();
-                page = page_of(ahead);
-            }
-            cp_async_commit();
-        }
         bool ok = true;
-        for (int u = 0; !at.done(); ++u, at.next()) {
-            const int stage = u % kTreeStages, buf = at.s, i = at.tile();
-            cp_async_wait<kTreeStages - 2>();
-            const uint32_t place = places[stage * 128 + t128];
-            uint32_t word = scale_words[stage * 128 + t128];
-            if constexpr (D == 64) word = place == 0xFFFFFFFFu ? 0u : word >> (16 * (place & 1));
-            const int j = token_of(at);
-            int top = 0, low = 255;                               // of the token's scale exponents
-            if (at.value) {
+        if (warp < 12) {
+            // values: groups of 8 tokens by 8 channels, word w of the tokens' codes
+            constexpr int kItems = kTreeTile / 8 * (D / 8) / 128;
+            const int id = tid - 256, g = id & 7, w = (id >> 3) % (D / 8);
+            uint32_t words[kItems][8], exps[kItems][8];           // exps: the words that hold the scale bytes
+            int pages[kItems];
+            auto group_at = [&](int u, int k) { return first_of(u) + 64 * (D == 128 ? k : id >> 6) + 8 * g; };
+            auto look = [&](int u) {
                 #pragma unroll
-                for (int k = 0; k < kB; ++k) {
-                    const uint32_t e = (word >> (8 * k)) & 255u;
-                    uint32_t f = e == 0u ? 0x0040u : e << 7;
-                    if (e == 255u) {
-                        // NaN: straight to the weighted sums where every row sees the token, at the end to
-                        // those rows that do where it is a node (a product with the weight 0 would give it to all)
-                        f = j < tree.context ? 0x7FC0u : 0u;
-                        if (j >= tree.context) *nan_nodes = 1;
-                    }
-                    vfac[((u & 1) * kB + k) * 128 + t128] = static_cast<uint16_t>(f);
-                }
-            } else {
-                const uint32_t gone = __ballot_sync(0xFFFFFFFFu, place == 0xFFFFFFFFu);
-                low = 255;
-                #pragma unroll
-                for (int k = 0; k < kB; ++k) {
-                    const int e = static_cast<int>((word >> (8 * k)) & 255u);
-                    if (e != 255) top = max(top, e);
-                    if (e != 255 && e != 0) low = min(low, e);    // (0: blocks of zeros, or the least there is)
-                }
-                const int most = __reduce_max_sync(0xFFFFFFFFu, top), least = __reduce_min_sync(0xFFFFFFFFu, low);
-                if (lane == 0) {
-                    hid[(buf * 2 + (i & 1)) * 8 + warp - 8] = gone;
-                    range[(u & 1) * 4 + warp - 8] = make_short2(static_cast<short>(most), static_cast<short>(least));
-                }
-            }
-            named_barrier_sync(1, 128);                           // every warp's codes are there
-            // the next tile but one takes the stage that was read before the barrier
-            if (!ahead.done()) {
-                issue(ahead, page, (u + kTreeStages - 1) % kTreeStages);
-                ahead.next();
-                page = page_of(ahead);
-            }
-            cp_async_commit();
-            const unsigned char* raw = smem + Cfg::kRawOffset + stage * Cfg::kRaw;
-            if (at.value) {
-                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&v_empty[buf], (i & 1) ^ 1));
-                if (!ok) continue;                                // (the barriers go on: no warp waits for one that left)
-                // groups of 8 tokens by 8 channels: word w of the tokens' codes
-                constexpr int kItems = kTreeTile / 8 * (D / 8) / 128;
+                for (int k = 0; k < kItems; ++k) pages[k] = u < units ? page_at(group_at(u, k)) : -1;
+            };
+            auto load = [&](int u) {
                 #pragma unroll
                 for (int k = 0; k < kItems; ++k) {
-                    const int g = t128 & 7, w = (t128 >> 3) % (D / 8), half = D == 128 ? k : t128 >> 6;
-                    uint32_t words[8];
+                    const int j = group_at(u, k);
                     #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        words[e] = *reinterpret_cast<const uint32_t*>(raw + raw_at(1, 64 * half + 8 * g + e, w >> 2) + (w & 3) * 4);
-                    const uint4 f4 = *reinterpret_cast<const uint4*>(vfac + ((u & 1) * kB + (w >> 2)) * 128 + 64 * half + 8 * g);
-                    const uint32_t f[4] = {f4.x, f4.y, f4.z, f4.w};
+                    for (int e = 0; e < 8; ++e) words[k][e] = exps[k][e] = 0u;
+                    if (a.page_bits >= 3) {                       // a group lies in one page
+                        const uint32_t place = place_of(pages[k], j, 1);
+                        if (place == 0xFFFFFFFFu) continue;
+                        const uint32_t* from = reinterpret_cast<const uint32_t*>(a.codes + static_cast<size_t>(place) * (D / 2)) + w;
+                        const uint8_t* scales = a.scales + static_cast<size_t>(place) * kB;
+                        if (j + 8 <= n) {
+                            #pragma unroll
+                            for (int e = 0; e < 8; ++e) words[k][e] = __ldg(from + e * (D / 8));
+                            if constexpr (D == 128) {
+                                const uint4 lo = __ldg(reinterpret_cast<const uint4*>(scales)), hi = __ldg(reinterpret_cast<const uint4*>(scales) + 1);
+                                exps[k][0] = lo.x; exps[k][1] = lo.y; exps[k][2] = lo.z; exps[k][3] = lo.w;
+                                exps[k][4] = hi.x; exps[k][5] = hi.y; exps[k][6] = hi.z; exps[k][7] = hi.w;
+                            } else {
+                                const uint4 x = __ldg(reinterpret_cast<const uint4*>(scales));
+                                exps[k][0] = x.x; exps[k][2] = x.y; exps[k][4] = x.z; exps[k][6] = x.w;
+                                #pragma unroll
+                                for (int e = 1; e < 8; e += 2) exps[k][e] = exps[k][e - 1] >> 16;
+                            }
+                        } else {
+                            #pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                if (j + e >= n) continue;
+                                words[k][e] = __ldg(from + e * (D / 8));
+                                exps[k][e] = D == 128 ? __ldg(reinterpret_cast<const uint32_t*>(scales) + e)
+                                                      : static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(scales) + e));
+                            }
+                        }
+                    } else {
+                        #pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t place = place_of(page_at(j + e), j + e, 1);
+                            if (place == 0xFFFFFFFFu) continue;
+                            words[k][e] = __ldg(reinterpret_cast<const uint32_t*>(a.codes + static_cast<size_t>(place) * (D / 2)) + w);
+                            exps[k][e] = D == 128 ? __ldg(reinterpret_cast<const uint32_t*>(a.scales) + place)
+                                                  : static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(a.scales) + place));
+                        }
+                    }
+                }
+            };
+            look(0);
+            load(0);
+            look(1);
+            for (int u = 0; u < units; ++u) {
+                const int buf = u % streams, i = u / streams;
+                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&v_empty[buf], (i & 1) ^ 1));
+                if (!ok) break;
+                #pragma unroll 1
+                for (int k = 0; k < kItems; ++k) {
+                    const int half = D == 128 ? k : id >> 6;
+                    uint32_t (&word)[8] = words[0], (&exp)[8] = exps[0];          // (the second item's move up below)
+                    uint32_t f[4];                                // scales of pairs of tokens as bf16
+                    bool odd_scale = false;
+                    #pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        const uint32_t x = exp[2 * p] >> (8 * (w >> 2)) & 255u, y = exp[2 * p + 1] >> (8 * (w >> 2)) & 255u;
+                        f[p] = x << 7 | y << 23;
+                        odd_scale |= x - 1u >= 254u || y - 1u >= 254u;
+                    }
+                    if (odd_scale) {
+                        // 0 is a subnormal. NaN goes straight to the weighted sums where every row sees the token, at
+                        // the end to those rows that do where it is a node (a product with the weight 0 would give it to all)
+                        #pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t x = exp[e] >> (8 * (w >> 2)) & 255u;
+                            const bool context = group_at(u, k) + e < tree.context;
+                            if (x == 255u && !context) *nan_nodes = 1;
+                            const uint32_t bits = x == 0u ? 0x0040u : x < 255u ? x << 7 : context ? 0x7FC0u : 0u;
+                            f[e / 2] = e % 2 ? (f[e / 2] & 0xFFFFu) | bits << 16 : bits;
+                        }
+                    }
                     uint32_t out[8][4];                           // [channel][pair of tokens]
                     #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        const uint32_t x = words[2 * p], y = words[2 * p + 1];
+                        const uint32_t x = word[2 * p], y = word[2 * p + 1];
                         uint32_t even[4], odd[4];
                         codes_to_bf16((x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u), even);
                         codes_to_bf16(((x >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u), odd);
@@ -377,56 +343,123 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                             out[2 * c + 1][p] = mul_bf16x2(odd[c], f[p]);
                         }
                     }
+                    // (rows are channels, 128 bytes of 64 tokens each: lanes of eight groups in distinct banks)
                     unsigned char* to = v_buf(buf) + half * Cfg::kVAtom + w * 1024;
                     #pragma unroll
                     for (int c = 0; c < 8; ++c)
                         *reinterpret_cast<uint4*>(to + c * 128 + ((g ^ c) << 4)) = make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
-                }
-                fence_proxy_async_smem();
-                mbar_arrive(&v_full[buf]);
-            } else {
-                // A code times 2^-23 is an f16 value exactly: where the tile's exponents lie no further apart
-                // one factor serves all columns.
-                uint32_t f[kB];
-                int most = 0, least = 255;
-                #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const short2 x = range[(u & 1) * 4 + k];
-                    most = max(most, static_cast<int>(x.x));
-                    least = min(least, static_cast<int>(x.y));
-                }
-                const bool apart = most - least > 23;
-                if (!apart) top = most;
-                #pragma unroll
-                for (int k = 0; k < kB; ++k) {
-                    const int e = static_cast<int>((word >> (8 * k)) & 255u);
-                    const float x = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(max(e - top + 127, 0)) << 23);
-                    f[k] = f16x2_bits(x, x);
-                }
-                fac[(buf * 2 + (i & 1)) * 128 + t128] = __uint_as_float(max(static_cast<uint32_t>(top) << 23, 0x00400000u));
-                if (t128 == 0) hid[(buf * 2 + (i & 1)) * 8 + 4] = apart;
-                mbar_arrive(&f_full[buf * 2 + (i & 1)]);
-                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&k_empty[buf], (i & 1) ^ 1));
-                if (!ok) continue;
-                #pragma unroll
-                for (int k = 0; k < kB; ++k) {
-                    const uint4 codes = *reinterpret_cast<const uint4*>(raw + raw_at(0, t128, k));
-                    const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
-                    unsigned char* to = k_buf(buf) + (k / 2) * Cfg::kAtom + t128 * 128;
                     #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t h[4];
-                        codes_to_f16(words[c], h);
-                        *reinterpret_cast<uint4*>(to + ((((k & 1) * 4 + c) ^ (t128 & 7)) << 4)) =
-                            make_uint4(hmul2_bits(h[0], f[k]), hmul2_bits(h[1], f[k]), hmul2_bits(h[2], f[k]), hmul2_bits(h[3], f[k]));
+                    for (int e = 0; e < 8; ++e) {
+                        word[e] = words[kItems - 1][e];
+                        exp[e] = exps[kItems - 1][e];
                     }
                 }
                 fence_proxy_async_smem();
+                mbar_arrive(&v_full[buf]);
+                if (u + 1 < units) {
+                    load(u + 1);
+                    look(u + 2);
+                }
+            }
+        } else {
+            // keys: a thread has tokens t and t + 64
+            const int id = tid - 384;
+            uint4 codes[2][kB];
+            uint32_t exps[2];
+            int pages[2];
+            bool held[2];
+            short2* range = reinterpret_cast<short2*>(smem + Cfg::kRangeOffset);
+            auto look = [&](int u) {
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) pages[k] = u < units ? page_at(first_of(u) + id + 64 * k) : -1;
+            };
+            auto load = [&](int u) {
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t place = place_of(pages[k], first_of(u) + id + 64 * k, 0);
+                    held[k] = place != 0xFFFFFFFFu;
+                    exps[k] = 0u;
+                    #pragma unroll
+                    for (int c = 0; c < kB; ++c) codes[k][c] = make_uint4(0, 0, 0, 0);
+                    if (!held[k]) continue;
+                    const uint4* from = reinterpret_cast<const uint4*>(a.codes + static_cast<size_t>(place) * (D / 2));
+                    #pragma unroll
+                    for (int c = 0; c < kB; ++c) codes[k][c] = __ldg(from + c);
+                    exps[k] = D == 128 ? __ldg(reinterpret_cast<const uint32_t*>(a.scales) + place)
+                                       : static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(a.scales) + place));
+                }
+            };
+            look(0);
+            load(0);
+            look(1);
+            for (int u = 0; u < units; ++u) {
+                const int buf = u % streams, i = u / streams, at = buf * 2 + (i & 1);
+                int top[2] = {0, 0}, low = 255;                   // scale exponents of the tokens
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    #pragma unroll
+                    for (int c = 0; c < kB; ++c) {
+                        const int e = static_cast<int>((exps[k] >> (8 * c)) & 255u);
+                        if (e != 255) top[k] = max(top[k], e);
+                        if (e != 255 && e != 0) low = min(low, e);                // (0: blocks of zeros, or the least there is)
+                    }
+                }
+                const uint32_t gone0 = __ballot_sync(0xFFFFFFFFu, !held[0]), gone1 = __ballot_sync(0xFFFFFFFFu, !held[1]);
+                int most = __reduce_max_sync(0xFFFFFFFFu, max(top[0], top[1])), least = __reduce_min_sync(0xFFFFFFFFu, low);
+                if (lane == 0) range[(u & 1) * 2 + warp - 12] = make_short2(static_cast<short>(most), static_cast<short>(least));
+                named_barrier_sync(1, 64);
+                // A code times 2^-23 is an f16 value exactly: where the tile's exponents lie no further apart
+                // one factor serves all columns.
+                const short2 other = range[(u & 1) * 2 + (warp & 1 ^ 1)];
+                most = max(most, static_cast<int>(other.x));
+                least = min(least, static_cast<int>(other.y));
+                const bool apart = most - least > 23;
+                // (the barriers of the two warps go on: neither waits for one that left)
+                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&k_empty[buf], (i & 1) ^ 1));
+                if (!ok) continue;
+                // the products of the tile before are done: the softmax of the tile that had these factors is, too
+                if (lane == 0) {
+                    hid[at * 8 + warp - 12] = gone0;
+                    hid[at * 8 + warp - 10] = gone1;
+                }
+                #pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (!apart) top[k] = most;
+                    fac[at * 128 + id + 64 * k] = __uint_as_float(max(static_cast<uint32_t>(top[k]) << 23, 0x00400000u));
+                }
+                if (id == 0) hid[at * 8 + 4] = apart;
+                mbar_arrive(&f_full[at]);
+                #pragma unroll 1
+                for (int k = 0; k < 2; ++k) {
+                    const int t = id + 64 * k;
+                    #pragma unroll
+                    for (int c = 0; c < kB; ++c) {
+                        const int e = static_cast<int>((exps[0] >> (8 * c)) & 255u);
+                        const float x = e == 255 ? NAN : __uint_as_float(static_cast<uint32_t>(max(e - top[0] + 127, 0)) << 23);
+                        const uint32_t f = f16x2_bits(x, x);
+                        const uint32_t words[4] = {codes[0][c].x, codes[0][c].y, codes[0][c].z, codes[0][c].w};
+                        unsigned char* to = k_buf(buf) + (c / 2) * Cfg::kAtom + t * 128;
+                        #pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            uint32_t h[4];
+                            codes_to_f16(words[y], h);
+                            *reinterpret_cast<uint4*>(to + ((((c & 1) * 4 + y) ^ (t & 7)) << 4)) =
+                                make_uint4(hmul2_bits(h[0], f), hmul2_bits(h[1], f), hmul2_bits(h[2], f), hmul2_bits(h[3], f));
+                        }
+                        codes[0][c] = codes[1][c];                // (the second token's, for the second round)
+                    }
+                    exps[0] = exps[1];
+                    top[0] = top[1];
+                }
+                fence_proxy_async_smem();
                 mbar_arrive(&k_full[buf]);
+                if (u + 1 < units) {
+                    load(u + 1);
+                    look(u + 2);
+                }
             }
         }
         if (!ok && lane == 0) tree_record_status(kMx4TimeoutProducer);
-        cp_async_wait<0>();
     } else {
         // ---------------- a stream's softmax, a thread a row
         const int s = warp >> 2, r = tid & 127;
@@ -528,8 +561,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             const bool slow = hides || gone[4] != 0u;
             const float sc = slow ? rs : rs * f[0];
             auto columns = [&](int c, uint32_t (&sr)[32]) {
-                if (!slow) return;
-                const uint32_t bits = hides ? seen[c] : 0xFFFFFFFFu;
+                const uint32_t bits = !hides ? 0xFFFFFFFFu : c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
                 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
                     const float x = __uint_as_float(sr[k]) * f[32 * c + k];
@@ -547,7 +579,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                     uint32_t sr[32];
                     tmem_ld_32x32b_x32(ts + 32 * c, sr);
                     tmem_ld_wait_regs(sr);
-                    columns(c, sr);
+                    if (slow) columns(c, sr);
                     #pragma unroll
                     for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(sr[k]));
                 }
@@ -579,41 +611,46 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                     tmem_st_32x32b_x32(ts + 32 * c, w);
                 }
             };
-            // a chunk's weights, in place; their sum
-            auto weights = [&](uint32_t (&sr)[32]) {
-                const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), by = make_float2(sc, sc);
-                float2 part[2] = {};
-                uint32_t lo[16];
-                #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const float2 y = ffma2_rn(make_float2(__uint_as_float(sr[2 * k]), __uint_as_float(sr[2 * k + 1])), by, less);
-                    const float2 w = make_float2(ex2(y.x), ex2(y.y));
-                    part[k & 1] = fadd2_rn(part[k & 1], w);
-                    split_bf16(w, sr[k], lo[k]);
-                }
-                #pragma unroll
-                for (int k = 0; k < 16; ++k) sr[16 + k] = lo[k];
-                return fadd2_rn(part[0], part[1]);
-            };
-            uint32_t sr[2][32];
-            tmem_ld_32x32b_x32(ts, sr[0]);
-            #pragma unroll
+            // chunk by chunk, the next one's scores on their way (rolled: with all roles unrolled, warps waited
+            // for instructions a fifth of the time)
+            uint32_t sr[32];
+            tmem_ld_32x32b_x32(ts, sr);
+            #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
-                uint32_t (&cur)[32] = sr[c & 1];
-                tmem_ld_wait_regs(cur);
-                if (c < 3) tmem_ld_32x32b_x32(ts + 32 * (c + 1), sr[(c + 1) & 1]);
-                columns(c, cur);
-                float2 here = weights(cur);
-                if (__any_sync(0xFFFFFFFFu, here.x + here.y > 6.1035156e-5f)) {
+                uint32_t w[32];                                   // weights, then their first and second terms
+                float2 here;
+                #pragma unroll 1
+                for (bool again = false;; again = true) {
+                    tmem_ld_wait_regs(sr);
+                    if (slow) columns(c, sr);
+                    const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), by = make_float2(sc, sc);
+                    #pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 y = ffma2_rn(make_float2(__uint_as_float(sr[2 * k]), __uint_as_float(sr[2 * k + 1])), by, less);
+                        w[2 * k] = __float_as_uint(y.x);
+                        w[2 * k + 1] = __float_as_uint(y.y);
+                    }
+                    if (c < 3) tmem_ld_32x32b_x32(ts + 32 * (c + 1), sr);
+                    float2 part[2] = {};
+                    #pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 x = make_float2(ex2(__uint_as_float(w[2 * k])), ex2(__uint_as_float(w[2 * k + 1])));
+                        part[k & 1] = fadd2_rn(part[k & 1], x);
+                        w[2 * k] = __float_as_uint(x.x);
+                        w[2 * k + 1] = __float_as_uint(x.y);
+                    }
+                    here = fadd2_rn(part[0], part[1]);
+                    if (again || !__any_sync(0xFFFFFFFFu, here.x + here.y > 6.1035156e-5f)) break;
                     tmem_ld_wait();
                     move(c);
-                    tmem_ld_32x32b_x32(ts + 32 * c, cur);
-                    tmem_ld_wait_regs(cur);
-                    columns(c, cur);
-                    here = weights(cur);
+                    tmem_ld_32x32b_x32(ts + 32 * c, sr);
                 }
                 sum = fadd2_rn(sum, here);
-                tmem_st_32x32b_x32(ts + 32 * c, cur);
+                uint32_t p[32];
+                #pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    split_bf16(make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1])), p[k], p[16 + k]);
+                tmem_st_32x32b_x32(ts + 32 * c, p);
             }
             l += sum.x + sum.y;
             tmem_st_wait();
@@ -715,7 +752,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 14) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
