@@ -12,7 +12,7 @@
 //               2^E goes to its column of S in fp32
 //   O = P V     values are bf16 exactly, whatever their scale; weights two bf16 terms (16 bits)
 //
-// S lies in tensor memory, the weights take its place (32 columns of S: 16 of the first terms, 16 of
+// S lies in tensor memory, the weights take its place (16 columns of S: 8 of the first terms, 8 of
 // the second), O beside it. The order of the MMAs is P_A V, Q_A K, P_B V, Q_B K, ..., so that
 // one stream's softmax runs under the other's products, and single buffers of K and V
 // (32 KB each at heads of 128) are refilled under the products that do not read them.
@@ -27,6 +27,7 @@ namespace convrot {
 constexpr int kTreeTile = 128;                 // tokens of a tile, rows of a stream
 constexpr int kTreeThreads = 15 * 32;
 constexpr float kTreeDown = 24.0f;
+constexpr float kTreeMost = 6.1035156e-5f;     // 2^-14: weights of a chunk above this move the reference
 
 template <int D>
 struct Mx4TreeCfg {
@@ -47,6 +48,26 @@ struct Mx4TreeCfg {
     static_assert(kSmemBytes <= 227 * 1024, "fits a multiprocessor");
     static constexpr uint32_t kIdescS = idesc_f16(kTreeTile, kTreeTile), kIdescO = idesc_bf16(kTreeTile, D);
 };
+
+// 32 lanes x 16 consecutive 32-bit columns from and to tensor memory.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_ld_wait_regs16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 
 // D (+)= A B^T, kind::f16, A from tensor memory.
 __device__ __forceinline__ void mma_f16kind_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -196,7 +217,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                         for (int j = 0; j < kTreeTile / 16; ++j)
                             #pragma unroll
                             for (int term = 0; term < 2; ++term)
-                                mma_f16kind_ts(tmem_o(s), tmem_s(s) + 32 * (j / 2) + 8 * (j % 2) + 16 * term,
+                                mma_f16kind_ts(tmem_o(s), tmem_s(s) + 16 * j + 8 * term,
                                                vd + (j / 4) * (Cfg::kVAtom / 16) + 2 * (j % 4), Cfg::kIdescO, t > 0 || j > 0 || term > 0);
                         if (last) mma_commit(&v_empty[buf]);
                         if (t == ns - 1) mma_commit(&o_done[s]);
@@ -543,116 +564,145 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             const uint32_t* gone = hid + (buf * 2 + (i & 1)) * 8;
             const int j0 = (first + i) * kTreeTile;
             const bool hides = !__all_sync(0xFFFFFFFFu, !node || (j0 + kTreeTile <= tree.context && (gone[0] | gone[1] | gone[2] | gone[3]) == 0));
-            uint32_t seen[4];                                     // columns that this row sees
-            if (hides) {
-                #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int from = j0 + 32 * c, known = min(max(tree.context - from, 0), 32);
-                    uint32_t bits = known == 32 ? 0xFFFFFFFFu : (1u << known) - 1u;
-                    const int end = min(32, n - from);
-                    if (node)
-                        for (int k = known; k < end; ++k)
-                            if (tree.sees(t, from + k)) bits |= 1u << k;
-                    seen[c] = bits & ~gone[c];
-                }
-            }
-            // Scores x and the factor sc to m's scale: what the products gave and the tile's own factor, or
-            // with columns that are hidden or keys far apart, column by column.
+            // Scores to m's scale: what the products gave times the tile's own factor, or with columns that are
+            // hidden or keys far apart, column by column.
             const bool slow = hides || gone[4] != 0u;
             const float sc = slow ? rs : rs * f[0];
-            auto columns = [&](int c, uint32_t (&sr)[32]) {
-                const uint32_t bits = !hides ? 0xFFFFFFFFu : c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
+            float sum = 0.0f;
+            auto weights = [&](const uint32_t (&x)[16], float2 (&w)[8]) {
+                const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), by = make_float2(sc, sc);
+                float2 part[2] = {};
                 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    const float x = __uint_as_float(sr[k]) * f[32 * c + k];
-                    sr[k] = bits >> k & 1u ? __float_as_uint(x) : 0xFF800000u;
+                for (int k = 0; k < 8; ++k) {
+                    const float2 y = ffma2_rn(make_float2(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), by, less);
+                    w[k] = make_float2(ex2(y.x), ex2(y.y));
+                    part[k & 1] = fadd2_rn(part[k & 1], w[k]);
                 }
+                const float2 both = fadd2_rn(part[0], part[1]);
+                return both.x + both.y;
             };
-            // The reference is one of earlier tiles as long as the weights stay below 2^-14 (their sum tells);
-            // where they do not, it moves to the largest of the scores from chunk `from` on, and what was
-            // summed and laid down gets the new scale.
-            float2 sum = make_float2(0.0f, 0.0f);
-            auto move = [&](int from) {
+            auto store = [&](int c, const float2 (&w)[8]) {
+                uint32_t p[16];
+                #pragma unroll
+                for (int k = 0; k < 8; ++k) split_bf16(w[k], p[k], p[8 + k]);
+                tmem_st_32x32b_x16(ts + 16 * c, p);
+            };
+            // The reference is one of earlier tiles, as long as the weights stay below 2^-14 (their sum tells).
+            // Chunks of 16 columns in three stages: scores on their way, weights of the next chunk, terms of
+            // this one, so that the unit of exp2 works while others do. (Two chunks a round and no more:
+            // with all roles' loops unrolled, warps waited for instructions a fifth of the time.)
+            int c = 0;
+            if (!slow) {
+                uint32_t sr[16];
+                float2 w[2][8];
+                float here[2];
+                tmem_ld_32x32b_x16(ts, sr);
+                tmem_ld_wait_regs16(sr);
+                here[0] = weights(sr, w[0]);
+                tmem_ld_32x32b_x16(ts + 16, sr);
+                #pragma unroll 1
+                for (; c < 6; c += 2) {
+                    tmem_ld_wait_regs16(sr);
+                    here[1] = weights(sr, w[1]);
+                    tmem_ld_32x32b_x16(ts + 16 * (c + 2), sr);
+                    if (__any_sync(0xFFFFFFFFu, here[0] > kTreeMost)) break;
+                    sum += here[0];
+                    store(c, w[0]);
+                    tmem_ld_wait_regs16(sr);
+                    here[0] = weights(sr, w[0]);
+                    tmem_ld_32x32b_x16(ts + 16 * (c + 3), sr);
+                    if (__any_sync(0xFFFFFFFFu, here[1] > kTreeMost)) { ++c; break; }
+                    sum += here[1];
+                    store(c + 1, w[1]);
+                }
+                tmem_ld_wait_regs16(sr);
+                if (c == 6) {
+                    here[1] = weights(sr, w[1]);
+                    if (!__any_sync(0xFFFFFFFFu, here[0] > kTreeMost)) {
+                        sum += here[0];
+                        store(6, w[0]);
+                        c = 7;
+                        if (!__any_sync(0xFFFFFFFFu, here[1] > kTreeMost)) {
+                            sum += here[1];
+                            store(7, w[1]);
+                            c = 8;
+                        }
+                    }
+                }
+            }
+            if (c < 8) {
+                // From chunk c on: the reference moves to the largest score, what was summed and laid down
+                // gets the new scale.
+                auto columns = [&](int at, uint32_t (&x)[16]) {
+                    if (!slow) return;
+                    const int from = j0 + 16 * at;
+                    uint32_t bits = 0xFFFFu;
+                    if (hides) {
+                        const int known = min(max(tree.context - from, 0), 16), end = min(16, n - from);
+                        bits = (1u << known) - 1u;
+                        if (node)
+                            for (int k = known; k < end; ++k)
+                                if (tree.sees(t, from + k)) bits |= 1u << k;
+                        bits &= ~(gone[at >> 1] >> (16 * (at & 1)));
+                    }
+                    #pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float y = __uint_as_float(x[k]) * f[16 * at + k];
+                        x[k] = bits >> k & 1u ? __float_as_uint(y) : 0xFF800000u;
+                    }
+                };
                 float top = -INFINITY;
                 #pragma unroll 1
-                for (int c = from; c < 4; ++c) {
-                    uint32_t sr[32];
-                    tmem_ld_32x32b_x32(ts + 32 * c, sr);
-                    tmem_ld_wait_regs(sr);
-                    if (slow) columns(c, sr);
+                for (int at = c; at < 8; ++at) {
+                    uint32_t x[16];
+                    tmem_ld_32x32b_x16(ts + 16 * at, x);
+                    tmem_ld_wait_regs16(x);
+                    columns(at, x);
                     #pragma unroll
-                    for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(sr[k]));
+                    for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(x[k]));
                 }
-                const float was = m;
-                m = fmaxf(m, top * sc);
-                const float down = ex2(was - m);
-                l *= down;
-                sum = fmul2_rn(sum, make_float2(down, down));
-                #pragma unroll 1
-                for (int c = 0; i > 0 && c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tmem_ld_32x32b_x32(to + 32 * c, o);
-                    tmem_ld_wait_regs(o);
-                    #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
-                    tmem_st_32x32b_x32(to + 32 * c, o);
-                }
-                #pragma unroll 1
-                for (int c = 0; c < from; ++c) {
-                    uint32_t w[32];
-                    tmem_ld_32x32b_x32(ts + 32 * c, w);
-                    tmem_ld_wait_regs(w);
-                    #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float x = (__uint_as_float(w[k] << 16) + __uint_as_float(w[16 + k] << 16)) * down;
-                        const float y = (__uint_as_float(w[k] & 0xFFFF0000u) + __uint_as_float(w[16 + k] & 0xFFFF0000u)) * down;
-                        split_bf16(make_float2(x, y), w[k], w[16 + k]);
+                top *= sc;
+                if (__any_sync(0xFFFFFFFFu, top > m + 6.0f)) {
+                    const float was = m;
+                    m = fmaxf(m, top);
+                    const float down = ex2(was - m);
+                    l *= down;
+                    sum *= down;
+                    #pragma unroll 1
+                    for (int at = 0; i > 0 && at < D / 16; ++at) {
+                        uint32_t o[16];
+                        tmem_ld_32x32b_x16(to + 16 * at, o);
+                        tmem_ld_wait_regs16(o);
+                        #pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+                        tmem_st_32x32b_x16(to + 16 * at, o);
                     }
-                    tmem_st_32x32b_x32(ts + 32 * c, w);
+                    #pragma unroll 1
+                    for (int at = 0; at < c; ++at) {
+                        uint32_t p[16];
+                        tmem_ld_32x32b_x16(ts + 16 * at, p);
+                        tmem_ld_wait_regs16(p);
+                        #pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const float x = (__uint_as_float(p[k] << 16) + __uint_as_float(p[8 + k] << 16)) * down;
+                            const float y = (__uint_as_float(p[k] & 0xFFFF0000u) + __uint_as_float(p[8 + k] & 0xFFFF0000u)) * down;
+                            split_bf16(make_float2(x, y), p[k], p[8 + k]);
+                        }
+                        tmem_st_32x32b_x16(ts + 16 * at, p);
+                    }
                 }
-            };
-            // chunk by chunk, the next one's scores on their way (rolled: with all roles unrolled, warps waited
-            // for instructions a fifth of the time)
-            uint32_t sr[32];
-            tmem_ld_32x32b_x32(ts, sr);
-            #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                uint32_t w[32];                                   // weights, then their first and second terms
-                float2 here;
                 #pragma unroll 1
-                for (bool again = false;; again = true) {
-                    tmem_ld_wait_regs(sr);
-                    if (slow) columns(c, sr);
-                    const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), by = make_float2(sc, sc);
-                    #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 y = ffma2_rn(make_float2(__uint_as_float(sr[2 * k]), __uint_as_float(sr[2 * k + 1])), by, less);
-                        w[2 * k] = __float_as_uint(y.x);
-                        w[2 * k + 1] = __float_as_uint(y.y);
-                    }
-                    if (c < 3) tmem_ld_32x32b_x32(ts + 32 * (c + 1), sr);
-                    float2 part[2] = {};
-                    #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 x = make_float2(ex2(__uint_as_float(w[2 * k])), ex2(__uint_as_float(w[2 * k + 1])));
-                        part[k & 1] = fadd2_rn(part[k & 1], x);
-                        w[2 * k] = __float_as_uint(x.x);
-                        w[2 * k + 1] = __float_as_uint(x.y);
-                    }
-                    here = fadd2_rn(part[0], part[1]);
-                    if (again || !__any_sync(0xFFFFFFFFu, here.x + here.y > 6.1035156e-5f)) break;
-                    tmem_ld_wait();
-                    move(c);
-                    tmem_ld_32x32b_x32(ts + 32 * c, sr);
+                for (; c < 8; ++c) {
+                    uint32_t x[16];
+                    float2 w[8];
+                    tmem_ld_32x32b_x16(ts + 16 * c, x);
+                    tmem_ld_wait_regs16(x);
+                    columns(c, x);
+                    sum += weights(x, w);
+                    store(c, w);
                 }
-                sum = fadd2_rn(sum, here);
-                uint32_t p[32];
-                #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    split_bf16(make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1])), p[k], p[16 + k]);
-                tmem_st_32x32b_x32(ts + 32 * c, p);
             }
-            l += sum.x + sum.y;
+            l += sum;
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(&p_full[s]);
