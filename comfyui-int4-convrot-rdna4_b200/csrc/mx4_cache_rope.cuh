@@ -1,11 +1,11 @@
 // Writing new tokens to the paged MX4 cache with their positions: queries and keys are
 // turned (rope.cuh), keys and values rotated and quantized (mx4_cache.cuh).
 //
-// Included by rope.cu. A warp's task is 32 units of keys, 32 units of values or as many
-// values of queries. Keys and values: the lanes read 16-byte chunks, pairs in one lane,
-// turn the keys in fp32 and lay 32 units down in shared memory as fp32; then a lane has a
-// unit, as in the append without positions, and gives the same codes for the same fp32
-// values. A lane's chunk stays the same from head to head, so a token's angles are
+// Included by rope.cu. A warp's task is up to 32 units of keys, as many of values or as many
+// values of queries. The lanes read 16-byte chunks, pairs in one lane, and turn them in
+// fp32; queries go out, keys and values are laid down in shared memory as fp32 units, of which
+// each lane then has one, as in the append without positions: the same codes for the same
+// fp32 values. A lane's chunk stays the same from head to head, so a token's angles are
 // computed once for all of its heads.
 #pragma once
 
@@ -18,64 +18,8 @@ struct Mx4AppendRope {
     const long long* slots;
     uint8_t *codes, *scales;
     int tokens, hq, units;                         // units of the keys
-    int kv_tasks, tasks;                           // tasks of the keys (and of the values), of all
-    int wide;                                      // 16-byte chunks (rows aligned, sections of whole chunks)
+    int size, kv_tasks, tasks;                     // units of a task, tasks of the keys (and of the values), of all
 };
-
-// Items (heads of D channels, token by token) first .. first + kItems of a task, `heads` a
-// token of which `held` exist; `sink(item, place, raw a, raw b)` or, for turned keys, floats.
-template <typename T, int D, int VP, typename Sink>
-__device__ __forceinline__ void rope_items(const T* src, long long st, long long sh, int tokens, int heads, int held, long long first,
-                                           bool turn, const RopeArgs& r, Sink sink) {
-    constexpr int kItems = 32 * 128 / D, kChunks = D / (2 * VP), kRuns = kChunks < 32 ? 32 / kChunks : 1, kPer = kItems / kRuns;
-    constexpr int kAhead = 4;
-    const int lane = threadIdx.x & 31;
-    #pragma unroll 1
-    for (int u = lane % kChunks; u < kChunks; u += 32) {
-        RopePlace<VP> at(r, u);
-        if (!turn && !r.interleaved) {                            // (values lie in a row of chunks: no pairs)
-            at.a = 2 * VP * u;
-            at.b = at.a + VP;
-        }
-        if (!turn) at.pair = -1;
-        const int from = lane / kChunks * kPer;
-        int t = static_cast<int>((first + from) / heads), h = static_cast<int>((first + from) % heads), known = -1;
-        RopeCoef<VP> w;
-        #pragma unroll 1
-        for (int i0 = 0; i0 < kPer; i0 += kAhead) {
-            RopeRaw<T, VP> ra[kAhead], rb[kAhead];
-            int it[kAhead], ih[kAhead];
-            #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                it[i] = t;
-                ih[i] = h;
-                if (t < tokens && h < held) {
-                    const T* p = src + t * st + h * sh;
-                    ra[i].load(p + at.a);
-                    rb[i].load(p + at.b);
-                } else {
-                    ra[i].zero();
-                    rb[i].zero();
-                }
-                if (++h == heads) { h = 0; ++t; }
-            }
-            #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                float fa[VP], fb[VP];
-                ra[i].get(fa);
-                rb[i].get(fb);
-                if (at.pair >= 0 && it[i] < tokens) {
-                    if (it[i] != known) {
-                        w.load(r, 0, it[i], at.pair);
-                        known = it[i];
-                    }
-                    rope_turn<VP>(fa, fb, w, r.interleaved);
-                }
-                sink(from + i0 + i, it[i], ih[i], at, fa, fb);
-            }
-        }
-    }
-}
 
 // Lays item `item`'s channels [c, c + VP) into the slab of 32 fp32 units.
 template <int D, int VP>
@@ -90,63 +34,95 @@ __device__ __forceinline__ void slab_put(unsigned char* slab, int item, int c, c
     }
 }
 
-template <typename T, int D, int G>
+template <typename T, int D, int G, int VP>
 __global__ void __launch_bounds__(kMx4QuantWarps * 32, 3)
-mx4_cache_append_rope_kernel(Mx4AppendRope a, Mx4CacheShape c, RopeArgs r) {
-    constexpr int kWide = 16 / static_cast<int>(sizeof(T));
+mx4_cache_append_rope_kernel(const __grid_constant__ Mx4AppendRope a, Mx4CacheShape c, const __grid_constant__ RopeArgs r) {
+    constexpr int kChunks = D / (2 * VP), kRuns = kChunks < 32 ? 32 / kChunks : 1, kAhead = 4;
     extern __shared__ __align__(128) unsigned char mx4slabs[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned char* slab = mx4slabs + warp * Mx4Slab<float>::kBytes;
     const int per = mx4_cache_units<D>(c.heads);                  // units of a token
-    const int padded = D == 64 ? 2 * per : c.heads;               // heads of a token with the missing one of its last unit
+    const int task = static_cast<int>(blockIdx.x) * kMx4QuantWarps + warp;
     griddep_wait();
     griddep_launch_dependents();
+    if (task >= a.tasks) return;
+    const int kind = task >= 2 * a.kv_tasks ? 2 : task >= a.kv_tasks;             // keys, values, queries
+    const int base = (task - kind * a.kv_tasks) * a.size;         // the first unit
+    const T* src = static_cast<const T*>(kind == 0 ? a.k : kind == 1 ? a.v : a.q);
+    const long long st = kind == 0 ? a.kst : kind == 1 ? a.vst : a.qst, sh = kind == 0 ? a.ksh : kind == 1 ? a.vsh : a.qsh;
+    // heads of a token, and with the missing one of heads of 64 whose last unit is half
+    const int held = kind == 2 ? a.hq : c.heads, heads = kind != 2 && D == 64 ? 2 * per : held;
+    const int items = a.size * 128 / D, share = (items + kRuns - 1) / kRuns;      // heads of the task, of a lane
+    const int first = static_cast<int>(static_cast<long long>(base) * 128 / D);
     #pragma unroll 1
-    for (int task = static_cast<int>(blockIdx.x) * kMx4QuantWarps + warp; task < a.tasks; task += static_cast<int>(gridDim.x) * kMx4QuantWarps) {
-        if (task >= 2 * a.kv_tasks) {                             // queries
-            const long long first = static_cast<long long>(task - 2 * a.kv_tasks) * (32 * 128 / D);
-            auto sink = [&](auto vp, int t, int h, auto& at, auto& fa, auto& fb) {
-                constexpr int VP = decltype(vp)::value;
-                if (t >= a.tokens) return;
-                T* to = static_cast<T*>(a.q_out) + (static_cast<long long>(t) * a.hq + h) * D;
-                RopeRaw<T, VP> o;
-                o.put(fa);
-                o.store(to + at.a);
-                o.put(fb);
-                o.store(to + at.b);
-            };
-            const T* q = static_cast<const T*>(a.q);
-            if (a.wide) rope_items<T, D, kWide>(q, a.qst, a.qsh, a.tokens, a.hq, a.hq, first, true, r,
-                [&](int, int t, int h, auto& at, auto& fa, auto& fb) { sink(std::integral_constant<int, kWide>{}, t, h, at, fa, fb); });
-            else rope_items<T, D, 1>(q, a.qst, a.qsh, a.tokens, a.hq, a.hq, first, true, r,
-                [&](int, int t, int h, auto& at, auto& fa, auto& fb) { sink(std::integral_constant<int, 1>{}, t, h, at, fa, fb); });
-            continue;
+    for (int u = lane % kChunks; u < kChunks; u += 32) {
+        const RopePlace<VP> at(r, D, u, kind != 1);               // (values are not turned)
+        const int from = lane / kChunks * share, count = min(share, items - from);
+        int t = (first + from) / heads, h = first + from - t * heads, known = -1;
+        RopeCoef<VP> w;
+        #pragma unroll 1
+        for (int i0 = 0; i0 < count; i0 += kAhead) {
+            RopeRaw<T, VP> ra[kAhead], rb[kAhead];
+            const int t0 = t, h_first = h;
+            #pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (i0 + i < count && t < a.tokens && h < held) {
+                    const T* p = src + t * st + h * sh;
+                    ra[i].load(p + at.a);
+                    rb[i].load(p + at.b);
+                } else {
+                    ra[i].zero();
+                    rb[i].zero();
+                }
+                if (++h == heads) { h = 0; ++t; }
+            }
+            int ti = t0, hi = h_first;
+            #pragma unroll 1
+            for (int i = 0; i < kAhead; ++i) {
+                // (rolled, the next item moved up: a short program, which a small call has to fetch)
+                if (i0 + i < count && ti < a.tokens && at.any() && ti != known) {
+                    w.load(r, 0, ti, at);
+                    known = ti;
+                }
+                float fa[VP], fb[VP];
+                ra[0].get(fa);
+                rb[0].get(fb);
+                if (at.any()) rope_turn<VP>(fa, fb, w, r.interleaved);
+                if (i0 + i < count) {
+                    if (kind == 2) {
+                        if (ti < a.tokens) {
+                            T* to = static_cast<T*>(a.q_out) + (static_cast<long long>(ti) * a.hq + hi) * D;
+                            RopeRaw<T, VP> o;
+                            o.put(fa);
+                            o.store(to + at.a);
+                            o.put(fb);
+                            o.store(to + at.b);
+                        }
+                    } else {
+                        slab_put<D, VP>(slab, from + i0 + i, at.a, fa);
+                        slab_put<D, VP>(slab, from + i0 + i, at.b, fb);
+                    }
+                }
+                #pragma unroll
+                for (int k = 0; k + 1 < kAhead; ++k) {
+                    ra[k] = ra[k + 1];
+                    rb[k] = rb[k + 1];
+                }
+                if (++hi == heads) { hi = 0; ++ti; }
+            }
         }
-        const bool value = task >= a.kv_tasks;
-        const int base = (value ? task - a.kv_tasks : task) * 32;
-        const T* src = static_cast<const T*>(value ? a.v : a.k);
-        const long long st = value ? a.vst : a.kst, sh = value ? a.vsh : a.ksh, first = static_cast<long long>(base) * 128 / D;
-        if (a.wide) rope_items<T, D, kWide>(src, st, sh, a.tokens, padded, c.heads, first, !value, r,
-            [&](int item, int, int, auto& at, auto& fa, auto& fb) {
-                slab_put<D, kWide>(slab, item, at.a, fa);
-                slab_put<D, kWide>(slab, item, at.b, fb);
-            });
-        else rope_items<T, D, 1>(src, st, sh, a.tokens, padded, c.heads, first, !value, r,
-            [&](int item, int, int, auto& at, auto& fa, auto& fb) {
-                slab_put<D, 1>(slab, item, at.a, fa);
-                slab_put<D, 1>(slab, item, at.b, fb);
-            });
-        __syncwarp();
-        float2 val[64];
-        slab_to_unit<float>(slab, val);
-        unit_rotate<G>(val);
-        uint4 codes[4];
-        const uint32_t word = unit_quantize(val, unit_factor<G>(), codes);
-        const int u = (base + lane) ^ (G == 256 ? 1 : 0);
-        const Mx4CacheUnit<D> at(value ? u + a.units : u, per, c.heads, 2 * a.units);
-        cache_store_unit<D>(a.codes, a.scales, c, u < a.units ? a.slots[at.t] : -1, at, codes, word);
-        __syncwarp();
     }
+    if (kind == 2) return;
+    __syncwarp();
+    // (lanes beyond a small task's units have what the slab happens to hold, and store nothing)
+    float2 val[64];
+    slab_to_unit<float>(slab, val);
+    unit_rotate<G>(val);
+    uint4 codes[4];
+    const uint32_t word = unit_quantize(val, unit_factor<G>(), codes);
+    const int mine = lane ^ (G == 256 ? 1 : 0), u = base + mine;
+    const Mx4CacheUnit<D> at(kind ? u + a.units : u, per, c.heads, 2 * a.units);
+    cache_store_unit<D>(a.codes, a.scales, c, mine < a.size && u < a.units ? a.slots[at.t] : -1, at, codes, word);
 }
 
 }  // namespace convrot

@@ -52,17 +52,19 @@ bool whole_chunks(const RopeArgs& r, int D, size_t size, long long strides) {
 }
 
 template <typename T, int VP>
-int launch_rope(const void* x, void* out, RopeShape s, long long tokens, const RopeArgs& r, cudaStream_t stream) {
+int launch_rope(const void* x, void* out, RopeShape s, const RopeArgs& r, cudaStream_t stream) {
     const long long chunks = s.D / (2 * VP);
-    // heads a thread: as many as leave every multiprocessor `kFull` threads
-    constexpr long long kFull = 1024;
-    s.heads = static_cast<int>(std::max(1LL, std::min(static_cast<long long>(s.H), tokens * chunks * s.H / (kFull * sm_count()))));
+    // heads a thread: all that leave one wave of blocks full (a token's angles serve a thread's heads)
+    const long long places = static_cast<long long>(kRopeResident) * kRopeThreads * sm_count();
+    s.runs = static_cast<int>(std::max(1LL, std::min(static_cast<long long>(s.H), places / std::max(1LL, s.tokens * chunks))));
+    s.heads = (s.H + s.runs - 1) / s.runs;
     s.runs = (s.H + s.heads - 1) / s.heads;
-    s.threads = tokens * chunks * s.runs;
-    const long long blocks = (s.threads + kRopeThreads - 1) / kRopeThreads;
-    if (blocks > 0x7FFFFFFFll) return fail("tensor too large");
-    return static_cast<int>(launch_pdl(rope_kernel<T, VP>, dim3(static_cast<unsigned>(blocks)), dim3(kRopeThreads), 0, stream,
-                                       static_cast<const T*>(x), static_cast<T*>(out), s, r));
+    const long long per = chunks * s.runs;                        // threads of a token
+    s.slice = static_cast<int>(std::max(1LL, std::min(s.tokens, (0x7FFFFFFFll - kRopeThreads) / per)));
+    const long long rows = (s.tokens + s.slice - 1) / s.slice;
+    if (rows > 65535 || per > 0x7FFFFFFFll - kRopeThreads) return fail("tensor too large");
+    const dim3 grid(static_cast<unsigned>((s.slice * per + kRopeThreads - 1) / kRopeThreads), static_cast<unsigned>(rows));
+    return static_cast<int>(launch_pdl(rope_kernel<T, VP>, grid, dim3(kRopeThreads), 0, stream, static_cast<const T*>(x), static_cast<T*>(out), s, r));
 }
 
 }  // namespace
@@ -80,12 +82,12 @@ CONVROT_API int ck_rope(const void* x, int dtype, long long x_batch, long long x
     if (!x || !out) return fail("null pointer");
     if (int rc = rope_pointers(r)) return rc;
     if (!aligned_to(x, type_size(dtype)) || !aligned_to(out, type_size(dtype))) return fail("x or out is not aligned to its type");
-    const RopeShape s{x_batch, x_token, x_head, T, H, D, 0, 0, 0};
+    const RopeShape s{x_batch, x_token, x_head, tokens, T, H, D, 0, 0, 0};
     return with_type(dtype, [&](auto* t) {
         using E = std::remove_pointer_t<decltype(t)>;
         const bool wide = aligned16(x) && aligned16(out) && whole_chunks(r, D, sizeof(E), x_batch | x_token | x_head);
-        if (wide) return launch_rope<E, 16 / sizeof(E)>(x, out, s, tokens, r, static_cast<cudaStream_t>(stream));
-        return launch_rope<E, 1>(x, out, s, tokens, r, static_cast<cudaStream_t>(stream));
+        if (wide) return launch_rope<E, 16 / sizeof(E)>(x, out, s, r, static_cast<cudaStream_t>(stream));
+        return launch_rope<E, 1>(x, out, s, r, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -124,16 +126,22 @@ CONVROT_API int ck_mx4_cache_append_rope(void* codes, void* scales, long long pa
             a.tokens = T;
             a.hq = q_heads;
             a.units = static_cast<int>(units);
-            a.kv_tasks = static_cast<int>((units + 31) / 32);
-            a.tasks = 2 * a.kv_tasks + static_cast<int>((q_items * D + 4095) / 4096);
+            // few tokens: smaller tasks, so that every warp has little to do
+            int size = 32;
+            while (size > 8 && (2 * units + q_items * D / 128) / size < 4LL * sm_count()) size /= 2;
+            a.size = size;
+            a.kv_tasks = static_cast<int>((units + size - 1) / size);
+            a.tasks = 2 * a.kv_tasks + static_cast<int>((q_items * D + 128 * size - 1) / (128 * size));
             const long long strides = k_token | k_head | v_token | v_head | (q_heads ? q_token | q_head : 0);
-            a.wide = aligned16(k) && aligned16(v) && (!q_heads || (aligned16(q) && aligned16(q_out))) && whole_chunks(r, d, sizeof(E), strides);
-            auto kernel = mx4_cache_append_rope_kernel<E, D, decltype(g)::value>;
-            const int smem = kMx4QuantWarps * Mx4Slab<float>::kBytes;
-            cudaError_t e = ensure_smem(kernel, smem);
-            if (e != cudaSuccess) return static_cast<int>(e);
-            const int blocks = std::min((a.tasks + kMx4QuantWarps - 1) / kMx4QuantWarps, 3 * sm_count());
-            return static_cast<int>(launch_pdl(kernel, dim3(blocks), dim3(kMx4QuantWarps * 32), smem, static_cast<cudaStream_t>(stream), a, c, r));
+            const bool wide = aligned16(k) && aligned16(v) && (!q_heads || (aligned16(q) && aligned16(q_out))) && whole_chunks(r, d, sizeof(E), strides);
+            const int smem = kMx4QuantWarps * Mx4Slab<float>::kBytes, blocks = (a.tasks + kMx4QuantWarps - 1) / kMx4QuantWarps;
+            auto launch = [&](auto kernel) {
+                cudaError_t e = ensure_smem(kernel, smem);
+                if (e != cudaSuccess) return static_cast<int>(e);
+                return static_cast<int>(launch_pdl(kernel, dim3(blocks), dim3(kMx4QuantWarps * 32), smem, static_cast<cudaStream_t>(stream), a, c, r));
+            };
+            if (wide) return launch(mx4_cache_append_rope_kernel<E, D, decltype(g)::value, 16 / sizeof(E)>);
+            return launch(mx4_cache_append_rope_kernel<E, D, decltype(g)::value, 1>);
         });
     });
 }

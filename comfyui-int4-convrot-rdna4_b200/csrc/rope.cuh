@@ -43,46 +43,70 @@ struct RopeArgs {
     }
 };
 
-// Cosine and sine of VP pairs of a token in a row.
+// Where a thread's 2 VP channels lie: VP from a and VP from b, so that neighbours' chunks are
+// neighbours in memory. In halves a pair has one channel in each; interleaved, each chunk holds VP / 2 pairs.
+// `pair`: the first pair, and of the second chunk's where they are interleaved; -1: none, a plain copy.
+template <int VP>
+struct RopePlace {
+    int a, b, pair, pair_b;
+    __device__ __forceinline__ RopePlace(const RopeArgs& r, int D, int u, bool turned) {
+        const int whole = r.pairs / VP;                           // chunks of pairs in halves
+        pair = pair_b = -1;
+        if (r.interleaved && VP > 1) {
+            a = VP * u;
+            b = D / 2 + a;
+            if (turned && a < 2 * r.pairs) pair = a / 2;
+            if (turned && b < 2 * r.pairs) pair_b = b / 2;
+        } else if (r.interleaved) {
+            a = 2 * u;
+            b = a + 1;
+            if (turned && u < r.pairs) pair = u;
+        } else if (u < whole) {
+            a = VP * u;
+            b = r.pairs + a;
+            if (turned) pair = a;
+        } else {
+            a = 2 * r.pairs + VP * (u - whole);
+            b = a + (D / 2 - r.pairs);
+        }
+    }
+    __device__ __forceinline__ bool any() const { return pair >= 0 || pair_b >= 0; }
+};
+
+// Cosine and sine of a thread's pairs, those of chunk a's first where they are interleaved.
 template <int VP>
 struct RopeCoef {
     float c[VP], s[VP];
-    __device__ __forceinline__ void none() {
-        #pragma unroll
-        for (int i = 0; i < VP; ++i) { c[i] = 1.0f; s[i] = 0.0f; }
-    }
-    __device__ __forceinline__ void load(const RopeArgs& r, long long b, long long t, int pair) {
+    // N pairs in a row to the places from FROM on.
+    template <int FROM, int N>
+    __device__ __forceinline__ void group(const RopeArgs& r, long long b, long long t, int pair) {
         int axis = 0;
         while (axis < r.axes - 1 && pair >= r.ends[axis]) ++axis;
+        int end = axis < r.axes - 1 ? r.ends[axis] : 0x7FFFFFFF;
         double p = r.position(b, t, axis);
         #pragma unroll
-        for (int i = 0; i < VP; ++i) {
-            if (axis < r.axes - 1 && pair + i >= r.ends[axis]) {
+        for (int i = 0; i < N; ++i) {
+            if (pair + i >= end) {
                 do ++axis; while (axis < r.axes - 1 && pair + i >= r.ends[axis]);
+                end = axis < r.axes - 1 ? r.ends[axis] : 0x7FFFFFFF;
                 p = r.position(b, t, axis);
             }
             const double turns = p * (r.freqs[pair + i] * 0.15915494309189533577);
-            sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s[i], &c[i]);
-            s[i] *= r.sign;
+            sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s[FROM + i], &c[FROM + i]);
+            s[FROM + i] *= r.sign;
         }
     }
-};
-
-// Where a thread's 2 VP channels lie: VP from a and VP from b, which are pairs (halves)
-// or hold pairs of neighbours (interleaved); behind the rotated channels, plain copies.
-template <int VP>
-struct RopePlace {
-    int a, b, pair;                // pair < 0: no pairs here
-    __device__ __forceinline__ RopePlace(const RopeArgs& r, int u) {
-        const int turned = r.pairs / VP;
-        if (u >= turned || r.interleaved) {
-            a = 2 * VP * u;
-            b = a + VP;
-            pair = u < turned ? VP * u : -1;
-        } else {
-            a = pair = VP * u;
-            b = r.pairs + VP * u;
+    __device__ __forceinline__ void load(const RopeArgs& r, long long b, long long t, const RopePlace<VP>& at) {
+        if (VP == 1 || !r.interleaved) {
+            group<0, VP>(r, b, t, at.pair);
+            return;
         }
+        constexpr int kHalf = VP > 1 ? VP / 2 : 1;
+        #pragma unroll
+        for (int i = 0; i < VP; ++i) { c[i] = 1.0f; s[i] = 0.0f; }
+        if (at.pair >= 0) group<0, kHalf>(r, b, t, at.pair);
+        if constexpr (VP > 1)
+            if (at.pair_b >= 0) group<kHalf, VP - kHalf>(r, b, t, at.pair_b);
     }
 };
 
@@ -148,32 +172,41 @@ struct RopeRaw {
 
 struct RopeShape {
     long long xb, xt, xh;          // strides of the input in elements: batch, token, head
+    long long tokens;
     int T, H, D;
-    int heads, runs;               // heads a thread takes, threads a chunk of a token needs
-    long long threads;
+    int heads, runs;               // heads a thread takes, threads that a chunk of a token needs
+    int slice;                     // tokens of a row of blocks
 };
 
 constexpr int kRopeThreads = 256;
+constexpr int kRopeResident = 2;   // blocks a multiprocessor holds
 
 // x [B, T, H, D] by strides -> out [B, T, H, D] without gaps. A thread has 2 VP channels
 // of one token and goes through its heads.
 template <typename T, int VP>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const T* __restrict__ x, T* __restrict__ out, RopeShape s, RopeArgs r) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const T* __restrict__ x, T* __restrict__ out, RopeShape s,
+                                                                         const __grid_constant__ RopeArgs r) {
     constexpr int kAhead = 4;
+    const int chunks = s.D / (2 * VP);
+    const unsigned id = blockIdx.x * static_cast<unsigned>(kRopeThreads) + threadIdx.x;
+    const unsigned rest = id / chunks, in_slice = rest / s.runs;
+    const int u = static_cast<int>(id - rest * chunks), run = static_cast<int>(rest - in_slice * s.runs);
+    const long long token = static_cast<long long>(blockIdx.y) * s.slice + in_slice;
     griddep_wait();
     griddep_launch_dependents();
-    const long long id = static_cast<long long>(blockIdx.x) * kRopeThreads + threadIdx.x;
-    if (id >= s.threads) return;
-    const int chunks = s.D / (2 * VP);
-    const int u = static_cast<int>(id % chunks);
-    const long long rest = id / chunks, token = rest / s.runs;
-    const int h0 = static_cast<int>(rest % s.runs) * s.heads, h1 = min(s.H, h0 + s.heads);
-    const long long b = token / s.T, t = token % s.T;
-    const RopePlace<VP> at(r, u);
+    if (in_slice >= static_cast<unsigned>(s.slice) || token >= s.tokens) return;
+    const int h0 = run * s.heads, h1 = min(s.H, h0 + s.heads);
+    long long b = 0, t = token;
+    if (token >= s.T) {
+        b = s.tokens <= 0x7FFFFFFF ? static_cast<int>(token) / s.T : token / s.T;
+        t = token - b * s.T;
+    }
+    const RopePlace<VP> at(r, s.D, u, true);
     const T* src = x + b * s.xb + t * s.xt;
     T* dst = out + token * s.H * s.D;
     RopeCoef<VP> w;
     bool known = false;
+    #pragma unroll 1
     for (int h = h0; h < h1; h += kAhead) {
         RopeRaw<T, VP> ra[kAhead], rb[kAhead];
         #pragma unroll
@@ -183,14 +216,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const T* __restrict_
                 rb[i].load(src + (h + i) * s.xh + at.b);
             }
         if (!known) {                                             // (the first loads are on their way)
-            if (at.pair >= 0) w.load(r, b, t, at.pair);
+            if (at.any()) w.load(r, b, t, at);
             known = true;
         }
         #pragma unroll
         for (int i = 0; i < kAhead; ++i)
             if (h + i < h1) {
                 T* to = dst + static_cast<long long>(h + i) * s.D;
-                if (at.pair >= 0) {
+                if (at.any()) {
                     float fa[VP], fb[VP];
                     ra[i].get(fa);
                     rb[i].get(fb);
