@@ -1435,6 +1435,13 @@ int dispatch_gemm_i8(const void* X, const void* W, const float* xs, const float*
 
 int run_gemm_i8(const void* X, const void* W, const float* xs, const float* ws, BiasRef bias, void* out, int out_dtype,
                 int M, int N, int K, cudaStream_t stream) {
+    if (out_dtype == 1 && N % 8 == 0 && aligned16(out)) {
+        // 192-column tiles where 256-column ones are the choice and the waves of tiles come out shorter
+        // (509 x 6144 x 4096: 64 tiles for 74 CTA pairs instead of 48, 13.4 against 17.6 us)
+        const long pairs = sm_count() / 2, rows = (M + 255) / 256, tiles256 = rows * ((N + 255) / 256), tiles192 = rows * ((N + 191) / 192);
+        if (2 * tiles256 >= pairs && (tiles192 + pairs - 1) / pairs * 3 < (tiles256 + pairs - 1) / pairs * 4)
+            return launch_pair_impl<192, false, kOutBF16, true, false, true>(X, W, xs, ws, bias, out, M, N, K, LoraArgs(), stream);
+    }
     if (out_dtype == 1) return dispatch_gemm_i8<kOutBF16>(X, W, xs, ws, bias, out, M, N, K, stream);
     return dispatch_gemm_i8<kOutF32>(X, W, xs, ws, bias, out, M, N, K, stream);
 }
@@ -1938,7 +1945,8 @@ CONVROT_API int ck_int8_convrot_gemm(const void* X, const void* W, const void* x
     const float* ws = static_cast<const float*>(wscale);
     const BiasRef b{bias, 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return run_gemm_i8(X, W, xs, ws, b, out, out_dtype, M, N, K, s);
+    if (out_dtype == 1) return dispatch_gemm_i8<kOutBF16>(X, W, xs, ws, b, out, M, N, K, s);
+    return dispatch_gemm_i8<kOutF32>(X, W, xs, ws, b, out, M, N, K, s);
 }
 
 CONVROT_API int ck_int8_gemm_s32(const void* X, const void* W, void* acc, int M, int N, int K, void* stream) {

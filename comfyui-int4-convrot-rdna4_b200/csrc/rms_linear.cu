@@ -12,13 +12,30 @@ using namespace convrot;
 namespace {
 
 template <typename T, int G>
-int launch_rms_quant(const RmsQuantArgs& a, int warps, cudaStream_t stream) {
-    auto kernel = rms_quant_int8_kernel<T, G>;
-    const int smem = rms_quant_smem<T>(warps, a.row_warps);
-    cudaError_t e = ensure_smem(kernel, rms_quant_smem<T>(4, 4));
-    if (e != cudaSuccess) return static_cast<int>(e);
-    const int blocks = std::min((a.M + a.rows - 1) / a.rows, 3 * sm_count());
-    return static_cast<int>(launch_pdl(kernel, dim3(blocks), dim3(warps * 32), smem, stream, a));
+int launch_rms_quant(const RmsQuantArgs& a, cudaStream_t stream) {
+    const int warps = a.rows * a.row_warps, blocks = std::min((a.M + a.rows - 1) / a.rows, 8 * sm_count());
+    auto launch = [&](auto kernel, int most) {
+        cudaError_t e = ensure_smem(kernel, most * kRmsWarpFloats * 4);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        return static_cast<int>(launch_pdl(kernel, dim3(blocks), dim3(warps * 32), warps * kRmsWarpFloats * 4, stream, a));
+    };
+    if (warps <= 8) return launch(rms_quant_int8_kernel<T, G, 256>, 8);
+    return launch(rms_quant_int8_kernel<T, G, 1024>, 32);
+}
+
+// Four warps a block, as many blocks as there are outputs by 16, or sixteen where those would
+// leave places empty (1 x 15360 x 3840: one wave of blocks, with eight warps it were two and a bit).
+template <int NT, typename T>
+int launch_few(const RmsQuantArgs& a, const void* W, const float* ws, BiasRef bias, void* out, int N, cudaStream_t stream) {
+    const int blocks = (N + 15) / 16, warps = blocks >= 2 * sm_count() ? 4 : 16;
+    return static_cast<int>(launch_pdl(few_i8_kernel<NT, T>, dim3(blocks), dim3(warps * 32), warps * 8 * NT * 17 * 4, stream, static_cast<const int8_t*>(a.codes),
+                                       static_cast<const int8_t*>(W), static_cast<const float*>(a.scales), ws, bias, static_cast<T*>(out), a.M, N, a.K));
+}
+
+template <typename T>
+int run_few(const RmsQuantArgs& a, const void* W, const float* ws, BiasRef bias, void* out, int N, cudaStream_t stream) {
+    if (a.M <= 8) return launch_few<1, T>(a, W, ws, bias, out, N, stream);
+    return launch_few<2, T>(a, W, ws, bias, out, N, stream);
 }
 
 }  // namespace
@@ -64,20 +81,23 @@ CONVROT_API int ck_convrot_w8a8_linear_rmsnorm(const void* x, const void* residu
     a.M = M;
     a.K = K;
     a.g_type = norm_dtype;
-    a.row_warps = (K + 4095) / 4096;
-    a.rows = 4 / a.row_warps;
+    a.row_warps = (K + 511) / 512;
+    a.rows = std::max(1, 8 / a.row_warps);
     a.vec_x = aligned16(x) && ldx * static_cast<long long>(size) % 16 == 0;
+    a.vec_g = aligned16(norm_weight);
     a.vec_r = aligned16(residual) && ldr * static_cast<long long>(size) % 16 == 0;
     a.eps = eps;
-    const int warps = a.rows * a.row_warps;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (int rc = with_type(dtype, [&](auto* t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            if (G == 16) return launch_rms_quant<T, 16>(a, warps, st);
-            if (G == 64) return launch_rms_quant<T, 64>(a, warps, st);
-            return launch_rms_quant<T, 256>(a, warps, st);
+            if (G == 16) return launch_rms_quant<T, 16>(a, st);
+            if (G == 64) return launch_rms_quant<T, 64>(a, st);
+            return launch_rms_quant<T, 256>(a, st);
         }))
         return rc;
     if (N == 0) return 0;
-    return run_gemm_i8(a.codes, W, a.scales, static_cast<const float*>(wscale), BiasRef{bias, bias_dtype}, out, out_dtype, M, N, K, st);
+    const float* s = static_cast<const float*>(wscale);
+    const BiasRef b{bias, bias_dtype};
+    if (M <= kFewI8Rows) return out_dtype == 1 ? run_few<__nv_bfloat16>(a, W, s, b, out, N, st) : run_few<float>(a, W, s, b, out, N, st);
+    return run_gemm_i8(a.codes, W, a.scales, s, b, out, out_dtype, M, N, K, st);
 }

@@ -4,13 +4,17 @@
 // R(h g), and a row needs one pass and one exchange (sum of squares and largest
 // magnitude together). All in fp32, without an intermediate rounding.
 //
-// A thread has 128 columns (a unit, mx4_unit.cuh), a row one to four warps; a block
-// goes through rows of the matrix and keeps g in shared memory.
+// A thread has 16 neighbouring columns, a warp 512 (two groups of 256). The steps of the
+// rotation at strides 1 and 4 stay in the thread; for those at 16 and 64 the 16 x 16 values
+// of a group are transposed through shared memory, codes go back the same way. A block
+// goes through rows, keeps its columns' g in registers and loads the next row's
+// values under the current one's work.
 #pragma once
 
 namespace convrot {
 
-constexpr int kRmsMostK = 16384;              // four warps a row, with g and two slabs of it in shared memory
+constexpr int kRmsMostK = 16384;              // 32 warps a row
+constexpr int kRmsWarpFloats = 512 + 16;      // a warp's values; the second group 16 floats on: other banks
 
 struct RmsQuantArgs {
     const void *x, *r, *g;                    // r null: no residual; g null: ones
@@ -20,141 +24,254 @@ struct RmsQuantArgs {
     float* scales;                            // [M]
     int M, K, g_type;
     int row_warps, rows;                      // warps of a row, rows of a block at a time
-    int vec_x, vec_r;                         // 16-byte aligned rows
+    int vec_x, vec_r, vec_g;                  // 16-byte aligned rows
     float eps;
 };
 
+// 16 values of a row from memory as they are.
 template <typename T>
-__host__ __device__ constexpr int rms_quant_smem(int warps, int row_warps) {
-    return warps * 2 * Mx4Slab<T>::kBytes + row_warps * Mx4Slab<float>::kBytes;
+struct RmsRaw {
+    static constexpr int kChunks = sizeof(T);                     // of 16 bytes: 16 values are as many as a value's bytes
+    uint4 v[kChunks];
+    __device__ __forceinline__ void load(const T* p, bool held, bool vec) {
+        #pragma unroll
+        for (int c = 0; c < kChunks; ++c) v[c] = make_uint4(0, 0, 0, 0);
+        if (!held) return;
+        if (vec) {
+            #pragma unroll
+            for (int c = 0; c < kChunks; ++c) v[c] = __ldg(reinterpret_cast<const uint4*>(p) + c);
+        } else {
+            T e[16];
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) e[i] = p[i];
+            memcpy(v, e, sizeof(e));
+        }
+    }
+    __device__ __forceinline__ void get(float (&f)[16]) const {
+        T e[16];
+        memcpy(e, v, sizeof(e));
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = mx4_to_f32(e[i]);
+    }
+    __device__ __forceinline__ void put(const float (&f)[16]) {
+        T e[16];
+        #pragma unroll
+        for (int i = 0; i < 16; ++i) e[i] = mx4_from_f32<T>(f[i]);
+        memcpy(v, e, sizeof(e));
+    }
+};
+
+// Steps at strides 1 and 4 of 16 values.
+__device__ __forceinline__ void rms_rotate16(float (&v)[16], bool second) {
+    #pragma unroll
+    for (int i = 0; i < 16; i += 4) h4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    if (second) {
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) h4(v[i], v[i + 4], v[i + 8], v[i + 12]);
+    }
 }
 
-template <typename T, int G>
-__global__ void __launch_bounds__(128, 3) rms_quant_int8_kernel(RmsQuantArgs a) {
-    using S = Mx4Slab<T>;
-    extern __shared__ __align__(128) unsigned char mx4slabs[];
-    __shared__ float2 part[4];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    unsigned char* slab = mx4slabs + warp * 2 * S::kBytes;
-    unsigned char* gains = mx4slabs + warps * 2 * S::kBytes;
-    const int in_row = warp % a.row_warps, col = (in_row * 32 + lane) * kMx4Unit;       // this thread's first column
-    auto start = [&](int row) {
-        const bool held = row < a.M && col < a.K;
-        const int chunks = held ? min(S::kChunks, (a.K - col) / S::kPer) : 0;
-        const T* x = static_cast<const T*>(a.x);
-        slab_load<false>(slab, Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(held ? x + row * a.ldx + col : x), chunks}, 0, a.vec_x);
-        if (a.r) {
-            const T* r = static_cast<const T*>(a.r);
-            slab_load<false>(slab + S::kBytes, Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(held ? r + row * a.ldr + col : r), chunks}, 0, a.vec_r);
-        }
-    };
+// THREADS: 256 (rows up to 4096 columns) or 1024.
+template <typename T, int G, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int8_kernel(const __grid_constant__ RmsQuantArgs a) {
+    extern __shared__ __align__(128) unsigned char rms_smem[];
+    __shared__ float2 part[2][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float* mine = reinterpret_cast<float*>(rms_smem) + warp * kRmsWarpFloats;
+    const int in_row = warp % a.row_warps, col = in_row * 512 + lane * 16;
+    const bool column = col < a.K;
+    const int group = lane >> 4, j = lane & 15;
     griddep_wait();
     griddep_launch_dependents();
-    const int first = static_cast<int>(blockIdx.x) * a.rows + warp / a.row_warps;
-    start(first);
-    cp_async_commit();
-    for (int i = threadIdx.x; i < a.row_warps * 4096; i += blockDim.x) {
-        float g = 0.0f;
-        if (i < a.K)
-            g = !a.g ? 1.0f : a.g_type == 0 ? static_cast<const float*>(a.g)[i] : a.g_type == 1 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.g)[i])
-                                                                                             : __half2float(static_cast<const __half*>(a.g)[i]);
-        *reinterpret_cast<float*>(gains + i / 4096 * Mx4Slab<float>::kBytes + Mx4Slab<float>::offset(i % 4096 / kMx4Unit, i % kMx4Unit / 4) + i % 4 * 4) = g;
+    int row = static_cast<int>(blockIdx.x) * a.rows + warp / a.row_warps;
+    RmsRaw<T> x, r;
+    auto load = [&](int at) {
+        const bool held = column && at < a.M;
+        x.load(static_cast<const T*>(a.x) + (held ? at * a.ldx + col : 0), held, a.vec_x);
+        if (a.r) r.load(static_cast<const T*>(a.r) + (held ? at * a.ldr + col : 0), held, a.vec_r);
+    };
+    load(row);
+    float g[16];
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) g[i] = 1.0f;
+    if (a.g) {
+        auto gains = [&](auto* p) {
+            RmsRaw<std::remove_const_t<std::remove_pointer_t<decltype(p)>>> raw;
+            raw.load(p + (column ? col : 0), column, a.vec_g);
+            raw.get(g);
+        };
+        if (a.g_type == 0) gains(static_cast<const float*>(a.g));
+        else if (a.g_type == 1) gains(static_cast<const __nv_bfloat16*>(a.g));
+        else gains(static_cast<const __half*>(a.g));
     }
-    __syncthreads();
-    for (int row0 = static_cast<int>(blockIdx.x) * a.rows; row0 < a.M; row0 += static_cast<int>(gridDim.x) * a.rows) {
-        const int row = row0 + warp / a.row_warps;
-        const bool held = row < a.M && col < a.K;
-        cp_async_wait<0>();
-        __syncwarp();
-        float2 v[64];
-        slab_to_unit<T>(slab, v);
+    // (every warp of the block makes as many rounds: they meet at barriers)
+    for (int row0 = static_cast<int>(blockIdx.x) * a.rows, round = 0; row0 < a.M; row0 += static_cast<int>(gridDim.x) * a.rows, ++round) {
+        float v[16];
+        x.get(v);
         if (a.r) {
-            float2 w[64];
-            slab_to_unit<T>(slab + S::kBytes, w);
+            float w[16];
+            r.get(w);
             #pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] = fadd2_rn(v[i], w[i]);
-            __syncwarp();
-            unit_to_slab<T>(slab, lane, v, 1.0f);
-            __syncwarp();
-            T* h = static_cast<T*>(a.h);
-            slab_store<T>(slab, Mx4UnitAt<T>{reinterpret_cast<const unsigned char*>(held ? h + static_cast<size_t>(row) * a.K + col : h),
-                                             held ? min(S::kChunks, (a.K - col) / S::kPer) : 0});
-        }
-        __syncwarp();
-        float2 sum[4] = {};
-        #pragma unroll
-        for (int i = 0; i < 64; ++i) sum[i & 3] = ffma2_rn(v[i], v[i], sum[i & 3]);
-        float ss = ((sum[0].x + sum[1].x) + (sum[2].x + sum[3].x)) + ((sum[0].y + sum[1].y) + (sum[2].y + sum[3].y));
-        {
-            const unsigned char* gs = gains + in_row * Mx4Slab<float>::kBytes;
-            #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-                const float4 lo = *reinterpret_cast<const float4*>(gs + Mx4Slab<float>::offset(lane, c));
-                const float4 hi = *reinterpret_cast<const float4*>(gs + Mx4Slab<float>::offset(lane, c + 16));
-                v[4 * c] = fmul2_rn(v[4 * c], make_float2(lo.x, hi.x));
-                v[4 * c + 1] = fmul2_rn(v[4 * c + 1], make_float2(lo.y, hi.y));
-                v[4 * c + 2] = fmul2_rn(v[4 * c + 2], make_float2(lo.z, hi.z));
-                v[4 * c + 3] = fmul2_rn(v[4 * c + 3], make_float2(lo.w, hi.w));
+            for (int i = 0; i < 16; ++i) v[i] = __fadd_rn(v[i], w[i]);
+            if (column && row < a.M) {
+                RmsRaw<T> o;
+                o.put(v);
+                uint4* h = reinterpret_cast<uint4*>(static_cast<T*>(a.h) + static_cast<size_t>(row) * a.K + col);
+                #pragma unroll
+                for (int c = 0; c < RmsRaw<T>::kChunks; ++c) h[c] = o.v[c];
             }
         }
-        unit_rotate<G>(v);
-        float top[4] = {};
+        const int now = row;
+        row += static_cast<int>(gridDim.x) * a.rows;
+        load(row);
+        float ss = 0.0f, amax = 0.0f;
         #pragma unroll
-        for (int i = 0; i < 64; ++i) top[i & 3] = max3_abs_nan(top[i & 3], v[i].x, v[i].y);
-        float amax = max3_abs_nan(max3_abs_nan(top[0], top[1], top[2]), top[3], 0.0f);
+        for (int i = 0; i < 16; ++i) {
+            ss = fmaf(v[i], v[i], ss);
+            v[i] *= g[i];
+        }
+        rms_rotate16(v, true);
+        if constexpr (G >= 64) {
+            // value 16 l + i of a group (of its thread l) lies in row l, its chunks of four XORed: neither
+            // side meets a bank conflict
+            float* base = mine + group * (256 + 16);
+            #pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *reinterpret_cast<float4*>(base + j * 16 + ((c ^ (j >> 1 & 3)) << 2)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+            __syncwarp();
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = base[i * 16 + (((j >> 2) ^ (i >> 1 & 3)) << 2) + (j & 3)];
+            rms_rotate16(v, G == 256);
+        }
+        #pragma unroll
+        for (int i = 0; i < 16; i += 2) amax = max3_abs_nan(amax, v[i], v[i + 1]);
         #pragma unroll
         for (int z = 16; z; z >>= 1) {
             ss += __shfl_xor_sync(0xFFFFFFFFu, ss, z);
             amax = max3_abs_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, z), 0.0f);
         }
-        if (a.row_warps > 1) {                                    // (every warp of the block passes the same barriers)
-            if (lane == 0) part[warp] = make_float2(ss, amax);
+        if (a.row_warps > 1) {
+            float2* p = part[round & 1];
+            if (lane == 0) p[warp] = make_float2(ss, amax);
             __syncthreads();
-            ss = amax = 0.0f;
-            for (int w = warp - in_row; w < warp - in_row + a.row_warps; ++w) {
-                ss += part[w].x;
-                amax = max3_abs_nan(amax, part[w].y, 0.0f);
+            const float2 y = lane < a.row_warps ? p[warp - in_row + lane] : make_float2(0.0f, 0.0f);
+            ss = y.x;
+            amax = y.y;
+            #pragma unroll
+            for (int z = 16; z; z >>= 1) {
+                ss += __shfl_xor_sync(0xFFFFFFFFu, ss, z);
+                amax = max3_abs_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, z), 0.0f);
             }
-            __syncthreads();
         }
         const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.K) + a.eps);
         const float y = amax * unit_factor<G>() * rstd;
         const float s = (y < 1e-10f ? 1e-10f : y) / 127.0f;       // (NaN stays)
         const float f = unit_factor<G>() * rstd / s;
-        const int mine = lane ^ (G == 256 ? 1 : 0);               // whose columns this lane has after the rotation
-        #pragma unroll
-        for (int c = 0; c < 4; ++c) {                             // 16 columns of each half of the unit
-            uint32_t wx[4], wy[4];
+        uint32_t out[4];
+        if constexpr (G >= 64) {
+            __syncwarp();
+            unsigned char* bytes = reinterpret_cast<unsigned char*>(mine);
             #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                wx[j] = wy[j] = 0;
+            for (int i = 0; i < 16; ++i)
+                bytes[group * 256 + i * 16 + j] = static_cast<unsigned char>(max(-127, min(127, __float2int_rn(v[i] * f))));
+            __syncwarp();
+            const uint4 o = *reinterpret_cast<const uint4*>(bytes + lane * 16);
+            out[0] = o.x; out[1] = o.y; out[2] = o.z; out[3] = o.w;
+            __syncwarp();
+        } else {
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                out[c] = 0;
                 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 z = fmul2_rn(v[16 * c + 4 * j + e], make_float2(f, f));
-                    const int ix = max(-127, min(127, __float2int_rn(z.x))), iy = max(-127, min(127, __float2int_rn(z.y)));
-                    wx[j] |= static_cast<uint32_t>(ix & 255) << (8 * e);
-                    wy[j] |= static_cast<uint32_t>(iy & 255) << (8 * e);
-                }
+                for (int e = 0; e < 4; ++e)
+                    out[c] |= static_cast<uint32_t>(max(-127, min(127, __float2int_rn(v[4 * c + e] * f))) & 255) << (8 * e);
             }
-            *reinterpret_cast<uint4*>(slab + mine * 128 + ((c ^ (mine & 7)) << 4)) = make_uint4(wx[0], wx[1], wx[2], wx[3]);
-            *reinterpret_cast<uint4*>(slab + mine * 128 + (((c + 4) ^ (mine & 7)) << 4)) = make_uint4(wy[0], wy[1], wy[2], wy[3]);
         }
-        __syncwarp();
-        if (row < a.M) {
-            int8_t* to = a.codes + static_cast<size_t>(row) * a.K + in_row * 4096;
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int unit = (i * 32 + lane) >> 3, c = lane & 7;
-                if (in_row * 4096 + unit * 128 + c * 16 < a.K)
-                    *reinterpret_cast<uint4*>(to + unit * 128 + c * 16) = *reinterpret_cast<const uint4*>(slab + unit * 128 + ((c ^ (unit & 7)) << 4));
-            }
-            if (in_row == 0 && lane == 0) a.scales[row] = s;
+        if (now < a.M) {
+            if (column) *reinterpret_cast<uint4*>(a.codes + static_cast<size_t>(now) * a.K + col) = make_uint4(out[0], out[1], out[2], out[3]);
+            if (in_row == 0 && lane == 0) a.scales[now] = s;
         }
-        __syncwarp();
-        start(row + static_cast<int>(gridDim.x) * a.rows);
-        cp_async_commit();
     }
-    cp_async_wait<0>();
+}
+
+// ---------------------------------------------------------------- few rows times the int8 weight
+
+// out[m, n] = ((float(D) xs[m]) ws[n]) + bias[n], D the exact product, for up to 8 NT rows (NT 1 or 2): bound by the
+// weight's bytes. A block takes 16 outputs, its warps a share of K each; products run on
+// mma.m16n8k32 with the weight on the side of 16 (tcgen05 wants 128 rows of it a tile,
+// and the tiles of a weight of some thousand rows do not fill the multiprocessors). The order of
+// the contraction is free, so a thread's operands are 16 bytes of a row as they lie. The weight
+// is not written by the kernel before (this library's quantizer), so its first loads
+// start under that kernel.
+constexpr int kFewI8Rows = 16;                 // (32 x 15360 x 3840: 33 us against 19 in tiles of 256 rows; 8: 11)
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int NT, typename T>
+__global__ void __launch_bounds__(512)
+few_i8_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, const float* __restrict__ xs, const float* __restrict__ ws,
+              BiasRef bias, T* __restrict__ out, int M, int N, int K) {
+    constexpr int kAhead = 4;                                     // segments of 64 columns on their way
+    extern __shared__ int few_sums[];                             // [warp][row][17]
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = static_cast<int>(blockIdx.x) * 16;
+    const int segs = (K + 63) / 64, per = (segs + warps - 1) / warps;
+    const int s0 = min(segs, warp * per), s1 = min(segs, s0 + per);
+    const int8_t* row0 = w + static_cast<size_t>(min(n0 + g, N - 1)) * K + 16 * t;
+    const int8_t* row1 = w + static_cast<size_t>(min(n0 + g + 8, N - 1)) * K + 16 * t;
+    uint4 a[kAhead][2];
+    auto load_w = [&](int s, uint4 (&to)[2]) {
+        const bool held = s < s1 && 64 * s + 16 * t < K;
+        to[0] = held ? __ldg(reinterpret_cast<const uint4*>(row0 + 64 * s)) : make_uint4(0, 0, 0, 0);
+        to[1] = held ? __ldg(reinterpret_cast<const uint4*>(row1 + 64 * s)) : make_uint4(0, 0, 0, 0);
+    };
+    #pragma unroll
+    for (int i = 0; i < kAhead; ++i) load_w(s0 + i, a[i]);
+    griddep_wait();
+    griddep_launch_dependents();
+    int d[NT][4] = {};
+    const int8_t* xr[NT];
+    #pragma unroll
+    for (int k = 0; k < NT; ++k) xr[k] = x + static_cast<size_t>(min(8 * k + g, M - 1)) * K + 16 * t;
+    #pragma unroll 1
+    for (int s = s0; s < s1; s += kAhead) {
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (s + i < s1) {
+                const uint4 lo = a[i][0], hi = a[i][1];
+                const bool held = 64 * (s + i) + 16 * t < K;
+                #pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    // (the rows' codes come from the kernel before: no read-only loads)
+                    const uint4 b = held ? *reinterpret_cast<const uint4*>(xr[k] + 64 * (s + i)) : make_uint4(0, 0, 0, 0);
+                    mma_s8(d[k], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+                    mma_s8(d[k], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+                }
+                load_w(s + i + kAhead, a[i]);
+            }
+        }
+    }
+    #pragma unroll
+    for (int k = 0; k < NT; ++k) {
+        int* to = few_sums + (warp * 8 * NT + 8 * k + 2 * t) * 17 + g;
+        to[0] = d[k][0];
+        to[17] = d[k][1];
+        to[8] = d[k][2];
+        to[25] = d[k][3];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * 8 * NT; i += blockDim.x) {
+        const int m = i >> 4, n = n0 + (i & 15);
+        if (m >= M || n >= N) continue;
+        int sum = 0;
+        for (int k = 0; k < warps; ++k) sum += few_sums[(k * 8 * NT + m) * 17 + (i & 15)];
+        float y = __fmul_rn(__fmul_rn(static_cast<float>(sum), xs[m]), ws[n]);
+        if (bias.ptr) y = __fadd_rn(y, bias.at(n));
+        out[static_cast<size_t>(m) * N + n] = mx4_from_f32<T>(y);
+    }
 }
 
 }  // namespace convrot
