@@ -85,6 +85,13 @@ struct Mx4Tree {
     }
     // Whether node t, one of the tree's, sees token j, one of the cache's.
     __device__ __forceinline__ bool sees(int t, int j) const { return j < context || mask[t * row + (j - context)] != 0; }
+    // The same for any t and j, without a branch: several loads are then on their way at once.
+    __device__ __forceinline__ bool sees_any(int t, int j) const {
+        const int last = nodes - 1, from = j - context;
+        if (last < 0) return false;
+        const uint8_t named = __ldg(mask + min(t, last) * row + min(max(from, 0), last));
+        return (t <= last) & ((from < 0) | ((from <= last) & (named != 0)));
+    }
 };
 
 constexpr int kMx4AttnWarps = 4;
@@ -527,11 +534,13 @@ mx4_attn_kernel(Mx4AttnArgs a) {
                 for (int h = 0; h < 2; ++h) {
                     const int r = 8 * i + 2 * t4 + h;
                     const int t = (row0 + r) / per_head;
-                    const int sees = r >= rows ? 0 : !TREE ? n - a.tq + t + 1 : t < tree.nodes ? n : 0;
+                    const int sees = r >= rows ? 0 : !TREE ? n - a.tq + t + 1 : n;
                     #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int j = ci * kMx4AttnChunk + 8 * c + ktok;
-                        if (j >= sees || (TREE && !tree.sees(t, j))) s[i][c >> 1][2 * (c & 1) + h] = -INFINITY;
+                        bool seen = j < sees;
+                        if constexpr (TREE) seen &= tree.sees_any(t, j);
+                        if (!seen) s[i][c >> 1][2 * (c & 1) + h] = -INFINITY;
                     }
                 }
             // a value's block of NaN: straight to the accumulators of the rows that see its

@@ -17,10 +17,10 @@ struct AttnPlan {
     size_t partials() const { return splits > 1 && !clustered ? static_cast<size_t>(tiles) * splits * tile_rows : 0; }
 };
 
-inline AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
+// With tiles of `tile_rows` of a cache head's `rows`.
+inline AttnPlan attn_plan_rows(int B, long long rows, int tile_rows, int hkv, int d, long long longest) {
     AttnPlan p;
-    const long long rows = static_cast<long long>(tq) * (hq / hkv);
-    p.tile_rows = rows <= 8 ? 8 : rows <= 16 || d == 256 ? 16 : 32;
+    p.tile_rows = tile_rows;
     p.row_tiles = static_cast<int>((rows + p.tile_rows - 1) / p.tile_rows);
     p.tiles = static_cast<long long>(B) * hkv * p.row_tiles;
     // splits: one full wave of blocks always, as far as every split has a group of
@@ -39,6 +39,11 @@ inline AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longe
     // (64 x 4096 tokens, 4 splits: 106 against 99 us)
     p.clustered = p.splits > 1 && p.splits <= 8 && tiles * p.splits <= 2LL * sm_count();
     return p;
+}
+
+inline AttnPlan attn_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
+    const long long rows = static_cast<long long>(tq) * (hq / hkv);
+    return attn_plan_rows(B, rows, rows <= 8 ? 8 : rows <= 16 || d == 256 ? 16 : 32, hkv, d, longest);
 }
 
 template <typename T, int D, int NT, bool TREE>
@@ -73,7 +78,7 @@ int launch_attention(const Mx4AttnArgs& a, const AttnPlan& p, cudaStream_t strea
 template <typename T, int D, bool TREE>
 int launch_attention_rows(const Mx4AttnArgs& a, const AttnPlan& p, cudaStream_t stream) {
     if (p.tile_rows == 8) return launch_attention<T, D, 1, TREE>(a, p, stream);
-    if constexpr (D < 256)
+    if constexpr (D < 256 && !TREE)
         if (p.tile_rows == 32) return launch_attention<T, D, 4, TREE>(a, p, stream);
     return launch_attention<T, D, 2, TREE>(a, p, stream);
 }

@@ -36,7 +36,7 @@ using namespace convrot;
 namespace {
 
 // How a call is cut. `tensor`: the kernel of this file's header, with 256 rows of a cache head a
-// block (pair) or 128; otherwise the one for few rows.
+// block (pair) or 128; otherwise the one for few rows, in tiles of 8 or 16.
 struct TreePlan {
     AttnPlan p;
     bool tensor, pair;
@@ -45,9 +45,17 @@ struct TreePlan {
 TreePlan tree_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
     TreePlan t{};
     const long long rows = static_cast<long long>(tq) * (hq / hkv);
-    t.tensor = d <= 128 && rows > 32;
+    // What is least by what was measured: a start, and a time for each tile of rows and 128 tokens. Tiles of
+    // 8 rows start first, and read the cache anew for each 8; 128 rows of the tensor kernel take as long
+    // as 22 of them. In ns; heads of 128: 1 x 777 tokens of 32 rows 8.9 us
+    // in tiles of 8, 19 in one tile of 32, 20 by the tensor kernel; 16 x 4096 tokens of 32 rows 112, 94 and 78 us; of
+    // 16 rows (tiles of 16) 57 against 78 us; heads of 64, 32 rows: 72 against 58 us.
+    const double units = static_cast<double>(B) * hkv * ((longest + kTreeTile - 1) / kTreeTile), per = d == 64 ? 0.57 : d / 128.0;
+    const double few8 = 8000 + 7 * per * units * ((rows + 7) / 8), few16 = 11000 + 14 * per * units * ((rows + 15) / 16);
+    const double many = 18000 + (d == 64 ? 10 : 19) * units * (rows <= kTreeTile ? 1.0 : 1.5 * ((rows + 2 * kTreeTile - 1) / (2 * kTreeTile)));
+    t.tensor = d <= 128 && many < std::min(few8, few16);
     if (!t.tensor) {
-        t.p = attn_plan(B, tq, hq, hkv, d, longest);
+        t.p = attn_plan_rows(B, rows, rows <= 8 || few8 <= few16 ? 8 : 16, hkv, d, longest);
         return t;
     }
     t.pair = rows > kTreeTile;

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             mbar_init(&p_full[i], 128);
             mbar_init(&o_done[i], 1);
         }
-        mbar_init(q_full, PAIR ? 256 : 128);
+        mbar_init(q_full, PAIR || D == 128 ? 256 : 128);
         mbar_init(drain, 1);
         *nan_nodes = 0;
         fence_mbar_init();
@@ -486,15 +486,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
         const int s = warp >> 2, r = tid & 127;
         const int row = row0 + (PAIR ? s * kTreeTile : 0) + r, t = row / per_head;
         const bool real = row < rows_all && (PAIR || r < rows);
-        if (PAIR || s == 0) {
+        {
+            // the row's queries: rotated, then two f16 terms of the row times a power of two. 64 channels at a
+            // time: where both streams have the same rows of 128, the second's threads take the second
+            // half; a pair's threads load their rows twice, for the largest value and as operands.
+            constexpr bool kSplit = !PAIR && D == 128;
             const T* q = static_cast<const T*>(a.q) + b * a.qsb + t * a.qst + (hk * per_head + row % per_head) * a.qsh;
-            // 64 channels at a time, rotated (twice: for the largest value, then as operands; a whole
-            // row of 128 does not fit the registers)
-            auto channels = [&](int from, float (&v)[64]) {
-                if (!real) {
-                    #pragma unroll
-                    for (int i = 0; i < 64; ++i) v[i] = 0.0f;
-                } else if (vec_q) {
+            float v[64], top = 0.0f;
+            auto channels = [&](int from) {
+                #pragma unroll
+                for (int i = 0; i < 64; ++i) v[i] = 0.0f;
+                if (real && vec_q) {
                     #pragma unroll
                     for (int i = 0; i < 64; i += 8) {
                         const uint4 x = __ldg(reinterpret_cast<const uint4*>(q + from + i));
@@ -503,30 +505,35 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                         #pragma unroll
                         for (int k = 0; k < 8; ++k) v[i + k] = mx4_to_f32(e[k]);
                     }
-                } else {
+                } else if (real) {
                     #pragma unroll
                     for (int i = 0; i < 64; ++i) v[i] = mx4_to_f32(q[from + i]);
                 }
                 tree_rotate(v, a.group);
             };
-            float top = 0.0f;
+            const bool mine = PAIR || kSplit || s == 0;
             #pragma unroll 1
-            for (int from = 0; from < D; from += 64) {
-                float v[64];
-                channels(from, v);
+            for (int from = kSplit ? 64 * s : 0; mine && from < D; from += 64) {
+                channels(from);
                 #pragma unroll
                 for (int i = 0; i < 64; ++i) top = fmaxf(top, fabsf(v[i]));
+                if (kSplit) break;
+            }
+            if constexpr (kSplit) {
+                row_scale[s * 128 + r] = top;
+                named_barrier_sync(2, 256);
+                top = fmaxf(top, row_scale[(s ^ 1) * 128 + r]);
+                named_barrier_sync(2, 256);
             }
             // 2^(8 - exponent of the row's largest value), within fp32's normal range
             const int e = static_cast<int>(__float_as_uint(top) >> 23);
             const int up = top > 0.0f ? min(max(135 - e, -120), 120) : 0;
             // (the scale's sign goes to the queries, and 0 to the smallest number: a hidden score stays -inf)
             const float to_f16 = copysignf(__uint_as_float(static_cast<uint32_t>(127 + up) << 23), a.scale);
-            row_scale[s * 128 + r] = fmaxf(fabsf(a.scale) * tree_factor(a.group) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
+            if (mine) row_scale[s * 128 + r] = fmaxf(fabsf(a.scale) * tree_factor(a.group) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
             #pragma unroll 1
-            for (int from = 0; from < D; from += 64) {
-                float v[64];
-                channels(from, v);
+            for (int from = kSplit ? 64 * s : 0; mine && from < D; from += 64) {
+                if (PAIR && D == 128) channels(from);
                 unsigned char* base = smem + (PAIR ? 2 * s : 0) * Cfg::kOperand + from / 64 * Cfg::kAtom + r * 128;
                 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
@@ -544,17 +551,20 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                     *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4*>(to + Cfg::kOperand) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
+                if (kSplit) break;
             }
-            fence_proxy_async_smem();
-            mbar_arrive(q_full);
+            if (mine) {
+                fence_proxy_async_smem();
+                mbar_arrive(q_full);
+            }
         }
         const int ns = s ? n1 : n0, first = s ? c1 : c0, buf = PAIR ? 0 : s;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem_s(s) + lanes, to = tmem_o(s) + lanes;
         float m = kMx4NoScore, l = 0.0f, rs = 0.0f;
         bool ok = true;
-        if (!PAIR && ns) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(q_full, 0));      // (both streams' rows are scaled by one of them)
-        if (ns) rs = row_scale[(PAIR ? s * 128 : 0) + r];
+        if (!PAIR && ns) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(q_full, 0));      // (heads of 64: the first stream's threads scale both's rows)
+        if (ns) rs = row_scale[(PAIR || D == 128 ? s * 128 : 0) + r];
         const bool node = real && t < tree.nodes;                 // (what other rows compute is not kept)
         for (int i = 0; ok && i < ns; ++i) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&s_full[s], i & 1) && mbar_wait_bounded(&f_full[buf * 2 + (i & 1)], (i >> 1) & 1));
@@ -633,18 +643,29 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             if (c < 8) {
                 // From chunk c on: the reference moves to the largest score, what was summed and laid down
                 // gets the new scale.
+                unsigned long long seen[2] = {~0ull, ~0ull};      // columns that this row sees
+                if (hides) {
+                    #pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        unsigned long long bits = 0;
+                        #pragma unroll 1
+                        for (int k = 0; k < 64; k += 16) {
+                            const int from = j0 + 64 * half + k;
+                            uint32_t some = 0;
+                            if (from + 16 <= tree.context) {
+                                some = 0xFFFFu;
+                            } else if (from < n) {
+                                #pragma unroll
+                                for (int e = 0; e < 16; ++e) some |= static_cast<uint32_t>(tree.sees_any(t, from + e)) << e;
+                            }
+                            bits |= static_cast<unsigned long long>(some) << k;
+                        }
+                        seen[half] = bits & ~(static_cast<unsigned long long>(gone[2 * half]) | static_cast<unsigned long long>(gone[2 * half + 1]) << 32);
+                    }
+                }
                 auto columns = [&](int at, uint32_t (&x)[16]) {
                     if (!slow) return;
-                    const int from = j0 + 16 * at;
-                    uint32_t bits = 0xFFFFu;
-                    if (hides) {
-                        const int known = min(max(tree.context - from, 0), 16), end = min(16, n - from);
-                        bits = (1u << known) - 1u;
-                        if (node)
-                            for (int k = known; k < end; ++k)
-                                if (tree.sees(t, from + k)) bits |= 1u << k;
-                        bits &= ~(gone[at >> 1] >> (16 * (at & 1)));
-                    }
+                    const uint32_t bits = static_cast<uint32_t>((at < 4 ? seen[0] : seen[1]) >> (16 * (at & 3)));
                     #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         const float y = __uint_as_float(x[k]) * f[16 * at + k];

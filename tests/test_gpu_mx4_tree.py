@@ -95,7 +95,11 @@ CASES = [  # lens, nodes (None: all), t, hq, hkv, D, page, group
     ([64, 513], [20, 31], 31, 4, 4, 128, 32, 16), ([1030, 129, 128, 127], [40, 3, 40, 17], 40, 8, 2, 128, 16, 64),
     ([260, 60], [60, 60], 60, 3, 1, 256, 16, 256), ([2100], None, 64, 16, 2, 128, 64, 64), ([500, 257], [129, 130], 130, 2, 1, 64, 64, 0),
     ([4000, 10, 200], [70, 10, 70], 70, 4, 2, 64, 128, 16), ([50, 3], [0, 70000], 9, 20, 4, 128, 16, 64), ([6, 20, 33], [9, 9, 9], 9, 32, 2, 64, 1, 64),
-    ([1500], None, 300, 1, 1, 128, 256, 64), ([900, 128, 1], [33, 33, 1], 33, 12, 3, 256, 64, 64)]
+    ([1500], None, 300, 1, 1, 128, 256, 64), ([900, 128, 1], [33, 33, 1], 33, 12, 3, 256, 64, 64),
+    # enough rows and tokens for the kernel that takes 128 or 256 rows at a time
+    ([1100, 0, 40, 1025], [40, 0, 40, 17], 40, 64, 2, 128, 64, 64), ([1200, 1, 700], [16, 1, 9], 16, 64, 8, 128, 16, 16),
+    ([900, 1300], None, 150, 64, 8, 64, 128, 64), ([1200, 1281, 31], [30, 29, 30], 30, 32, 8, 64, 16, 0), ([1290, 640], None, 17, 128, 8, 128, 1, 64),
+    ([1153, 1152, 1151], [65, 64, 3], 65, 16, 2, 128, 2, 0), ([1400, 129], [128, 128], 128, 16, 8, 64, 4, 16), ([2000, 1500], [257, 256], 257, 4, 2, 128, 256, 64)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -117,11 +121,11 @@ def test_tree(mx, case, dtype):
     assert torch.equal(out.view(torch.int16), again.view(torch.int16))
 
 
-@pytest.mark.parametrize("t,hq,hkv,d", [(4, 8, 2, 128), (48, 8, 2, 128), (150, 3, 3, 64)])
+@pytest.mark.parametrize("t,hq,hkv,d", [(4, 8, 2, 128), (48, 8, 2, 128), (150, 3, 3, 64), (40, 64, 2, 128), (16, 64, 8, 128), (150, 64, 8, 64), (30, 32, 8, 64)])
 def test_any_mask(mx, t, hq, hkv, d):
     """Masks that are no trees: rows that see nothing of a sequence without context, forward references, one mask for all,
     views with strides."""
-    lens, nodes = [t, 500, t - 1], [t, t, t]
+    lens, nodes = [t, 500 if hq < 32 else 1200, t - 1], [t, t, t]
     codes, scales, table = make_cache(mx, lens, 16, hkv, d, 64, t)
     q = torch.randn(3, t, hq, d, generator=torch.Generator().manual_seed(t)).bfloat16().cuda()
     n = torch.tensor(lens, dtype=torch.int32, device="cuda")
@@ -153,9 +157,9 @@ def test_sequence_shorter_than_its_nodes(mx):
     assert near.all()
 
 
-@pytest.mark.parametrize("t,hq", [(6, 4), (60, 8)])
+@pytest.mark.parametrize("t,hq", [(6, 4), (60, 8), (60, 64)])
 def test_strides_scale_lengths_and_bad_pages(mx, t, hq):
-    lens = [90, 64]
+    lens = [90, 64] if hq < 64 else [1500, 1000]
     codes, scales, table = make_cache(mx, lens, 16, 2, 64, 64, 4)
     qkv = torch.randn(2, t, 3, hq, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
     q = qkv[:, :, 1]
@@ -176,53 +180,54 @@ def test_strides_scale_lengths_and_bad_pages(mx, t, hq):
     check(cut, reference(q, codes, scales, table[:, :4], [64, 0], [t, t], mask, 64 ** -0.5, 64), q)
 
 
-@pytest.mark.parametrize("t,d", [(5, 128), (70, 128), (70, 64), (20, 256)])
-def test_nan_in_the_cache(mx, t, d):
+@pytest.mark.parametrize("t,d,hq", [(5, 128, 4), (70, 128, 4), (70, 64, 4), (20, 256, 4), (70, 128, 128), (100, 64, 128)])
+def test_nan_in_the_cache(mx, t, d, hq):
     """A NaN block of a key or a value reaches the nodes that see its token, and no others."""
-    lens = [200]
+    many = hq // 2
+    lens = [200] if hq < 64 else [200 + 1040]
     codes, scales, table = make_cache(mx, lens, 16, 2, d, 0, 7)
-    q = torch.randn(1, t, 4, d, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    q = torch.randn(1, t, hq, d, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
     n = torch.tensor(lens, dtype=torch.int32, device="cuda")
     mask = mx.tree_mask(trees(1, t, 5))[0].cuda()
     clean = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask, convrot_groupsize=0)
 
     def at(j):
         return int(table[0, j // 16]), j % 16
-    node = t // 2
-    for kind, j in ((0, 200 - t + node), (1, 200 - t + node), (1, 200 - t)):
+    node, n0 = t // 2, lens[0]
+    for kind, j in ((0, n0 - t + node), (1, n0 - t + node), (1, n0 - t)):
         held = scales.clone()
         p, o = at(j)
         held[p, kind, 1, o, 1] = 255
         out = mx.convrot_mx4_tree_attention(q, codes, held, table, n, mask, convrot_groupsize=0)
-        sees = mask[0, :, j - (200 - t)]
+        sees = mask[0, :, j - (n0 - t)]
         bad = out.isnan()
         want = torch.zeros_like(bad)
-        want[0, sees, 2:, (slice(None) if kind == 0 else slice(32, 64))] = True
+        want[0, sees, many:, (slice(None) if kind == 0 else slice(32, 64))] = True
         assert torch.equal(bad, want), (kind, j)
         assert torch.equal(out[~want], clean[~want])
     held = scales.clone()                                                         # in the context: all nodes
     p, o = at(3)
     held[p, 1, 0, o, 0] = 255
     out = mx.convrot_mx4_tree_attention(q, codes, held, table, n, mask, convrot_groupsize=0)
-    assert out[0, :, :2, :32].isnan().all() and int(out.isnan().sum()) == t * 2 * 32
+    assert out[0, :, :many, :32].isnan().all() and int(out.isnan().sum()) == t * many * 32
     held = scales.clone()                                                         # behind the sequence: nobody
-    held[at(200)[0], :, :, at(200)[1]:] = 255
+    held[at(n0)[0], :, :, at(n0)[1]:] = 255
     assert torch.equal(mx.convrot_mx4_tree_attention(q, codes, held, table, n, mask, convrot_groupsize=0), clean)
 
 
-@pytest.mark.parametrize("t,d", [(5, 128), (70, 128), (70, 64)])
+@pytest.mark.parametrize("t,d,hq", [(5, 128, 4), (70, 128, 4), (70, 64, 4), (50, 128, 64), (60, 64, 64)])
 @pytest.mark.parametrize("spread", [30.0, 1e4])
-def test_values_and_keys_of_mixed_magnitudes(mx, t, d, spread):
-    lens = [333, 150]
+def test_values_and_keys_of_mixed_magnitudes(mx, t, d, hq, spread):
+    lens = [333, 150] if hq < 64 else [1333, 150]
     codes, scales, table = make_cache(mx, lens, 16, 2, d, 64, 11, spread)
-    q = (torch.randn(2, t, 4, d, generator=torch.Generator().manual_seed(3)) * 4).bfloat16().cuda()
+    q = (torch.randn(2, t, hq, d, generator=torch.Generator().manual_seed(3)) * 4).bfloat16().cuda()
     mask = mx.tree_mask(trees(2, t, 6))[0].cuda()
     n = torch.tensor(lens, dtype=torch.int32, device="cuda")
     out = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask)
     check(out, reference(q, codes, scales, table, lens, [t, t], mask, d ** -0.5, 64), q)
 
 
-@pytest.mark.parametrize("t,hq", [(8, 8), (64, 8)])
+@pytest.mark.parametrize("t,hq", [(8, 8), (64, 8), (64, 32)])
 def test_streams_and_graphs(mx, t, hq):
     """A captured call replayed with other tables, lengths and masks, and two graphs at once on two streams."""
     lens = [3000, 700]
@@ -251,3 +256,26 @@ def test_streams_and_graphs(mx, t, hq):
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("t,d,hq", [(6, 128, 4), (50, 128, 64), (60, 64, 64)])
+def test_keys_far_apart_and_scores_that_grow(mx, t, d, hq):
+    """Keys of one tile whose scales lie more than 2^23 apart, and scores that rise from tile to tile, so that the
+    reference moves and what was summed gets a new scale."""
+    lens = [1300]
+    codes, scales, table = make_cache(mx, lens, 16, 2, d, 64, 21)
+    j = torch.arange(lens[0])
+    slots = (table[0].cpu().long()[j // 16] * 16 + j % 16).cuda()
+    k, v = mx.convrot_mx4_cache_read(codes, scales, slots, torch.float32, 64)
+    k = k * (0.02 * 1.003 ** j.cuda())[:, None, None]                             # 0.02 .. 1: a row's largest score moves up and up
+    k[::7] *= 2.0 ** -40
+    mx.convrot_mx4_cache_append(codes, scales, k, v, slots, 64)
+    q = (torch.randn(1, t, hq, d, generator=torch.Generator().manual_seed(3)) * 20).bfloat16().cuda()
+    mask = mx.tree_mask(trees(1, t, 6))[0].cuda()
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask)
+    check(out, reference(q, codes, scales, table, lens, [t], mask, d ** -0.5, 64), q)
+    back = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask, softmax_scale=-0.05)
+    check(back, reference(q, codes, scales, table, lens, [t], mask, -0.05, 64), q)
+    flat = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask, softmax_scale=0.0)
+    check(flat, reference(q, codes, scales, table, lens, [t], mask, 0.0, 64), q)
