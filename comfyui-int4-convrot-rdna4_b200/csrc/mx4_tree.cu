@@ -79,7 +79,7 @@ TreePlan tree_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
 
 template <typename T, int D, bool PAIR>
 int launch_tree(const Mx4AttnArgs& a, const AttnPlan& p, int vec_q, cudaStream_t stream) {
-    using Cfg = Mx4TreeCfg<D>;
+    using Cfg = Mx4TreeCfg<D, PAIR>;
     auto kernel = mx4_tree_kernel<T, D, PAIR>;
     cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
     if (e != cudaSuccess) return static_cast<int>(e);

@@ -14,8 +14,8 @@
 //
 // S lies in tensor memory, the weights take its place (16 columns of S: 8 of the first terms, 8 of
 // the second), O beside it. The order of the MMAs is P_A V, Q_A K, P_B V, Q_B K, ..., so that
-// one stream's softmax runs under the other's products, and single buffers of K and V
-// (32 KB each at heads of 128) are refilled under the products that do not read them.
+// one stream's softmax runs under the other's products, and K and V (32 KB a tile at heads of 128)
+// are refilled under the products that do not read them.
 //
 // Weights are 2^(s - m - 24), m near the row's maximum: sums of up to 2^24 of them stay
 // below one, so that O does not leave fp32's range where the mean does not. m moves when a score
@@ -29,18 +29,19 @@ constexpr int kTreeThreads = 15 * 32;
 constexpr float kTreeDown = 24.0f;
 constexpr float kTreeMost = 6.1035156e-5f;     // 2^-14: weights of a chunk above this move the reference
 
-template <int D>
+template <int D, bool PAIR>
 struct Mx4TreeCfg {
     static constexpr int kOperand = kTreeTile * D * 2;            // a term of a stream's queries, a tile of K or V
     static constexpr int kAtom = kTreeTile * 128;                 // 128 rows of 64 16-bit columns, 128-byte swizzle
     static constexpr int kVAtom = D * 128;                        // D rows (channels) of 64 tokens
     static constexpr int kBlocks = D / 32;
-    static constexpr int kFacOffset = 6 * kOperand;               // (four terms of queries, or two and the second K and V; K, V)
-                                                                  // [buffer][parity][128] fp32: factors of a tile's keys
-    static constexpr int kHidOffset = kFacOffset + 2048;          // [buffer][parity][8]: hidden tokens' bits, keys far apart
-    static constexpr int kRangeOffset = kHidOffset + 128;         // [2][2] largest and least exponents of a tile's keys
-    static constexpr int kRowOffset = kRangeOffset + 32;                            // [256] fp32: the rows' scales
-    static constexpr int kBarOffset = kRowOffset + 1024;
+    // a pair: four terms of queries, K, two tiles of V; otherwise two terms, then K and V of each stream
+    static constexpr int kFacOffset = (PAIR ? 7 : 6) * kOperand;  // [buffer][parity][128] fp32: factors of a tile's keys
+    static constexpr int kBufs = PAIR ? 1 : 2;                    // buffers of K
+    static constexpr int kHidOffset = kFacOffset + kBufs * 1024;  // [buffer][parity][8]: hidden tokens' bits, keys far apart
+    static constexpr int kRangeOffset = kHidOffset + kBufs * 64;  // [2][2] largest and least exponents of a tile's keys
+    static constexpr int kRowOffset = kRangeOffset + 32;          // [256] fp32: the rows' scales (both streams' the same rows)
+    static constexpr int kBarOffset = kRowOffset + (PAIR ? 0 : 1024);
     static constexpr int kBars = 2 * 4 + 2 * 2 + 2 * 3 + 2;
     static constexpr int kEnd = kBarOffset + kBars * 8 + 16;
     // (all of the tensor memory is taken: one block a multiprocessor, by shared memory too)
@@ -137,7 +138,7 @@ __device__ __forceinline__ float tree_factor(int group) { return group == 16 ? 0
 
 template <typename T, int D, bool PAIR>
 __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a, int vec_q) {
-    using Cfg = Mx4TreeCfg<D>;
+    using Cfg = Mx4TreeCfg<D, PAIR>;
     constexpr int kB = Cfg::kBlocks;
     extern __shared__ __align__(1024) unsigned char tree_smem_raw[];
     unsigned char* smem = tree_smem_raw + ((1024u - (smem_u32(tree_smem_raw) & 1023u)) & 1023u);
@@ -194,7 +195,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
     auto tmem_s = [&](int s) { return tmem + s * kTreeTile; };
     auto tmem_o = [&](int s) { return tmem + 2 * kTreeTile + s * D; };
     auto k_buf = [&](int i) { return smem + (PAIR || i == 0 ? 4 : 2) * Cfg::kOperand; };
-    auto v_buf = [&](int i) { return smem + (PAIR || i == 0 ? 5 : 3) * Cfg::kOperand; };
+    auto v_buf = [&](int i) { return smem + (PAIR ? 5 + i : i == 0 ? 5 : 3) * Cfg::kOperand; };
+    // a tile's place among the values: a pair's tiles take turns, otherwise each stream has one
+    auto v_at = [](int s, int i) { return PAIR ? i & 1 : s; };
+    auto v_use = [](int i) { return PAIR ? i >> 1 : i; };
     float* fac = reinterpret_cast<float*>(smem + Cfg::kFacOffset);
     uint32_t* hid = reinterpret_cast<uint32_t*>(smem + Cfg::kHidOffset);
 
@@ -207,11 +211,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 const int ns = s ? n1 : n0, buf = PAIR ? 0 : s;
                 const bool last = !PAIR || s == streams - 1;      // of those that read the buffers
                 if (i > 0 && i - 1 < ns) {
-                    const int t = i - 1;
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&v_full[buf], t & 1) && mbar_wait_bounded(&p_full[s], t & 1));
+                    const int t = i - 1, vb = v_at(s, t);
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&v_full[vb], v_use(t) & 1) && mbar_wait_bounded(&p_full[s], t & 1));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t vd = smem_desc_kmajor(smem_u32(v_buf(buf)), 1024, 2);
+                    const uint64_t vd = smem_desc_kmajor(smem_u32(v_buf(vb)), 1024, 2);
                     if (elect_one()) {
                         #pragma unroll
                         for (int j = 0; j < kTreeTile / 16; ++j)
@@ -219,7 +223,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                             for (int term = 0; term < 2; ++term)
                                 mma_f16kind_ts(tmem_o(s), tmem_s(s) + 16 * j + 8 * term,
                                                vd + (j / 4) * (Cfg::kVAtom / 16) + 2 * (j % 4), Cfg::kIdescO, t > 0 || j > 0 || term > 0);
-                        if (last) mma_commit(&v_empty[buf]);
+                        if (last) mma_commit(&v_empty[vb]);
                         if (t == ns - 1) mma_commit(&o_done[s]);
                     }
                     __syncwarp();
@@ -324,8 +328,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             load(0);
             look(1);
             for (int u = 0; u < units; ++u) {
-                const int buf = u % streams, i = u / streams;
-                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&v_empty[buf], (i & 1) ^ 1));
+                const int buf = v_at(u % streams, u / streams), use = v_use(u / streams);
+                ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&v_empty[buf], (use & 1) ^ 1));
                 if (!ok) break;
                 #pragma unroll 1
                 for (int k = 0; k < kItems; ++k) {
@@ -486,6 +490,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
         const int s = warp >> 2, r = tid & 127;
         const int row = row0 + (PAIR ? s * kTreeTile : 0) + r, t = row / per_head;
         const bool real = row < rows_all && (PAIR || r < rows);
+        float rs = 0.0f;                                          // the row's scale
         {
             // the row's queries: rotated, then two f16 terms of the row times a power of two. 64 channels at a
             // time: where both streams have the same rows of 128, the second's threads take the second
@@ -530,7 +535,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             const int up = top > 0.0f ? min(max(135 - e, -120), 120) : 0;
             // (the scale's sign goes to the queries, and 0 to the smallest number: a hidden score stays -inf)
             const float to_f16 = copysignf(__uint_as_float(static_cast<uint32_t>(127 + up) << 23), a.scale);
-            if (mine) row_scale[s * 128 + r] = fmaxf(fabsf(a.scale) * tree_factor(a.group) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
+            rs = fmaxf(fabsf(a.scale) * tree_factor(a.group) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
+            if (!PAIR && D == 64 && mine) row_scale[r] = rs;
             #pragma unroll 1
             for (int from = kSplit ? 64 * s : 0; mine && from < D; from += 64) {
                 if (PAIR && D == 128) channels(from);
@@ -561,10 +567,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
         const int ns = s ? n1 : n0, first = s ? c1 : c0, buf = PAIR ? 0 : s;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem_s(s) + lanes, to = tmem_o(s) + lanes;
-        float m = kMx4NoScore, l = 0.0f, rs = 0.0f;
+        float m = kMx4NoScore, l = 0.0f;
         bool ok = true;
-        if (!PAIR && ns) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(q_full, 0));      // (heads of 64: the first stream's threads scale both's rows)
-        if (ns) rs = row_scale[(PAIR || D == 128 ? s * 128 : 0) + r];
+        if (!PAIR && D == 64 && s == 1 && ns) {                   // (the first stream's threads have scaled the rows)
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(q_full, 0));
+            rs = row_scale[r];
+        }
         const bool node = real && t < tree.nodes;                 // (what other rows compute is not kept)
         for (int i = 0; ok && i < ns; ++i) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&s_full[s], i & 1) && mbar_wait_bounded(&f_full[buf * 2 + (i & 1)], (i >> 1) & 1));
