@@ -281,16 +281,11 @@ CONVROT_API int ck_mx4_linear(const void* x, int dtype, long long ldx, const voi
     });
 }
 
-CONVROT_API int ck_mx4_cache_append(void* codes, void* scales, long long pages, int heads, int d, int page, int G,
-                                    const void* k, const void* v, int in_dtype, long long k_token, long long k_head,
-                                    long long v_token, long long v_head, const void* slots, int T, void* stream) {
-    if (int rc = check_cache(codes, scales, pages, heads, d, page, G)) return rc;
-    if (T < 0) return fail("T must not be negative");
-    if (in_dtype < 0 || in_dtype > 2) return fail("dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
-    if (T == 0) return 0;
-    if (!k || !v || !slots) return fail("null pointer");
-    if (!aligned_to(k, type_size(in_dtype)) || !aligned_to(v, type_size(in_dtype)) || !aligned_to(slots, 8))
-        return fail("keys, values or slots are not aligned to their type");
+namespace convrot {
+
+int run_cache_append(void* codes, void* scales, long long pages, int heads, int d, int page, int G, const void* k, const void* v, int in_dtype,
+                     long long k_token, long long k_head, long long v_token, long long v_head, const void* slots, int T, bool values_only,
+                     cudaStream_t stream) {
     const Mx4CacheShape c{pages * page, heads, d, page_bits(page)};
     return with_type(in_dtype, [&](auto* t) {
         using E = std::remove_pointer_t<decltype(t)>;
@@ -304,12 +299,28 @@ CONVROT_API int ck_mx4_cache_append(void* codes, void* scales, long long pages, 
             const bool vec = aligned16(k) && aligned16(v) && strides * static_cast<long long>(sizeof(E)) % 16 == 0;
             const bool linear = vec && k_head == d && v_head == d && k_token == static_cast<long long>(heads) * d &&
                                 v_token == k_token && (d != 64 || heads % 2 == 0);
-            return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<E>(),
-                                               static_cast<cudaStream_t>(stream), static_cast<uint8_t*>(codes),
+            return static_cast<int>(launch_pdl(kernel, dim3(unit_blocks(values_only ? units / 2 : units)), dim3(kMx4QuantWarps * 32), mx4_quant_smem<E>(),
+                                               stream, static_cast<uint8_t*>(codes),
                                                static_cast<uint8_t*>(scales), static_cast<const E*>(k), static_cast<const E*>(v),
-                                               k_token, k_head, v_token, v_head, static_cast<const long long*>(slots), static_cast<int>(units), c, vec, linear));
+                                               k_token, k_head, v_token, v_head, static_cast<const long long*>(slots), static_cast<int>(values_only ? units / 2 : 0), static_cast<int>(units), c, vec, linear));
         });
     });
+}
+
+}  // namespace convrot
+
+CONVROT_API int ck_mx4_cache_append(void* codes, void* scales, long long pages, int heads, int d, int page, int G,
+                                    const void* k, const void* v, int in_dtype, long long k_token, long long k_head,
+                                    long long v_token, long long v_head, const void* slots, int T, void* stream) {
+    if (int rc = check_cache(codes, scales, pages, heads, d, page, G)) return rc;
+    if (T < 0) return fail("T must not be negative");
+    if (in_dtype < 0 || in_dtype > 2) return fail("dtype must be 0 (f32), 1 (bf16) or 2 (f16)");
+    if (T == 0) return 0;
+    if (!k || !v || !slots) return fail("null pointer");
+    if (!aligned_to(k, type_size(in_dtype)) || !aligned_to(v, type_size(in_dtype)) || !aligned_to(slots, 8))
+        return fail("keys, values or slots are not aligned to their type");
+    return run_cache_append(codes, scales, pages, heads, d, page, G, k, v, in_dtype, k_token, k_head, v_token, v_head, slots, T, false,
+                            static_cast<cudaStream_t>(stream));
 }
 
 CONVROT_API int ck_mx4_cache_read(const void* codes, const void* scales, long long pages, int heads, int d, int page, int G,

@@ -75,14 +75,14 @@ template <typename T, int D, int G>
 __global__ void __launch_bounds__(kMx4QuantWarps * 32, 3)
 mx4_cache_append_kernel(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const T* __restrict__ k,
                         const T* __restrict__ v, long long kst, long long ksh, long long vst, long long vsh,
-                        const long long* __restrict__ slots, int units, Mx4CacheShape c, bool vec, bool linear) {
+                        const long long* __restrict__ slots, int first_unit, int units, Mx4CacheShape c, bool vec, bool linear) {
     using S = Mx4Slab<T>;
     extern __shared__ __align__(128) unsigned char mx4slabs[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned char* slab = mx4slabs + warp * 2 * S::kBytes;
     const int per = mx4_cache_units<D>(c.heads);
     const int step = static_cast<int>(gridDim.x) * kMx4QuantWarps * 32;
-    int base = (static_cast<int>(blockIdx.x) * kMx4QuantWarps + warp) * 32;
+    int base = first_unit + (static_cast<int>(blockIdx.x) * kMx4QuantWarps + warp) * 32;          // (units / 2: values alone)
     auto load = [&](unsigned char* to, int first) {
         const int u = first + lane;
         if (linear && first + 32 <= units && (first + 32 <= units / 2 || first >= units / 2)) {

@@ -18,7 +18,7 @@ struct Mx4AppendRope {
     const long long* slots;
     uint8_t *codes, *scales;
     int tokens, hq, units;                         // units of the keys
-    int size, kv_tasks, tasks;                     // units of a task, tasks of the keys (and of the values), of all
+    int size, k_tasks, v_tasks, tasks;             // units of a task, tasks of the keys, of the values, of all
 };
 
 // Lays item `item`'s channels [c, c + VP) into the slab of 32 fp32 units.
@@ -46,8 +46,8 @@ mx4_cache_append_rope_kernel(const __grid_constant__ Mx4AppendRope a, Mx4CacheSh
     griddep_wait();
     griddep_launch_dependents();
     if (task >= a.tasks) return;
-    const int kind = task >= 2 * a.kv_tasks ? 2 : task >= a.kv_tasks;             // keys, values, queries
-    const int base = (task - kind * a.kv_tasks) * a.size;         // the first unit
+    const int kind = task < a.k_tasks ? 0 : task < a.k_tasks + a.v_tasks ? 1 : 2;  // keys, values, queries
+    const int base = (task - (kind > 0 ? a.k_tasks : 0) - (kind > 1 ? a.v_tasks : 0)) * a.size;      // the first unit
     const T* src = static_cast<const T*>(kind == 0 ? a.k : kind == 1 ? a.v : a.q);
     const long long st = kind == 0 ? a.kst : kind == 1 ? a.vst : a.qst, sh = kind == 0 ? a.ksh : kind == 1 ? a.vsh : a.qsh;
     // heads of a token, and with the missing one of heads of 64 whose last unit is half

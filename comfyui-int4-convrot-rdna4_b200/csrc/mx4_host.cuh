@@ -87,4 +87,9 @@ inline int check_cache(const void* codes, const void* scales, long long pages, i
     return 0;
 }
 
+// Keys and values [T, heads, d] to their slots (mx4.cu), or the values alone; arguments checked by the caller.
+int run_cache_append(void* codes, void* scales, long long pages, int heads, int d, int page, int G, const void* k, const void* v, int in_dtype,
+                     long long k_token, long long k_head, long long v_token, long long v_head, const void* slots, int T, bool values_only,
+                     cudaStream_t stream);
+
 }  // namespace convrot

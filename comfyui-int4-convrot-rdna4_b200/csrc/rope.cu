@@ -112,7 +112,8 @@ CONVROT_API int ck_mx4_cache_append_rope(void* codes, void* scales, long long pa
         using E = std::remove_pointer_t<decltype(t)>;
         return with_head(d, G, [&](auto dim, auto g) {
             constexpr int D = decltype(dim)::value;
-            const long long units = static_cast<long long>(T) * mx4_cache_units<D>(heads), q_items = static_cast<long long>(T) * q_heads;
+            const long long units = static_cast<long long>(T) * mx4_cache_units<D>(heads);
+            long long q_items = static_cast<long long>(T) * q_heads;
             if (2 * units > kMx4MostUnits || q_items > 0x7FFFFFFFll - 4096) return fail("too many tokens in one call");
             Mx4AppendRope a{};
             a.q = q;
@@ -126,19 +127,33 @@ CONVROT_API int ck_mx4_cache_append_rope(void* codes, void* scales, long long pa
             a.tokens = T;
             a.hq = q_heads;
             a.units = static_cast<int>(units);
-            // few tokens: smaller tasks, so that every warp has little to do
+            // Few tokens: one launch, in small tasks, so that every warp has little to do (7 tokens of 32 query heads
+            // on 8 of 128: 5.5 us; queries apart 9). Many: queries and values by the kernels that do nothing
+            // else, which hold more loads (32768 tokens: 164 us; in one launch 178).
+            const bool apart = (2 * units + q_items * D / 128) / 32 > 64LL * sm_count();
+            cudaStream_t st = static_cast<cudaStream_t>(stream);
+            if (apart && q_items) {
+                const RopeShape shape{0, q_token, q_head, T, T, q_heads, D, 0, 0, 0};
+                const bool wide = aligned16(q) && aligned16(q_out) && whole_chunks(r, d, sizeof(E), q_token | q_head);
+                const int rc = wide ? launch_rope<E, 16 / sizeof(E)>(q, q_out, shape, r, st) : launch_rope<E, 1>(q, q_out, shape, r, st);
+                if (rc) return rc;
+                q_items = 0;
+            }
+            if (apart)
+                if (int rc = run_cache_append(codes, scales, pages, heads, d, page, G, v, v, dtype, v_token, v_head, v_token, v_head, slots, T, true, st)) return rc;
             int size = 32;
             while (size > 8 && (2 * units + q_items * D / 128) / size < 4LL * sm_count()) size /= 2;
             a.size = size;
-            a.kv_tasks = static_cast<int>((units + size - 1) / size);
-            a.tasks = 2 * a.kv_tasks + static_cast<int>((q_items * D + 128 * size - 1) / (128 * size));
-            const long long strides = k_token | k_head | v_token | v_head | (q_heads ? q_token | q_head : 0);
-            const bool wide = aligned16(k) && aligned16(v) && (!q_heads || (aligned16(q) && aligned16(q_out))) && whole_chunks(r, d, sizeof(E), strides);
+            a.k_tasks = static_cast<int>((units + size - 1) / size);
+            a.v_tasks = apart ? 0 : a.k_tasks;
+            a.tasks = a.k_tasks + a.v_tasks + static_cast<int>((q_items * D + 128 * size - 1) / (128 * size));
+            const long long strides = k_token | k_head | v_token | v_head | (q_items ? q_token | q_head : 0);
+            const bool wide = aligned16(k) && aligned16(v) && (!q_items || (aligned16(q) && aligned16(q_out))) && whole_chunks(r, d, sizeof(E), strides);
             const int smem = kMx4QuantWarps * Mx4Slab<float>::kBytes, blocks = (a.tasks + kMx4QuantWarps - 1) / kMx4QuantWarps;
             auto launch = [&](auto kernel) {
                 cudaError_t e = ensure_smem(kernel, smem);
                 if (e != cudaSuccess) return static_cast<int>(e);
-                return static_cast<int>(launch_pdl(kernel, dim3(blocks), dim3(kMx4QuantWarps * 32), smem, static_cast<cudaStream_t>(stream), a, c, r));
+                return static_cast<int>(launch_pdl(kernel, dim3(blocks), dim3(kMx4QuantWarps * 32), smem, st, a, c, r));
             };
             if (wide) return launch(mx4_cache_append_rope_kernel<E, D, decltype(g)::value, 16 / sizeof(E)>);
             return launch(mx4_cache_append_rope_kernel<E, D, decltype(g)::value, 1>);

@@ -5,10 +5,11 @@
 // channels behind the 2P first stay as they are. The pairs are cut into sections, one an
 // axis (text: one; images and video: index, height, width).
 //
-// The angle is taken in turns and in 64 bits, t = p (f / 2 pi), and only its fraction
-// t - round(t) goes to fp32: at position 10^6 an fp32 product would be 0.06 radians
-// off, this is 2^-24 turns off wherever the token stands. (64-bit products run at half
-// the fp32 rate here, and a token's angles serve all of its heads.)
+// The angle p f and its sine and cosine are taken in 64 bits and rounded once: at position 10^6 an
+// fp32 product would be 0.06 radians off. (64-bit products run at half the fp32 rate here, some 25 a
+// pair, and a token's angles serve all of its heads.) Products and sums of the turn are fp32 operations
+// each of its own: the values are those of the formula computed step by step in fp32, which matters
+// where they are quantized to 4 bits afterwards.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -73,6 +74,30 @@ struct RopePlace {
     __device__ __forceinline__ bool any() const { return pair >= 0 || pair_b >= 0; }
 };
 
+// Sine and cosine of a (radians, finite and below some 2^50 in magnitude), rounded to fp32: reduced to
+// |x| <= pi / 4 around a quarter turn with 1 / (2 pi) in two terms, then the Taylor polynomials of degree 13
+// and 14, whose remainders are below 2 * 10^-14.
+__device__ __forceinline__ void rope_sincos(double a, float& s, float& c) {
+    const double hi = a * 0.15915494309189535, lo = fma(a, 0.15915494309189535, -hi) + a * -9.839338337591243e-18;
+    const double r = (hi - rint(hi)) + lo, q = rint(4.0 * r), x = fma(-0.25, q, r) * 6.283185307179586, y = x * x;
+    double u = fma(y, 1.0 / 6227020800.0, -1.0 / 39916800.0), v = fma(y, -1.0 / 87178291200.0, 1.0 / 479001600.0);
+    u = fma(u, y, 1.0 / 362880.0);
+    v = fma(v, y, -1.0 / 3628800.0);
+    u = fma(u, y, -1.0 / 5040.0);
+    v = fma(v, y, 1.0 / 40320.0);
+    u = fma(u, y, 1.0 / 120.0);
+    v = fma(v, y, -1.0 / 720.0);
+    u = fma(u, y, -1.0 / 6.0);
+    v = fma(v, y, 1.0 / 24.0);
+    v = fma(v, y, -0.5);
+    const float sx = static_cast<float>(fma(u * y, x, x)), cx = static_cast<float>(fma(v, y, 1.0));
+    const int quarter = static_cast<int>(q);                      // -2 .. 2
+    s = quarter & 1 ? cx : sx;
+    c = quarter & 1 ? sx : cx;
+    if (quarter & 2) s = -s;
+    if ((quarter + 1) & 2) c = -c;
+}
+
 // Cosine and sine of a thread's pairs, those of chunk a's first where they are interleaved.
 template <int VP>
 struct RopeCoef {
@@ -91,8 +116,7 @@ struct RopeCoef {
                 end = axis < r.axes - 1 ? r.ends[axis] : 0x7FFFFFFF;
                 p = r.position(b, t, axis);
             }
-            const double turns = p * (r.freqs[pair + i] * 0.15915494309189533577);
-            sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s[FROM + i], &c[FROM + i]);
+            rope_sincos(p * r.freqs[pair + i], s[FROM + i], c[FROM + i]);
             s[FROM + i] *= r.sign;
         }
     }
@@ -112,22 +136,20 @@ struct RopeCoef {
 
 template <int VP>
 __device__ __forceinline__ void rope_turn(float (&a)[VP], float (&b)[VP], const RopeCoef<VP>& w, bool interleaved) {
+    auto turn = [](float& x, float& y, float c, float s) {
+        const float z = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+        y = __fadd_rn(__fmul_rn(x, s), __fmul_rn(y, c));
+        x = z;
+    };
     if (VP > 1 && interleaved) {
         #pragma unroll
         for (int i = 0; i + 1 < VP; i += 2) {
-            const float x = a[i], y = a[i + 1], z = b[i], t = b[i + 1];
-            a[i] = fmaf(x, w.c[i / 2], -y * w.s[i / 2]);
-            a[i + 1] = fmaf(x, w.s[i / 2], y * w.c[i / 2]);
-            b[i] = fmaf(z, w.c[(VP + i) / 2], -t * w.s[(VP + i) / 2]);
-            b[i + 1] = fmaf(z, w.s[(VP + i) / 2], t * w.c[(VP + i) / 2]);
+            turn(a[i], a[i + 1], w.c[i / 2], w.s[i / 2]);
+            turn(b[i], b[i + 1], w.c[(VP + i) / 2], w.s[(VP + i) / 2]);
         }
     } else {
         #pragma unroll
-        for (int i = 0; i < VP; ++i) {
-            const float x = a[i], y = b[i];
-            a[i] = fmaf(x, w.c[i], -y * w.s[i]);
-            b[i] = fmaf(x, w.s[i], y * w.c[i]);
-        }
+        for (int i = 0; i < VP; ++i) turn(a[i], b[i], w.c[i], w.s[i]);
     }
 }
 

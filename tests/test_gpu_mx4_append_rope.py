@@ -3,7 +3,7 @@
 Keys go through the fp32 steps of ``apply_rope`` and then those of ``convrot_mx4_cache_append``, so their
 codes are those of the two calls on float32 tensors, bit for bit, and values those of the plain append.
 Against 64 bits a code may differ only where the value lies within the steps' rounding error of a
-midpoint: (|a| + |b|) 2^-21 from the positions and 12 roundings of 2^-24 of the group's magnitudes.
+midpoint: (|a| + |b|) 2^-22 from the positions and 12 roundings of 2^-24 of the group's magnitudes.
 """
 import numpy as np
 import pytest
@@ -36,7 +36,8 @@ CASES = [  # tokens, hq, hkv, D, page, group, sections, interleaved
     (1, 4, 1, 64, 16, 64, (32,), False), (1, 0, 1, 128, 16, 0, (64,), True), (7, 32, 8, 128, 16, 64, (64,), False),
     (33, 6, 3, 64, 32, 16, (8, 12, 12), False), (5, 2, 2, 256, 64, 256, (128,), False), (65, 3, 1, 256, 16, 64, (64,), True),
     (130, 5, 5, 64, 1, 0, (13,), False), (19, 8, 4, 128, 128, 64, (8, 28, 28), True), (300, 1, 1, 128, 64, 16, (32,), False),
-    (12, 14, 7, 128, 16, 64, (3, 5), True), (257, 24, 8, 64, 16, 64, (16,), True), (40, 9, 3, 256, 32, 0, (20, 44, 64), False)]
+    (12, 14, 7, 128, 16, 64, (3, 5), True), (257, 24, 8, 64, 16, 64, (16,), True), (40, 9, 3, 256, 32, 0, (20, 44, 64), False),
+    (4001, 32, 8, 128, 64, 64, (64,), False), (5003, 15, 5, 64, 16, 16, (13,), False), (2049, 0, 8, 256, 128, 256, (16, 56, 56), True)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])

@@ -1,10 +1,9 @@
 """GPU tests of the rotary positions against the definition in 64 bits.
 
-Tolerance. The fraction of the angle goes to fp32 (2^-25 of a half turn, 2^-23.3 radians), sine and
-cosine are off by 2 units at most (2^-22), the two products and the sum by 2^-24 each: an output is
-off by (|a| + |b|) 2^-21 at most for a pair (a, b), then by half a step of its type. In 64 bits an angle
-A itself carries four roundings of 2^-53: the frequency over 2 pi, that constant, the product, and
-the reference's own product. They count from positions of some 2^30 on: (|a| + |b|) |A| 2^-51.
+Tolerance. Sine and cosine are rounded to fp32 (2^-25), the two products and their sum by 2^-24 each: an
+output is off by (|a| + |b|) 2^-22 at most for a pair (a, b), then by half a step of its type. In 64 bits
+an angle A itself carries the product's rounding here and in the reference, 2^-53 each, which counts
+from positions of some 2^30 on: (|a| + |b|) |A| 2^-51.
 """
 import pytest
 import torch
@@ -39,7 +38,7 @@ def turned64(x, positions, freqs, sections, interleaved, inverse):
             angle = (p[..., axis] * f[i] * (-1 if inverse else 1))[..., None]
             out[..., a] = x[..., a] * angle.cos() - x[..., b] * angle.sin()
             out[..., b] = x[..., a] * angle.sin() + x[..., b] * angle.cos()
-            size[..., a] = size[..., b] = (x[..., a].abs() + x[..., b].abs()) * (2.0 ** -21 + angle.abs() * 2.0 ** -51)
+            size[..., a] = size[..., b] = (x[..., a].abs() + x[..., b].abs()) * (2.0 ** -22 + angle.abs() * 2.0 ** -51)
             i += 1
     return out, size
 
