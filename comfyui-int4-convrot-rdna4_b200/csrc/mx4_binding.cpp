@@ -433,10 +433,10 @@ PyObject* cache_append_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         q = tensor(a[2], "q");
         TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == t && q.size(2) == c.d && q.scalar_type() == k.scalar_type(), "queries ", q.sizes(),
                           " must be [", t, ", heads, ", c.d, "] in the keys' dtype");
-        on_device(q, codes.device());
     }
     Rope r = rope_of(k.sizes().slice(0, 1), c.d, a[6], a[7], a[8], a[9]);
     for (const Tensor* x : std::initializer_list<const Tensor*>{&codes, &scales, &k, &v, &slots, &r.positions, &r.freqs}) on_device(*x, codes.device());
+    if (q.defined()) on_device(q, codes.device());
     const c10::cuda::CUDAGuard guard(codes.device());
     if (k.stride(2) != 1) k = k.contiguous();
     if (v.stride(2) != 1) v = v.contiguous();
@@ -476,10 +476,10 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         nodes = tensor(a[6], "tree_lens");
         TORCH_CHECK_VALUE(nodes.scalar_type() == at::kInt && nodes.dim() == 1 && nodes.size(0) == b && nodes.is_contiguous(),
                           "tree_lens must be a contiguous int32 vector [B]");
-        on_device(nodes, codes.device());
     }
     const double scale = scale_of(a[7], c);
     for (const Tensor* x : std::initializer_list<const Tensor*>{&q, &codes, &scales, &table, &lens, &mask}) on_device(*x, codes.device());
+    if (nodes.defined()) on_device(nodes, codes.device());
     const c10::cuda::CUDAGuard guard(codes.device());
     if (q.stride(3) != 1) q = q.contiguous();
     if (mask.stride(-1) != 1 && t > 1) mask = mask.contiguous();
@@ -516,16 +516,12 @@ PyObject* linear_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int code = dtype_code(x.scalar_type());
     const double eps = PyFloat_AsDouble(a[6]);
     if (eps == -1.0 && PyErr_Occurred()) return nullptr;
-    on_device(x, x.device());
-    on_device(w, x.device());
-    on_device(ws, x.device());
     auto vector = [&](PyObject* o, const char* what, int64_t size) {
         Tensor v;
         if (o == Py_None) return v;
         v = tensor(o, what);
         TORCH_CHECK_VALUE(v.dim() == 1 && v.size(0) == size && code_of(v.scalar_type()) >= 0, what, " must be [", size,
                           "] in float32, bfloat16 or float16");
-        on_device(v, x.device());
         return v;
     };
     bias = vector(a[3], "bias", outs);
@@ -534,8 +530,9 @@ PyObject* linear_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         residual = tensor(a[5], "residual");
         TORCH_CHECK_VALUE(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type(), "residual ", residual.sizes(),
                           " must have the shape and dtype of x ", x.sizes());
-        on_device(residual, x.device());
     }
+    for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &w, &ws, &bias, &gain, &residual})
+        if (t->defined()) on_device(*t, x.device());
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor m = rows_of(x);
     w = w.contiguous();
