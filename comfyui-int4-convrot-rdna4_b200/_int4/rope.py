@@ -36,4 +36,4 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, se
     leading sizes a copy is made where they are not one stride); q and k as heads of one
     tensor take one launch.
     """
-    return mx4.native().rope(x, positions, freqs, sections, interleaved, inverse)
+    return (mx4._native or mx4.native()).rope(x, positions, freqs, sections, interleaved, inverse)

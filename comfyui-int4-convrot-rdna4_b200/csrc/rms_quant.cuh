@@ -214,19 +214,25 @@ template <int NT, typename T>
 __global__ void __launch_bounds__(512)
 few_i8_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, const float* __restrict__ xs, const float* __restrict__ ws,
               BiasRef bias, T* __restrict__ out, int M, int N, int K) {
-    constexpr int kAhead = 4;                                     // segments of 64 columns on their way
+    constexpr int kAhead = 2;                                     // segments of 128 columns on their way
     extern __shared__ int few_sums[];                             // [warp][row][17]
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n0 = static_cast<int>(blockIdx.x) * 16;
-    const int segs = (K + 63) / 64, per = (segs + warps - 1) / warps;
+    const int segs = (K + 127) / 128, per = (segs + warps - 1) / warps;
     const int s0 = min(segs, warp * per), s1 = min(segs, s0 + per);
-    const int8_t* row0 = w + static_cast<size_t>(min(n0 + g, N - 1)) * K + 16 * t;
-    const int8_t* row1 = w + static_cast<size_t>(min(n0 + g + 8, N - 1)) * K + 16 * t;
-    uint4 a[kAhead][2];
-    auto load_w = [&](int s, uint4 (&to)[2]) {
-        const bool held = s < s1 && 64 * s + 16 * t < K;
-        to[0] = held ? __ldg(reinterpret_cast<const uint4*>(row0 + 64 * s)) : make_uint4(0, 0, 0, 0);
-        to[1] = held ? __ldg(reinterpret_cast<const uint4*>(row1 + 64 * s)) : make_uint4(0, 0, 0, 0);
+    // (a thread's 32 bytes of a segment, so that four threads ask for a whole line of a row)
+    const int8_t* row0 = w + static_cast<size_t>(min(n0 + g, N - 1)) * K + 32 * t;
+    const int8_t* row1 = w + static_cast<size_t>(min(n0 + g + 8, N - 1)) * K + 32 * t;
+    uint4 a[kAhead][2][2];
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    auto load_w = [&](int s, uint4 (&to)[2][2]) {
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = 128 * s + 16 * h;
+            const bool held = s < s1 && at + 32 * t < K;
+            to[h][0] = held ? __ldg(reinterpret_cast<const uint4*>(row0 + at)) : zero;
+            to[h][1] = held ? __ldg(reinterpret_cast<const uint4*>(row1 + at)) : zero;
+        }
     };
     #pragma unroll
     for (int i = 0; i < kAhead; ++i) load_w(s0 + i, a[i]);
@@ -235,20 +241,23 @@ few_i8_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, const 
     int d[NT][4] = {};
     const int8_t* xr[NT];
     #pragma unroll
-    for (int k = 0; k < NT; ++k) xr[k] = x + static_cast<size_t>(min(8 * k + g, M - 1)) * K + 16 * t;
+    for (int k = 0; k < NT; ++k) xr[k] = x + static_cast<size_t>(min(8 * k + g, M - 1)) * K + 32 * t;
     #pragma unroll 1
     for (int s = s0; s < s1; s += kAhead) {
         #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             if (s + i < s1) {
-                const uint4 lo = a[i][0], hi = a[i][1];
-                const bool held = 64 * (s + i) + 16 * t < K;
                 #pragma unroll
-                for (int k = 0; k < NT; ++k) {
-                    // (the rows' codes come from the kernel before: no read-only loads)
-                    const uint4 b = held ? *reinterpret_cast<const uint4*>(xr[k] + 64 * (s + i)) : make_uint4(0, 0, 0, 0);
-                    mma_s8(d[k], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
-                    mma_s8(d[k], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 lo = a[i][h][0], hi = a[i][h][1];
+                    const int at = 128 * (s + i) + 16 * h;
+                    #pragma unroll
+                    for (int k = 0; k < NT; ++k) {
+                        // (the rows' codes come from the kernel before: no read-only loads)
+                        const uint4 b = at + 32 * t < K ? *reinterpret_cast<const uint4*>(xr[k] + at) : zero;
+                        mma_s8(d[k], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+                        mma_s8(d[k], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+                    }
                 }
                 load_w(s + i + kAhead, a[i]);
             }
