@@ -194,17 +194,27 @@ class Mx4SelfAttention(torch.nn.Module):
         y = self.qkv(x).unflatten(-1, (self.heads + 2 * self.kv_heads, self.head_dim))
         return y.split((self.heads, self.kv_heads, self.kv_heads), dim=-2)
 
-    def _positions(self, positions: torch.Tensor | None, tokens: int) -> torch.Tensor | None:
-        """The tokens' positions as the cache takes them; ValueError where they do not fit the block."""
+    def _apply(self, fn, recurse=True):
+        freqs = self.freqs                                        # (64 bits also where the block is cast)
+        super()._apply(fn, recurse)
+        if freqs is not None and self.freqs.dtype != freqs.dtype:
+            self.freqs = freqs.to(self.freqs.device)
+        return self
+
+    def _positions(self, positions: torch.Tensor | None, *lead: int) -> torch.Tensor | None:
+        """The positions of tokens [*lead] as the cache takes them; ValueError where they do not fit the block."""
         if (positions is None) != (self.freqs is None):
             raise ValueError("a block with frequencies needs its tokens' positions" if positions is None
                              else "positions were given to a block without frequencies")
         if positions is None:
             return None
-        shape = (tokens,) if self.sections is None or len(self.sections) == 1 else (tokens, len(self.sections))
-        if positions.numel() != math.prod(shape) or positions.dtype not in (torch.int32, torch.int64, torch.float32):
-            raise ValueError(f"positions {tuple(positions.shape)} of {positions.dtype}: int32, int64 or float32 {shape} expected")
-        return positions.reshape(shape)
+        axes = () if self.sections is None or len(self.sections) == 1 else (len(self.sections),)
+        flat = (math.prod(lead), *axes)
+        if tuple(positions.shape) not in ((*lead, *axes), flat) or positions.dtype not in (torch.int32, torch.int64, torch.float32):
+            raise ValueError(f"positions {tuple(positions.shape)} of {positions.dtype}: int32, int64 or float32 {(*lead, *axes)} expected")
+        if positions.device != self.freqs.device:
+            raise ValueError(f"positions on {positions.device}, the block's frequencies on {self.freqs.device}")
+        return positions.reshape(flat)
 
     def _store(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Mx4KVCache, slots: torch.Tensor,
                positions: torch.Tensor | None) -> torch.Tensor:
@@ -224,12 +234,12 @@ class Mx4SelfAttention(torch.nn.Module):
         tree_mask (and tree_lens) the tokens are a tree's nodes, as in
         ``convrot_mx4_tree_attention``; slots of padding behind them are -1."""
         b, t, _ = x.shape
-        positions = self._positions(positions, b * t)
+        if tree_lens is not None and tree_mask is None:
+            raise ValueError("tree_lens were given without a tree_mask")
+        positions = self._positions(positions, b, t)
         q = self._store(*self.project(x.flatten(0, 1)), cache, slots, positions).unflatten(0, (b, t))
         if tree_mask is not None:
             y = cache.attend_tree(q, block_table, seq_lens, tree_mask, tree_lens)
-        elif tree_lens is not None:
-            raise ValueError("tree_lens were given without a tree_mask")
         else:
             y = cache.attend(q, block_table, seq_lens)
         return self.out(y.reshape(b, t, self.heads * self.head_dim))

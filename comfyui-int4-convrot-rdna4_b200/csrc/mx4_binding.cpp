@@ -403,8 +403,11 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(x.device());
     Tensor out = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
     if (x.dim() > 4) {                                            // [B, T, heads, D], by a copy where strides do not allow a view
-        r.positions = r.positions.reshape(r.axes > 1 ? at::DimVector{-1, x.size(-3), r.axes} : at::DimVector{-1, x.size(-3)});
-        x = x.reshape({-1, x.size(-3), heads, d});
+        const int64_t t = x.size(-3);
+        int64_t b = 1;
+        for (int64_t i = 0; i < x.dim() - 3; ++i) b *= x.size(i);
+        r.positions = r.positions.reshape(r.axes > 1 ? at::DimVector{b, t, r.axes} : at::DimVector{b, t});
+        x = x.reshape({b, t, heads, d});
     }
     if (x.stride(-1) != 1) x = x.contiguous();
     r.freqs = r.freqs.contiguous();

@@ -7,6 +7,11 @@
 // each lane then has one, as in the append without positions: the same codes for the same
 // fp32 values. A lane's chunk stays the same from head to head, so a token's angles are
 // computed once for all of its heads.
+//
+// 32768 tokens of 8 heads of 128 in bf16, keys alone: 52 us (2.9 TB/s; issue 54 % of the cycles: angles,
+// the turn, the rotation and the codes); 7 tokens of 32 query heads on 8: 5.5 us in a graph, one
+// task's latency. Blocks are not kept for several tasks: a wave that counts on three blocks a
+// multiprocessor has fewer where it starts under the kernel before it.
 #pragma once
 
 namespace convrot {

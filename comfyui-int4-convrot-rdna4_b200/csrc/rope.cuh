@@ -10,6 +10,11 @@
 // pair, and a token's angles serve all of its heads.) Products and sums of the turn are fp32 operations
 // each of its own: the values are those of the formula computed step by step in fp32, which matters
 // where they are quantized to 4 bits afterwards.
+//
+// Bound by its bytes where it is large: 4608 tokens of 60 heads of 128 in bf16 take 27.9 us, 5.1 TB/s
+// (a copy of the tensor 28.7). A thread keeps a token's angles for as many heads as leave one wave of
+// blocks, four heads' loads ahead; one head a thread took 37.5 us, most of it for angles. One token
+// of 40 heads is a launch (2.9 us in a graph).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -188,3 +188,21 @@ def test_block_positions_that_do_not_fit():
             block.prefill(torch.zeros(5, 64), cache, seq, given)
         assert cache.length(seq) == 0
     assert "freqs" not in turned.state_dict()
+
+
+def test_block_positions_of_other_orders_and_a_cast_block():
+    freqs = _int4.rope_freqs(32, device="cpu")
+    turned = Mx4SelfAttention(64, 2, 1, 64, device="cpu", freqs=freqs)
+    axes = Mx4SelfAttention(64, 2, 1, 64, device="cpu", freqs=freqs, sections=(8, 24))
+    assert torch.equal(turned._positions(torch.arange(6).view(2, 3), 2, 3), torch.arange(6))
+    assert axes._positions(torch.zeros(2, 3, 2), 2, 3).shape == (6, 2) and axes._positions(torch.zeros(6, 2), 2, 3).shape == (6, 2)
+    # as many numbers, but not in the tokens' order
+    for block, bad in ((turned, torch.zeros(3, 2)), (axes, torch.zeros(2, 6)), (axes, torch.zeros(2, 2, 3)), (axes, torch.zeros(12))):
+        with pytest.raises(ValueError, match="expected"):
+            block._positions(bad, 2, 3)
+    with pytest.raises(ValueError, match="frequencies on"):
+        turned._positions(torch.zeros(6, device="meta"), 2, 3)
+    for cast in (turned.half(), turned.to(torch.bfloat16), turned.float()):
+        assert cast.freqs.dtype == torch.float64 and torch.equal(cast.freqs, freqs)
+    with pytest.raises(ValueError, match="tree_mask"):            # (before anything is written)
+        turned(torch.zeros(1, 2, 64), None, None, None, None, torch.arange(2), tree_lens=torch.ones(1, dtype=torch.int32))

@@ -151,7 +151,7 @@ def test_special_values_streams_and_graphs(lib):
 
 def test_empty(lib):
     freqs = lib.rope_freqs(32)
-    for shape in ((0, 4, 64), (2, 0, 4, 64), (3, 0, 64)):
+    for shape in ((0, 4, 64), (2, 0, 4, 64), (3, 0, 64), (2, 3, 0, 4, 64), (0, 2, 3, 4, 64), (2, 3, 5, 0, 64)):
         assert lib.apply_rope(torch.empty(shape, device="cuda"), torch.zeros(shape[:-2], dtype=torch.int64, device="cuda"), freqs).shape == shape
     x = torch.randn(3, 2, 64, device="cuda")
     assert torch.equal(lib.apply_rope(x, torch.arange(3, device="cuda"), freqs[:0]), x)        # no pair is turned
