@@ -10,9 +10,10 @@
 // goes through rows, keeps its columns' g in registers and loads the next row's
 // values under the current one's work.
 //
-// 16384 x 3840 in bf16: 38 us, 5.0 TB/s; issue 67 % of the cycles (the rotation, two passes through
-// shared memory, the codes). The product behind it is the int8 GEMM of the other linears: with
-// 15360 outputs 853 us in all, where the product alone takes 690 by itself.
+// 16384 x 3840 in bf16: 64 us, 2.9 TB/s (a copy of the rows 41); the fp32 pipe, shared memory and issue are each
+// busy half to two thirds of the time, and a row's exchange and divisions leave 24 warps a
+// multiprocessor waiting in turns. Single operations instead of pairs, and codes by conversions, took 78; four
+// blocks a multiprocessor (64 registers) 73. The product behind it is the int8 GEMM of the other linears.
 #pragma once
 
 namespace convrot {
@@ -51,28 +52,54 @@ struct RmsRaw {
             memcpy(v, e, sizeof(e));
         }
     }
-    __device__ __forceinline__ void get(float (&f)[16]) const {
+    __device__ __forceinline__ void get(float2 (&f)[8]) const {
         T e[16];
         memcpy(e, v, sizeof(e));
         #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = mx4_to_f32(e[i]);
+        for (int i = 0; i < 8; ++i) f[i] = make_float2(mx4_to_f32(e[2 * i]), mx4_to_f32(e[2 * i + 1]));
     }
-    __device__ __forceinline__ void put(const float (&f)[16]) {
+    __device__ __forceinline__ void put(const float2 (&f)[8]) {
         T e[16];
         #pragma unroll
-        for (int i = 0; i < 16; ++i) e[i] = mx4_from_f32<T>(f[i]);
+        for (int i = 0; i < 8; ++i) {
+            e[2 * i] = mx4_from_f32<T>(f[i].x);
+            e[2 * i + 1] = mx4_from_f32<T>(f[i].y);
+        }
         memcpy(v, e, sizeof(e));
     }
 };
 
-// Steps at strides 1 and 4 of 16 values.
-__device__ __forceinline__ void rms_rotate16(float (&v)[16], bool second) {
+// Steps at strides 1 and 4 of 16 values in pairs (two fp32 operations an instruction). Value e is then
+// in place e ^ 3: a step at stride 1 gives its sums in reverse where it need not swap halves.
+__device__ __forceinline__ void rms_rotate16(float2 (&v)[8], bool second) {
+    const float2 less = make_float2(-2.0f, -2.0f);
     #pragma unroll
-    for (int i = 0; i < 16; i += 4) h4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    for (int i = 0; i < 8; i += 2) {
+        const float2 t = fadd2_rn(v[i], v[i + 1]);
+        const float2 sum = make_float2(t.x + t.y, t.x + t.y);
+        v[i] = ffma2_rn(less, v[i], sum);
+        v[i + 1] = ffma2_rn(less, v[i + 1], sum);
+    }
     if (second) {
         #pragma unroll
-        for (int i = 0; i < 4; ++i) h4(v[i], v[i + 4], v[i + 8], v[i + 12]);
+        for (int i = 0; i < 2; ++i) {
+            const float2 sum = fadd2_rn(fadd2_rn(v[i], v[i + 2]), fadd2_rn(v[i + 4], v[i + 6]));
+            const float2 w0 = ffma2_rn(less, v[i + 6], sum), w1 = ffma2_rn(less, v[i + 4], sum), w2 = ffma2_rn(less, v[i + 2], sum);
+            v[i + 6] = ffma2_rn(less, v[i], sum);
+            v[i] = w0;
+            v[i + 2] = w1;
+            v[i + 4] = w2;
+        }
     }
+}
+
+// The sum of `ss` and the largest `amax` (NaN above all; neither is negative) over the lanes
+// that differ in the bits below WIDTH, and of `amax` over the warp.
+template <int WIDTH>
+__device__ __forceinline__ void rms_reduce(float& ss, float& amax) {
+    amax = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax)));
+    #pragma unroll
+    for (int z = WIDTH / 2; z; z >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, z);
 }
 
 // THREADS: 256 (rows up to 4096 columns) or 1024.
@@ -95,9 +122,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
         if (a.r) r.load(static_cast<const T*>(a.r) + (held ? at * a.ldr + col : 0), held, a.vec_r);
     };
     load(row);
-    float g[16];
+    float2 g[8];
     #pragma unroll
-    for (int i = 0; i < 16; ++i) g[i] = 1.0f;
+    for (int i = 0; i < 8; ++i) g[i] = make_float2(1.0f, 1.0f);
     if (a.g) {
         auto gains = [&](auto* p) {
             RmsRaw<std::remove_const_t<std::remove_pointer_t<decltype(p)>>> raw;
@@ -108,15 +135,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
         else if (a.g_type == 1) gains(static_cast<const __nv_bfloat16*>(a.g));
         else gains(static_cast<const __half*>(a.g));
     }
+    const float per_k = 1.0f / static_cast<float>(a.K);
     // (every warp of the block makes as many rounds: they meet at barriers)
     for (int row0 = static_cast<int>(blockIdx.x) * a.rows, round = 0; row0 < a.M; row0 += static_cast<int>(gridDim.x) * a.rows, ++round) {
-        float v[16];
+        float2 v[8];
         x.get(v);
         if (a.r) {
-            float w[16];
+            float2 w[8];
             r.get(w);
             #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = __fadd_rn(v[i], w[i]);
+            for (int i = 0; i < 8; ++i) v[i] = fadd2_rn(v[i], w[i]);
             if (column && row < a.M) {
                 RmsRaw<T> o;
                 o.put(v);
@@ -128,12 +156,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
         const int now = row;
         row += static_cast<int>(gridDim.x) * a.rows;
         load(row);
-        float ss = 0.0f, amax = 0.0f;
+        float2 squares = make_float2(0.0f, 0.0f);
         #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            ss = fmaf(v[i], v[i], ss);
-            v[i] *= g[i];
+        for (int i = 0; i < 8; ++i) {
+            squares = ffma2_rn(v[i], v[i], squares);
+            v[i] = fmul2_rn(v[i], g[i]);
         }
+        float ss = squares.x + squares.y, amax = 0.0f;
         rms_rotate16(v, true);
         if constexpr (G >= 64) {
             // value 16 l + i of a group (of its thread l) lies in row l, its chunks of four XORed: neither
@@ -141,54 +170,54 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
             float* base = mine + group * (256 + 16);
             #pragma unroll
             for (int c = 0; c < 4; ++c)
-                *reinterpret_cast<float4*>(base + j * 16 + ((c ^ (j >> 1 & 3)) << 2)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                *reinterpret_cast<float4*>(base + j * 16 + ((c ^ (j >> 1 & 3)) << 2)) = make_float4(v[2 * c].x, v[2 * c].y, v[2 * c + 1].x, v[2 * c + 1].y);
             __syncwarp();
+            const float* from = base + (j & 3 ^ 3);
             #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = base[i * 16 + (((j >> 2) ^ (i >> 1 & 3)) << 2) + (j & 3)];
+            for (int i = 0; i < 8; ++i)
+                v[i] = make_float2(from[2 * i * 16 + (((j >> 2) ^ (i & 3)) << 2)], from[(2 * i + 1) * 16 + (((j >> 2) ^ (i & 3)) << 2)]);
             rms_rotate16(v, G == 256);
         }
         #pragma unroll
-        for (int i = 0; i < 16; i += 2) amax = max3_abs_nan(amax, v[i], v[i + 1]);
-        #pragma unroll
-        for (int z = 16; z; z >>= 1) {
-            ss += __shfl_xor_sync(0xFFFFFFFFu, ss, z);
-            amax = max3_abs_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, z), 0.0f);
-        }
+        for (int i = 0; i < 8; ++i) amax = max3_abs_nan(amax, v[i].x, v[i].y);
+        rms_reduce<32>(ss, amax);
         if (a.row_warps > 1) {
+            constexpr int kMost = THREADS / 32;                   // warps of a row
             float2* p = part[round & 1];
             if (lane == 0) p[warp] = make_float2(ss, amax);
             __syncthreads();
-            const float2 y = lane < a.row_warps ? p[warp - in_row + lane] : make_float2(0.0f, 0.0f);
+            const float2 y = lane % kMost < a.row_warps ? p[warp - in_row + lane % kMost] : make_float2(0.0f, 0.0f);
             ss = y.x;
             amax = y.y;
-            #pragma unroll
-            for (int z = 16; z; z >>= 1) {
-                ss += __shfl_xor_sync(0xFFFFFFFFu, ss, z);
-                amax = max3_abs_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, z), 0.0f);
-            }
+            rms_reduce<kMost>(ss, amax);
         }
-        const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.K) + a.eps);
+        const float rstd = 1.0f / sqrtf(fmaf(ss, per_k, a.eps));
         const float y = amax * unit_factor<G>() * rstd;
         const float s = (y < 1e-10f ? 1e-10f : y) / 127.0f;       // (NaN stays)
-        const float f = unit_factor<G>() * rstd / s;
+        // |v f| is 127 and roundings at most: a sum with 1.5 * 2^23 has the code in its last byte. (f finite: 0 stays 0)
+        const float f = fminf(unit_factor<G>() * rstd / s, 3.4e38f);
+        const float2 by = make_float2(f, f), shift = make_float2(12582912.0f, 12582912.0f);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = ffma2_rn(v[i], by, shift);
         uint32_t out[4];
         if constexpr (G >= 64) {
             __syncwarp();
-            unsigned char* bytes = reinterpret_cast<unsigned char*>(mine);
+            unsigned char* bytes = reinterpret_cast<unsigned char*>(mine) + group * (256 + 16);
             #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                bytes[group * 256 + i * 16 + j] = static_cast<unsigned char>(max(-127, min(127, __float2int_rn(v[i] * f))));
+            for (int i = 0; i < 8; ++i) {                         // (places 2i and 2i + 1: values 2i ^ 3 and 2i ^ 2)
+                bytes[(2 * i ^ 3) * 16 + j] = static_cast<unsigned char>(__float_as_uint(v[i].x));
+                bytes[(2 * i ^ 2) * 16 + j] = static_cast<unsigned char>(__float_as_uint(v[i].y));
+            }
             __syncwarp();
-            const uint4 o = *reinterpret_cast<const uint4*>(bytes + lane * 16);
+            const uint4 o = *reinterpret_cast<const uint4*>(bytes + j * 16);
             out[0] = o.x; out[1] = o.y; out[2] = o.z; out[3] = o.w;
             __syncwarp();
         } else {
             #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                out[c] = 0;
-                #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    out[c] |= static_cast<uint32_t>(max(-127, min(127, __float2int_rn(v[4 * c + e] * f))) & 255) << (8 * e);
+                const uint32_t hi = __byte_perm(__float_as_uint(v[2 * c].x), __float_as_uint(v[2 * c].y), 0x0004);      // values 2, 3
+                const uint32_t lo = __byte_perm(__float_as_uint(v[2 * c + 1].x), __float_as_uint(v[2 * c + 1].y), 0x0004);
+                out[c] = __byte_perm(lo, hi, 0x5410);
             }
         }
         if (now < a.M) {
