@@ -83,7 +83,8 @@ int launch_tree(const Mx4AttnArgs& a, const AttnPlan& p, int vec_q, cudaStream_t
     auto kernel = mx4_tree_kernel<T, D, PAIR>;
     cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
-    e = launch_pdl(kernel, dim3(static_cast<unsigned>(p.tiles), p.splits), dim3(kTreeThreads), Cfg::kSmemBytes, stream, a, vec_q);
+    e = launch_pdl(kernel, dim3(static_cast<unsigned>(p.tiles), p.splits), dim3(kTreeThreads), Cfg::kSmemBytes, stream, a, vec_q,
+                   static_cast<int>(a.B > 1 && a.B <= kTreeThreads && p.tiles * p.splits > sm_count()));
     if (e == cudaSuccess && p.splits > 1) {
         const unsigned rows = static_cast<unsigned>(a.B * a.tq * a.hq);
         const int wide = p.splits > 16;

@@ -24,8 +24,8 @@
 // What bounds it: a stream's softmax (load, exp2, split, store: some 3500 cycles a tile, by the
 // latency of its 128 threads) takes turns with its own two products, and two streams a block
 // are what registers and tensor memory hold; a block starts in 3 to 9 us and ends in 6. 8 x 16384 tokens, 64
-// nodes of 64 query heads on 8 of 128: 467 us (1.18 PFLOP/s with both terms counted, 0.59 of the formula's;
-// tensor pipe 53 % of the active time, exp2's 27 %); 37 x 4096, 24 nodes of 24 on 8 of 64: 93 us.
+// nodes of 64 query heads on 8 of 128: 465 us (1.18 PFLOP/s with both terms counted, 0.59 of the formula's;
+// tensor pipe 53 % of the active time, exp2's 27 %); 37 x 4096, 24 nodes of 24 on 8 of 64: 76 us.
 // The kernel for few rows took 1820 and 277. Tiles in halves of 64 tokens: 541 and 103.
 #pragma once
 
@@ -144,7 +144,7 @@ __device__ __forceinline__ void tree_rotate(float (&v)[64], int group) {
 __device__ __forceinline__ float tree_factor(int group) { return group == 16 ? 0.25f : group == 64 ? 0.125f : 1.0f; }
 
 template <typename T, int D, bool PAIR>
-__global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a, int vec_q) {
+__global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a, int vec_q, int by_length) {
     using Cfg = Mx4TreeCfg<D, PAIR>;
     constexpr int kB = Cfg::kBlocks;
     extern __shared__ __align__(1024) unsigned char tree_smem_raw[];
@@ -158,14 +158,33 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
     int* nan_nodes = reinterpret_cast<int*>(tmem_slot + 1);       // a node's values hold a block of NaN
     float* row_scale = reinterpret_cast<float*>(smem + Cfg::kRowOffset);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int tile = blockIdx.x, split = blockIdx.y;
-    const int rt = tile % a.row_tiles, hk = tile / a.row_tiles % a.hkv, b = tile / a.row_tiles / a.hkv;
+    const int split = blockIdx.y;
+    const int rt = blockIdx.x % a.row_tiles, hk = blockIdx.x / a.row_tiles % a.hkv;
+    int b = blockIdx.x / a.row_tiles / a.hkv;
     const int per_head = a.hq / a.hkv, rows_all = a.tq * per_head;
     constexpr int kTileRows = PAIR ? 2 * kTreeTile : kTreeTile;
     const int row0 = rt * kTileRows, rows = min(kTileRows, rows_all - row0);
     griddep_wait();
     griddep_launch_dependents();
-    const int n = max(0, static_cast<int>(min(static_cast<long long>(a.lens[b]), a.cap)));
+    auto tokens_of = [&](int i) { return max(0, static_cast<int>(min(static_cast<long long>(a.lens[i]), a.cap))); };
+    if (by_length) {
+        // More blocks than multiprocessors: long sequences first, so that what is left at the end is short (37 sequences
+        // of up to 4096 tokens, 296 blocks: 76 against 93 to 99 us). A sequence's place is the number of longer ones,
+        // of the same length those before it.
+        int* held = reinterpret_cast<int*>(smem);                 // [threads] lengths, behind them the block's sequence
+        const int mine = tid < a.B ? tokens_of(tid) : -1;
+        held[tid] = mine;
+        __syncthreads();
+        if (tid < a.B) {
+            int place = 0;
+            for (int i = 0; i < a.B; ++i) place += held[i] > mine || (held[i] == mine && i < tid);
+            if (place == b) held[kTreeThreads] = tid;
+        }
+        __syncthreads();
+        b = held[kTreeThreads];
+    }
+    const int tile = (b * a.hkv + hk) * a.row_tiles + rt;
+    const int n = tokens_of(b);
     const Mx4Tree tree(a, b, n);
     const int per_split = mx4_split_groups(n, a.splits), groups = mx4_groups(n);
     const int c0 = min(groups, split * per_split), count = min(groups, c0 + per_split) - c0;
