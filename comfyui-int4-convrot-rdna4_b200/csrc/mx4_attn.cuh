@@ -60,7 +60,7 @@ struct Mx4AttnArgs {
     const int* lens;
     void* out;
     float* part;                   // per (tile, split, row): the mean of the split's values, D floats ...
-    float2* part_ml;               // ... and {reference, sum of weights}
+    float2* part_ml;               // ... and {reference, sum of weights}; in a tree's first split below zero: the row is written
     int B, tq, hq, hkv, page_bits, pages, group, row_tiles, splits;
     int clustered;                 // a sequence's splits are one cluster and join themselves
     float scale;                   // softmax scale times log2(e)
@@ -868,6 +868,7 @@ __global__ void __launch_bounds__(256) mx4_attn_join_kernel(Mx4AttnArgs a, int t
     const int held = per_split ? (mx4_groups(n) + per_split - 1) / per_split : 0;          // splits that hold tokens
     const size_t at = ((static_cast<size_t>(b) * a.hkv + hk) * a.row_tiles + row / tile_rows) * a.splits * tile_rows + row % tile_rows;
     const float2* ml = a.part_ml + at;
+    if (a.mask && held && ml->y < 0.0f) return;                   // (the row is written)
     float top = -INFINITY, sum = 0.0f;
     for (int s = lane; s < held; s += 32) top = fmaxf(top, ml[static_cast<size_t>(s) * tile_rows].x);
     #pragma unroll

@@ -42,6 +42,10 @@ struct TreePlan {
     bool tensor, pair;
 };
 
+// Whether blocks take the sequences in the order of their lengths: more of them than multiprocessors, and no
+// more sequences than a block has threads.
+bool tree_order(int B, long long blocks) { return B > 1 && B <= kTreeThreads && blocks > sm_count(); }
+
 TreePlan tree_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
     TreePlan t{};
     const long long rows = static_cast<long long>(tq) * (hq / hkv);
@@ -62,13 +66,21 @@ TreePlan tree_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
     t.p.tile_rows = t.pair ? 2 * kTreeTile : kTreeTile;
     t.p.row_tiles = static_cast<int>((rows + t.p.tile_rows - 1) / t.p.tile_rows);
     t.p.tiles = static_cast<long long>(B) * hkv * t.p.row_tiles;
-    // as many splits as give the least waves of blocks times tiles of a block, a block's start and
-    // end counted as two tiles
+    // Splits by the estimated time of two batches of that longest length, in us (a block's start and end 13, a split's
+    // mean on its way out 3, the join 9 and memory's time). All sequences that long: waves of blocks; whole
+    // sequences where blocks go by length and are enough. Lengths evenly spread: the longest
+    // one's blocks, or the work and a part of a block at the end. One split where more are not a
+    // tenth better. Two instead of one: 8 ragged sequences of up to 16384 tokens of 512 rows 334
+    // against 432 us, all of 16384 444 against 433; up to 4096 (where it takes one) 139 against 126.
     const long long groups = std::max(1LL, (longest + kTreeTile - 1) / kTreeTile), sms = sm_count();
-    long long best = -1;
-    t.p.splits = 1;
+    const double tile = 3.6 * d / 128 * (t.pair ? 1.0 : 0.5), join = static_cast<double>(t.p.tiles) * t.p.tile_rows * d * 8 / 6.5e6;
+    double best = -1;
     for (long long s = 1; s <= std::min(groups, 64LL) && t.p.tiles * s <= 16 * sms + t.p.tiles; ++s) {
-        const long long cost = (t.p.tiles * s + sms - 1) / sms * ((groups + s - 1) / s + 2 + (s > 1));
+        const double block = (groups + s - 1) / s * tile + (s > 1 ? 16 : 13);
+        const bool whole = tree_order(B, t.p.tiles * s) && t.p.tiles * 5 >= sms * 4;
+        const double equal = whole ? (t.p.tiles + sms - 1) / sms * (groups * tile + 13) : (t.p.tiles * s + sms - 1) / sms * block;
+        const double spread = std::max(block, t.p.tiles * s * (block - (groups + s - 1) / s * tile / 2) / sms + block / 6);
+        const double both = equal + (B > 1 ? spread : equal), cost = s > 1 ? both + 18 + join * s : 0.9 * both;
         if (best < 0 || cost < best) {
             best = cost;
             t.p.splits = static_cast<int>(s);
@@ -84,7 +96,7 @@ int launch_tree(const Mx4AttnArgs& a, const AttnPlan& p, int vec_q, cudaStream_t
     cudaError_t e = ensure_smem(kernel, Cfg::kSmemBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
     e = launch_pdl(kernel, dim3(static_cast<unsigned>(p.tiles), p.splits), dim3(kTreeThreads), Cfg::kSmemBytes, stream, a, vec_q,
-                   static_cast<int>(a.B > 1 && a.B <= kTreeThreads && p.tiles * p.splits > sm_count()));
+                   tree_order(a.B, p.tiles * p.splits) ? sm_count() : 0);
     if (e == cudaSuccess && p.splits > 1) {
         const unsigned rows = static_cast<unsigned>(a.B * a.tq * a.hq);
         const int wide = p.splits > 16;

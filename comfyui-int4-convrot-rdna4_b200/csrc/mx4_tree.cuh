@@ -24,8 +24,8 @@
 // What bounds it: a stream's softmax (load, exp2, split, store: some 3500 cycles a tile, by the
 // latency of its 128 threads) takes turns with its own two products, and two streams a block
 // are what registers and tensor memory hold; a block starts in 3 to 9 us and ends in 6. 8 x 16384 tokens, 64
-// nodes of 64 query heads on 8 of 128: 465 us (1.18 PFLOP/s with both terms counted, 0.59 of the formula's;
-// tensor pipe 53 % of the active time, exp2's 27 %); 37 x 4096, 24 nodes of 24 on 8 of 64: 76 us.
+// nodes of 64 query heads on 8 of 128: 467 to 478 us (1.15 PFLOP/s with both terms counted, 0.59 of the formula's;
+// tensor pipe 53 % of the active time, exp2's 27 %); 37 x 4096, 24 nodes of 24 on 8 of 64: 74 us.
 // The kernel for few rows took 1820 and 277. Tiles in halves of 64 tokens: 541 and 103.
 #pragma once
 
@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
     float* row_scale = reinterpret_cast<float*>(smem + Cfg::kRowOffset);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.y;
+    int splits = a.splits;                                        // of the sequence
     const int rt = blockIdx.x % a.row_tiles, hk = blockIdx.x / a.row_tiles % a.hkv;
     int b = blockIdx.x / a.row_tiles / a.hkv;
     const int per_head = a.hq / a.hkv, rows_all = a.tq * per_head;
@@ -169,26 +170,34 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
     auto tokens_of = [&](int i) { return max(0, static_cast<int>(min(static_cast<long long>(a.lens[i]), a.cap))); };
     if (by_length) {
         // More blocks than multiprocessors: long sequences first, so that what is left at the end is short (37 sequences
-        // of up to 4096 tokens, 296 blocks: 76 against 93 to 99 us). A sequence's place is the number of longer ones,
-        // of the same length those before it.
-        int* held = reinterpret_cast<int*>(smem);                 // [threads] lengths, behind them the block's sequence
+        // of up to 4096 tokens, 296 blocks: 74 against 93 to 99 us). A sequence's place is the number of longer ones,
+        // of the same length those before it. Splits are cut by the table's width; a sequence that is no
+        // more than a quarter above a multiprocessor's share of all tiles stays whole.
+        int* held = reinterpret_cast<int*>(smem);                 // [threads] lengths, behind them the block's sequence, whether it stays whole
         const int mine = tid < a.B ? tokens_of(tid) : -1;
         held[tid] = mine;
         __syncthreads();
         if (tid < a.B) {
             int place = 0;
             for (int i = 0; i < a.B; ++i) place += held[i] > mine || (held[i] == mine && i < tid);
-            if (place == b) held[kTreeThreads] = tid;
+            if (place == b) {
+                float tiles = 0.0f;
+                for (int i = 0; splits > 1 && i < a.B; ++i) tiles += mx4_groups(held[i]);
+                held[kTreeThreads] = tid;
+                held[kTreeThreads + 1] = mx4_groups(mine) * static_cast<float>(by_length) <= 1.25f * tiles * (a.hkv * a.row_tiles);
+            }
         }
         __syncthreads();
         b = held[kTreeThreads];
+        if (held[kTreeThreads + 1]) splits = 1;
     }
+    if (split >= splits) return;
     const int tile = (b * a.hkv + hk) * a.row_tiles + rt;
     const int n = tokens_of(b);
     const Mx4Tree tree(a, b, n);
-    const int per_split = mx4_split_groups(n, a.splits), groups = mx4_groups(n);
+    const int per_split = mx4_split_groups(n, splits), groups = mx4_groups(n);
     const int c0 = min(groups, split * per_split), count = min(groups, c0 + per_split) - c0;
-    if (a.splits > 1 && count == 0) return;                       // (the join knows how many splits hold tokens)
+    if (splits > 1 && count == 0) return;                         // (the join knows how many splits hold tokens)
     // tiles of each stream, and where the second starts
     const int n0 = PAIR ? count : (count + 1) / 2, n1 = PAIR ? (rows > kTreeTile ? count : 0) : count - n0;
     const int c1 = PAIR ? c0 : c0 + n0;
@@ -834,11 +843,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                         }
                 }
             }
-            if (a.splits > 1) {
-                const size_t at = (static_cast<size_t>(tile) * a.splits + split) * kTileRows + (row - row0);
+            const size_t at = (static_cast<size_t>(tile) * a.splits + split) * kTileRows + (row - row0);
+            // (a whole sequence's rows need no join, which the sum below zero tells it)
+            if (from == 0 && a.splits > 1) a.part_ml[at] = splits > 1 ? make_float2(m, l) : make_float2(0.0f, -1.0f);
+            if (splits > 1) {
                 #pragma unroll
                 for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4*>(a.part + at * D + from + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                if (from == 0) a.part_ml[at] = make_float2(m, l);
             } else {
                 tree_rotate(v, a.group);
                 const float f = tree_factor(a.group);
