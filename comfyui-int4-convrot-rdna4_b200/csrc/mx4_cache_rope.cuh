@@ -92,16 +92,15 @@ mx4_cache_append_rope_kernel(const __grid_constant__ Mx4AppendRope a, Mx4CacheSh
                 float fa[VP], fb[VP];
                 ra[0].get(fa);
                 rb[0].get(fb);
-                if (at.any()) rope_turn<VP>(fa, fb, w, r.interleaved);
+                if (at.any()) rope_turn<VP>(fa, fb, w, at, r.interleaved);
                 if (i0 + i < count) {
                     if (kind == 2) {
                         if (ti < a.tokens) {
                             T* to = static_cast<T*>(a.q_out) + (static_cast<long long>(ti) * a.hq + hi) * D;
-                            RopeRaw<T, VP> o;
-                            o.put(fa);
-                            o.store(to + at.a);
-                            o.put(fb);
-                            o.store(to + at.b);
+                            if (at.pair >= 0) ra[0].put(fa);
+                            if (at.pair_b >= 0) rb[0].put(fb);
+                            ra[0].store(to + at.a);
+                            rb[0].store(to + at.b);
                         }
                     } else {
                         slab_put<D, VP>(slab, from + i0 + i, at.a, fa);

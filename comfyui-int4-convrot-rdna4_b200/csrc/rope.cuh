@@ -51,7 +51,7 @@ struct RopeArgs {
 
 // Where a thread's 2 VP channels lie: VP from a and VP from b, so that neighbours' chunks are
 // neighbours in memory. In halves a pair has one channel in each; interleaved, each chunk holds VP / 2 pairs.
-// `pair`: the first pair, and of the second chunk's where they are interleaved; -1: none, a plain copy.
+// `pair`, `pair_b`: the first pair of each chunk; -1: none, the chunk is copied as it is.
 template <int VP>
 struct RopePlace {
     int a, b, pair, pair_b;
@@ -66,11 +66,11 @@ struct RopePlace {
         } else if (r.interleaved) {
             a = 2 * u;
             b = a + 1;
-            if (turned && u < r.pairs) pair = u;
+            if (turned && u < r.pairs) pair = pair_b = u;
         } else if (u < whole) {
             a = VP * u;
             b = r.pairs + a;
-            if (turned) pair = a;
+            if (turned) pair = pair_b = a;
         } else {
             a = 2 * r.pairs + VP * (u - whole);
             b = a + (D / 2 - r.pairs);
@@ -131,16 +131,15 @@ struct RopeCoef {
             return;
         }
         constexpr int kHalf = VP > 1 ? VP / 2 : 1;
-        #pragma unroll
-        for (int i = 0; i < VP; ++i) { c[i] = 1.0f; s[i] = 0.0f; }
         if (at.pair >= 0) group<0, kHalf>(r, b, t, at.pair);
         if constexpr (VP > 1)
             if (at.pair_b >= 0) group<kHalf, VP - kHalf>(r, b, t, at.pair_b);
     }
 };
 
+// (A chunk of interleaved channels without pairs stays: a turn by 0 would give a neighbour's infinity or NaN to it.)
 template <int VP>
-__device__ __forceinline__ void rope_turn(float (&a)[VP], float (&b)[VP], const RopeCoef<VP>& w, bool interleaved) {
+__device__ __forceinline__ void rope_turn(float (&a)[VP], float (&b)[VP], const RopeCoef<VP>& w, const RopePlace<VP>& at, bool interleaved) {
     auto turn = [](float& x, float& y, float c, float s) {
         const float z = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
         y = __fadd_rn(__fmul_rn(x, s), __fmul_rn(y, c));
@@ -149,8 +148,8 @@ __device__ __forceinline__ void rope_turn(float (&a)[VP], float (&b)[VP], const 
     if (VP > 1 && interleaved) {
         #pragma unroll
         for (int i = 0; i + 1 < VP; i += 2) {
-            turn(a[i], a[i + 1], w.c[i / 2], w.s[i / 2]);
-            turn(b[i], b[i + 1], w.c[(VP + i) / 2], w.s[(VP + i) / 2]);
+            if (at.pair >= 0) turn(a[i], a[i + 1], w.c[i / 2], w.s[i / 2]);
+            if (at.pair_b >= 0) turn(b[i], b[i + 1], w.c[(VP + i) / 2], w.s[(VP + i) / 2]);
         }
     } else {
         #pragma unroll
@@ -254,9 +253,9 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
                     float fa[VP], fb[VP];
                     ra[i].get(fa);
                     rb[i].get(fb);
-                    rope_turn<VP>(fa, fb, w, r.interleaved);
-                    ra[i].put(fa);
-                    rb[i].put(fb);
+                    rope_turn<VP>(fa, fb, w, at, r.interleaved);
+                    if (at.pair >= 0) ra[i].put(fa);
+                    if (at.pair_b >= 0) rb[i].put(fb);
                 }
                 ra[i].store(to + at.a);
                 rb[i].store(to + at.b);
