@@ -2,7 +2,9 @@
 // s = max |y| / 127, codes = y / s to nearest, ties to even. R is the ConvRot rotation,
 // which is linear, so 1 / rms goes to the scale alone: the codes are those of
 // R(h g), and a row needs one pass and one exchange (sum of squares and largest
-// magnitude together). All in fp32, without an intermediate rounding.
+// magnitude together). All in fp32, without an intermediate rounding. Rows that leave its range on the
+// way (squares from 1.8 10^19, h g beyond 3.4 10^38, squares that vanish) are left to a second loop
+// of the block, which takes them times powers of two.
 //
 // A thread has 16 neighbouring columns, a warp 512 (two groups of 256). The steps of the
 // rotation at strides 1 and 4 stay in the thread; for those at 16 and 64 the 16 x 16 values
@@ -19,6 +21,7 @@
 namespace convrot {
 
 constexpr int kRmsMostK = 16384;              // 32 warps a row
+constexpr float kRmsLeast = 0x1p-100f;        // a mean of squares below it has lost some of them
 constexpr int kRmsWarpFloats = 512 + 16;      // a warp's values; the second group 16 floats on: other banks
 
 struct RmsQuantArgs {
@@ -136,33 +139,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
         else gains(static_cast<const __half*>(a.g));
     }
     const float per_k = 1.0f / static_cast<float>(a.K);
-    // (every warp of the block makes as many rounds: they meet at barriers)
-    for (int row0 = static_cast<int>(blockIdx.x) * a.rows, round = 0; row0 < a.M; row0 += static_cast<int>(gridDim.x) * a.rows, ++round) {
-        float2 v[8];
-        x.get(v);
-        if (a.r) {
-            float2 w[8];
-            r.get(w);
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fadd2_rn(v[i], w[i]);
-            if (column && row < a.M) {
-                RmsRaw<T> o;
-                o.put(v);
-                uint4* h = reinterpret_cast<uint4*>(static_cast<T*>(a.h) + static_cast<size_t>(row) * a.K + col);
-                #pragma unroll
-                for (int c = 0; c < RmsRaw<T>::kChunks; ++c) h[c] = o.v[c];
-            }
-        }
-        const int now = row;
-        row += static_cast<int>(gridDim.x) * a.rows;
-        load(row);
-        float2 squares = make_float2(0.0f, 0.0f);
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            squares = ffma2_rn(v[i], v[i], squares);
-            v[i] = fmul2_rn(v[i], g[i]);
-        }
-        float ss = squares.x + squares.y, amax = 0.0f;
+    // The row's codes and scale from its h times a power of two up_h, and v, h g times up_v; the sum of squares and the
+    // largest magnitude meet in p. In the first loop (both powers 1) a row that left fp32's range gets instead
+    // of a scale -(1 + 3 i + j), with which powers it has to be taken; whether it did is returned.
+    auto quantize = [&](auto first, float2 (&v)[8], float ss, int now, bool kept, float2* p, float up_h, float up_v) -> bool {
+        constexpr bool kFirst = decltype(first)::value;
+        float amax = 0.0f;
         rms_rotate16(v, true);
         if constexpr (G >= 64) {
             // value 16 l + i of a group (of its thread l) lies in row l, its chunks of four XORed: neither
@@ -183,7 +165,6 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
         rms_reduce<32>(ss, amax);
         if (a.row_warps > 1) {
             constexpr int kMost = THREADS / 32;                   // warps of a row
-            float2* p = part[round & 1];
             if (lane == 0) p[warp] = make_float2(ss, amax);
             __syncthreads();
             const float2 y = lane % kMost < a.row_warps ? p[warp - in_row + lane % kMost] : make_float2(0.0f, 0.0f);
@@ -191,14 +172,22 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
             amax = y.y;
             rms_reduce<kMost>(ss, amax);
         }
-        const float rstd = 1.0f / sqrtf(fmaf(ss, per_k, a.eps));
+        const float mean = fmaf(ss, per_k, kFirst ? a.eps : a.eps * up_h * up_h);
+        float rstd = 1.0f / sqrtf(mean);
+        if (!kFirst) rstd *= up_h / up_v;                          // (for h g as it is scaled)
         const float y = amax * unit_factor<G>() * rstd;
-        const float s = (y < 1e-10f ? 1e-10f : y) / 127.0f;       // (NaN stays)
+        float s = (y < 1e-10f ? 1e-10f : y) / 127.0f;             // (NaN stays)
         // |v f| is 127 and roundings at most: a sum with 1.5 * 2^23 has the code in its last byte. (f finite: 0 stays 0)
         const float f = fminf(unit_factor<G>() * rstd / s, 3.4e38f);
         const float2 by = make_float2(f, f), shift = make_float2(12582912.0f, 12582912.0f);
         #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = ffma2_rn(v[i], by, shift);
+        const bool odd = kFirst && !(mean >= kRmsLeast && mean < INFINITY && amax < INFINITY);
+        if (odd) {
+            // What 2^-100 takes below the range is less than 2^-60 of the row's largest; 2^100 is for rows below 2^-43.
+            const bool small = mean < kRmsLeast, large = !(mean < INFINITY), wide = !(amax < INFINITY);
+            s = -1.0f - (small ? 3.0f : large ? 6.0f : 0.0f) - (wide || (large && amax >= 1.0f) ? 2.0f : small && amax < 0x1p-60f ? 1.0f : 0.0f);
+        }
         uint32_t out[4];
         if constexpr (G >= 64) {
             __syncwarp();
@@ -220,10 +209,63 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
                 out[c] = __byte_perm(lo, hi, 0x5410);
             }
         }
-        if (now < a.M) {
+        if (kept) {
             if (column) *reinterpret_cast<uint4*>(a.codes + static_cast<size_t>(now) * a.K + col) = make_uint4(out[0], out[1], out[2], out[3]);
             if (in_row == 0 && lane == 0) a.scales[now] = s;
         }
+        return odd && kept;
+    };
+    auto sum_of = [&](float2 (&v)[8]) {                           // x + r
+        x.get(v);
+        if (!a.r) return;
+        float2 w[8];
+        r.get(w);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fadd2_rn(v[i], w[i]);
+    };
+    // (every warp of the block makes as many rounds: they meet at barriers)
+    const int stride = static_cast<int>(gridDim.x) * a.rows;
+    bool odd = false;
+    for (int row0 = static_cast<int>(blockIdx.x) * a.rows, round = 0; row0 < a.M; row0 += stride, ++round) {
+        float2 v[8];
+        sum_of(v);
+        if (a.r && column && row < a.M) {
+            RmsRaw<T> o;
+            o.put(v);
+            uint4* h = reinterpret_cast<uint4*>(static_cast<T*>(a.h) + static_cast<size_t>(row) * a.K + col);
+            #pragma unroll
+            for (int c = 0; c < RmsRaw<T>::kChunks; ++c) h[c] = o.v[c];
+        }
+        const int now = row;
+        row += stride;
+        load(row);
+        float2 squares = make_float2(0.0f, 0.0f);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            squares = ffma2_rn(v[i], v[i], squares);
+            v[i] = fmul2_rn(v[i], g[i]);
+        }
+        odd |= quantize(std::true_type{}, v, squares.x + squares.y, now, now < a.M, part[round & 1], 1.0f, 1.0f);
+    }
+    if (!__syncthreads_or(odd)) return;
+    row = static_cast<int>(blockIdx.x) * a.rows + warp / a.row_warps;
+    #pragma unroll 1
+    for (int row0 = static_cast<int>(blockIdx.x) * a.rows; row0 < a.M; row0 += stride, row += stride) {
+        const float mark = row < a.M ? __ldcg(a.scales + row) : 0.0f;
+        if (!__syncthreads_or(mark < 0.0f)) continue;             // (a round's exchange is over, too, before the next)
+        const int code = mark < 0.0f ? static_cast<int>(-mark) - 1 : 0;
+        const float up_h = code >= 6 ? 0x1p-100f : code >= 3 ? 0x1p100f : 1.0f, up_v = code % 3 == 2 ? 0x1p-100f : code % 3 == 1 ? 0x1p100f : 1.0f;
+        load(row);
+        float2 v[8];
+        sum_of(v);
+        float2 squares = make_float2(0.0f, 0.0f);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 h = fmul2_rn(v[i], make_float2(up_h, up_h));
+            squares = ffma2_rn(h, h, squares);
+            v[i] = fmul2_rn(fmul2_rn(v[i], make_float2(up_v, up_v)), g[i]);
+        }
+        quantize(std::false_type{}, v, squares.x + squares.y, row, mark < 0.0f, part[0], up_h, up_v);
     }
 }
 

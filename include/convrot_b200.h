@@ -416,7 +416,8 @@ size_t ck_convrot_w8a8_linear_rmsnorm_workspace_size(int M, int K);
 /* The W8A8 linear behind a root-mean-square norm: hidden = x + residual (rounded to dtype; residual NULL:
  * hidden is not written), y = R(h / sqrt(mean h^2 + eps) * norm_weight), xs = max(max |y|, 1e-10) / 127,
  * codes = y / xs to nearest even, out = ((float(D) * xs[m]) * wscale[n]) + bias[n] with the exact product
- * D. fp32 throughout, h unrounded; a row with an infinity or a NaN gives NaN.
+ * D. fp32 throughout, h unrounded; a row with an infinity or a NaN gives NaN, finite rows of any
+ * magnitude are normalised. hidden must not overlap x or residual.
  *   x, residual [M, K] (row strides ldx, ldr >= K), hidden [M, K] (16-byte aligned) in dtype;
  *   norm_weight [K] in norm_dtype or NULL (ones); W [N, K] int8 and out [M, N] 16-byte aligned, wscale [N]
  *   f32, bias [N] in bias_dtype or NULL; out_dtype 0 f32, 1 bf16; G in {16, 64, 256}, K a multiple of G and
