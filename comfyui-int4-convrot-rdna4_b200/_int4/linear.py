@@ -116,10 +116,14 @@ class Int4ConvRotLinear(torch.nn.Module):
     def forward_rmsnorm(self, x: torch.Tensor, norm_weight: torch.Tensor | None = None, residual: torch.Tensor | None = None,
                         eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
         """``self(rms_norm(x + residual) * norm_weight)`` and x + residual, as a transformer block takes
-        them. Plain int8 layers run it in one pass over x (``_int4.convrot_w8a8_linear_rmsnorm``);
-        int4 layers and layers with Dynamic-LoRA adapters, whose down projection needs the
-        normalised rows, add and normalise in torch first."""
-        if self._qmode == "int8" and not self._dyn_lora:
+        them. Plain int8 layers run it in one pass over x (``_int4.convrot_w8a8_linear_rmsnorm``),
+        up to its 16384 inputs, in its rotation groups and with a residual of x's type; other int8
+        layers, int4 layers and layers with Dynamic-LoRA adapters, whose down projection needs the
+        normalised rows, add and normalise in torch first (some eight kernels, and rows rounded to
+        x's type before they are quantized)."""
+        fused = (self.in_features <= 16384 and self._qgs in (16, 64, 256) and x.dtype in (torch.float32, torch.bfloat16, torch.float16)
+                 and (residual is None or residual.dtype == x.dtype))
+        if self._qmode == "int8" and not self._dyn_lora and fused:
             return convrot_w8a8_linear_rmsnorm(x, self._q, self._qs, self.bias, norm_weight, residual, eps, self._qgs)
         h = x.float() if residual is None else x.float() + residual.float()
         y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps)
