@@ -255,10 +255,14 @@ class Mx4SelfAttention(torch.nn.Module):
         positions = self._positions(positions, t)
         q, k, v = self.project(x)
         new = torch.tensor(cache.extend(seq, t), dtype=torch.int64, device=device)
-        q = self._store(q, k, v, cache, new, positions)
-        ks, vs = cache.read(torch.tensor(cache.slots(seq), dtype=torch.int64, device=device), x.dtype)
-        n = ks.shape[0]
-        seen = torch.ones(t, n, dtype=torch.bool, device=device).tril(n - t)
-        y = torch.nn.functional.scaled_dot_product_attention(
-            q.transpose(0, 1)[None], ks.transpose(0, 1)[None], vs.transpose(0, 1)[None], attn_mask=seen, enable_gqa=True)
-        return self.out(y[0].transpose(0, 1).reshape(t, self.heads * self.head_dim))
+        try:
+            q = self._store(q, k, v, cache, new, positions)
+            ks, vs = cache.read(torch.tensor(cache.slots(seq), dtype=torch.int64, device=device), x.dtype)
+            n = ks.shape[0]
+            seen = torch.ones(t, n, dtype=torch.bool, device=device).tril(n - t)
+            y = torch.nn.functional.scaled_dot_product_attention(
+                q.transpose(0, 1)[None], ks.transpose(0, 1)[None], vs.transpose(0, 1)[None], attn_mask=seen, enable_gqa=True)
+            return self.out(y[0].transpose(0, 1).reshape(t, self.heads * self.head_dim))
+        except BaseException:
+            cache.accept(seq, t, ())                              # (the new tokens' slots are given back)
+            raise

@@ -1,0 +1,23 @@
+"""Bookkeeping of the cache and the trees where a call fails or has nothing to do (no GPU needed)."""
+import pytest
+import torch
+
+import _int4
+from _int4.mx4_layers import Mx4KVCache, Mx4SelfAttention
+
+
+def test_a_prefill_that_fails_on_its_way_to_the_cache_reserves_no_tokens():
+    """Frequencies of the wrong type, of more pairs than a head, sections that do not add up, tensors that the kernels
+    do not take: the sequence keeps its length and its pages."""
+    f = _int4.rope_freqs(32, device="cpu")
+    for how in (dict(freqs=f.float()), dict(freqs=_int4.rope_freqs(64, device="cpu")), dict(freqs=f, sections=(8, 25)), dict(freqs=f), dict()):
+        block = Mx4SelfAttention(64, 2, 1, 64, device="cpu", **how)
+        block.project = lambda x: (torch.zeros(len(x), 2, 64), torch.zeros(len(x), 1, 64), torch.zeros(len(x), 1, 64))
+        cache = Mx4KVCache(4, 1, 64, page=16, device="cpu")
+        seq = cache.add()
+        cache.extend(seq, 7)
+        free, held = list(cache._free), list(cache._pages[seq])
+        axes = (2,) if "sections" in how else ()
+        with pytest.raises(ValueError):
+            block.prefill(torch.zeros(20, 64), cache, seq, torch.zeros(20, *axes) if "freqs" in how else None)
+        assert cache.length(seq) == 7 and cache._pages[seq] == held and sorted(cache._free) == sorted(free)
