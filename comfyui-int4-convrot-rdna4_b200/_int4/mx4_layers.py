@@ -160,9 +160,10 @@ class Mx4KVCache:
         slots = self.slots(seq)
         moved = [(slots[start + i], slots[start + to]) for to, i in enumerate(kept) if i != to]
         if moved:
-            src, dst = torch.tensor(moved, dtype=torch.int64, device=self.codes.device).unbind(1)
-            for t in (self.codes, self.scales):                   # (read as a whole before it is written)
-                t[dst // self.page, :, :, dst % self.page] = t[src // self.page, :, :, src % self.page]
+            with torch.inference_mode(self.codes.is_inference()):  # (a cache made there can be written there alone)
+                src, dst = torch.tensor(moved, dtype=torch.int64, device=self.codes.device).unbind(1)
+                for t in (self.codes, self.scales):               # (read as a whole before it is written)
+                    t[dst // self.page, :, :, dst % self.page] = t[src // self.page, :, :, src % self.page]
         self._len[seq] = start + len(kept)
         pages = self._pages[seq]
         while len(pages) > -(-self._len[seq] // self.page):

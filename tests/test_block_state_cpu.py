@@ -21,3 +21,23 @@ def test_a_prefill_that_fails_on_its_way_to_the_cache_reserves_no_tokens():
         with pytest.raises(ValueError):
             block.prefill(torch.zeros(20, 64), cache, seq, torch.zeros(20, *axes) if "freqs" in how else None)
         assert cache.length(seq) == 7 and cache._pages[seq] == held and sorted(cache._free) == sorted(free)
+
+
+def test_accept_takes_caches_made_in_inference_mode():
+    with torch.inference_mode():
+        cache = Mx4KVCache(2, 1, 64, page=4, device="cpu")
+        codes = torch.randint(0, 255, cache.codes.shape, dtype=torch.uint8)
+        cache.codes.copy_(codes)
+    seq = cache.add()
+    new = cache.extend(seq, 6)
+    cache.accept(seq, 5, [1, 3])
+    assert cache.length(seq) == 3
+    for to, node in enumerate((1, 3)):
+        s, t = cache.slots(seq)[1 + to], new[1 + node]
+        assert torch.equal(cache.codes[s // 4, :, :, s % 4], codes[t // 4, :, :, t % 4])
+    plain = Mx4KVCache(2, 1, 64, page=4, device="cpu")
+    seq = plain.add()
+    plain.extend(seq, 6)
+    before = plain.codes._version
+    plain.accept(seq, 5, [1, 3])
+    assert plain.codes._version > before                          # (written in place)
