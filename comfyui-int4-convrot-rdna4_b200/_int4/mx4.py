@@ -203,9 +203,10 @@ def tree_mask(parents) -> tuple[torch.Tensor, torch.Tensor]:
     position context + depth. Worked out on the host and given back on the parents' device.
     """
     given = torch.as_tensor(parents)
-    if given.dim() not in (1, 2) or given.is_floating_point() or given.dtype == torch.bool:
+    if given.dim() not in (1, 2) or given.is_floating_point() or given.is_complex() or given.dtype == torch.bool:
         raise ValueError("parents must be whole numbers [T] or [B, T]")
-    p = given.cpu().long().reshape(-1, given.shape[-1])
+    p = given.cpu().long()
+    p = p[None] if given.dim() == 1 else p
     b, t = p.shape
     if bool(((p >= torch.arange(t)) | (p < -1)).any()):
         raise ValueError("a node's parent must be a node before it, or -1")

@@ -41,3 +41,11 @@ def test_accept_takes_caches_made_in_inference_mode():
     before = plain.codes._version
     plain.accept(seq, 5, [1, 3])
     assert plain.codes._version > before                          # (written in place)
+
+
+def test_trees_without_nodes():
+    for shape in ((0,), (3, 0), (0, 0), (0, 5)):
+        mask, depth = _int4.tree_mask(torch.zeros(shape, dtype=torch.int64))
+        assert mask.shape == (*shape, shape[-1]) and mask.dtype == torch.bool and depth.shape == shape and depth.dtype == torch.int64
+    with pytest.raises(ValueError, match="whole numbers"):
+        _int4.tree_mask(torch.zeros(3, dtype=torch.complex64))
