@@ -741,6 +741,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                         for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
                         tmem_st_32x32b_x16(to + 16 * at, o);
                     }
+                    if (c > 0) tmem_st_wait();                    // (what was laid down is read back)
                     #pragma unroll 1
                     for (int at = 0; at < c; ++at) {
                         uint32_t p[16];
