@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             const int up = top > 0.0f ? min(max(135 - e, -120), 120) : 0;
             // (the scale's sign goes to the queries, and 0 to the smallest number: a hidden score stays -inf)
             const float to_f16 = copysignf(__uint_as_float(static_cast<uint32_t>(127 + up) << 23), a.scale);
-            rs = fmaxf(fabsf(a.scale) * tree_factor(a.group) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-37f);
+            rs = fmaxf(fabsf(a.scale) * tree_factor(a.group) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1.4e-45f);
             if (!PAIR && D == 64 && mine) row_scale[r] = rs;
             #pragma unroll 1
             for (int from = kSplit ? 64 * s : 0; mine && from < D; from += 64) {

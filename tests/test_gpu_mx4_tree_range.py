@@ -10,6 +10,8 @@ pytestmark = pytest.mark.gpu
 
 SIZES = [(6, 128, 4), (50, 128, 64), (60, 64, 64), (16, 128, 64), (16, 64, 64)]        # nodes, D, query heads (on 2)
 
+LONG = [(6, 128, 4, 1250), (50, 128, 64, 1250), (60, 64, 64, 1250), (16, 128, 16, 9000), (16, 64, 16, 20000)]     # and tokens
+
 
 @pytest.fixture(scope="module")
 def mx():
@@ -43,3 +45,17 @@ def test_scores_that_jump_within_a_tile(mx, t, d, hq):
     n = torch.tensor(lens, dtype=torch.int32, device="cuda")
     out = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask)
     check(out, reference(q, codes, scales, table, lens, [t], mask, d ** -0.5, 64), q)
+
+
+@pytest.mark.parametrize("t,d,hq,tokens", LONG)
+def test_tiny_queries_meet_huge_keys(mx, t, d, hq, tokens):
+    """Queries of 2^-113 and keys of 2^104: scores that count, of rows whose factor is about the least normal number."""
+    lens = [tokens]
+    codes, scales, table = make_cache(mx, lens, 16, 2, d, 64, 33)
+    scales[:, 0] = (scales[:, 0].int() + 104).clamp(max=254).to(torch.uint8)
+    q = (torch.randn(1, t, hq, d, generator=torch.Generator().manual_seed(3)) * 2.0 ** -113).bfloat16().cuda()
+    mask = mx.tree_mask(trees(1, t, 6))[0].cuda()
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for scale in (2.0 ** -4, -2.0 ** -3, 2.0 ** 5):
+        out = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask, softmax_scale=scale)
+        check(out, reference(q, codes, scales, table, lens, [t], mask, scale, 64), q)
