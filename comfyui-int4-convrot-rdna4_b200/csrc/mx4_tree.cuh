@@ -9,7 +9,8 @@
 //
 //   S = Q K^T   queries rotated in fp32, then two f16 terms (22 bits) of the row times a power of two;
 //               a key's codes times 2^(E_b - E), E its largest scale exponent, are f16 values, and
-//               2^E goes to its column of S in fp32
+//               2^E goes to its column of S in fp32; blocks more than 2^23 below it are left out there and
+//               added to the scores by fp32 products (tree_far_scores)
 //   O = P V     values are bf16 exactly, whatever their scale; weights two bf16 terms (16 bits)
 //
 // S lies in tensor memory, the weights take its place (16 columns of S: 8 of the first terms, 8 of
@@ -35,6 +36,8 @@ constexpr int kTreeTile = 128;                 // tokens of a tile, rows of a st
 constexpr int kTreeThreads = 15 * 32;
 constexpr float kTreeDown = 24.0f;
 constexpr float kTreeMost = 6.1035156e-5f;     // 2^-14: weights of a chunk above this move the reference
+constexpr int kTreeBits = 23;                  // a code times 2^-23 is an f16 value exactly
+constexpr uint32_t kTreeApart = 1, kTreeFar = 2;          // of a tile: keys, or blocks of one key, lie further apart
 
 template <int D, bool PAIR>
 struct Mx4TreeCfg {
@@ -45,9 +48,10 @@ struct Mx4TreeCfg {
     // a pair: four terms of queries, K, two tiles of V; otherwise two terms, then K and V of each stream
     static constexpr int kFacOffset = (PAIR ? 7 : 6) * kOperand;  // [buffer][parity][128] fp32: factors of a tile's keys
     static constexpr int kBufs = PAIR ? 1 : 2;                    // buffers of K
-    static constexpr int kHidOffset = kFacOffset + kBufs * 1024;  // [buffer][parity][8]: hidden tokens' bits, keys far apart
-    static constexpr int kRangeOffset = kHidOffset + kBufs * 64;  // [2][2] largest and least exponents of a tile's keys
-    static constexpr int kRowOffset = kRangeOffset + 32;          // [256] fp32: the rows' scales (both streams' the same rows)
+    static constexpr int kHidOffset = kFacOffset + kBufs * 1024;  // [buffer][parity][8]: hidden tokens' bits, kTreeApart | kTreeFar
+    static constexpr int kRangeOffset = kHidOffset + kBufs * 64;  // [2][2] largest and least exponents of a tile's keys, [2][2] of a closer look
+    static constexpr int kOneOffset = kRangeOffset + 32;          // [16] fp32 ones: factors of columns that have theirs already
+    static constexpr int kRowOffset = kOneOffset + 64;            // [256] fp32: the rows' scales (both streams' the same rows)
     static constexpr int kBarOffset = kRowOffset + (PAIR ? 0 : 1024);
     static constexpr int kBars = 2 * 4 + 2 * 2 + 2 * 3 + 2;
     static constexpr int kEnd = kBarOffset + kBars * 8 + 16;
@@ -98,6 +102,12 @@ __device__ __forceinline__ uint32_t bf16x2_bits(float lo, float hi) {
     return r;
 }
 
+__device__ __forceinline__ float2 half2_bits(uint32_t x) {
+    __half2 h;
+    memcpy(&h, &x, 4);
+    return __half22float2(h);
+}
+
 // Two weights as the sum of two bf16 terms each: the upper halves as they are, and what they leave out.
 __device__ __forceinline__ void split_bf16(float2 w, uint32_t& hi, uint32_t& lo) {
     const uint32_t x = __float_as_uint(w.x), y = __float_as_uint(w.y);
@@ -142,6 +152,85 @@ __device__ __forceinline__ void tree_rotate(float (&v)[64], int group) {
 }
 
 __device__ __forceinline__ float tree_factor(int group) { return group == 16 ? 0.25f : group == 64 ? 0.125f : 1.0f; }
+
+// A tile's scores in tensor memory times its keys' factors, with what the products left out: the blocks of a key more
+// than 2^kTreeBits below its largest, times their own scales. All lanes of a warp take the same tokens, each its row r
+// of those that begin at `q`. Not inlined: few tiles need it, and the loop that calls it has no register to give. (8 x 4096 tokens
+// of 64 nodes, 64 query heads on 8 of 128: 133 us, with one such key among 64 387, with every key 3150.)
+template <int D>
+__device__ __noinline__ void tree_far_scores(uint32_t ts, const unsigned char* q, int r, const uint8_t* codes, const uint8_t* scales, const int* table,
+                                             int page_bits, int pages, int hkv, int hk, int j0, int n, const float* f) {
+    constexpr int kB = D / 32, kAtom = kTreeTile * 128, kOperand = kTreeTile * D * 2;
+    auto place_of = [&](int j) -> long long {
+        const int page = j < n ? table[j >> page_bits] : -1;
+        if (page < 0 || page >= pages) return -1;
+        return (((static_cast<long long>(page) * 2 * hkv + hk) << page_bits) + (j & ((1 << page_bits) - 1)));
+    };
+    auto exps_of = [&](long long place) -> uint32_t {
+        return D == 128 ? reinterpret_cast<const uint32_t*>(scales)[place] : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(scales)[place]);
+    };
+    auto exp_at = [](uint32_t exps, int c) { return static_cast<int>((exps >> (8 * c)) & 255u); };
+    auto top_of = [&](uint32_t exps) {
+        int top = 0;
+        #pragma unroll
+        for (int c = 0; c < kB; ++c)
+            if (exp_at(exps, c) != 255) top = max(top, exp_at(exps, c));
+        return top;
+    };
+    #pragma unroll 1
+    for (int at = 0; at < kTreeTile; at += 16) {
+        const long long mine = place_of(j0 + at + (threadIdx.x & 15));
+        const uint32_t own = mine < 0 ? 0u : exps_of(mine);
+        bool far = false;
+        #pragma unroll
+        for (int c = 0; c < kB; ++c) far |= exp_at(own, c) != 255 && top_of(own) - exp_at(own, c) > kTreeBits;
+        uint32_t left = __ballot_sync(0xFFFFFFFFu, far) & 0xFFFFu;
+        float more[16];
+        #pragma unroll
+        for (int k = 0; k < 16; ++k) more[k] = 0.0f;
+        #pragma unroll 1
+        for (; left; left &= left - 1) {
+            const int k = __ffs(left) - 1;
+            const long long place = __shfl_sync(0xFFFFFFFFu, mine, k);
+            const uint32_t exps = __shfl_sync(0xFFFFFFFFu, own, k);
+            const int top = top_of(exps);
+            float all = 0.0f;
+            #pragma unroll 1
+            for (int c = 0; c < kB; ++c) {
+                const int e = exp_at(exps, c);
+                if (e == 255 || top - e <= kTreeBits) continue;
+                const uint4 x = *reinterpret_cast<const uint4*>(codes + place * (D / 2) + c * 16);
+                const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+                float sum = 0.0f;
+                #pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t h[4];
+                    codes_to_f16(words[w], h);
+                    const unsigned char* row = q + (c / 2) * kAtom + r * 128 + ((((c & 1) * 4 + w) ^ (r & 7)) << 4);
+                    const uint4 hi = *reinterpret_cast<const uint4*>(row), lo = *reinterpret_cast<const uint4*>(row + kOperand);
+                    const uint32_t a[4] = {hi.x, hi.y, hi.z, hi.w}, b[4] = {lo.x, lo.y, lo.z, lo.w};
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 u = half2_bits(a[i]), v = half2_bits(b[i]), z = half2_bits(h[i]);
+                        sum = fmaf(u.x + v.x, z.x, fmaf(u.y + v.y, z.y, sum));
+                    }
+                }
+                all = fmaf(sum, __uint_as_float(max(static_cast<uint32_t>(e) << 23, 0x00400000u)), all);
+            }
+            #pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i == k) more[i] = all;
+        }
+        uint32_t x[16];
+        __syncwarp();
+        tmem_ld_32x32b_x16(ts + at, x);
+        tmem_ld_wait_regs16(x);
+        #pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), f[at + k], more[k]));
+        tmem_st_32x32b_x16(ts + at, x);
+    }
+    tmem_st_wait();
+}
 
 template <typename T, int D, bool PAIR>
 __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a, int vec_q, int by_length) {
@@ -219,6 +308,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
         *nan_nodes = 0;
         fence_mbar_init();
     }
+    if (tid < 16) reinterpret_cast<float*>(smem + Cfg::kOneOffset)[tid] = 1.0f;
     if (warp == 14) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
@@ -461,19 +551,44 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                     for (int c = 0; c < kB; ++c) {
                         const int e = static_cast<int>((exps[k] >> (8 * c)) & 255u);
                         if (e != 255) top[k] = max(top[k], e);
-                        if (e != 255 && e != 0) low = min(low, e);                // (0: blocks of zeros, or the least there is)
+                        if (e != 255 && held[k]) low = min(low, e);
                     }
                 }
                 const uint32_t gone0 = __ballot_sync(0xFFFFFFFFu, !held[0]), gone1 = __ballot_sync(0xFFFFFFFFu, !held[1]);
                 int most = __reduce_max_sync(0xFFFFFFFFu, max(top[0], top[1])), least = __reduce_min_sync(0xFFFFFFFFu, low);
                 if (lane == 0) range[(u & 1) * 2 + warp - 12] = make_short2(static_cast<short>(most), static_cast<short>(least));
                 named_barrier_sync(1, 64);
-                // A code times 2^-23 is an f16 value exactly: where the tile's exponents lie no further apart
-                // one factor serves all columns.
+                // Where the tile's exponents lie no further apart than kTreeBits one factor serves all columns.
                 const short2 other = range[(u & 1) * 2 + (warp & 1 ^ 1)];
                 most = max(most, static_cast<int>(other.x));
                 least = min(least, static_cast<int>(other.y));
-                const bool apart = most - least > 23;
+                uint32_t spread = 0;
+                if (most - least > kTreeBits) {                   // (the same in both warps)
+                    // Once more without blocks of zeros, whose exponent is 0, and for each token by itself.
+                    int own[2] = {255, 255};
+                    #pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        #pragma unroll
+                        for (int c = 0; c < kB; ++c) {
+                            const int e = static_cast<int>((exps[k] >> (8 * c)) & 255u);
+                            const uint4 x = codes[k][c];
+                            if (e != 255 && (e != 0 || ((x.x | x.y | x.z | x.w) & 0x77777777u) != 0u)) own[k] = min(own[k], e);
+                        }
+                    const bool far = __any_sync(0xFFFFFFFFu, max(top[0] - own[0], top[1] - own[1]) > kTreeBits);
+                    least = __reduce_min_sync(0xFFFFFFFFu, min(own[0], own[1]));
+                    if (lane == 0) range[4 + (u & 1) * 2 + warp - 12] = make_short2(far, static_cast<short>(least));
+                    named_barrier_sync(1, 64);
+                    const short2 there = range[4 + (u & 1) * 2 + (warp & 1 ^ 1)];
+                    spread = (most - min(least, static_cast<int>(there.y)) > kTreeBits ? kTreeApart : 0u) | (far || there.x ? kTreeFar : 0u);
+                    #pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        #pragma unroll
+                        for (int c = 0; c < kB; ++c) {
+                            const int e = static_cast<int>((exps[k] >> (8 * c)) & 255u);
+                            if (e != 255 && top[k] - e > kTreeBits) codes[k][c] = make_uint4(0, 0, 0, 0);      // (tree_far_scores takes it)
+                        }
+                }
+                const bool apart = spread != 0u;
                 // (the barriers of the two warps go on: neither waits for one that left)
                 ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&k_empty[buf], (i & 1) ^ 1));
                 if (!ok) continue;
@@ -487,7 +602,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                     if (!apart) top[k] = most;
                     fac[at * 128 + id + 64 * k] = __uint_as_float(max(static_cast<uint32_t>(top[k]) << 23, 0x00400000u));
                 }
-                if (id == 0) hid[at * 8 + 4] = apart;
+                if (id == 0) hid[at * 8 + 4] = spread;
                 mbar_arrive(&f_full[at]);
                 #pragma unroll 1
                 for (int k = 0; k < 2; ++k) {
@@ -686,6 +801,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             if (c < 8) {
                 // From chunk c on: the reference moves to the largest score, what was summed and laid down
                 // gets the new scale.
+                const bool far = slow && (gone[4] & kTreeFar);
+                if (far) tree_far_scores<D>(ts, smem + (PAIR ? 2 * s : 0) * Cfg::kOperand, r, a.codes, a.scales, a.table + b * a.table_ld, a.page_bits, a.pages,
+                                            a.hkv, hk, j0, n, f);
                 unsigned long long seen[2] = {~0ull, ~0ull};      // columns that this row sees
                 if (hides) {
                     #pragma unroll
@@ -709,9 +827,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 auto columns = [&](int at, uint32_t (&x)[16]) {
                     if (!slow) return;
                     const uint32_t bits = static_cast<uint32_t>((at < 4 ? seen[0] : seen[1]) >> (16 * (at & 3)));
+                    const float* by = far ? reinterpret_cast<const float*>(smem + Cfg::kOneOffset) : f + 16 * at;
                     #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float y = __uint_as_float(x[k]) * f[16 * at + k];
+                        const float y = __uint_as_float(x[k]) * by[k];
                         x[k] = bits >> k & 1u ? __float_as_uint(y) : 0xFF800000u;
                     }
                 };

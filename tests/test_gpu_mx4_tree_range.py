@@ -59,3 +59,52 @@ def test_tiny_queries_meet_huge_keys(mx, t, d, hq, tokens):
     for scale in (2.0 ** -4, -2.0 ** -3, 2.0 ** 5):
         out = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask, softmax_scale=scale)
         check(out, reference(q, codes, scales, table, lens, [t], mask, scale, 64), q)
+
+
+@pytest.mark.parametrize("every", [1, 9])
+@pytest.mark.parametrize("t,d,hq,tokens", LONG)
+def test_blocks_of_a_key_far_apart(mx, t, d, hq, tokens, every):
+    """Blocks of 32 channels of one key whose scales lie up to 2^90 apart, and heads whose queries look at one block each:
+    every block keeps its own precision, that of scale byte 0 included."""
+    lens = [tokens]
+    codes, scales, table = make_cache(mx, lens, 16, 2, d, 0, 35)
+    blocks = d // 32
+    step = 24 if blocks == 4 else 40
+    low = [step * (blocks - 1 - c) - step * (blocks - 1) // 2 for c in range(blocks)]          # exponents added to the blocks'
+    far = torch.zeros(codes.shape[0] * 16, dtype=torch.bool)
+    far[::every] = True
+    far = far.reshape(-1, 1, 16, 1).cuda()
+    shift = torch.tensor(low, dtype=torch.int32, device="cuda")
+    scales[:, 0] = torch.where(far, scales[:, 0].int() + shift, scales[:, 0].int()).clamp(1, 254).to(torch.uint8)
+    g = torch.Generator().manual_seed(3)
+    q = torch.zeros(1, t, hq, d)
+    for h in range(hq):
+        c = h % blocks
+        q[:, :, h, 32 * c:32 * c + 32] = torch.randn(1, t, 32, generator=g) * 2.0 ** -low[c]
+    q = q.bfloat16().cuda()
+    mask = mx.tree_mask(trees(1, t, 6))[0].cuda()
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+    def run(q, scales):
+        out = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask, convrot_groupsize=0)
+        check(out, reference(q, codes, scales, table, lens, [t], mask, d ** -0.5, 0), q)
+        again = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask, convrot_groupsize=0)
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+    if every == 1:
+        run(q, scales)
+    else:
+        # (ordinary keys beside them: queries that are moderate for both)
+        run(q * torch.tensor([2.0 ** min(0, x) for x in low], device="cuda").repeat_interleave(32).bfloat16(), scales)
+    # a block of scale byte 0, 2^-127, beside ordinary ones, and one that is NaN
+    least = scales.clone()
+    least[:, 0] = torch.where(far, scales[:, 0] * 0 + 127, scales[:, 0])
+    least[:, 0, :, :, 1] = torch.where(far[..., 0], 0, least[:, 0, :, :, 1])
+    q = torch.zeros(1, t, hq, d)
+    q[..., 32:64] = torch.randn(1, t, hq, 32, generator=g) * 2.0 ** 124
+    q = q.bfloat16().cuda()
+    if every == 1:
+        run(q, least)
+        j = lens[0] - t - 3
+        held = least.clone()
+        held[int(table[0, j // 16]), 0, :, j % 16, 0] = 255
+        assert mx.convrot_mx4_tree_attention(q, codes, held, table, n, mask, convrot_groupsize=0).isnan().all()
