@@ -1436,10 +1436,12 @@ int dispatch_gemm_i8(const void* X, const void* W, const float* xs, const float*
 int run_gemm_i8(const void* X, const void* W, const float* xs, const float* ws, BiasRef bias, void* out, int out_dtype,
                 int M, int N, int K, cudaStream_t stream) {
     if (out_dtype == 1 && N % 8 == 0 && aligned16(out)) {
-        // 192-column tiles where 256-column ones are the choice and the waves of tiles come out shorter
-        // (509 x 6144 x 4096: 64 tiles for 74 CTA pairs instead of 48, 13.4 against 17.6 us)
+        // 192-column tiles where 256-column ones are the choice and the waves of tiles come out shorter by more than a
+        // tenth. K 1024 to 15360, us with 256 and with 192 columns (quantizer included): 509 x 6144, one wave of either,
+        // 12.4 : 11.5 to 63 : 58 (K 4096 22.5 : 18.2); 4096 x 6144, 6 : 7 waves, 35.3 : 34.7 to 341 : 329; but 4096 x 12288,
+        // 11 : 14, 71.5 : 81.3 to 577 : 584, and 4096 x 4096, 4 : 5, the same within 2 %
         const long pairs = sm_count() / 2, rows = (M + 255) / 256, tiles256 = rows * ((N + 255) / 256), tiles192 = rows * ((N + 191) / 192);
-        if (2 * tiles256 >= pairs && (tiles192 + pairs - 1) / pairs * 3 < (tiles256 + pairs - 1) / pairs * 4)
+        if (2 * tiles256 >= pairs && (tiles192 + pairs - 1) / pairs * 5 < (tiles256 + pairs - 1) / pairs * 6)
             return launch_pair_impl<192, false, kOutBF16, true, false, true>(X, W, xs, ws, bias, out, M, N, K, LoraArgs(), stream);
     }
     if (out_dtype == 1) return dispatch_gemm_i8<kOutBF16>(X, W, xs, ws, bias, out, M, N, K, stream);

@@ -280,7 +280,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) rms_quant_int
 // start under that kernel. A thread has 32 neighbouring bytes of each of two rows, so that four threads
 // ask for a whole line: 1 x 15360 x 3840 takes 14.8 us with the quantizer, against 16.2 in
 // pieces of 16 bytes (9.0 by the weight's bytes; a start of two kernels is some 4).
-constexpr int kFewI8Rows = 16;                 // (32 x 15360 x 3840: 33 us against 19 in tiles of 256 rows; 8: 11)
+// (16 rows here and 17 in tiles of 256 rows, us with the quantizer: 15360 x 3840 14.3 and 19.8, 4096 x 4096 8.1 and 12.8,
+// 3840 x 15360 17.0 and 27.5. 32 rows of 15360 x 3840 took 33 here, and 20 in tiles.)
+constexpr int kFewI8Rows = 16;
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
