@@ -97,7 +97,7 @@ mx4_cache_append_rope_kernel(const __grid_constant__ Mx4AppendRope a, Mx4CacheSh
                     if (kind == 2) {
                         if (ti < a.tokens) {
                             T* to = static_cast<T*>(a.q_out) + (static_cast<long long>(ti) * a.hq + hi) * D;
-                            if (at.pair >= 0) ra[0].put(fa);
+                            if (at.any()) ra[0].put(fa);
                             if (at.pair_b >= 0) rb[0].put(fb);
                             ra[0].store(to + at.a);
                             rb[0].store(to + at.b);

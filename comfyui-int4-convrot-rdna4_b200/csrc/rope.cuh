@@ -51,7 +51,7 @@ struct RopeArgs {
 
 // Where a thread's 2 VP channels lie: VP from a and VP from b, so that neighbours' chunks are
 // neighbours in memory. In halves a pair has one channel in each; interleaved, each chunk holds VP / 2 pairs.
-// `pair`, `pair_b`: the first pair of each chunk; -1: none, the chunk is copied as it is.
+// `pair`, `pair_b`: the first pair of each chunk; -1: none, the chunk is copied as it is (b if a is: it lies behind).
 template <int VP>
 struct RopePlace {
     int a, b, pair, pair_b;
@@ -76,7 +76,7 @@ struct RopePlace {
             b = a + (D / 2 - r.pairs);
         }
     }
-    __device__ __forceinline__ bool any() const { return pair >= 0 || pair_b >= 0; }
+    __device__ __forceinline__ bool any() const { return pair >= 0; }
 };
 
 // Sine and cosine of a (radians, finite and below some 2^50 in magnitude), rounded to fp32: reduced to
@@ -131,7 +131,7 @@ struct RopeCoef {
             return;
         }
         constexpr int kHalf = VP > 1 ? VP / 2 : 1;
-        if (at.pair >= 0) group<0, kHalf>(r, b, t, at.pair);
+        group<0, kHalf>(r, b, t, at.pair);
         if constexpr (VP > 1)
             if (at.pair_b >= 0) group<kHalf, VP - kHalf>(r, b, t, at.pair_b);
     }
@@ -148,7 +148,7 @@ __device__ __forceinline__ void rope_turn(float (&a)[VP], float (&b)[VP], const 
     if (VP > 1 && interleaved) {
         #pragma unroll
         for (int i = 0; i + 1 < VP; i += 2) {
-            if (at.pair >= 0) turn(a[i], a[i + 1], w.c[i / 2], w.s[i / 2]);
+            turn(a[i], a[i + 1], w.c[i / 2], w.s[i / 2]);
             if (at.pair_b >= 0) turn(b[i], b[i + 1], w.c[(VP + i) / 2], w.s[(VP + i) / 2]);
         }
     } else {
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) rope_kernel(const
                     ra[i].get(fa);
                     rb[i].get(fb);
                     rope_turn<VP>(fa, fb, w, at, r.interleaved);
-                    if (at.pair >= 0) ra[i].put(fa);
+                    ra[i].put(fa);
                     if (at.pair_b >= 0) rb[i].put(fb);
                 }
                 ra[i].store(to + at.a);
