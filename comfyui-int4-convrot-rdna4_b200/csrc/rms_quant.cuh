@@ -291,8 +291,7 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 
 template <int NT, typename T>
 __global__ void __launch_bounds__(512)
-few_i8_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, const float* __restrict__ xs, const float* __restrict__ ws,
-              BiasRef bias, T* __restrict__ out, int M, int N, int K) {
+few_i8_kernel(const int8_t* x, const int8_t* __restrict__ w, const float* xs, const float* __restrict__ ws, BiasRef bias, T* out, int M, int N, int K) {
     constexpr int kAhead = 2;                                     // segments of 128 columns on their way
     extern __shared__ int few_sums[];                             // [warp][row][17]
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -332,7 +331,7 @@ few_i8_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, const 
                     const int at = 128 * (s + i) + 16 * h;
                     #pragma unroll
                     for (int k = 0; k < NT; ++k) {
-                        // (the rows' codes come from the kernel before: no read-only loads)
+                        // (the rows' codes come from the kernel before, which may still write: no read-only loads)
                         const uint4 b = at + 32 * t < K ? *reinterpret_cast<const uint4*>(xr[k] + at) : zero;
                         mma_s8(d[k], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
                         mma_s8(d[k], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
