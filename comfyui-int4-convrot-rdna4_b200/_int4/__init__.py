@@ -349,7 +349,9 @@ def convrot_w8a8_linear_rmsnorm(
     returned is rounded to x's dtype). x, residual [..., K] of one dtype (float32,
     bfloat16 or float16), K a multiple of the group (16, 64 or 256) and at most 16384;
     qweight int8 [N, K], wscales [N], norm_weight [K] and bias [N] in any of the three
-    types or None. Without a residual the second value is x itself. out is in x's dtype;
-    a row with an infinity or a NaN gives NaN. Forward only.
+    types or None. Without a residual the second value is x itself. out is in x's dtype (for
+    float16 written in fp32 and cast by torch: 10 bytes an output instead of 2, 1080 us against
+    830 for 16384 x 15360 x 3840); a row with an infinity or a NaN gives NaN, finite rows of any
+    magnitude are normalised. Forward only.
     """
     return _native().linear_rmsnorm(x, qweight, wscales, bias, norm_weight, residual, eps, convrot_groupsize)

@@ -187,7 +187,8 @@ def convrot_mx4_cache_append_rope(codes: torch.Tensor, scales: torch.Tensor, q: 
     and returned in its dtype, k is turned in fp32 and goes on to the cache without a
     rounding between, v is written as by ``convrot_mx4_cache_append``. q, k and v have one
     dtype and any token and head strides; positions [T] or, with several sections,
-    [T, axes], freqs, sections and interleaved as in ``apply_rope``. A slot outside the
+    [T, axes], freqs, sections and interleaved as in ``apply_rope``, whose default for
+    ``interleaved`` is the other one: name it where both serve one model. A slot outside the
     cache writes nothing (its query is turned all the same); two tokens of one call must
     not share a slot.
     """
@@ -229,6 +230,9 @@ def convrot_mx4_tree_attention(q: torch.Tensor, codes: torch.Tensor, scales: tor
     itself only if named). tree_mask bool [T, T] for all sequences or [B, T, T].
     tree_lens int32 [B]: nodes of each sequence, its newest tokens (cut to 0 .. T; None: T
     each); the rows behind them are zeros. q [B, T, Hq, D], block_table and seq_lens (nodes
-    included) as there; a node that sees nothing gives zeros.
+    included) as there; a node that sees nothing gives zeros. Calls of the same shapes repeat bit
+    for bit; by the rows of a cache head and the table's width one of two kernels runs, which hold the
+    softmax weights to 22 bits (few rows, heads of 256) or 16: within the output's rounding of each other for
+    means of ordinary size, which lose bits from some 2^-115 down.
     """
     return (_native or native()).tree_attention(q, codes, scales, block_table, seq_lens, tree_mask, tree_lens, softmax_scale, convrot_groupsize)

@@ -152,7 +152,8 @@ class Mx4KVCache:
         """Ends a tree's verification: of the sequence's ``nodes`` newest tokens those numbered
         ``kept`` stay (in rising order, a path from the root), the others' tokens and the pages
         behind the last are given back. Keys carry their positions already: a node's depth must
-        be its place on the path."""
+        be its place on the path. Worked out on the host, one sequence a call, four indexing kernels
+        where a token moves; it cannot be captured into a graph."""
         kept = [int(i) for i in kept]
         start = self._len[seq] - nodes
         if nodes < 0 or start < 0 or any(not 0 <= i < nodes for i in kept) or any(b <= a for a, b in zip(kept, kept[1:])):
@@ -174,7 +175,8 @@ class Mx4SelfAttention(torch.nn.Module):
     """Causal self-attention of new tokens over a paged MX4 cache, with MX4 projections.
 
     freqs (float64 [pairs], ``rope_freqs``): rotary positions for queries and keys, with
-    sections and interleaved as in ``apply_rope``; None: no position embedding. A model that
+    sections and interleaved as in ``apply_rope`` (there neighbours are the default, here halves); None:
+    no position embedding. A model that
     has another one calls the parts itself: ``project``, its embedding of q and k,
     ``cache.append``, ``cache.attend``, ``out``.
     """

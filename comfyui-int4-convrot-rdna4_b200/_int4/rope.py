@@ -27,10 +27,13 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, se
     """Turns the heads x [..., H, D] by their tokens' positions; returns a new tensor in x's dtype.
 
     Pair i of a head is channels (2i, 2i + 1) where ``interleaved``, else (i, i + P), of P
-    pairs; channels behind the 2P first stay as they are. Its angle is position times
+    pairs; channels behind the 2P first are copied. Its angle is position times
     freqs[i] (float64 [P], radians a position). sections: pairs of each position axis,
     adding up to P (None: one axis). positions int32, int64 or float32, broadcast to x's
     leading sizes [...], with several sections to [..., axes]. Angles are taken in 64 bits.
+
+    ``convrot_mx4_cache_append_rope`` and the layers on it have ``interleaved=False`` by default: name
+    the order where queries and keys go through both.
 
     x float32, bfloat16 or float16, any strides but a contiguous D (with more than two
     leading sizes a copy is made where they are not one stride); q and k as heads of one

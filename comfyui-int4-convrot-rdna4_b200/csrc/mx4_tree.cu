@@ -70,8 +70,9 @@ TreePlan tree_plan(int B, int tq, int hq, int hkv, int d, long long longest) {
     // mean on its way out 3, the join 9 and memory's time). All sequences that long: waves of blocks; whole
     // sequences where blocks go by length and are enough. Lengths evenly spread: the longest
     // one's blocks, or the work and a part of a block at the end. One split where more are not a
-    // tenth better. Two instead of one: 8 ragged sequences of up to 16384 tokens of 512 rows 334
-    // against 432 us, all of 16384 444 against 433; up to 4096 (where it takes one) 139 against 126.
+    // tenth better. Two instead of one, three draws of lengths each: 8 sequences of up to 16384 tokens of 512 rows 344, 376
+    // and 446 against 441 to 446 us, all of 16384 465 against 444 to 460 (it takes two); up to 4096 153 to 165 against 132 to
+    // 138, all of 4096 153 against 136; 37 of up to 4096, heads of 64, 93 to 105 against 84 to 94 (it takes one in both).
     const long long groups = std::max(1LL, (longest + kTreeTile - 1) / kTreeTile), sms = sm_count();
     const double tile = 3.6 * d / 128 * (t.pair ? 1.0 : 0.5), join = static_cast<double>(t.p.tiles) * t.p.tile_rows * d * 8 / 6.5e6;
     double best = -1;

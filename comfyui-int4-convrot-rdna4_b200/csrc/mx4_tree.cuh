@@ -18,15 +18,19 @@
 // one stream's softmax runs under the other's products, and K and V (32 KB a tile at heads of 128)
 // are refilled under the products that do not read them.
 //
-// Weights are 2^(s - m - 24), m near the row's maximum: sums of up to 2^24 of them stay
-// below one, so that O does not leave fp32's range where the mean does not. m moves when a score
-// is 2^8 above it.
+// Weights are 2^(s - m - 24). m lags the row's maximum by 2^10 at most: a chunk of 16 columns whose weights sum to
+// more than 2^-14 moves it, where scores go column by column a score 2^6 above it. A stream's sum is then below one up to
+// 2^18 tokens, below 2^13 at the longest table, so that O stays in fp32's range for values up to 2^114; and
+// values below 2^-102 give products below its normal numbers: means lose bits from some 2^-115 down.
+// 16 bits a weight (the kernel for few rows has 22): what they leave out is 2^-16 of the mean of the
+// magnitudes at most, and by its random sign far less of the mean; a third term has no room in tensor memory.
 //
 // What bounds it: a stream's softmax (load, exp2, split, store: some 3500 cycles a tile, by the
 // latency of its 128 threads) takes turns with its own two products, and two streams a block
 // are what registers and tensor memory hold; a block starts in 3 to 9 us and ends in 6. 8 x 16384 tokens, 64
-// nodes of 64 query heads on 8 of 128: 467 to 478 us (1.15 PFLOP/s with both terms counted, 0.59 of the formula's;
-// tensor pipe 53 % of the active time, exp2's 27 %); 37 x 4096, 24 nodes of 24 on 8 of 64: 74 us.
+// nodes of 64 query heads on 8 of 128: 474 to 482 us (1.14 PFLOP/s with both terms counted, 0.57 of the formula's;
+// tensor pipe 44 to 53 % of the active time, exp2's 22 to 27 %); 37 x 4096, 24 nodes of 24 on 8 of 64: 72 to 79 us.
+// Registers are full: heads of 128 spill 32 to 40 bytes, heads of 64 none.
 // The kernel for few rows took 1820 and 277. Tiles in halves of 64 tokens: 541 and 103.
 #pragma once
 

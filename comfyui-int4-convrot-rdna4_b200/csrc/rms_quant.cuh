@@ -12,10 +12,13 @@
 // goes through rows, keeps its columns' g in registers and loads the next row's
 // values under the current one's work.
 //
-// 16384 x 3840 in bf16: 64 us, 2.9 TB/s (a copy of the rows 41); the fp32 pipe, shared memory and issue are each
-// busy half to two thirds of the time, and a row's exchange and divisions leave 24 warps a
-// multiprocessor waiting in turns. Single operations instead of pairs, and codes by conversions, took 78; four
-// blocks a multiprocessor (64 registers) 73. The product behind it is the int8 GEMM of the other linears.
+// 16384 x 3840 in bf16, caches cold: 72 us, 2.6 TB/s (a copy of the rows 41); the fp32 pipe, shared memory and issue
+// are each busy half to two thirds of the time, and a row's exchange and divisions leave 24 warps a
+// multiprocessor waiting in turns. With a residual 86 us (5.1 TB/s); 8192 x 8192 with one 108 (4.3), 4096 x 15360 113 (3.9; fp32
+// 246, 3.3). Above 4096 columns a row's warps are a block of 64 registers a thread: 52 to 64 bytes spill (fp32 304; below,
+// fp32 24 to 52). The second loop inside the first, instead of behind it, took 80 us; single operations instead of pairs, and codes
+// by conversions, 78 against 64 without that loop; four blocks a multiprocessor (64 registers) 73. The product behind it is the
+// int8 GEMM of the other linears.
 #pragma once
 
 namespace convrot {
