@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 most = max(most, static_cast<int>(other.x));
                 least = min(least, static_cast<int>(other.y));
                 uint32_t spread = 0;
-                if (most - least > kTreeBits) {                   // (the same in both warps)
+                if (__builtin_expect(most - least > kTreeBits, 0)) {          // (the same in both warps)
                     // Once more without blocks of zeros, whose exponent is 0, and for each token by itself.
                     int own[2] = {255, 255};
                     #pragma unroll
@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 // From chunk c on: the reference moves to the largest score, what was summed and laid down
                 // gets the new scale.
                 const bool far = slow && (gone[4] & kTreeFar);
-                if (far) tree_far_scores<D>(ts, smem + (PAIR ? 2 * s : 0) * Cfg::kOperand, r, a.codes, a.scales, a.table + b * a.table_ld, a.page_bits, a.pages,
+                if (__builtin_expect(far, 0)) tree_far_scores<D>(ts, smem + (PAIR ? 2 * s : 0) * Cfg::kOperand, r, a.codes, a.scales, a.table + b * a.table_ld, a.page_bits, a.pages,
                                             a.hkv, hk, j0, n, f);
                 unsigned long long seen[2] = {~0ull, ~0ull};      // columns that this row sees
                 if (hides) {
