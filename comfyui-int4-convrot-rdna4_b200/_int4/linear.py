@@ -119,8 +119,8 @@ class Int4ConvRotLinear(torch.nn.Module):
         them. Plain int8 layers run it in one pass over x (``_int4.convrot_w8a8_linear_rmsnorm``),
         up to its 16384 inputs, in its rotation groups and with a residual of x's type; other int8
         layers, int4 layers and layers with Dynamic-LoRA adapters, whose down projection needs the
-        normalised rows, add and normalise in torch first (some eight kernels, and rows rounded to
-        x's type before they are quantized)."""
+        normalised rows, add and normalise in torch first (some eight kernels, rows rounded to x's
+        type before they are quantized, and magnitudes up to 1.8e19, where the squares leave fp32)."""
         fused = (self.in_features <= 16384 and self._qgs in (16, 64, 256) and x.dtype in (torch.float32, torch.bfloat16, torch.float16)
                  and (residual is None or residual.dtype == x.dtype))
         if self._qmode == "int8" and not self._dyn_lora and fused:
