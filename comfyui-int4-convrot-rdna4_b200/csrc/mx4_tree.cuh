@@ -41,6 +41,7 @@ constexpr int kTreeThreads = 15 * 32;
 constexpr float kTreeDown = 24.0f;
 constexpr float kTreeMost = 6.1035156e-5f;     // 2^-14: weights of a chunk above this move the reference
 constexpr int kTreeBits = 23;                  // a code times 2^-23 is an f16 value exactly
+constexpr float kTreeHuge = 268435456.0f;      // 2^28: scores whose own step is 16 and more
 constexpr uint32_t kTreeApart = 1, kTreeFar = 2;          // of a tile: keys, or blocks of one key, lie further apart
 
 template <int D, bool PAIR>
@@ -728,6 +729,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             rs = row_scale[r];
         }
         const bool node = real && t < tree.nodes;                 // (what other rows compute is not kept)
+        bool huge = false;                                        // some row's reference is beyond kTreeHuge
         for (int i = 0; ok && i < ns; ++i) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&s_full[s], i & 1) && mbar_wait_bounded(&f_full[buf * 2 + (i & 1)], (i >> 1) & 1));
             if (!ok) break;
@@ -738,11 +740,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             const bool hides = !__all_sync(0xFFFFFFFFu, !node || (j0 + kTreeTile <= tree.context && (gone[0] | gone[1] | gone[2] | gone[3]) == 0));
             // Scores to m's scale: what the products gave times the tile's own factor, or with columns that are
             // hidden or keys far apart, column by column.
-            const bool slow = hides || gone[4] != 0u;
+            const bool slow = hides || gone[4] != 0u || huge;
             const float sc = slow ? rs : rs * f[0];
             float sum = 0.0f;
-            auto weights = [&](const uint32_t (&x)[16], float2 (&w)[8]) {
-                const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), by = make_float2(sc, sc);
+            auto weights = [&](const uint32_t (&x)[16], float2 (&w)[8], float scale) {
+                const float2 less = make_float2(-(m + kTreeDown), -(m + kTreeDown)), by = make_float2(scale, scale);
                 float2 part[2] = {};
                 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -770,18 +772,18 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 float here[2];
                 tmem_ld_32x32b_x16(ts, sr);
                 tmem_ld_wait_regs16(sr);
-                here[0] = weights(sr, w[0]);
+                here[0] = weights(sr, w[0], sc);
                 tmem_ld_32x32b_x16(ts + 16, sr);
                 #pragma unroll 1
                 for (; c < 6; c += 2) {
                     tmem_ld_wait_regs16(sr);
-                    here[1] = weights(sr, w[1]);
+                    here[1] = weights(sr, w[1], sc);
                     tmem_ld_32x32b_x16(ts + 16 * (c + 2), sr);
                     if (__any_sync(0xFFFFFFFFu, here[0] > kTreeMost)) break;
                     sum += here[0];
                     store(c, w[0]);
                     tmem_ld_wait_regs16(sr);
-                    here[0] = weights(sr, w[0]);
+                    here[0] = weights(sr, w[0], sc);
                     tmem_ld_32x32b_x16(ts + 16 * (c + 3), sr);
                     if (__any_sync(0xFFFFFFFFu, here[1] > kTreeMost)) { ++c; break; }
                     sum += here[1];
@@ -789,7 +791,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 }
                 tmem_ld_wait_regs16(sr);
                 if (c == 6) {
-                    here[1] = weights(sr, w[1]);
+                    here[1] = weights(sr, w[1], sc);
                     if (!__any_sync(0xFFFFFFFFu, here[0] > kTreeMost)) {
                         sum += here[0];
                         store(6, w[0]);
@@ -852,6 +854,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 if (__any_sync(0xFFFFFFFFu, top > m + 6.0f)) {
                     const float was = m;
                     m = fmaxf(m, top);
+                    huge = __any_sync(0xFFFFFFFFu, fabsf(m) >= kTreeHuge);
                     const float down = ex2(was - m);
                     l *= down;
                     sum *= down;
@@ -886,7 +889,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                     tmem_ld_32x32b_x16(ts + 16 * c, x);
                     tmem_ld_wait_regs16(x);
                     columns(c, x);
-                    sum += weights(x, w);
+                    if (__builtin_expect(huge, 0)) {
+                        // (rounded like the reference: half a step between the two would be more than an exponent holds)
+                        #pragma unroll
+                        for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(__fmul_rn(__uint_as_float(x[k]), sc));
+                    }
+                    sum += weights(x, w, huge ? 1.0f : sc);
                     store(c, w);
                 }
             }

@@ -108,3 +108,21 @@ def test_blocks_of_a_key_far_apart(mx, t, d, hq, tokens, every):
         held = least.clone()
         held[int(table[0, j // 16]), 0, :, j % 16, 0] = 255
         assert mx.convrot_mx4_tree_attention(q, codes, held, table, n, mask, convrot_groupsize=0).isnan().all()
+
+
+@pytest.mark.parametrize("up", [20, 34, 60, 90])
+@pytest.mark.parametrize("t,d,hq,tokens", LONG)
+def test_scores_of_any_finite_size(mx, t, d, hq, tokens, up):
+    """Scores of 2^20 to 2^90 pick the largest; steps of their own fp32 values, 2^66 there, are far above 1."""
+    lens = [tokens]
+    codes, scales, table = make_cache(mx, lens, 16, 2, d, 64, 37)
+    scales[:, 0] = (scales[:, 0].int() + up).clamp(max=254).to(torch.uint8)
+    q = torch.randn(1, t, hq, d, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    mask = mx.tree_mask(trees(1, t, 6))[0].cuda()
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for scale in (0.1, -0.3):
+        out = mx.convrot_mx4_tree_attention(q, codes, scales, table, n, mask, softmax_scale=scale)
+        ref, err = reference(q, codes, scales, table, lens, [t], mask, scale, 64)
+        check(out, (ref, err), q)
+        # (that tolerance grows with the scores, beyond the values: the means are finite and of the values' size)
+        assert out.isfinite().all() and float(out.abs().max()) <= 16 * float(abs(ref).max())
