@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
             rs = row_scale[r];
         }
         const bool node = real && t < tree.nodes;                 // (what other rows compute is not kept)
-        bool huge = false;                                        // some row's reference is beyond kTreeHuge
+        bool huge = false;                                        // some row's reference is beyond kTreeHuge (one without a score has none)
         for (int i = 0; ok && i < ns; ++i) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&s_full[s], i & 1) && mbar_wait_bounded(&f_full[buf * 2 + (i & 1)], (i >> 1) & 1));
             if (!ok) break;
@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) mx4_tree_kernel(Mx4AttnArgs a
                 if (__any_sync(0xFFFFFFFFu, top > m + 6.0f)) {
                     const float was = m;
                     m = fmaxf(m, top);
-                    huge = __any_sync(0xFFFFFFFFu, fabsf(m) >= kTreeHuge);
+                    huge = __any_sync(0xFFFFFFFFu, fabsf(m) >= kTreeHuge && m > kMx4NoScore);
                     const float down = ex2(was - m);
                     l *= down;
                     sum *= down;
