@@ -28,7 +28,7 @@
 // What bounds it: a stream's softmax (load, exp2, split, store: some 3500 cycles a tile, by the
 // latency of its 128 threads) takes turns with its own two products, and two streams a block
 // are what registers and tensor memory hold; a block starts in 3 to 9 us and ends in 6. 8 x 16384 tokens, 64
-// nodes of 64 query heads on 8 of 128: 474 to 482 us (1.14 PFLOP/s with both terms counted, 0.57 of the formula's;
+// nodes of 64 query heads on 8 of 128: 464 to 484 us (1.16 PFLOP/s with both terms counted, 0.58 of the formula's;
 // tensor pipe 44 to 53 % of the active time, exp2's 22 to 27 %); 37 x 4096, 24 nodes of 24 on 8 of 64: 72 to 79 us.
 // Registers are full: heads of 128 spill 32 to 40 bytes, heads of 64 none.
 // The kernel for few rows took 1820 and 277. Tiles in halves of 64 tokens: 541 and 103.
